@@ -480,6 +480,21 @@ int tt_tree_conv_bwd_ex(int dtype, int32_t C, int32_t S, int32_t K, const void* 
                         void* dx, float* dweight, float* dbias, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* ---- rotary positions ---------------------------------------------------- *
+ * Turns the first R dims (R even) of every head of q [n_tok, hq, D] and
+ * k [n_tok, hk, D] by the angle of the token's position; the other D - R dims
+ * are copied.  Pairs are (i, i + R/2), or (2i, 2i + 1) with `interleaved`.
+ * `table` [n_positions, R] fp32 holds R/2 cosines then R/2 sines a row;
+ * `inverse` turns the other way (the gradient).  Token and head strides of q
+ * and k are in elements, outputs are contiguous; hq or hk may be 0.  positions
+ * are int64 (positions64) or int32; a position outside the table makes the
+ * turned dims NaN and writes TT_ERR_INVALID_ARG into *status. */
+int tt_rotary(int dtype, int64_t n_tok, int32_t hq, int32_t hk, int32_t D, int32_t R,
+              int interleaved, int inverse, const void* q, int64_t q_st, int64_t q_sh,
+              const void* k, int64_t k_st, int64_t k_sh, const void* positions, int positions64,
+              const float* table, int64_t n_positions, void* q_out, void* k_out,
+              int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

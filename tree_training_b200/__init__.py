@@ -10,11 +10,13 @@ from .packer import (TreeNode, DFSTreeInfo, TreeAttnMeta, build_dfs_tree_info,  
 from .attention import (tree_attention, tree_attention_forward, register_hf_attention,  # noqa: F401
                         tree_mask_placeholder, meta_from_dense_mask, check_device_status,
                         prefetch_tree_meta, ATTN_IMPL_NAME)
+from .rotary import apply_rotary, rotary_table  # noqa: F401
 from ._lib import LIB_PATH, TTError  # noqa: F401
 
 __all__ = [
     "TreeNode", "DFSTreeInfo", "TreeAttnMeta", "build_dfs_tree_info",
     "gateway_intervals_from_bias", "tree_attention", "tree_attention_forward",
     "register_hf_attention", "tree_mask_placeholder", "meta_from_dense_mask",
-    "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
+    "apply_rotary", "rotary_table",
+        "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
 ]

@@ -1,0 +1,96 @@
+// Packs of V elements moved as one load or store of V * sizeof(T) bytes (2 to
+// 16), converted to and from fp32 registers.  A pack's address must be a
+// multiple of its size.
+#pragma once
+
+#include <type_traits>
+
+#include "tt_common.cuh"
+
+namespace tt {
+namespace vec {
+
+constexpr int kSMs = 148;   // of a B200: grids are sized by it
+
+template <int Bytes>
+struct RawOf;
+template <>
+struct RawOf<16> { using type = uint4; };
+template <>
+struct RawOf<8> { using type = uint2; };
+template <>
+struct RawOf<4> { using type = uint32_t; };
+template <>
+struct RawOf<2> { using type = uint16_t; };
+
+template <typename T, int V>
+using Raw = typename RawOf<(int)sizeof(T) * V>::type;
+
+// Read-only data used once: keeps it out of L1.
+template <typename R>
+__device__ __forceinline__ R ld_stream(const void* p) {
+  return __ldg(reinterpret_cast<const R*>(p));
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
+  return ld_stream<Raw<T, V>>(p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&v)[V]) {
+  union {
+    Raw<T, V> raw;
+    uint32_t w[(sizeof(T) * V + 3) / 4];
+    uint16_t h[(sizeof(T) * V + 1) / 2];
+  } u;
+  u.raw = r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      v[i] = __uint_as_float(u.w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      if constexpr (V == 1)
+        v[i] = __uint_as_float((uint32_t)u.h[0] << 16);
+      else
+        v[i] = __uint_as_float((i & 1) ? (u.w[i / 2] & 0xffff0000u) : (u.w[i / 2] << 16));
+    } else {
+      v[i] = __half2float(__ushort_as_half(u.h[i]));
+    }
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+  unpack<T, V>(load_raw<T, V>(p), v);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> pack(const float (&v)[V]) {
+  union {
+    Raw<T, V> raw;
+    T e[V];
+  } u = {};
+#pragma unroll
+  for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+  return u.raw;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+  *reinterpret_cast<Raw<T, V>*>(p) = pack<T, V>(v);
+}
+
+// Calls f with a value of the C++ type of a TT_* floating dtype.
+template <typename F>
+int dispatch_float(int dtype, F f) {
+  switch (dtype) {
+    case TT_BF16: return f(__nv_bfloat16());
+    case TT_F16: return f(__half());
+    case TT_F32: return f(float());
+    default: return TT_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace vec
+}  // namespace tt
