@@ -495,6 +495,32 @@ int tt_rotary(int dtype, int64_t n_tok, int32_t hq, int32_t hk, int32_t D, int32
               const float* table, int64_t n_positions, void* q_out, void* k_out,
               int32_t* status, void* stream);
 
+/* ---- norm after a block, gate, residual sum, norm before the next --------- *
+ *   h = x, or RMSNorm(x) * (offset + post_weight) where post_weight is given
+ *   r = residual + scale * gate * h;  y = RMSNorm(r) * (offset + weight)
+ * x, y [rows, D] of `dtype`, residual (null: zeros) and r of `res_dtype`
+ * (`dtype` or TT_F32), row strides in elements, outputs contiguous, D <= 16384.
+ * gate_mode: 0 none, 1 [D], 2 one value a row, 3 [rows, D]; gate of `dtype`,
+ * weights of fp32 (weight_f32) or `dtype`.  stats (may be null) [rows][2]
+ * fp32 keeps the two reciprocal root mean squares for the backward. */
+int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int32_t D, const void* x,
+                         int64_t x_st, const void* residual, int64_t res_st, const void* weight,
+                         const void* post_weight, int weight_f32, float weight_offset,
+                         const void* gate, int64_t gate_st, int gate_mode, float scale, float eps,
+                         void* y, void* r, float* stats, void* stream);
+/* Rows of fp32 partials the backward writes: `part` is [3][blocks][D]. */
+int tt_residual_norm_bwd_blocks(int64_t rows, int32_t D);
+/* dy, dr (null: zeros) are the gradients of y and r; every output may be null
+ * if it is not wanted.  dx, dres, dgate have the shape and type of their
+ * inputs, contiguous; dweight and dpost [D] have the weights' type. */
+int tt_residual_norm_bwd(int dtype, int res_dtype, int64_t rows, int32_t D, const void* x,
+                         int64_t x_st, const void* residual, int64_t res_st, const void* weight,
+                         const void* post_weight, int weight_f32, float weight_offset,
+                         const void* gate, int64_t gate_st, int gate_mode, float scale,
+                         const float* stats, const void* dy, int64_t dy_st, const void* dr,
+                         int64_t dr_st, void* dx, void* dres, void* dgate, void* dweight,
+                         void* dpost, float* part, int32_t blocks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@ from .attention import (tree_attention, tree_attention_forward, register_hf_atte
                         tree_mask_placeholder, meta_from_dense_mask, check_device_status,
                         prefetch_tree_meta, ATTN_IMPL_NAME)
 from .rotary import apply_rotary, rotary_table  # noqa: F401
+from .residual_norm import residual_norm  # noqa: F401
 from ._lib import LIB_PATH, TTError  # noqa: F401
 
 __all__ = [
@@ -18,5 +19,5 @@ __all__ = [
     "gateway_intervals_from_bias", "tree_attention", "tree_attention_forward",
     "register_hf_attention", "tree_mask_placeholder", "meta_from_dense_mask",
     "apply_rotary", "rotary_table",
-        "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
+    "residual_norm",     "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
 ]

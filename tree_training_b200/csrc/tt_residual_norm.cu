@@ -1,0 +1,558 @@
+// The edge between two blocks of a decoder layer in one pass each way: the norm
+// after a block, its gate, the residual sum and the norm before the next block.
+//
+//   h = x                              or  x i1 (o + w1),  i1 = rsqrt(mean x^2 + eps)
+//   r = residual + scale g h           g: 1, one value a channel, a row or an element
+//   y = r i2 (o + w2),                 i2 = rsqrt(mean r^2 + eps)
+//
+// and, given dy and dr (the gradients of y and r), with a = dr + i2 dy (o + w2)
+// and c = i2^3 / D * sum dy (o + w2) r:
+//
+//   d  = a - c r                        gradient of the residual
+//   dh = scale g d;  dg = scale h d     (summed over what g was spread over)
+//   dx = i1 dh (o + w1) - x i1^3 / D * sum dh (o + w1) x     (dh without w1)
+//   dw2 = sum over rows of dy r i2;  dw1 = sum over rows of dh x i1
+//
+// All sums over a row that the backward needs come out of one reduction: the
+// sum in dx splits into sum scale g (o + w1) x a  -  c sum scale g (o + w1) x r,
+// and both terms are known before c is.  r is recomputed from x and residual,
+// so no rounding of the stored r enters the gradients; i1 and i2 are kept from
+// the forward (8 bytes a row).
+//
+// A row lies in the registers of `tpr` threads, E elements each; a block of
+// 256 threads or one row takes whole rows and goes on to further ones, so the
+// weights, and in the backward the column sums of dw, are kept in registers.
+// The columns' sums leave as one row of partials a block, which a second
+// kernel adds up in a fixed order (no atomics).  Everything is fp32, rounded
+// once at the store.
+#include <algorithm>
+
+#include "tt_vec.cuh"
+
+namespace tt {
+namespace resnorm {
+namespace {
+
+enum Gate { kNone = 0, kChannel = 1, kRow = 2, kFull = 3 };
+
+struct Args {
+  int64_t rows;
+  int D, tpr;               // threads a row
+  const void *x, *res, *gate, *w2, *w1;
+  int64_t x_st, res_st, gate_st;
+  int gate_mode, w_f32;
+  float scale, offset, eps;
+  void *y, *r;
+  float* stats;             // [rows][2] i1, i2
+  const void *dy, *dr;
+  int64_t dy_st, dr_st;
+  void *dx, *dres, *dgate;
+  float* part;              // [3][blocks][D]: dw2, dw1, dgate of the channels
+};
+
+// Column of element e of thread t of a row: packs of 8 where rows are aligned,
+// single elements tpr apart otherwise.
+template <bool kVec>
+__device__ __forceinline__ int column(int e, int t, int tpr) {
+  return kVec ? (e / 8) * tpr * 8 + t * 8 + (e & 7) : e * tpr + t;
+}
+
+template <typename T, bool kVec, int E>
+struct Row {
+  // raw packs as loaded, so that a row can be fetched ahead at its own width
+  static constexpr int P = (int)sizeof(T) / 2;                 // 16-byte loads a pack of 8
+  uint4 raw[kVec ? E / 8 * P : 1];
+  T one[kVec ? 1 : E];
+
+  __device__ __forceinline__ void fetch(const T* row, int t, int tpr, int D, bool live) {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int b = 0; b < E / 8; ++b) {
+        const int c = column<true>(b * 8, t, tpr);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          raw[b * P + p] = (live && c < D)
+                               ? __ldg(reinterpret_cast<const uint4*>(row + c) + p)
+                               : make_uint4(0, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = column<false>(e, t, tpr);
+        one[e] = (live && c < D) ? row[c] : from_f32<T>(0.f);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void get(float (&v)[E]) const {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < E / 8 * P; ++i) {
+        constexpr int W = 16 / (int)sizeof(T);
+        float o[W];
+        vec::unpack<T, W>(raw[i], o);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[i * W + j] = o[j];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = to_f32(one[e]);
+    }
+  }
+};
+
+template <typename T, bool kVec, int E>
+__device__ __forceinline__ void put(T* row, int t, int tpr, int D, const float (&v)[E]) {
+  if constexpr (kVec) {
+    constexpr int W = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < E / W; ++i) {
+      const int c = column<true>(i * W, t, tpr);
+      if (c < D) {
+        float o[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[j] = v[i * W + j];
+        vec::store<T, W>(row + c, o);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = column<false>(e, t, tpr);
+      if (c < D) row[c] = from_f32<T>(v[e]);
+    }
+  }
+}
+
+template <typename T, bool kVec, int E>
+__device__ __forceinline__ void weights(const void* w, int f32, float offset, int t, int tpr,
+                                        int D, float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int c = column<kVec>(e, t, tpr);
+    v[e] = c >= D ? 0.f
+                  : offset + (f32 ? reinterpret_cast<const float*>(w)[c]
+                                  : to_f32(reinterpret_cast<const T*>(w)[c]));
+  }
+}
+
+// Sums of N values over the tpr threads of a row, the same in all of them.
+// tpr is a power of two up to 32, or a multiple of 32 (then `red`, N floats a
+// warp, is used; the caller alternates between two such areas, so that one
+// barrier a call is enough).
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* red) {
+  const int width = tpr < 32 ? tpr : 32;
+  for (int o = width >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  if (tpr <= 32) return;
+  const int warp = threadIdx.x >> 5, nw = tpr >> 5;
+  const int first = warp / nw * nw;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[warp * N + i] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int q = 0; q < nw; ++q) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += red[(first + q) * N + i];
+  }
+}
+
+constexpr int kMaxWarps = 32;
+
+template <typename T, typename R, bool kVec, int E, int kMaxThreads, bool kFullForm>
+__global__ void __launch_bounds__(kMaxThreads) fwd_kernel(const Args a) {
+  __shared__ float red[2][kMaxWarps];
+  const int t = threadIdx.x % a.tpr, slot = threadIdx.x / a.tpr;
+  const int per = blockDim.x / a.tpr;
+  const int D = a.D, tpr = a.tpr;
+  const bool post = kFullForm && a.w1 != nullptr;
+  const int mode = kFullForm ? a.gate_mode : kNone;
+  float w2[E], w1[E], gc[E];
+  weights<T, kVec, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
+  if (post) weights<T, kVec, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
+  if (mode == kChannel) weights<T, kVec, E>(a.gate, 0, 0.f, t, tpr, D, gc);
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.rows;
+    Row<T, kVec, E> rx;
+    Row<R, kVec, E> rr;
+    Row<T, kVec, E> rg;
+    rx.fetch(reinterpret_cast<const T*>(a.x) + row * a.x_st, t, tpr, D, live);
+    rr.fetch(reinterpret_cast<const R*>(a.res) + row * a.res_st, t, tpr, D, live && a.res);
+    if (mode == kFull)
+      rg.fetch(reinterpret_cast<const T*>(a.gate) + row * a.gate_st, t, tpr, D, live);
+    float h[E], r[E];
+    rx.get(h);
+    rr.get(r);
+    float i1 = 1.f;
+    if (post) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[0] = fmaf(h[e], h[e], s[0]);
+      row_sum<1>(s, tpr, red[turn]);
+      turn ^= 1;
+      i1 = rsqrtf(s[0] / D + a.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] *= i1 * w1[e];
+    }
+    float k = a.scale;
+    if (mode == kRow && live)
+      k *= to_f32(reinterpret_cast<const T*>(a.gate)[row * a.gate_st]);
+    if (mode == kChannel) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] *= gc[e];
+    } else if (mode == kFull) {
+      float g[E];
+      rg.get(g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] *= g[e];
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      r[e] = fmaf(k, h[e], r[e]);
+      s[0] = fmaf(r[e], r[e], s[0]);
+    }
+    row_sum<1>(s, tpr, red[turn]);
+    turn ^= 1;
+    const float i2 = rsqrtf(s[0] / D + a.eps);
+    if (live) {
+      put<R, kVec, E>(reinterpret_cast<R*>(a.r) + row * D, t, tpr, D, r);
+#pragma unroll
+      for (int e = 0; e < E; ++e) r[e] *= i2 * w2[e];
+      put<T, kVec, E>(reinterpret_cast<T*>(a.y) + row * D, t, tpr, D, r);
+      if (t == 0 && a.stats) {
+        a.stats[2 * row] = i1;
+        a.stats[2 * row + 1] = i2;
+      }
+    }
+  }
+}
+
+template <typename T, typename R, bool kVec, int E, int kMaxThreads, bool kFullForm>
+__global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
+  constexpr int N = kFullForm ? 3 : 1;
+  __shared__ float red[2][kMaxWarps * N];
+  extern __shared__ float cols[];           // [rows a block][D], where that is over one
+  const int t = threadIdx.x % a.tpr, slot = threadIdx.x / a.tpr;
+  const int per = blockDim.x / a.tpr;
+  const int D = a.D, tpr = a.tpr;
+  const bool post = kFullForm && a.w1 != nullptr;
+  const int mode = kFullForm ? a.gate_mode : kNone;
+  float w2[E], w1[E], gc[E], dw2[E], dw1[E], dgc[E];
+  weights<T, kVec, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
+  if (kFullForm) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) w1[e] = gc[e] = 1.f;
+    if (post) weights<T, kVec, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
+    if (mode == kChannel) weights<T, kVec, E>(a.gate, 0, 0.f, t, tpr, D, gc);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw2[e] = dw1[e] = dgc[e] = 0.f;
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.rows;
+    Row<T, kVec, E> rx, ry, rg;
+    Row<R, kVec, E> rr, rd;
+    rx.fetch(reinterpret_cast<const T*>(a.x) + row * a.x_st, t, tpr, D, live);
+    rr.fetch(reinterpret_cast<const R*>(a.res) + row * a.res_st, t, tpr, D, live && a.res);
+    ry.fetch(reinterpret_cast<const T*>(a.dy) + row * a.dy_st, t, tpr, D, live && a.dy);
+    rd.fetch(reinterpret_cast<const R*>(a.dr) + row * a.dr_st, t, tpr, D, live && a.dr);
+    if (mode == kFull)
+      rg.fetch(reinterpret_cast<const T*>(a.gate) + row * a.gate_st, t, tpr, D, live);
+    // a block's rows past the last hold zeros: they add nothing to any sum
+    const float i1 = live ? a.stats[2 * row] : 0.f, i2 = live ? a.stats[2 * row + 1] : 0.f;
+    float k = a.scale;
+    if (mode == kRow) k *= live ? to_f32(reinterpret_cast<const T*>(a.gate)[row * a.gate_st]) : 0.f;
+    float x[E], u[E], r[E], d[E], dy[E];
+    rx.get(x);
+    rr.get(r);
+    ry.get(dy);
+    rd.get(d);
+    if (mode == kFull) rg.get(u);
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (kFullForm) {
+        u[e] = mode == kFull ? u[e] : gc[e];     // the gate without a row's own
+        r[e] = fmaf(k * i1 * u[e] * w1[e], x[e], r[e]);
+      } else {
+        r[e] = fmaf(k, x[e], r[e]);
+      }
+      const float gy = dy[e] * w2[e];
+      dw2[e] = fmaf(dy[e] * i2, r[e], dw2[e]);
+      d[e] = fmaf(i2, gy, d[e]);                 // a
+      s[0] = fmaf(gy, r[e], s[0]);
+      if constexpr (kFullForm) {
+        const float ux = u[e] * w1[e] * x[e];
+        s[1] = fmaf(ux, d[e], s[1]);
+        s[2] = fmaf(ux, r[e], s[2]);
+      }
+    }
+    row_sum<N>(s, tpr, red[turn]);
+    turn ^= 1;
+    const float c = i2 * i2 * i2 * s[0] / D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = fmaf(-c, r[e], d[e]);
+    if (live && a.dres) put<R, kVec, E>(reinterpret_cast<R*>(a.dres) + row * D, t, tpr, D, d);
+    if constexpr (!kFullForm) {
+      if (live && a.dx) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] *= k;
+        put<T, kVec, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, d);
+      }
+    } else {
+      const float dot = s[1] - c * s[2];         // sum of u w1 x d
+      const float back = post ? k * i1 * i1 * i1 * dot / D : 0.f;
+      if (mode == kRow && live && t == 0 && a.dgate)
+        reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(a.scale * i1 * dot);
+      float dx[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float xd = i1 * x[e] * d[e];
+        const float dh = k * u[e] * d[e];        // gradient of h
+        dw1[e] = fmaf(k * u[e], xd, dw1[e]);
+        dgc[e] += xd;                            // times scale (o + w1) at the end
+        dx[e] = fmaf(-back, x[e], i1 * dh * w1[e]);
+        d[e] = a.scale * w1[e] * xd;             // gradient of the element's gate
+      }
+      if (live && a.dx) put<T, kVec, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, dx);
+      if (mode == kFull && live && a.dgate)
+        put<T, kVec, E>(reinterpret_cast<T*>(a.dgate) + row * D, t, tpr, D, d);
+    }
+  }
+  // the block's column sums: its rows' slots added in order
+  float* part = a.part + (int64_t)blockIdx.x * D;
+  const int64_t plane = (int64_t)gridDim.x * D;
+  auto leave = [&](const float (&v)[E], float* out) {
+    if (per == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = column<kVec>(e, t, tpr);
+        if (c < D) out[c] = v[e];
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = column<kVec>(e, t, tpr);
+      if (c < D) cols[slot * D + c] = v[e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += blockDim.x) {
+      float sum = 0.f;
+      for (int q = 0; q < per; ++q) sum += cols[q * D + c];
+      out[c] = sum;
+    }
+  };
+  leave(dw2, part);
+  if constexpr (kFullForm) {
+    if (post) leave(dw1, part + plane);
+    if (mode == kChannel) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) dgc[e] *= a.scale * w1[e];
+      leave(dgc, part + 2 * plane);
+    }
+  }
+}
+
+// out[c] = sum over the blocks' partials, in a fixed order: 16 threads a
+// column, each over every 16th block.
+constexpr int kSumRows = 16;
+
+struct Out {
+  void* p[3];
+  int dtype[3];
+};
+
+__global__ void __launch_bounds__(32 * kSumRows)
+sum_partials(int blocks, int D, const float* __restrict__ part, const Out out) {
+  if (!out.p[blockIdx.y]) return;
+  __shared__ float red[kSumRows][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const float* src = part + (int64_t)blockIdx.y * blocks * D;
+  float s = 0.f;
+  if (c < D)
+    for (int b = threadIdx.y; b < blocks; b += kSumRows) s += src[(int64_t)b * D + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < D) {
+    s = 0.f;
+    for (int q = 0; q < kSumRows; ++q) s += red[q][threadIdx.x];
+    void* p = out.p[blockIdx.y];
+    switch (out.dtype[blockIdx.y]) {
+      case TT_F32: reinterpret_cast<float*>(p)[c] = s; break;
+      case TT_BF16: reinterpret_cast<__nv_bfloat16*>(p)[c] = from_f32<__nv_bfloat16>(s); break;
+      default: reinterpret_cast<__half*>(p)[c] = from_f32<__half>(s); break;
+    }
+  }
+}
+
+// Threads of a row and rows of a block for D columns, E elements a thread.
+struct Shape {
+  int E, tpr, per;
+};
+
+constexpr int kMaxD = 16384;
+
+Shape shape_of(int D) {
+  Shape s;
+  s.E = D <= 4096 ? 8 : 16;
+  const int need = (D + s.E - 1) / s.E;
+  if (need <= 32) {
+    s.tpr = 1;
+    while (s.tpr < need) s.tpr *= 2;
+  } else {
+    s.tpr = (need + 31) / 32 * 32;
+  }
+  s.per = std::max(1, 256 / s.tpr);
+  return s;
+}
+
+bool aligned(const void* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+}
+
+template <typename T, typename R, bool kBwd>
+int launch(const Args& a, bool vec, bool full, Shape s, int blocks, cudaStream_t st) {
+  const int threads = s.tpr * s.per;
+  const size_t smem = kBwd && s.per > 1 ? sizeof(float) * s.per * a.D : 0;
+  auto go = [&](auto v, auto e, auto m, auto f) {
+    constexpr bool V = decltype(v)::value, F = decltype(f)::value;
+    constexpr int E = decltype(e)::value, M = decltype(m)::value;
+    if constexpr (kBwd)
+      bwd_kernel<T, R, V, E, M, F><<<blocks, threads, smem, st>>>(a);
+    else
+      fwd_kernel<T, R, V, E, M, F><<<blocks, threads, smem, st>>>(a);
+  };
+  using Y = std::true_type;
+  using N = std::false_type;
+  std::integral_constant<int, 8> e8;
+  std::integral_constant<int, 16> e16;
+  std::integral_constant<int, 512> m512;
+  std::integral_constant<int, 1024> m1024;
+  if (!vec) {
+    s.E == 8 ? go(N(), e8, m512, Y()) : go(N(), e16, m1024, Y());
+  } else if (s.E == 8) {
+    full ? go(Y(), e8, m512, Y()) : go(Y(), e8, m512, N());
+  } else if (threads <= 512) {
+    full ? go(Y(), e16, m512, Y()) : go(Y(), e16, m512, N());
+  } else {
+    full ? go(Y(), e16, m1024, Y()) : go(Y(), e16, m1024, N());
+  }
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
+template <bool kBwd>
+int dispatch(int dtype, int res_dtype, const Args& a, bool vec, Shape s, int blocks,
+             cudaStream_t st) {
+  const bool full = a.w1 || a.gate_mode != kNone;
+  return vec::dispatch_float(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    if (res_dtype == dtype) return launch<T, T, kBwd>(a, vec, full, s, blocks, st);
+    if (res_dtype == TT_F32) return launch<T, float, kBwd>(a, vec, full, s, blocks, st);
+    return TT_ERR_UNSUPPORTED;
+  });
+}
+
+bool bad_sizes(int64_t rows, int32_t D, int gate_mode, const void* gate) {
+  return rows < 0 || D <= 0 || D > kMaxD || gate_mode < kNone || gate_mode > kFull ||
+         (gate_mode != kNone && rows > 0 && !gate);
+}
+
+}  // namespace
+}  // namespace resnorm
+}  // namespace tt
+
+extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int32_t D,
+                                    const void* x, int64_t x_st, const void* residual,
+                                    int64_t res_st, const void* weight, const void* post_weight,
+                                    int weight_f32, float weight_offset, const void* gate,
+                                    int64_t gate_st, int gate_mode, float scale, float eps,
+                                    void* y, void* r, float* stats, void* stream) {
+  using namespace tt::resnorm;
+  if (bad_sizes(rows, D, gate_mode, gate) || (rows > 0 && (!x || !weight || !y || !r)))
+    return TT_ERR_INVALID_ARG;
+  if (rows == 0) return TT_OK;
+  Args a{};
+  a.rows = rows, a.D = D;
+  a.x = x, a.res = residual, a.gate = gate, a.w2 = weight, a.w1 = post_weight;
+  a.x_st = x_st, a.res_st = res_st, a.gate_st = gate_st;
+  a.gate_mode = gate_mode, a.w_f32 = weight_f32;
+  a.scale = scale, a.offset = weight_offset, a.eps = eps;
+  a.y = y, a.r = r, a.stats = stats;
+  Shape s = shape_of(D);
+  a.tpr = s.tpr;
+  const bool vec = D % 8 == 0 && aligned(x, x_st) && aligned(residual, residual ? res_st : 0) &&
+                   aligned(y, D) && aligned(r, D) &&
+                   (gate_mode != kFull || aligned(gate, gate_st));
+  const int64_t want = (rows + s.per - 1) / s.per;
+  const int blocks = (int)std::min<int64_t>(want, tt::vec::kSMs * 16ll);
+  const int rc = dispatch<false>(dtype, res_dtype, a, vec, s, blocks, (cudaStream_t)stream);
+  if (rc == TT_OK) tt_count_launches(1);
+  return rc;
+}
+
+extern "C" int tt_residual_norm_bwd_blocks(int64_t rows, int32_t D) {
+  using namespace tt::resnorm;
+  if (rows <= 0 || D <= 0 || D > kMaxD) return 1;
+  const Shape s = shape_of(D);
+  const int64_t want = (rows + s.per - 1) / s.per;
+  return (int)std::max<int64_t>(
+      1, std::min<int64_t>(want, tt::vec::kSMs * (int64_t)std::max(1, 1024 / (s.tpr * s.per))));
+}
+
+extern "C" int tt_residual_norm_bwd(
+    int dtype, int res_dtype, int64_t rows, int32_t D, const void* x, int64_t x_st,
+    const void* residual, int64_t res_st, const void* weight, const void* post_weight,
+    int weight_f32, float weight_offset, const void* gate, int64_t gate_st, int gate_mode,
+    float scale, const float* stats, const void* dy, int64_t dy_st, const void* dr,
+    int64_t dr_st, void* dx, void* dres, void* dgate, void* dweight, void* dpost, float* part,
+    int32_t blocks, void* stream) {
+  using namespace tt::resnorm;
+  if (bad_sizes(rows, D, gate_mode, gate) || blocks <= 0 ||
+      (rows > 0 && (!x || !weight || !stats || !part)))
+    return TT_ERR_INVALID_ARG;
+  if (rows == 0) return TT_OK;
+  Args a{};
+  a.rows = rows, a.D = D;
+  a.x = x, a.res = residual, a.gate = gate, a.w2 = weight, a.w1 = post_weight;
+  a.x_st = x_st, a.res_st = res_st, a.gate_st = gate_st;
+  a.gate_mode = gate_mode, a.w_f32 = weight_f32;
+  a.scale = scale, a.offset = weight_offset;
+  a.stats = const_cast<float*>(stats);
+  a.dy = dy, a.dr = dr, a.dy_st = dy_st, a.dr_st = dr_st;
+  a.dx = dx, a.dres = dres, a.dgate = gate_mode == kChannel ? nullptr : dgate;
+  a.part = part;
+  Shape s = shape_of(D);
+  a.tpr = s.tpr;
+  const bool vec = D % 8 == 0 && aligned(x, x_st) && aligned(residual, residual ? res_st : 0) &&
+                   aligned(dy, dy ? dy_st : 0) && aligned(dr, dr ? dr_st : 0) && aligned(dx, D) &&
+                   aligned(dres, D) &&
+                   (gate_mode != kFull || (aligned(gate, gate_st) && aligned(dgate, D)));
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rc = dispatch<true>(dtype, res_dtype, a, vec, s, blocks, st);
+  if (rc != TT_OK) return rc;
+  Out out{};
+  out.p[0] = dweight;
+  out.p[1] = post_weight ? dpost : nullptr;
+  out.p[2] = gate_mode == kChannel ? dgate : nullptr;
+  out.dtype[0] = out.dtype[1] = weight_f32 ? TT_F32 : dtype;
+  out.dtype[2] = dtype;
+  const int planes = out.p[2] ? 3 : out.p[1] ? 2 : out.p[0] ? 1 : 0;
+  if (planes)
+    sum_partials<<<dim3((D + 31) / 32, planes), dim3(32, kSumRows), 0, st>>>(blocks, D, part, out);
+  tt_count_launches(planes ? 2 : 1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
