@@ -521,6 +521,34 @@ int tt_residual_norm_bwd(int dtype, int res_dtype, int64_t rows, int32_t D, cons
                          int64_t dr_st, void* dx, void* dres, void* dgate, void* dweight,
                          void* dpost, float* part, int32_t blocks, void* stream);
 
+/* ---- tokens sorted by expert ---------------------------------------------- *
+ * Stable counting sort of n_entries = n_tok * k choices (entry t * k + j) by
+ * expert id (int64 with ids64, else int32).  slots[entry]: its sorted row, -1
+ * where the id is outside [0, n_experts) (dropped); entries[row]: its entry,
+ * -1 past the last kept row; offsets[n_experts + 1]: first row of each expert
+ * and the number of kept rows.  n_experts <= 1024, n_entries < 2^31. */
+int64_t tt_moe_plan_workspace_size(int64_t n_entries, int32_t n_experts);
+int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_t n_experts, int32_t* slots,
+                int32_t* entries, int32_t* offsets, void* workspace, int64_t workspace_bytes,
+                void* stream);
+/* xs[slots[t, j]] = x[t]; rows past the last kept one are zeroed. */
+int tt_moe_dispatch(int dtype, int64_t n_tok, int32_t k, int32_t H, int32_t n_experts,
+                    const int32_t* slots, const int32_t* offsets, const void* x, void* xs,
+                    void* stream);
+/* dx[t] = sum_j dxs[slots[t, j]]: the gradient of tt_moe_dispatch. */
+int tt_moe_collect(int dtype, int64_t n_tok, int32_t k, int32_t H, int32_t n_experts,
+                   const int32_t* slots, const int32_t* offsets, const void* dxs, void* dx,
+                   void* stream);
+/* y[t] = sum_j weights[t, j] ys[slots[t, j]]. */
+int tt_moe_combine(int dtype, int weight_dtype, int64_t n_tok, int32_t k, int32_t H,
+                   int32_t n_experts, const int32_t* slots, const int32_t* offsets,
+                   const void* ys, const void* weights, void* y, void* stream);
+/* The gradient of tt_moe_combine: dys[slots[t, j]] = weights[t, j] dy[t] (zero
+ * past the last kept row), dweights[t, j] = <dy[t], ys[slots[t, j]]>. */
+int tt_moe_spread(int dtype, int weight_dtype, int64_t n_tok, int32_t k, int32_t H,
+                  int32_t n_experts, const int32_t* slots, const int32_t* offsets, const void* dy,
+                  const void* ys, const void* weights, void* dys, void* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ from .attention import (tree_attention, tree_attention_forward, register_hf_atte
                         prefetch_tree_meta, ATTN_IMPL_NAME)
 from .rotary import apply_rotary, rotary_table  # noqa: F401
 from .residual_norm import residual_norm  # noqa: F401
+from .moe import ExpertPlan, expert_combine, expert_dispatch, expert_plan  # noqa: F401
 from ._lib import LIB_PATH, TTError  # noqa: F401
 
 __all__ = [
@@ -19,5 +20,6 @@ __all__ = [
     "gateway_intervals_from_bias", "tree_attention", "tree_attention_forward",
     "register_hf_attention", "tree_mask_placeholder", "meta_from_dense_mask",
     "apply_rotary", "rotary_table",
-    "residual_norm",     "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
+    "residual_norm", "ExpertPlan", "expert_plan", "expert_dispatch", "expert_combine",
+    "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
 ]

@@ -101,6 +101,13 @@ SIGNATURES = {
     "tt_residual_norm_bwd": (_INT, [_INT, _INT, _I64, _I32, _P, _I64, _P, _I64, _P, _P, _INT,
                                     _F32, _P, _I64, _INT, _F32, _P, _P, _I64, _P, _I64, _P, _P,
                                     _P, _P, _P, _P, _I32, _P]),
+    "tt_moe_plan_workspace_size": (_I64, [_I64, _I32]),
+    "tt_moe_plan": (_INT, [_P, _INT, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
+    "tt_moe_dispatch": (_INT, [_INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
+    "tt_moe_collect": (_INT, [_INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
+    "tt_moe_combine": (_INT, [_INT, _INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
+    "tt_moe_spread": (_INT, [_INT, _INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P,
+                             _P]),
     "tt_conv_predecessors": (_INT, [_I32, _P, _P, _I32, _P]),
     "tt_conv_successors": (_INT, [_I32, _I32, _P, _P, _P, _P, _I64]),
     "tt_tree_conv_fwd": (_INT, [_INT, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
