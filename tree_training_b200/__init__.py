@@ -10,6 +10,7 @@ from .packer import (TreeNode, DFSTreeInfo, TreeAttnMeta, build_dfs_tree_info,  
 from .attention import (tree_attention, tree_attention_forward, register_hf_attention,  # noqa: F401
                         tree_mask_placeholder, meta_from_dense_mask, check_device_status,
                         prefetch_tree_meta, ATTN_IMPL_NAME)
+from .logprob import TokenLogprobs, token_logprobs, tree_next_tokens  # noqa: F401
 from .rotary import apply_rotary, rotary_table  # noqa: F401
 from .residual_norm import residual_norm  # noqa: F401
 from .moe import ExpertPlan, expert_combine, expert_dispatch, expert_plan  # noqa: F401
@@ -19,7 +20,7 @@ __all__ = [
     "TreeNode", "DFSTreeInfo", "TreeAttnMeta", "build_dfs_tree_info",
     "gateway_intervals_from_bias", "tree_attention", "tree_attention_forward",
     "register_hf_attention", "tree_mask_placeholder", "meta_from_dense_mask",
-    "apply_rotary", "rotary_table",
+    "TokenLogprobs", "token_logprobs", "tree_next_tokens", "apply_rotary", "rotary_table",
     "residual_norm", "ExpertPlan", "expert_plan", "expert_dispatch", "expert_combine",
     "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
 ]

@@ -108,6 +108,10 @@ SIGNATURES = {
     "tt_moe_combine": (_INT, [_INT, _INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
     "tt_moe_spread": (_INT, [_INT, _INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P,
                              _P]),
+    "tt_token_logprobs_fwd": (_INT, [_INT, _I64, _I32, _P, _I64, _P, _I32, _F32, _I32, _P, _P,
+                                     _P, _P, _P, _P]),
+    "tt_token_logprobs_bwd": (_INT, [_INT, _I64, _I32, _P, _I64, _P, _I32, _F32, _I32, _P, _P,
+                                     _P, _P, _P, _P, _P]),
     "tt_conv_predecessors": (_INT, [_I32, _P, _P, _I32, _P]),
     "tt_conv_successors": (_INT, [_I32, _I32, _P, _P, _P, _P, _I64]),
     "tt_tree_conv_fwd": (_INT, [_INT, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
