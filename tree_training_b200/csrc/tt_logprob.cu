@@ -13,11 +13,19 @@
 // probability 0, no gradient).  -inf logits have probability 0; a row of
 // nothing but -inf has log probabilities -inf, entropy 0 and no gradient.
 //
-// Forward: each thread keeps a running (reference, sum, weighted sum) in base
-// 2 and the row is read once.
+// Both directions are bound by HBM.  Forward: the row is read once, in 16-byte
+// packs; each thread keeps running sums in base 2 (two fp32 values relative to a
+// reference that moves only when the maximum is 2^12 above it) and its largest
+// logit, from which the alternatives' candidates are found (block_top).  Few
+// rows are split over the blocks of a cluster, which meet in shared memory.
+// Backward: one pass from the four statistics a row that the forward keeps.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "tt_vec.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace tt {
 namespace logprob {
@@ -87,24 +95,62 @@ __device__ __forceinline__ Sums merged(Sums a, Sums b, float c) {
   return {ref, a.s + b.s, a.u + b.u};
 }
 
+__device__ __forceinline__ Sums shfl_xor(const Sums& a, int o) {
+  return {__shfl_xor_sync(0xffffffffu, a.ref, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+          __shfl_xor_sync(0xffffffffu, a.u, o)};
+}
+
+// A row as 16-byte packs that start on 16-byte boundaries: pack v holds the
+// elements [v N - shift, (v + 1) N - shift), of which those of the row are
+// loaded and the others are -inf (no probability, and no candidates: their
+// index is out of range).
+template <typename T>
+struct Packs {
+  static constexpr int N = 16 / (int)sizeof(T);
+  const T* x;
+  int V, shift;
+  int n, whole0, whole1;        // packs; those that lie in the row as a whole
+
+  __device__ __forceinline__ Packs(const T* row, int vocab) : x(row), V(vocab) {
+    shift = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % N);
+    n = (int)(((int64_t)shift + vocab + N - 1) / N);
+    whole0 = shift ? 1 : 0;
+    whole1 = (int)(((int64_t)shift + vocab) / N);
+  }
+  __device__ __forceinline__ bool whole(int v) const { return v >= whole0 && v < whole1; }
+  __device__ __forceinline__ int64_t first(int v) const { return (int64_t)v * N - shift; }
+  __device__ __forceinline__ uint4 raw(int v) const {
+    if (whole(v)) return __ldg(reinterpret_cast<const uint4*>(x - shift) + v);
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t e = first(v) + i;
+      o[i] = (e >= 0 && e < V) ? to_f32(x[e]) : -INFINITY;
+    }
+    return vec::pack<T, N>(o);
+  }
+  __device__ __forceinline__ void load(int v, float (&o)[N]) const {
+    vec::unpack<T, N>(raw(v), o);
+  }
+};
+
 template <int N>
-__device__ __forceinline__ void accumulate(const float (&x)[N], float c, Sums& a, float& best) {
+__device__ __forceinline__ float accumulate(const float (&x)[N], float c, Sums& a) {
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) mx = max_nan(mx, x[i]);
-  best = max_nan(best, mx);
   if ((mx - a.ref) * c > kSlack || (a.s == 0.f && mx > -INFINITY)) rebase(a, mx, c);
+  float s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float t = max_nan((x[i] - a.ref) * c, kFloor);
     const float e = ex2(t);
-    a.s += e;
-    a.u = fmaf(t, e, a.u);
+    s[i & 1] += e;
+    u[i & 1] = fmaf(t, e, u[i & 1]);
   }
-}
-
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  return __shfl_xor_sync(0xffffffffu, (unsigned long long)v, o);
+  a.s += s[0] + s[1];
+  a.u += u[0] + u[1];
+  return mx;
 }
 
 struct Args {
@@ -125,81 +171,252 @@ __device__ __forceinline__ float logp_of(float x, float m, float ln_s, float inv
   return (x / temp - m / temp) - ln_s;
 }
 
+constexpr int kUnroll = 4;        // packs in flight a thread
+constexpr int kCandidates = 2048;
+constexpr int kMaxCluster = 8;
+
+struct TopShared {
+  uint64_t keys[kWarps * 8];      // the best threads' keys
+  uint64_t found[kCandidates];
+  uint64_t list[kMaxTop];         // this block's largest, in order
+  uint64_t lists[kMaxCluster][kMaxTop];   // block 0: every block's
+  uint64_t bar;                   // the k-th largest of keys: a lower bound
+  int n_threads, n_found;
+  int threads[kThreads];
+};
+
+// The k largest keys of the block's packs [begin, end) into sh.list, in order
+// (0 where there are fewer).  `best` orders this thread's largest logit and
+// `best_pack` is the first pack that has it (-1: none).  The k-th largest key of
+// any elements is a lower bound of the k-th largest of all, so: take it from the
+// threads' largest (up to 8 of each warp), look once more through the packs of
+// the threads that reach it (about k of them), and rank what is found.  Should
+// more than kCandidates elements reach the bound, the list is made one pass an
+// entry.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
-  __shared__ Sums sums[kWarps];
-  __shared__ float maxes[kWarps];
-  __shared__ uint64_t keys[kWarps];
-  __shared__ float st[4];
+__device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int end, int k,
+                                          uint32_t best, int best_pack, TopShared& sh) {
+  constexpr int N = Packs<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
+  if (threadIdx.x == 0) sh.bar = 0, sh.n_threads = 0, sh.n_found = 0;
+  // a key no larger than that of the thread's largest: its pack's last index
+  uint32_t order = best_pack < 0 ? 0u : best;
+  const uint32_t last = (uint32_t)(row.first(best_pack) + N - 1);
+  const int rounds = min(8, k);
+  for (int r = 0; r < rounds; ++r) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, order);
+    const uint32_t at = __reduce_min_sync(0xffffffffu, order == top ? last : 0xffffffffu);
+    if (lane == 0) sh.keys[warp * rounds + r] = top ? key_of(top, at) : 0;
+    if (order == top && last == at) order = 0;
+  }
+  __syncthreads();
+  const int n_keys = kWarps * rounds;
+  if ((int)threadIdx.x < n_keys) {
+    const uint64_t mine = sh.keys[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < n_keys; ++i) above += sh.keys[i] > mine;
+    if (above == k - 1 && mine) sh.bar = mine;    // keys differ unless they are 0
+  }
+  __syncthreads();
+  const uint64_t bar = sh.bar;
+  if (best_pack >= 0 && key_of(best, max((int64_t)0, row.first(best_pack))) >= bar)
+    sh.threads[atomicAdd(&sh.n_threads, 1)] = threadIdx.x;
+  __syncthreads();
+  const int n_threads = sh.n_threads;
+  for (int q = warp; q < n_threads; q += kWarps) {
+    for (int v = begin + sh.threads[q] + lane * kThreads; v < end; v += 32 * kThreads) {
+      float x[N];
+      row.load(v, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t e = row.first(v) + i;
+        const uint64_t key = key_of(order_of(x[i]), e);
+        if (key >= bar && e >= 0 && e < row.V) {
+          const int at = atomicAdd(&sh.n_found, 1);
+          if (at < kCandidates) sh.found[at] = key;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh.n_found;
+  if (n <= kCandidates) {
+    for (int c = threadIdx.x; c < max(n, k); c += kThreads) {
+      if (c >= n) {
+        sh.list[c] = 0;
+        continue;
+      }
+      const uint64_t mine = sh.found[c];
+      int above = 0;
+      for (int i = 0; i < n; ++i) above += sh.found[i] > mine;
+      if (above < k) sh.list[above] = mine;
+    }
+    __syncthreads();
+    return;
+  }
+  uint64_t below = ~0ull;
+  for (int j = 0; j < k; ++j) {
+    uint64_t mine = 0;
+    for (int v = begin + threadIdx.x; v < end; v += kThreads) {
+      float x[N];
+      row.load(v, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t e = row.first(v) + i;
+        const uint64_t key = key_of(order_of(x[i]), e);
+        if (key < below && key > mine && e >= 0 && e < row.V) mine = key;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, (unsigned long long)mine, o);
+      mine = other > mine ? other : mine;
+    }
+    __syncthreads();
+    if (lane == 0) sh.keys[warp] = mine;
+    __syncthreads();
+    below = sh.keys[0];
+    for (int w = 1; w < kWarps; ++w) below = sh.keys[w] > below ? sh.keys[w] : below;
+    if (threadIdx.x == 0) sh.list[j] = below;
+  }
+  __syncthreads();
+}
+
+struct Part {
+  Sums sums;
+  float best;
+};
+
+// One row a cluster: its blocks take equal runs of the row's packs and block 0
+// brings their sums and lists together.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
+  constexpr int N = Packs<T>::N;
+  __shared__ Part warps[kWarps];
+  __shared__ Part parts[kMaxCluster];
+  __shared__ float st[3];
+  extern __shared__ uint64_t top_raw[];
+  TopShared& sh = *reinterpret_cast<TopShared*>(top_raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x / blocks;
+  // block 0 must be running before another block writes into its shared memory
+  if (blocks > 1) cluster.barrier_arrive();
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  const Packs<T> packs(x, a.V);
+  const int per = (packs.n + blocks - 1) / blocks;
+  const int begin = min(packs.n, rank * per), end = min(packs.n, begin + per);
   const float c = kLog2e / a.temperature;
+
+  // the first given tokens' logits are fetched along with the row
+  int64_t tok0 = -1;
+  float x0 = 0.f;
+  if (rank == 0 && (int)threadIdx.x < a.M) {
+    tok0 = a.tokens[row * a.M + threadIdx.x];
+    if (tok0 >= 0 && tok0 < a.V) x0 = to_f32(x[tok0]);
+  }
+
   Sums acc{0.f, 0.f, 0.f};
   float best = -INFINITY;
-  for (int i = threadIdx.x; i < a.V; i += kThreads) {
-    const float v[1] = {to_f32(x[i])};
-    accumulate<1>(v, c, acc, best);
+  uint32_t best_order = 0;
+  int best_pack = -1;
+  auto take = [&](const uint4& raw, int v) {
+    float f[N];
+    vec::unpack<T, N>(raw, f);
+    const float mx = accumulate<N>(f, c, acc);
+    if constexpr (kTop) {
+      const uint32_t o = order_of(mx);
+      if (o > best_order) best_order = o, best_pack = v;
+    } else {
+      best = max_nan(best, mx);
+    }
+  };
+  int v = begin + threadIdx.x;
+  for (; v + (kUnroll - 1) * kThreads < end; v += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) raw[i] = packs.raw(v + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * kThreads);
   }
+  for (; v < end; v += kThreads) take(packs.raw(v), v);
+  if constexpr (kTop)
+    if (best_pack >= 0) best = of_order(best_order);
+
+  float wb = best;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, acc.ref, o), __shfl_xor_sync(0xffffffffu, acc.s, o),
-                 __shfl_xor_sync(0xffffffffu, acc.u, o)};
-    acc = merged(acc, b, c);
-    best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, o));
+    acc = merged(acc, shfl_xor(acc, o), c);
+    wb = max_nan(wb, __shfl_xor_sync(0xffffffffu, wb, o));
   }
-  if (lane == 0) sums[warp] = acc, maxes[warp] = best;
-  __syncthreads();
+  if (lane == 0) warps[warp] = {acc, wb};
+  if constexpr (kTop)
+    block_top<T>(packs, begin, end, a.k, best_order, best_pack, sh);
+  else
+    __syncthreads();
+  if (blocks > 1) {
+    cluster.barrier_wait();
+    if (threadIdx.x == 0) {
+      Part p = warps[0];
+      for (int w = 1; w < kWarps; ++w)
+        p = {merged(p.sums, warps[w].sums, c), max_nan(p.best, warps[w].best)};
+      *cluster.map_shared_rank(&parts[rank], 0) = p;
+    }
+    if constexpr (kTop)
+      for (int j = threadIdx.x; j < a.k; j += kThreads)
+        *cluster.map_shared_rank(&sh.lists[rank][j], 0) = sh.list[j];
+    cluster.sync();
+    if (rank != 0) return;
+  }
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) {
-      acc = merged(acc, sums[w], c);
-      best = max_nan(best, maxes[w]);
-    }
+    const Part* from = blocks > 1 ? parts : warps;
+    Part p = from[0];
+    for (int i = 1; i < (blocks > 1 ? blocks : kWarps); ++i)
+      p = {merged(p.sums, from[i].sums, c), max_nan(p.best, from[i].best)};
     float ln_s = 0.f, inv_s = 0.f, H = 0.f;
-    if (acc.s != 0.f) {
-      rebase(acc, best, c);
-      ln_s = logf(acc.s);
-      inv_s = 1.f / acc.s;
-      H = ln_s - kLn2 * (acc.u / acc.s);
+    if (p.sums.s != 0.f) {
+      rebase(p.sums, p.best, c);
+      ln_s = logf(p.sums.s);
+      inv_s = 1.f / p.sums.s;
+      H = ln_s - kLn2 * (p.sums.u / p.sums.s);
     }
-    st[0] = best, st[1] = ln_s, st[2] = inv_s, st[3] = H;
+    st[0] = p.best, st[1] = ln_s, st[2] = inv_s;
     a.ent[row] = H;
-    if (a.stats) {
-      float4* out = reinterpret_cast<float4*>(a.stats) + row;
-      *out = make_float4(best, ln_s, inv_s, H);
+    if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(p.best, ln_s, inv_s, H);
+  }
+  if constexpr (kTop) {
+    if (blocks > 1) {
+      // of the blocks' lists, which share no element
+      const int n = blocks * a.k;
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t mine = sh.lists[i / a.k][i % a.k];
+        int above = 0;
+        for (int b = 0; b < blocks; ++b)
+          for (int j = 0; j < a.k && sh.lists[b][j] > mine; ++j) ++above;
+        if (mine && above < a.k) sh.list[above] = mine;
+      }
     }
   }
   __syncthreads();
   const float m = st[0], ln_s = st[1], inv_s = st[2];
   for (int j = threadIdx.x; j < a.M; j += kThreads) {
-    const int64_t tok = a.tokens[row * a.M + j];
+    int64_t tok = tok0;
+    float xt = x0;
+    if (j != (int)threadIdx.x) {
+      tok = a.tokens[row * a.M + j];
+      if (tok >= 0 && tok < a.V) xt = to_f32(x[tok]);
+    }
     a.logp[row * a.M + j] =
-        (tok < 0 || tok >= a.V) ? 0.f : logp_of(to_f32(x[tok]), m, ln_s, inv_s, a.temperature);
+        (tok < 0 || tok >= a.V) ? 0.f : logp_of(xt, m, ln_s, inv_s, a.temperature);
   }
-  // the alternatives, one a pass: the largest key below the one before
-  uint64_t below = ~0ull;
-  for (int j = 0; j < a.k; ++j) {
-    uint64_t mine = 0;
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const uint64_t key = key_of(order_of(to_f32(x[i])), i);
-      if (key < below && key > mine) mine = key;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t other = shfl_xor64(mine, o);
-      mine = other > mine ? other : mine;
-    }
-    __syncthreads();
-    if (lane == 0) keys[warp] = mine;
-    __syncthreads();
-    below = keys[0];
-    for (int w = 1; w < kWarps; ++w) below = keys[w] > below ? keys[w] : below;
-    if (threadIdx.x == 0) {
-      a.top_tok[row * a.k + j] = (int64_t)(uint32_t)~(uint32_t)below;
+  if constexpr (kTop)
+    for (int j = threadIdx.x; j < a.k; j += kThreads) {
+      const uint64_t key = sh.list[j];
+      a.top_tok[row * a.k + j] = (int64_t)(uint32_t)~(uint32_t)key;
       a.top_logp[row * a.k + j] =
-          logp_of(of_order((uint32_t)(below >> 32)), m, ln_s, inv_s, a.temperature);
+          logp_of(of_order((uint32_t)(key >> 32)), m, ln_s, inv_s, a.temperature);
     }
-  }
 }
 
 struct BwdArgs {
@@ -212,18 +429,28 @@ struct BwdArgs {
   const float *g_logp, *g_ent, *g_top;   // any of them null: zero
   const float* stats;
   void* dx;
+  int chunks, per;                       // blocks of a row, packs of a block
 };
 
+// With t = (x - m) c (c = log2(e) / temperature), p = 2^t / s and
+// logp = t ln 2 - ln s:
+//   dx = 2^t (A + B t) + g / temperature at the given tokens,
+//   A = -(G + g_H (H - ln s)) / (s temperature), B = -g_H ln 2 / (s temperature).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
-  const int64_t row = blockIdx.x;
+  constexpr int N = Packs<T>::N;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x / a.chunks;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
   T* dx = reinterpret_cast<T*>(a.dx) + row * a.V;
+  const Packs<T> to(dx, a.V);              // packs by dx's alignment
+  const bool same = Packs<T>(x, a.V).shift == to.shift;
+  const int begin = min((int64_t)to.n, (int64_t)(blockIdx.x % a.chunks) * a.per);
+  const int end = min((int64_t)to.n, (int64_t)begin + a.per);
   const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
-  const float m = st.x, ln_s = st.y, inv_s = st.z, H = st.w;
-  const bool empty = inv_s == 0.f;
+  const bool empty = st.z == 0.f;
   const float c = kLog2e / a.temperature, inv_t = 1.f / a.temperature;
-  const float ref = empty ? 0.f : m;
+  const float ref = empty ? 0.f : st.x;
   const int n = a.M + (a.g_top ? a.k : 0);
   // entry j: a given token or an alternative
   auto token = [&](int j) {
@@ -233,24 +460,60 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
     return j < a.M ? (a.g_logp ? a.g_logp[row * a.M + j] : 0.f) : a.g_top[row * a.k + j - a.M];
   };
   float G = 0.f;
-  if (!empty)
-    for (int j = 0; j < n; ++j) {
-      const int64_t tok = token(j);
-      if (tok >= 0 && tok < a.V) G += grad(j);
-    }
-  const float gH = a.g_ent && !empty ? a.g_ent[row] : 0.f;
+  for (int j = lane; j < n; j += 32) {
+    const int64_t tok = token(j);
+    if (tok >= 0 && tok < a.V) G += grad(j);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) G += __shfl_xor_sync(0xffffffffu, G, o);
+  const float gH = a.g_ent ? a.g_ent[row] : 0.f;
+  const float A = empty ? 0.f : -(G + gH * (st.w - st.y)) * st.z * inv_t;
+  const float B = empty ? 0.f : -gH * kLn2 * st.z * inv_t;
   auto base = [&](float v) {
     const float t = max_nan((v - ref) * c, kFloor);
-    const float p = ex2(t) * inv_s;
-    return -p * (G + gH * (fmaf(t, kLn2, -ln_s) + H));
+    return ex2(t) * fmaf(B, t, A);
   };
-  for (int i = threadIdx.x; i < a.V; i += kThreads)
-    dx[i] = from_f32<T>(base(to_f32(x[i])) * inv_t);
-  __syncthreads();
+  auto fetch = [&](int v) -> uint4 {
+    if (same && to.whole(v))
+      return __ldg(reinterpret_cast<const uint4*>(x - to.shift) + v);
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t e = to.first(v) + i;
+      o[i] = (e >= 0 && e < a.V) ? to_f32(x[e]) : 0.f;
+    }
+    return vec::pack<T, N>(o);
+  };
+  auto leave = [&](const uint4& raw, int v) {
+    float o[N];
+    vec::unpack<T, N>(raw, o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = base(o[i]);
+    if (to.whole(v)) {
+      vec::store<T, N>(dx + to.first(v), o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t e = to.first(v) + i;
+        if (e >= 0 && e < a.V) dx[e] = from_f32<T>(o[i]);
+      }
+    }
+  };
+  int v = begin + threadIdx.x;
+  for (; v + (kUnroll - 1) * kThreads < end; v += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) raw[i] = fetch(v + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) leave(raw[i], v + i * kThreads);
+  }
+  for (; v < end; v += kThreads) leave(fetch(v), v);
   if (empty) return;
+  __syncthreads();
+  // the given tokens in this block's part: equal ones add up in order
   for (int j = threadIdx.x; j < n; j += kThreads) {
     const int64_t tok = token(j);
-    if (tok < 0 || tok >= a.V) continue;
+    if (tok < 0 || tok >= a.V || tok < to.first(begin) || tok >= to.first(end)) continue;
     float g = 0.f;
     bool first = true;
     for (int i = 0; i < n; ++i) {
@@ -258,7 +521,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
       if (i < j) first = false;
       g += grad(i);
     }
-    if (first) dx[tok] = from_f32<T>((base(to_f32(x[tok])) + g) * inv_t);
+    if (first) dx[tok] = from_f32<T>(fmaf(g, inv_t, base(to_f32(x[tok]))));
   }
 }
 
@@ -266,6 +529,33 @@ bool bad(int64_t rows, int32_t V, int32_t M, int32_t k, const void* x, int64_t l
          const int64_t* tokens, float temperature) {
   return rows < 0 || rows > 0x7fffffff || V <= 0 || M < 0 || k < 0 || k > kMaxTop || k > V ||
          ld < V || !(temperature > 0.f) || (rows > 0 && (!x || (M > 0 && !tokens)));
+}
+
+// Blocks that share a row: enough that every SM has work, as long as each still
+// has two packs a thread.
+int cluster_of(int64_t rows, int64_t packs) {
+  int c = 1;
+  while (c < kMaxCluster && rows * c * 2 <= vec::kSMs * 8 && packs / (2 * c) >= 2 * kThreads)
+    c *= 2;
+  return c;
+}
+
+template <typename T, bool kTop>
+int launch_fwd(const Args& a, cudaStream_t st) {
+  const int c = cluster_of(a.rows, a.V / Packs<T>::N);
+  if (a.rows * c > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * c));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kTop ? sizeof(TopShared) : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fwd_kernel<T, kTop>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
 }  // namespace
@@ -286,8 +576,9 @@ extern "C" int tt_token_logprobs_fwd(int dtype, int64_t n_rows, int32_t vocab, c
   Args a{n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature,
          logprobs, entropy, top_logprobs, top_tokens, stats};
   const int rc = tt::vec::dispatch_float(dtype, [&](auto tag) -> int {
-    fwd_kernel<decltype(tag)><<<(unsigned)n_rows, kThreads, 0, (cudaStream_t)stream>>>(a);
-    return TT_OK;
+    using T = decltype(tag);
+    return top_k ? launch_fwd<T, true>(a, (cudaStream_t)stream)
+                 : launch_fwd<T, false>(a, (cudaStream_t)stream);
   });
   if (rc != TT_OK) return rc;
   tt_count_launches(1);
@@ -306,9 +597,18 @@ extern "C" int tt_token_logprobs_bwd(int dtype, int64_t n_rows, int32_t vocab, c
     return TT_ERR_INVALID_ARG;
   if (n_rows == 0) return TT_OK;
   BwdArgs a{n_rows, vocab, n_tokens, top_k, logits, ld, tokens, top_tokens, temperature,
-            g_logprobs, g_entropy, g_top, stats, dlogits};
+            g_logprobs, g_entropy, g_top, stats, dlogits, 1, 0};
   const int rc = tt::vec::dispatch_float(dtype, [&](auto tag) -> int {
-    bwd_kernel<decltype(tag)><<<(unsigned)n_rows, kThreads, 0, (cudaStream_t)stream>>>(a);
+    using T = decltype(tag);
+    // a block takes 4 x kUnroll packs a thread; kUnroll where rows are few
+    const int64_t packs = vocab / Packs<T>::N + 2;
+    const int64_t one = (int64_t)kUnroll * kThreads;
+    int64_t per = 4 * one;
+    if (n_rows * ((packs + per - 1) / per) < tt::vec::kSMs * 8) per = one;
+    a.per = (int)per;
+    a.chunks = (int)((packs + per - 1) / per);
+    if (n_rows * a.chunks > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+    bwd_kernel<T><<<(unsigned)(n_rows * a.chunks), kThreads, 0, (cudaStream_t)stream>>>(a);
     return TT_OK;
   });
   if (rc != TT_OK) return rc;
