@@ -23,6 +23,7 @@
 
 #include <algorithm>
 
+#include "tt_sm100.cuh"
 #include "tt_vec.cuh"
 
 namespace cg = cooperative_groups;
@@ -48,9 +49,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// 2^x; the forward's sums do without results under 2^-126 (three instructions
+// less), gradients keep them.
+template <bool kSubnormal = false>
 __device__ __forceinline__ float ex2(float x) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  if constexpr (kSubnormal)
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  else
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -134,24 +141,60 @@ struct Packs {
   }
 };
 
-template <int N>
-__device__ __forceinline__ float accumulate(const float (&x)[N], float c, Sums& a) {
-  float mx = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) mx = max_nan(mx, x[i]);
-  if ((mx - a.ref) * c > kSlack || (a.s == 0.f && mx > -INFINITY)) rebase(a, mx, c);
-  float s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float t = max_nan((x[i] - a.ref) * c, kFloor);
-    const float e = ex2(t);
-    s[i & 1] += e;
-    u[i & 1] = fmaf(t, e, u[i & 1]);
+// The largest of a pack (NaN aside).
+template <typename T>
+__device__ __forceinline__ float pack_max(const uint4& r) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                 fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2,
+                                         __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(&r);
+    const T2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(to_f32(m.x), to_f32(m.y));
   }
-  a.s += s[0] + s[1];
-  a.u += u[0] + u[1];
-  return mx;
 }
+
+// A thread's sums, the even and the odd elements' apart (paired arithmetic).
+struct Running {
+  float ref, over;              // over: the maximum that moves ref
+  float2 s, u;
+
+  __device__ __forceinline__ Running() : ref(0.f), over(-INFINITY) {
+    s = u = make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ void move(float mx, float c) {
+    const float d = max_nan((ref - mx) * c, kFloor), f = ex2(d);
+    if (s.x != 0.f) u.x = f * fmaf(s.x, d, u.x), s.x *= f;
+    if (s.y != 0.f) u.y = f * fmaf(s.y, d, u.y), s.y *= f;
+    ref = mx;
+    over = mx + kSlack / c;
+  }
+  template <typename T>
+  __device__ __forceinline__ float add(const uint4& raw, float c) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const float mx = pack_max<T>(raw);
+    if (mx > over) move(mx, c);
+    float x[N];
+    vec::unpack<T, N>(raw, x);
+    const float2 c2 = make_float2(c, c), r2 = make_float2(-ref, -ref);
+    float2 ps = make_float2(0.f, 0.f), pu = ps;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float2 t = sm100::fmul2(sm100::fadd2(make_float2(x[i], x[i + 1]), r2), c2);
+      t.x = max_nan(t.x, kFloor);
+      t.y = max_nan(t.y, kFloor);
+      const float2 e = make_float2(ex2(t.x), ex2(t.y));
+      ps = i ? sm100::fadd2(ps, e) : e;
+      pu = i ? sm100::ffma2(t, e, pu) : sm100::fmul2(t, e);
+    }
+    s = sm100::fadd2(s, ps);
+    u = sm100::fadd2(u, pu);
+    return mx;
+  }
+  __device__ __forceinline__ Sums sums() const { return {ref, s.x + s.y, u.x + u.y}; }
+};
 
 struct Args {
   int64_t rows;
@@ -186,21 +229,24 @@ struct TopShared {
 };
 
 // The k largest keys of the block's packs [begin, end) into sh.list, in order
-// (0 where there are fewer).  `best` orders this thread's largest logit and
-// `best_pack` is the first pack that has it (-1: none).  The k-th largest key of
+// (0 where there are fewer).  `best` is this thread's largest logit and
+// `best_pack` the first pack that has it (-1: none); `nan` is set where a sum of
+// the block is NaN, as then `best` may have missed a NaN.  The k-th largest key of
 // any elements is a lower bound of the k-th largest of all, so: take it from the
 // threads' largest (up to 8 of each warp), look once more through the packs of
 // the threads that reach it (about k of them), and rank what is found.  Should
-// more than kCandidates elements reach the bound, the list is made one pass an
-// entry.
+// more than kCandidates elements reach the bound, or with NaN, the list is made
+// one pass an entry.
 template <typename T>
 __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int end, int k,
-                                          uint32_t best, int best_pack, TopShared& sh) {
+                                          float best, int best_pack, bool nan,
+                                          TopShared& sh) {
   constexpr int N = Packs<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) sh.bar = 0, sh.n_threads = 0, sh.n_found = 0;
   // a key no larger than that of the thread's largest: its pack's last index
-  uint32_t order = best_pack < 0 ? 0u : best;
+  const uint32_t best_order = order_of(best);
+  uint32_t order = best_pack < 0 ? 0u : best_order;
   const uint32_t last = (uint32_t)(row.first(best_pack) + N - 1);
   const int rounds = min(8, k);
   for (int r = 0; r < rounds; ++r) {
@@ -219,10 +265,10 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   }
   __syncthreads();
   const uint64_t bar = sh.bar;
-  if (best_pack >= 0 && key_of(best, max((int64_t)0, row.first(best_pack))) >= bar)
+  if (best_pack >= 0 && key_of(best_order, max((int64_t)0, row.first(best_pack))) >= bar)
     sh.threads[atomicAdd(&sh.n_threads, 1)] = threadIdx.x;
   __syncthreads();
-  const int n_threads = sh.n_threads;
+  const int n_threads = nan ? 0 : sh.n_threads;
   for (int q = warp; q < n_threads; q += kWarps) {
     for (int v = begin + sh.threads[q] + lane * kThreads; v < end; v += 32 * kThreads) {
       float x[N];
@@ -240,7 +286,7 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   }
   __syncthreads();
   const int n = sh.n_found;
-  if (n <= kCandidates) {
+  if (n <= kCandidates && !nan) {
     for (int c = threadIdx.x; c < max(n, k); c += kThreads) {
       if (c >= n) {
         sh.list[c] = 0;
@@ -317,22 +363,16 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     if (tok0 >= 0 && tok0 < a.V) x0 = to_f32(x[tok0]);
   }
 
-  Sums acc{0.f, 0.f, 0.f};
+  Running run;
   float best = -INFINITY;
-  uint32_t best_order = 0;
   int best_pack = -1;
   auto take = [&](const uint4& raw, int v) {
-    float f[N];
-    vec::unpack<T, N>(raw, f);
-    const float mx = accumulate<N>(f, c, acc);
-    if constexpr (kTop) {
-      const uint32_t o = order_of(mx);
-      if (o > best_order) best_order = o, best_pack = v;
-    } else {
-      best = max_nan(best, mx);
-    }
+    const float mx = run.add<T>(raw, c);
+    if (kTop && mx > best) best_pack = v;
+    best = fmaxf(best, mx);
   };
   int v = begin + threadIdx.x;
+  if (v < end) best_pack = v;
   for (; v + (kUnroll - 1) * kThreads < end; v += kUnroll * kThreads) {
     uint4 raw[kUnroll];
 #pragma unroll
@@ -341,18 +381,18 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * kThreads);
   }
   for (; v < end; v += kThreads) take(packs.raw(v), v);
-  if constexpr (kTop)
-    if (best_pack >= 0) best = of_order(best_order);
 
+  Sums acc = run.sums();
+  const bool nan = acc.s != acc.s;
   float wb = best;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     acc = merged(acc, shfl_xor(acc, o), c);
-    wb = max_nan(wb, __shfl_xor_sync(0xffffffffu, wb, o));
+    wb = fmaxf(wb, __shfl_xor_sync(0xffffffffu, wb, o));
   }
   if (lane == 0) warps[warp] = {acc, wb};
   if constexpr (kTop)
-    block_top<T>(packs, begin, end, a.k, best_order, best_pack, sh);
+    block_top<T>(packs, begin, end, a.k, best, best_pack, __syncthreads_or(nan), sh);
   else
     __syncthreads();
   if (blocks > 1) {
@@ -360,7 +400,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     if (threadIdx.x == 0) {
       Part p = warps[0];
       for (int w = 1; w < kWarps; ++w)
-        p = {merged(p.sums, warps[w].sums, c), max_nan(p.best, warps[w].best)};
+        p = {merged(p.sums, warps[w].sums, c), fmaxf(p.best, warps[w].best)};
       *cluster.map_shared_rank(&parts[rank], 0) = p;
     }
     if constexpr (kTop)
@@ -373,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     const Part* from = blocks > 1 ? parts : warps;
     Part p = from[0];
     for (int i = 1; i < (blocks > 1 ? blocks : kWarps); ++i)
-      p = {merged(p.sums, from[i].sums, c), max_nan(p.best, from[i].best)};
+      p = {merged(p.sums, from[i].sums, c), fmaxf(p.best, from[i].best)};
     float ln_s = 0.f, inv_s = 0.f, H = 0.f;
     if (p.sums.s != 0.f) {
       rebase(p.sums, p.best, c);
@@ -471,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
   const float B = empty ? 0.f : -gH * kLn2 * st.z * inv_t;
   auto base = [&](float v) {
     const float t = max_nan((v - ref) * c, kFloor);
-    return ex2(t) * fmaf(B, t, A);
+    return ex2<true>(t) * fmaf(B, t, A);
   };
   auto fetch = [&](int v) -> uint4 {
     if (same && to.whole(v))
