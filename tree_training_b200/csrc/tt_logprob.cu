@@ -248,7 +248,8 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   const uint32_t best_order = order_of(best);
   uint32_t order = best_pack < 0 ? 0u : best_order;
   const uint32_t last = (uint32_t)(row.first(best_pack) + N - 1);
-  const int rounds = min(8, k);
+  // two of each warp for each eight wanted: twice as many keys as entries
+  const int rounds = min(8, 2 * ((k + 7) / 8));
   for (int r = 0; r < rounds; ++r) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, order);
     const uint32_t at = __reduce_min_sync(0xffffffffu, order == top ? last : 0xffffffffu);
@@ -269,10 +270,13 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
     sh.threads[atomicAdd(&sh.n_threads, 1)] = threadIdx.x;
   __syncthreads();
   const int n_threads = nan ? 0 : sh.n_threads;
+  const uint32_t bar_order = (uint32_t)(bar >> 32);
   for (int q = warp; q < n_threads; q += kWarps) {
     for (int v = begin + sh.threads[q] + lane * kThreads; v < end; v += 32 * kThreads) {
+      const uint4 raw = row.raw(v);
+      if (order_of(pack_max<T>(raw)) < bar_order) continue;
       float x[N];
-      row.load(v, x);
+      vec::unpack<T, N>(raw, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int64_t e = row.first(v) + i;
