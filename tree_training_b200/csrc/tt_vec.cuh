@@ -65,14 +65,28 @@ __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
   unpack<T, V>(load_raw<T, V>(p), v);
 }
 
+// (Pairs are converted by one instruction.)
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> pack(const float (&v)[V]) {
-  union {
+  union U {
     Raw<T, V> raw;
     T e[V];
-  } u = {};
+    __nv_bfloat162 b2[(V + 1) / 2];
+    __half2 h2[(V + 1) / 2];
+    __device__ U() {}
+  } u;
+  if constexpr (V == 1 || sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        u.b2[i / 2] = __floats2bfloat162_rn(v[i], v[i + 1]);
+      else
+        u.h2[i / 2] = __floats2half2_rn(v[i], v[i + 1]);
+    }
+  }
   return u.raw;
 }
 
