@@ -507,7 +507,7 @@ int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int32_t D, cons
                          int64_t x_st, const void* residual, int64_t res_st, const void* weight,
                          const void* post_weight, int weight_f32, float weight_offset,
                          const void* gate, int64_t gate_st, int gate_mode, float scale, float eps,
-                         void* y, void* r, float* stats, void* stream);
+                         void* y, void* r, float* stats, int32_t* status, void* stream);
 /* Rows of fp32 partials the backward writes: `part` is [3][blocks][D]. */
 int tt_residual_norm_bwd_blocks(int64_t rows, int32_t D);
 /* dy, dr (null: zeros) are the gradients of y and r; every output may be null
@@ -519,7 +519,7 @@ int tt_residual_norm_bwd(int dtype, int res_dtype, int64_t rows, int32_t D, cons
                          const void* gate, int64_t gate_st, int gate_mode, float scale,
                          const float* stats, const void* dy, int64_t dy_st, const void* dr,
                          int64_t dr_st, void* dx, void* dres, void* dgate, void* dweight,
-                         void* dpost, float* part, int32_t blocks, void* stream);
+                         void* dpost, float* part, int32_t blocks, int32_t* status, void* stream);
 
 /* ---- tokens sorted by expert ---------------------------------------------- *
  * Stable counting sort of n_entries = n_tok * k choices (entry t * k + j) by

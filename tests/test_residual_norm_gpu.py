@@ -107,7 +107,7 @@ def test_every_form(T, D, dtype, res, post, gate):
 
 
 @pytest.mark.parametrize("T,D,dtype", [
-    (1, 1, F32), (3, 2, BF), (1, 4096, BF), (2, 4097, F16), (5, 4104, F32), (6, 8192, BF),
+    (1500, 1032, BF), (2000, 2560, F32), (1300, 4096, BF), (1, 1, F32), (3, 2, BF), (1, 4096, BF), (2, 4097, F16), (5, 4104, F32), (6, 8192, BF),
     (3, 8200, BF), (2, 16384, F32), (2, 16383, BF), (1500, 40, BF), (5000, 128, BF),
 ])
 @pytest.mark.parametrize("full", [False, True])

@@ -96,11 +96,11 @@ SIGNATURES = {
     "tt_rotary": (_INT, [_INT, _I64, _I32, _I32, _I32, _I32, _INT, _INT, _P, _I64, _I64, _P,
                          _I64, _I64, _P, _INT, _P, _I64, _P, _P, _P, _P]),
     "tt_residual_norm_fwd": (_INT, [_INT, _INT, _I64, _I32, _P, _I64, _P, _I64, _P, _P, _INT,
-                                    _F32, _P, _I64, _INT, _F32, _F32, _P, _P, _P, _P]),
+                                    _F32, _P, _I64, _INT, _F32, _F32, _P, _P, _P, _P, _P]),
     "tt_residual_norm_bwd_blocks": (_INT, [_I64, _I32]),
     "tt_residual_norm_bwd": (_INT, [_INT, _INT, _I64, _I32, _P, _I64, _P, _I64, _P, _P, _INT,
                                     _F32, _P, _I64, _INT, _F32, _P, _P, _I64, _P, _I64, _P, _P,
-                                    _P, _P, _P, _P, _I32, _P]),
+                                    _P, _P, _P, _P, _I32, _P, _P]),
     "tt_moe_plan_workspace_size": (_I64, [_I64, _I32]),
     "tt_moe_plan": (_INT, [_P, _INT, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
     "tt_moe_dispatch": (_INT, [_INT, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),

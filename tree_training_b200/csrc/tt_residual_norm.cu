@@ -27,6 +27,7 @@
 // once at the store.
 #include <algorithm>
 
+#include "tt_sm100.cuh"
 #include "tt_vec.cuh"
 
 namespace tt {
@@ -367,6 +368,382 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
   }
 }
 
+// ---- rows through shared memory ---------------------------------------------
+//
+// The same for long aligned rows (one a block, weights of x's type): thread 0
+// keeps a ring of `stages` rows filled by bulk copies, so that the next rows
+// arrive while this one is reduced and stored, and raw 16-bit packs instead of
+// fp32 values are what stays in registers across the reduction.  A stage is
+// filled again only behind a barrier that every thread reaches after it has used
+// what it read.  A wait that gives up records its error and lets the block run
+// on over what is in the ring, so all threads keep meeting at the same barriers.
+
+struct Ring {
+  int stages, stage_bytes;
+  int32_t* status;
+};
+
+constexpr int kMaxStages = 8;
+
+// After a wait that gave up: the copies in flight land (stage i took the issues
+// i, i + S, ... of `issued`) before the block ends.
+__device__ __forceinline__ void land(uint64_t* full, int S, int64_t issued) {
+  for (int i = 0; i < S; ++i)
+    if (issued > i) sm100::mbar_wait(&full[i], (uint32_t)((issued - 1 - i) / S) & 1, nullptr);
+}
+
+// Sums over the block's warps; red: [N][32] floats.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i * 32 + (threadIdx.x >> 5)] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane < nw ? red[i * 32 + lane] : 0.f;
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+}
+
+// Eight elements of a row as they lie in shared memory.
+template <typename T>
+struct Raw8 {
+  static constexpr int P = (int)sizeof(T) / 2;
+  uint4 r[P];
+  __device__ __forceinline__ void read(const uint8_t* row, int t) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) r[p] = reinterpret_cast<const uint4*>(row)[t * P + p];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int p = 0; p < P; ++p) r[p] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    constexpr int W = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float o[W];
+      vec::unpack<T, W>(r[p], o);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[p * W + j] = o[j];
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void put8(T* row, int t, const float (&v)[8]) {
+  constexpr int W = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int p = 0; p < 8 / W; ++p) {
+    float o[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = v[p * W + j];
+    vec::store<T, W>(row + t * 8 + p * W, o);
+  }
+}
+
+template <typename T, typename R, bool kFullForm>
+__global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][32];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ int32_t abort_flag;
+  const int D = a.D, t = threadIdx.x, S = ring.stages;
+  const bool in = t * 8 < D;
+  const bool post = kFullForm && a.w1, gated = kFullForm && a.gate_mode == kFull;
+  const bool by_row = kFullForm && a.gate_mode == kRow;
+  const int x_bytes = D * (int)sizeof(T), r_bytes = a.res ? D * (int)sizeof(R) : 0;
+  const float inv_D = 1.f / D;
+  if (t == 0) {
+    for (int i = 0; i < S; ++i) sm100::mbar_init(&full[i], 1);
+    abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
+  __syncthreads();
+  int64_t issued = 0;
+  auto issue = [&](int64_t row, int stage) {
+    if (row >= a.rows || *(volatile int32_t*)&abort_flag) return;
+    ++issued;
+    uint8_t* to = smem + stage * ring.stage_bytes;
+    sm100::mbar_arrive_expect_tx(&full[stage], ring.stage_bytes);
+    sm100::bulk_load(to, reinterpret_cast<const T*>(a.x) + row * a.x_st, x_bytes, &full[stage]);
+    if (a.res)
+      sm100::bulk_load(to + x_bytes, reinterpret_cast<const R*>(a.res) + row * a.res_st, r_bytes,
+                       &full[stage]);
+    if (gated)
+      sm100::bulk_load(to + x_bytes + r_bytes,
+                       reinterpret_cast<const T*>(a.gate) + row * a.gate_st, x_bytes,
+                       &full[stage]);
+  };
+  if (t == 0)
+    for (int i = 0; i < S; ++i) issue(blockIdx.x + (int64_t)i * gridDim.x, i);
+  Raw8<T> w2, w1;
+  w2.zero(), w1.zero();
+  if (in) {
+    w2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
+    if (post) w1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
+  }
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (!sm100::mbar_wait(&full[stage], phase, &abort_flag)) {
+      set_status(ring.status, TT_ERR_DEVICE_TIMEOUT);
+      *(volatile int32_t*)&abort_flag = 1;
+    }
+    const uint8_t* at = smem + stage * ring.stage_bytes;
+    Raw8<T> raw;
+    float h[8], r[8], g[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = r[e] = g[e] = 0.f;
+    if (in) {
+      raw.read(at, t);
+      raw.get(h);
+      if (a.res) {
+        Raw8<R> rr;
+        rr.read(at + x_bytes, t);
+        rr.get(r);
+      }
+      if (gated) {
+        raw.read(at + x_bytes + r_bytes, t);
+        raw.get(g);
+      }
+    }
+    float k = a.scale, i1 = 1.f;
+    if (by_row) k *= to_f32(reinterpret_cast<const T*>(a.gate)[row * a.gate_st]);
+    if (post) {
+      float s[1] = {0.f}, w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[0] = fmaf(h[e], h[e], s[0]);
+      block_sum<1>(s, red[0]);
+      i1 = rsqrtf(fmaf(s[0], inv_D, a.eps));
+      w1.get(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] *= i1 * (a.offset + w[e]);
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (gated) h[e] *= g[e];
+      r[e] = fmaf(k, h[e], r[e]);
+      s[0] = fmaf(r[e], r[e], s[0]);
+    }
+    block_sum<1>(s, red[1]);
+    if (t == 0) issue(row + (int64_t)S * gridDim.x, stage);
+    if (++stage == S) stage = 0, phase ^= 1;
+    const float i2 = rsqrtf(fmaf(s[0], inv_D, a.eps));
+    if (in) {
+      put8<R>(reinterpret_cast<R*>(a.r) + row * D, t, r);
+      float w[8];
+      w2.get(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] *= i2 * (a.offset + w[e]);
+      put8<T>(reinterpret_cast<T*>(a.y) + row * D, t, r);
+    }
+    if (t == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = make_float2(i1, i2);
+    // without the first sum, a barrier before the second area is written again
+    if (!post) __syncthreads();
+  }
+  if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
+}
+
+template <typename T, typename R, bool kFullForm, int kBlocks>
+__global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Ring ring) {
+  constexpr int N = kFullForm ? 3 : 1;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][N * 32];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ int32_t abort_flag;
+  const int D = a.D, t = threadIdx.x, S = ring.stages;
+  const bool in = t * 8 < D;
+  const bool post = kFullForm && a.w1, gated = kFullForm && a.gate_mode == kFull;
+  const bool by_row = kFullForm && a.gate_mode == kRow;
+  const int x_bytes = D * (int)sizeof(T), r_bytes = D * (int)sizeof(R);
+  const int at_dy = x_bytes, at_g = at_dy + (a.dy ? x_bytes : 0);
+  const int at_r = at_g + (gated ? x_bytes : 0), at_dr = at_r + (a.res ? r_bytes : 0);
+  const float inv_D = 1.f / D;
+  if (t == 0) {
+    for (int i = 0; i < S; ++i) sm100::mbar_init(&full[i], 1);
+    abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
+  __syncthreads();
+  int64_t issued = 0;
+  auto issue = [&](int64_t row, int stage) {
+    if (row >= a.rows || *(volatile int32_t*)&abort_flag) return;
+    ++issued;
+    uint8_t* to = smem + stage * ring.stage_bytes;
+    uint64_t* bar = &full[stage];
+    sm100::mbar_arrive_expect_tx(bar, ring.stage_bytes);
+    sm100::bulk_load(to, reinterpret_cast<const T*>(a.x) + row * a.x_st, x_bytes, bar);
+    if (a.dy)
+      sm100::bulk_load(to + at_dy, reinterpret_cast<const T*>(a.dy) + row * a.dy_st, x_bytes, bar);
+    if (gated)
+      sm100::bulk_load(to + at_g, reinterpret_cast<const T*>(a.gate) + row * a.gate_st, x_bytes,
+                       bar);
+    if (a.res)
+      sm100::bulk_load(to + at_r, reinterpret_cast<const R*>(a.res) + row * a.res_st, r_bytes,
+                       bar);
+    if (a.dr)
+      sm100::bulk_load(to + at_dr, reinterpret_cast<const R*>(a.dr) + row * a.dr_st, r_bytes, bar);
+  };
+  if (t == 0)
+    for (int i = 0; i < S; ++i) issue(blockIdx.x + (int64_t)i * gridDim.x, i);
+  Raw8<T> rw2, rw1;
+  rw2.zero(), rw1.zero();
+  if (in) {
+    rw2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
+    if (post) rw1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
+  }
+  float dw2[8], dw1[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dw2[e] = dw1[e] = 0.f;
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  // a row's own values are fetched a row ahead
+  float2 next = make_float2(0.f, 0.f);
+  float next_g = 1.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+    next = reinterpret_cast<const float2*>(a.stats)[row];
+    if (by_row) next_g = to_f32(reinterpret_cast<const T*>(a.gate)[row * a.gate_st]);
+  };
+  fetch(blockIdx.x);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float i1 = next.x, i2 = next.y, k = a.scale * next_g;
+    fetch(row + gridDim.x);
+    if (!sm100::mbar_wait(&full[stage], phase, &abort_flag)) {
+      set_status(ring.status, TT_ERR_DEVICE_TIMEOUT);
+      *(volatile int32_t*)&abort_flag = 1;
+    }
+    const uint8_t* at = smem + stage * ring.stage_bytes;
+    Raw8<T> rx, rg;
+    float r[8], d[8], s[N];
+    rx.zero(), rg.zero();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = d[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.f;
+    if (in) {
+      rx.read(at, t);
+      if (gated) rg.read(at + at_g, t);
+      if (a.res) {
+        Raw8<R> q;
+        q.read(at + at_r, t);
+        q.get(r);
+      }
+      if (a.dr) {
+        Raw8<R> q;
+        q.read(at + at_dr, t);
+        q.get(d);
+      }
+      float x[8], u[8], w[8], dy[8];
+      Raw8<T> ry;
+      if (a.dy)
+        ry.read(at + at_dy, t);
+      else
+        ry.zero();
+      ry.get(dy);
+      rx.get(x);
+      if (kFullForm) {
+        // u x: the block's output without scale, row gate and i1
+        if (post) {
+          rw1.get(u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= a.offset + u[e];
+        }
+        if (gated) {
+          rg.get(u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= u[e];
+        }
+      }
+      const float ki = kFullForm ? k * i1 : k;
+      rw2.get(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        r[e] = fmaf(ki, x[e], r[e]);
+        const float gy = dy[e] * (a.offset + w[e]);
+        dw2[e] = fmaf(dy[e] * i2, r[e], dw2[e]);
+        d[e] = fmaf(i2, gy, d[e]);               // a
+        s[0] = fmaf(gy, r[e], s[0]);
+        if constexpr (kFullForm) {
+          s[1] = fmaf(x[e], d[e], s[1]);
+          s[2] = fmaf(x[e], r[e], s[2]);
+        }
+      }
+    }
+    block_sum<N>(s, red[turn]);
+    turn ^= 1;
+    if (t == 0) issue(row + (int64_t)S * gridDim.x, stage);
+    if (++stage == S) stage = 0, phase ^= 1;
+    const float c = i2 * i2 * i2 * s[0] * inv_D;
+    if (in) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = fmaf(-c, r[e], d[e]);
+      if (a.dres) put8<R>(reinterpret_cast<R*>(a.dres) + row * D, t, d);
+    }
+    if constexpr (!kFullForm) {
+      if (in && a.dx) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] *= k;
+        put8<T>(reinterpret_cast<T*>(a.dx) + row * D, t, d);
+      }
+    } else {
+      const float dot = s[1] - c * s[2];         // sum of u x d
+      const float back = post ? k * i1 * i1 * i1 * dot * inv_D : 0.f;
+      if (by_row && t == 0 && a.dgate)
+        reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(a.scale * i1 * dot);
+      if (in) {
+        float x[8], w[8], g[8];
+        rx.get(x);
+        if (post) {
+          rw1.get(w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] += a.offset;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = 1.f;
+        }
+        if (gated) {
+          rg.get(g);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = 1.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float xd = i1 * x[e] * d[e], kg = k * g[e];
+          dw1[e] = fmaf(kg, xd, dw1[e]);
+          r[e] = fmaf(-back, x[e], i1 * (kg * d[e]) * w[e]);     // dx
+          d[e] = a.scale * w[e] * xd;                            // the element's gate
+        }
+        if (a.dx) put8<T>(reinterpret_cast<T*>(a.dx) + row * D, t, r);
+        if (gated && a.dgate) put8<T>(reinterpret_cast<T*>(a.dgate) + row * D, t, d);
+      }
+    }
+  }
+  if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
+  if (in) {
+    float* part = a.part + (int64_t)blockIdx.x * D + t * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[e] = dw2[e];
+    if (post) {
+      part += (int64_t)gridDim.x * D;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[e] = dw1[e];
+    }
+  }
+}
+
 // out[c] = sum over the blocks' partials, in a fixed order: 16 threads a
 // column, each over every 16th block.
 constexpr int kSumRows = 16;
@@ -454,6 +831,69 @@ int launch(const Args& a, bool vec, bool full, Shape s, int blocks, cudaStream_t
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
+// The ring's shape: as many blocks an SM as threads and registers allow (64 a
+// thread) while each has two stages or more; blocks 0: rows go straight to
+// registers.
+struct RingShape {
+  int blocks, stages, stage_bytes, per_sm;
+};
+
+constexpr int kSharedPerSM = 225 * 1024, kSharedOwn = 2048;   // kSharedOwn: static, reserved
+
+RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes) {
+  RingShape best{0, 0, stage_bytes, 0};
+  for (int per = 1024 / threads; per > 0; --per) {
+    const int stages = std::min(kMaxStages, (kSharedPerSM / per - kSharedOwn) / stage_bytes);
+    if (stages >= 2) {
+      best.blocks = (int)std::min<int64_t>(rows, (int64_t)vec::kSMs * per);
+      best.stages = stages;
+      best.per_sm = per;
+      break;
+    }
+  }
+  return best;
+}
+
+bool rows_by_ring(int D, int dtype, bool vec, const Args& a) {
+  return vec && D > 1024 && D <= 4096 && (!a.w_f32 || dtype == TT_F32) &&
+         a.gate_mode != kChannel && reinterpret_cast<uintptr_t>(a.w2) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(a.w1) % 16 == 0;
+}
+
+template <typename T, typename R, bool kBwd>
+int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, int32_t* status,
+                cudaStream_t st) {
+  const Ring ring{shape.stages, shape.stage_bytes, status};
+  const int smem = shape.stages * shape.stage_bytes;
+  auto go = [&](auto kern) -> int {
+    TT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<shape.blocks, threads, smem, st>>>(a, ring);
+    return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  };
+  if constexpr (kBwd)
+    // alone on its SM a block of 512 threads may use 128 registers each
+    return !full               ? go(ring_bwd<T, R, false, 2>)
+           : shape.per_sm == 1 ? go(ring_bwd<T, R, true, 1>)
+                               : go(ring_bwd<T, R, true, 2>);
+  else
+    return full ? go(ring_fwd<T, R, true>) : go(ring_fwd<T, R, false>);
+}
+
+template <bool kBwd>
+int dispatch_ring(int dtype, int res_dtype, const Args& a, int threads, const RingShape& shape,
+                  int32_t* status, cudaStream_t st) {
+  const bool full = a.w1 || a.gate_mode != kNone;
+  return vec::dispatch_float(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    if (res_dtype == dtype) return launch_ring<T, T, kBwd>(a, full, threads, shape, status, st);
+    if (res_dtype == TT_F32)
+      return launch_ring<T, float, kBwd>(a, full, threads, shape, status, st);
+    return TT_ERR_UNSUPPORTED;
+  });
+}
+
+int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
+
 template <bool kBwd>
 int dispatch(int dtype, int res_dtype, const Args& a, bool vec, Shape s, int blocks,
              cudaStream_t st) {
@@ -480,9 +920,11 @@ extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int3
                                     int64_t res_st, const void* weight, const void* post_weight,
                                     int weight_f32, float weight_offset, const void* gate,
                                     int64_t gate_st, int gate_mode, float scale, float eps,
-                                    void* y, void* r, float* stats, void* stream) {
+                                    void* y, void* r, float* stats, int32_t* status,
+                                    void* stream) {
   using namespace tt::resnorm;
-  if (bad_sizes(rows, D, gate_mode, gate) || (rows > 0 && (!x || !weight || !y || !r)))
+  if (bad_sizes(rows, D, gate_mode, gate) || (rows > 0 && (!x || !weight || !y || !r)) ||
+      reinterpret_cast<uintptr_t>(stats) % 8)
     return TT_ERR_INVALID_ARG;
   if (rows == 0) return TT_OK;
   Args a{};
@@ -499,7 +941,15 @@ extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int3
                    (gate_mode != kFull || aligned(gate, gate_st));
   const int64_t want = (rows + s.per - 1) / s.per;
   const int blocks = (int)std::min<int64_t>(want, tt::vec::kSMs * 16ll);
-  const int rc = dispatch<false>(dtype, res_dtype, a, vec, s, blocks, (cudaStream_t)stream);
+  RingShape ring{};
+  if (rows_by_ring(D, dtype, vec, a))
+    ring = ring_of(rows, D, s.tpr,
+                   D * (size_of(dtype) * (gate_mode == kFull ? 2 : 1) +
+                        (residual ? size_of(res_dtype) : 0)));
+  const int rc = ring.blocks
+                     ? dispatch_ring<false>(dtype, res_dtype, a, s.tpr, ring, status,
+                                            (cudaStream_t)stream)
+                     : dispatch<false>(dtype, res_dtype, a, vec, s, blocks, (cudaStream_t)stream);
   if (rc == TT_OK) tt_count_launches(1);
   return rc;
 }
@@ -519,10 +969,10 @@ extern "C" int tt_residual_norm_bwd(
     int weight_f32, float weight_offset, const void* gate, int64_t gate_st, int gate_mode,
     float scale, const float* stats, const void* dy, int64_t dy_st, const void* dr,
     int64_t dr_st, void* dx, void* dres, void* dgate, void* dweight, void* dpost, float* part,
-    int32_t blocks, void* stream) {
+    int32_t blocks, int32_t* status, void* stream) {
   using namespace tt::resnorm;
   if (bad_sizes(rows, D, gate_mode, gate) || blocks <= 0 ||
-      (rows > 0 && (!x || !weight || !stats || !part)))
+      (rows > 0 && (!x || !weight || !stats || !part)) || reinterpret_cast<uintptr_t>(stats) % 8)
     return TT_ERR_INVALID_ARG;
   if (rows == 0) return TT_OK;
   Args a{};
@@ -542,7 +992,15 @@ extern "C" int tt_residual_norm_bwd(
                    aligned(dres, D) &&
                    (gate_mode != kFull || (aligned(gate, gate_st) && aligned(dgate, D)));
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = dispatch<true>(dtype, res_dtype, a, vec, s, blocks, st);
+  RingShape ring{};
+  if (rows_by_ring(D, dtype, vec, a))
+    ring = ring_of(rows, D, s.tpr,
+                   D * (size_of(dtype) * (1 + (dy ? 1 : 0) + (gate_mode == kFull ? 1 : 0)) +
+                        size_of(res_dtype) * ((residual ? 1 : 0) + (dr ? 1 : 0))));
+  if (ring.blocks) ring.blocks = blocks = std::min(blocks, ring.blocks);
+  const int rc = ring.blocks
+                     ? dispatch_ring<true>(dtype, res_dtype, a, s.tpr, ring, status, st)
+                     : dispatch<true>(dtype, res_dtype, a, vec, s, blocks, st);
   if (rc != TT_OK) return rc;
   Out out{};
   out.p[0] = dweight;

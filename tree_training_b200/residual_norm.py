@@ -11,6 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, _ops
+from .attention import _status_word
 
 MAX_DIM = 16384
 _NONE, _CHANNEL, _ROW, _FULL = 0, 1, 2, 3
@@ -30,7 +31,7 @@ def _forward(x, res, w, post, gate, mode, scale, eps, offset, keep):
               x.data_ptr(), x.stride(0), _ptr(res), 0 if res is None else res.stride(0),
               w.data_ptr(), _ptr(post), w.dtype == torch.float32, offset, _ptr(gate),
               0 if gate is None else gate.stride(0), mode, scale, eps, y.data_ptr(),
-              r.data_ptr(), _ptr(stats))
+              r.data_ptr(), _ptr(stats), _status_word(x.device).data_ptr())
     return y, r, stats
 
 
@@ -71,7 +72,7 @@ class _ResidualNorm(torch.autograd.Function):
                   0 if gate is None else gate.stride(0), mode, scale, stats.data_ptr(),
                   _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dr),
                   0 if dr is None else dr.stride(0), _ptr(dx), _ptr(dres), _ptr(dgate), _ptr(dw),
-                  _ptr(dpost), part.data_ptr(), blocks)
+                  _ptr(dpost), part.data_ptr(), blocks, _status_word(dev).data_ptr())
         if same and need[0]:
             dx = dres
         return dx, dres if need[1] else None, dw, dpost, dgate, None, None, None, None
