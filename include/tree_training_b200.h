@@ -526,7 +526,8 @@ int tt_residual_norm_bwd(int dtype, int res_dtype, int64_t rows, int32_t D, cons
  * expert id (int64 with ids64, else int32).  slots[entry]: its sorted row, -1
  * where the id is outside [0, n_experts) (dropped); entries[row]: its entry,
  * -1 past the last kept row; offsets[n_experts + 1]: first row of each expert
- * and the number of kept rows.  n_experts <= 1024, n_entries < 2^31. */
+ * and the number of kept rows.  n_experts <= 1024, n_entries < 2^31; the calls
+ * below take k <= 64. */
 int64_t tt_moe_plan_workspace_size(int64_t n_entries, int32_t n_experts);
 int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_t n_experts, int32_t* slots,
                 int32_t* entries, int32_t* offsets, void* workspace, int64_t workspace_bytes,

@@ -78,6 +78,7 @@ def test_large_plans(T, k, E):
     (1, 1, 1, 1, F32, F32), (47, 2, 4, 128, F32, F32), (130, 8, 32, 2048, BF, F32),
     (65, 3, 7, 77, F16, F16), (33, 11, 16, 520, BF, BF), (20, 4, 8, 8192, BF, F32),
     (300, 2, 5, 64, F16, F32), (9, 1, 3, 4100, F32, BF), (17, 17, 40, 96, BF, F32),
+    (11, 64, 90, 32, F32, BF), (5, 33, 40, 5000, BF, F16),
 ])
 def test_there_and_back(T, k, E, H, dtype, wdtype, kind):
     g = torch.Generator(device=DEV).manual_seed(1)
@@ -189,7 +190,7 @@ def test_refusals():
         tt.expert_plan(ids.cpu(), 4)
     with pytest.raises(TypeError):
         tt.expert_plan(ids.float(), 4)
-    for a in ((ids[0], 4), (ids, 0), (ids, 1025)):
+    for a in ((ids[0], 4), (ids, 0), (ids, 1025), (ids[:, :1].expand(4, 65), 4)):
         with pytest.raises(ValueError):
             tt.expert_plan(*a)
     plan = tt.expert_plan(ids, 4)

@@ -248,8 +248,9 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   const uint32_t best_order = order_of(best);
   uint32_t order = best_pack < 0 ? 0u : best_order;
   const uint32_t last = (uint32_t)(row.first(best_pack) + N - 1);
-  // two of each warp for each eight wanted: twice as many keys as entries
-  const int rounds = min(8, 2 * ((k + 7) / 8));
+  // (with fewer keys a warp, a row of equal logits has its bound set by later
+  // warps' and many more candidates)
+  const int rounds = min(8, k);
   for (int r = 0; r < rounds; ++r) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, order);
     const uint32_t at = __reduce_min_sync(0xffffffffu, order == top ? last : 0xffffffffu);

@@ -23,9 +23,16 @@ namespace {
 
 // ---- plan --------------------------------------------------------------------
 
+// Two launches: blocks take runs of the entries, count them by expert and leave
+// each entry's rank among its block's entries of the same expert; then each block
+// adds up the counts of all blocks and of the earlier ones, and places its
+// entries. One block does both in one launch where it is enough. Bound by
+// latency, not by the 20 bytes an entry: many blocks of few steps each (eight
+// blocks that meet in a cluster took 14.5 us for 65,528 entries).
+
 constexpr int kPlanWarps = 8;
 constexpr int kMaxExperts = 1024;
-constexpr int kChunk = 2048;       // entries of a block, at least
+constexpr int kSteps = 8;          // of 32 entries, fetched together
 
 __device__ __forceinline__ int expert_of(const void* ids, int ids64, int64_t i, int E) {
   const int64_t e = ids64 ? reinterpret_cast<const int64_t*>(ids)[i]
@@ -33,117 +40,180 @@ __device__ __forceinline__ int expert_of(const void* ids, int ids64, int64_t i, 
   return (e >= 0 && e < E) ? (int)e : E;      // E: dropped, sorted behind the others
 }
 
-// Entries [begin, end) of a warp: hist[e] += their number of each expert.
-__device__ __forceinline__ void warp_count(const void* ids, int ids64, int64_t begin, int64_t end,
-                                           int E, int* hist) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t i0 = begin; i0 < end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = i < end ? expert_of(ids, ids64, i, E) : E + 1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e <= E && lane == __ffs(same) - 1) hist[e] += __popc(same);
-    __syncwarp();
+// The lanes whose e is this lane's, by one vote a bit (a match instruction takes
+// several times as long over 32 different values).
+__device__ __forceinline__ unsigned same_as(int e, int bits) {
+  unsigned m = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (e >> b) & 1;
+    const unsigned v = __ballot_sync(0xffffffffu, one);
+    m &= one ? v : ~v;
   }
+  return m;
 }
 
-// Block b's entries are [b chunk, (b + 1) chunk), warp w's the w-th eighth.
-__device__ __forceinline__ void warp_range(int64_t n, int64_t chunk, int64_t* begin, int64_t* end) {
-  const int64_t part = chunk / kPlanWarps;
-  const int64_t b = blockIdx.x * chunk + (threadIdx.x >> 5) * part;
-  *begin = min(b, n);
-  *end = min(b + part, n);
-}
+struct PlanArgs {
+  const void* ids;
+  int ids64;
+  int64_t n, run;                  // entries, and those of a warp (a multiple of 32)
+  int E;
+  int32_t *slots, *entries, *offsets;
+  int32_t* counts;                 // [blocks][E + 1]
+};
 
-__global__ void __launch_bounds__(32 * kPlanWarps)
-plan_count(const void* ids, int ids64, int64_t n, int64_t chunk, int E, int* __restrict__ counts) {
-  extern __shared__ int hist[];              // [warps][E + 1]
-  for (int i = threadIdx.x; i < kPlanWarps * (E + 1); i += blockDim.x) hist[i] = 0;
-  __syncthreads();
-  int64_t begin, end;
-  warp_range(n, chunk, &begin, &end);
-  warp_count(ids, ids64, begin, end, E, hist + (threadIdx.x >> 5) * (E + 1));
-  __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    int s = 0;
-    for (int w = 0; w < kPlanWarps; ++w) s += hist[w * (E + 1) + e];
-    counts[(int64_t)blockIdx.x * (E + 1) + e] = s;
-  }
-}
-
-// counts: [blocks][E + 1] of plan_count, or null with a single block (which
-// then counts for itself).
-__global__ void __launch_bounds__(32 * kPlanWarps)
-plan_place(const void* ids, int ids64, int64_t n, int64_t chunk, int E,
-           const int* __restrict__ counts, int32_t* __restrict__ slots,
-           int32_t* __restrict__ entries, int32_t* __restrict__ offsets) {
-  extern __shared__ int sm[];
-  int* hist = sm;                            // [warps][E + 1], then first rows
-  int* total = sm + kPlanWarps * (E + 1);    // [E + 1]
-  int* before = total + (E + 1);             // [E + 1]: in earlier blocks
-  __shared__ int warp_sum[kPlanWarps];
+// The exclusive sums over the experts of `all` (each thread's experts are
+// x0 = threadIdx.x * per, ...): the first of them.
+__device__ __forceinline__ int scan_experts(int sum, int* warp_sum) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kPlanWarps * (E + 1); i += blockDim.x) hist[i] = 0;
-  __syncthreads();
-  int64_t begin, end;
-  warp_range(n, chunk, &begin, &end);
-  int* mine = hist + warp * (E + 1);
-  warp_count(ids, ids64, begin, end, E, mine);
-  __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    int all = 0, pre = 0;
-    if (counts) {
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int c = counts[(int64_t)b * (E + 1) + e];
-        if (b < (int)blockIdx.x) pre += c;
-        all += c;
-      }
-    } else {
-      for (int w = 0; w < kPlanWarps; ++w) all += hist[w * (E + 1) + e];
-    }
-    total[e] = all;
-    before[e] = pre;
-  }
-  __syncthreads();
-  // exclusive sum of total over the experts: each thread a run of them
-  const int per = (E + 1 + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int e0 = min((int)threadIdx.x * per, E + 1), e1 = min(e0 + per, E + 1);
-  int run = 0;
-  for (int e = e0; e < e1; ++e) run += total[e];
-  int scan = run;
+  int scan = sum;
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= o) scan += up;
   }
   if (lane == 31) warp_sum[warp] = scan;
   __syncthreads();
-  int first = scan - run;
+  int first = scan - sum;
   for (int w = 0; w < warp; ++w) first += warp_sum[w];
-  for (int e = e0; e < e1; ++e) {
-    const int c = total[e];
-    if (blockIdx.x == 0) offsets[e] = first;   // offsets[E]: the rows that are kept
-    int at = first + before[e];
-    for (int w = 0; w < kPlanWarps; ++w) {
-      const int h = hist[w * (E + 1) + e];
-      hist[w * (E + 1) + e] = at;
-      at += h;
+  return first;
+}
+
+template <bool kSingle>
+__global__ void __launch_bounds__(32 * kPlanWarps) plan_rank(const PlanArgs a) {
+  extern __shared__ int sm[];
+  int* hist = sm;                             // [warps][E + 1]: counts, then next ranks
+  __shared__ int warp_sum[kPlanWarps];
+  const int E = a.E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t begin = min(a.n, ((int64_t)blockIdx.x * kPlanWarps + warp) * a.run);
+  const int64_t end = min(a.n, begin + a.run);
+  for (int i = threadIdx.x; i < kPlanWarps * (E + 1); i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  int* mine = hist + warp * (E + 1);
+  const int bits = 32 - __clz(E + 1);
+  int e[kSteps];
+  unsigned same[kSteps];
+  auto fetch = [&](int64_t from) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int64_t i = from + s * 32 + lane;
+      e[s] = i < end ? expert_of(a.ids, a.ids64, i, E) : E + 1;
     }
-    first += c;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      if (from + s * 32 < end) same[s] = same_as(e[s], bits);
+  };
+  for (int64_t from = begin; from < end; from += 32 * kSteps) {
+    fetch(from);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      if (e[s] <= E && lane == __ffs(same[s]) - 1) atomicAdd(mine + e[s], __popc(same[s]));
   }
   __syncthreads();
-  for (int64_t i0 = begin; i0 < end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = i < end ? expert_of(ids, ids64, i, E) : E + 1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int base = e <= E ? mine[e] : 0;
-    __syncwarp();
-    if (e <= E) {
-      const int row = base + __popc(same & ((1u << lane) - 1));
-      slots[i] = e < E ? row : -1;
-      entries[row] = e < E ? (int32_t)i : -1;
-      if (lane == __ffs(same) - 1) mine[e] = base + __popc(same);
+  // counts become the ranks that each warp starts with
+  const int per = kSingle ? (E + (int)blockDim.x) / (int)blockDim.x : 1;
+  const int stride = kSingle ? 1 : (int)blockDim.x;
+  int sum = 0, first = 0;
+  auto warps_of = [&](int x, int at, bool write) {
+    int c[kPlanWarps], all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) c[w] = hist[w * (E + 1) + x];
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) {
+      if (write) hist[w * (E + 1) + x] = at + all;
+      all += c[w];
     }
-    __syncwarp();
+    return all;
+  };
+  if constexpr (kSingle) {
+    const int x0 = threadIdx.x * per, x1 = min(x0 + per, E + 1);
+    for (int x = x0; x < x1; ++x) sum += warps_of(x, 0, false);
+    first = scan_experts(sum, warp_sum);
+    for (int x = x0; x < x1; ++x) {
+      a.offsets[x] = first;                   // offsets[E]: the rows that are kept
+      first += warps_of(x, first, true);
+    }
+  } else {
+    for (int x = threadIdx.x; x <= E; x += stride)
+      a.counts[(int64_t)blockIdx.x * (E + 1) + x] = warps_of(x, 0, true);
   }
+  __syncthreads();
+  // a warp's atomics on its own counters take effect in the order of its steps
+  const bool kept = end - begin <= 32 * kSteps;        // the ids are still in e
+  for (int64_t from = begin; from < end; from += 32 * kSteps) {
+    if (!kept) fetch(from);
+    int base[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      base[s] = 0;
+      if (e[s] <= E && lane == __ffs(same[s]) - 1)
+        base[s] = atomicAdd(mine + e[s], __popc(same[s]));
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int64_t i = from + s * 32 + lane;
+      if (from + s * 32 >= end) continue;
+      const int rank = __shfl_sync(0xffffffffu, base[s], __ffs(same[s]) - 1) +
+                       __popc(same[s] & ((1u << lane) - 1));
+      if (e[s] > E) continue;
+      if constexpr (kSingle) {
+        a.slots[i] = e[s] < E ? rank : -1;
+        a.entries[rank] = e[s] < E ? (int32_t)i : -1;
+      } else {
+        a.slots[i] = rank;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(32 * kPlanWarps) plan_place(const PlanArgs a) {
+  extern __shared__ int sm[];
+  int* total = sm;                            // [E + 1]
+  int* first = sm + a.E + 1;                  // [E + 1]: this block's first rows
+  __shared__ int warp_sum[kPlanWarps];
+  const int E = a.E, blocks = gridDim.x, b0 = blockIdx.x;
+  for (int x = threadIdx.x; x <= E; x += blockDim.x) {
+    int all = 0, before = 0;
+    for (int b = 0; b < blocks; b += 16) {
+      int c[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        c[j] = b + j < blocks ? __ldg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        all += c[j];
+        before += b + j < b0 ? c[j] : 0;
+      }
+    }
+    total[x] = all;
+    first[x] = before;
+  }
+  __syncthreads();
+  const int per = (E + (int)blockDim.x) / (int)blockDim.x;
+  const int x0 = threadIdx.x * per, x1 = min(x0 + per, E + 1);
+  int sum = 0;
+  for (int x = x0; x < x1; ++x) sum += total[x];
+  int at = scan_experts(sum, warp_sum);
+  for (int x = x0; x < x1; ++x) {
+    if (b0 == 0) a.offsets[x] = at;           // offsets[E]: the rows that are kept
+    first[x] += at;
+    at += total[x];
+  }
+  __syncthreads();
+  const int64_t begin = min(a.n, (int64_t)b0 * kPlanWarps * a.run);
+  const int64_t end = min(a.n, begin + kPlanWarps * a.run);
+  for (int64_t i = begin + threadIdx.x; i < end; i += blockDim.x) {
+    const int e = expert_of(a.ids, a.ids64, i, E);
+    const int row = first[e] + a.slots[i];
+    a.slots[i] = e < E ? row : -1;
+    a.entries[row] = e < E ? (int32_t)i : -1;
+  }
+}
+
+// Blocks of the two-launch form (each adds up `blocks` counts an expert), 1: the
+// one-launch form, whose warps take up to two fetches.
+int plan_blocks(int64_t n, int E) {
+  if (n <= 32 * kSteps * kPlanWarps) return 1;
+  const int64_t most = std::max<int64_t>(8, std::min<int64_t>(64, 32768 / (E + 1)));
+  return (int)std::min<int64_t>(most, (n + 32 * kPlanWarps - 1) / (32 * kPlanWarps));
 }
 
 // ---- rows --------------------------------------------------------------------
@@ -157,15 +227,8 @@ struct Args {
   void *dst, *dw;
   const void* w;
   int w_dtype;
+  int by_four;               // slots can be read four at a time
 };
-
-__device__ __forceinline__ float weight_of(const void* w, int dtype, int64_t i) {
-  switch (dtype) {
-    case TT_F32: return reinterpret_cast<const float*>(w)[i];
-    case TT_BF16: return to_f32(reinterpret_cast<const __nv_bfloat16*>(w)[i]);
-    default: return to_f32(reinterpret_cast<const __half*>(w)[i]);
-  }
-}
 
 // Zeroes the rows past the last kept one; the blocks share them out.
 template <typename T, int V>
@@ -181,101 +244,197 @@ __device__ __forceinline__ void zero_tail(const Args& a) {
       vec::store<T, V>(reinterpret_cast<T*>(a.dst) + r * a.H + p * V, z);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256) dispatch_kernel(const Args a) {
-  const int t = threadIdx.x % a.group;
-  const int64_t tok = (int64_t)blockIdx.x * (blockDim.x / a.group) + threadIdx.x / a.group;
+// A block's threads are groups of `group`, one token each; a token's slots and
+// weights are fetched KC at a time, and so are the rows they lead to, so that
+// KC loads of 16 bytes a thread are in flight.
+struct Place {
+  int t, slot;               // thread of its group, group of the block
+  int64_t tok;
+  bool live;
+};
+
+__device__ __forceinline__ Place place(const Args& a) {
+  const int q = threadIdx.x / a.group;
+  Place p;
+  p.t = threadIdx.x - q * a.group;
+  p.slot = q;
+  p.tok = (int64_t)blockIdx.x * (blockDim.x / a.group) + q;
+  p.live = p.tok < a.T;
+  return p;
+}
+
+template <int KC>
+__device__ __forceinline__ void slots_of(const Args& a, int64_t tok, int k0, int (&r)[KC]) {
+  const int32_t* at = a.slots + tok * a.K + k0;
+  if (KC >= 4 && a.by_four) {
+#pragma unroll
+    for (int k = 0; k < KC; k += 4) {
+      const int4 q = k0 + k < a.K ? __ldg(reinterpret_cast<const int4*>(at + k))
+                                  : make_int4(-1, -1, -1, -1);
+      r[k] = q.x, r[k + 1] = q.y, r[k + 2] = q.z, r[k + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < KC; ++k) r[k] = k0 + k < a.K ? __ldg(at + k) : -1;
+  }
+}
+
+__device__ __forceinline__ float weight_of(const Args& a, const Place& pl, int k) {
+  if (!pl.live || k >= a.K) return 0.f;
+  const int64_t i = pl.tok * a.K + k;
+  switch (a.w_dtype) {
+    case TT_F32: return reinterpret_cast<const float*>(a.w)[i];
+    case TT_BF16: return to_f32(reinterpret_cast<const __nv_bfloat16*>(a.w)[i]);
+    default: return to_f32(reinterpret_cast<const __half*>(a.w)[i]);
+  }
+}
+
+constexpr int kMaxK = 64;
+constexpr int kMaxTokens = 8;                      // of a block
+
+template <typename T, int V, int KC>
+__global__ void __launch_bounds__(512) dispatch_kernel(const Args a) {
+  const Place pl = place(a);
   const int packs = a.H / V;
-  if (tok < a.T) {
-    const T* src = reinterpret_cast<const T*>(a.src) + tok * a.H;
-    const int32_t* slot = a.slots + tok * a.K;
-    for (int p = t; p < packs; p += a.group) {
-      const vec::Raw<T, V> v = vec::load_raw<T, V>(src + p * V);
-      for (int k = 0; k < a.K; ++k) {
-        const int64_t r = __ldg(slot + k);
-        if (r >= 0)
-          *reinterpret_cast<vec::Raw<T, V>*>(reinterpret_cast<T*>(a.dst) + r * a.H + p * V) = v;
+  if (pl.live) {
+    const T* src = reinterpret_cast<const T*>(a.src) + pl.tok * a.H;
+    for (int k0 = 0; k0 < a.K; k0 += KC) {
+      int r[KC];
+      slots_of<KC>(a, pl.tok, k0, r);
+      for (int p = pl.t; p < packs; p += a.group) {
+        const vec::Raw<T, V> v = vec::load_raw<T, V>(src + p * V);
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+          if (r[k] >= 0)
+            *reinterpret_cast<vec::Raw<T, V>*>(reinterpret_cast<T*>(a.dst) + (int64_t)r[k] * a.H +
+                                               p * V) = v;
       }
     }
   }
   zero_tail<T, V>(a);
 }
 
-// kWeighted: combine, else collect.
-template <typename T, int V, bool kWeighted>
-__global__ void __launch_bounds__(256) combine_kernel(const Args a) {
-  const int t = threadIdx.x % a.group;
-  const int64_t tok = (int64_t)blockIdx.x * (blockDim.x / a.group) + threadIdx.x / a.group;
-  if (tok >= a.T) return;
+// One choice after another in 32 registers, so that an SM is full of warps: the
+// loads of other warps stand in for those of other choices.  With KC rows in
+// flight a thread, as in collect, this took 60 us against 57 (8,191 tokens of 8 x
+// 2,048) and 162 against 150 (32,768 of 4 x 2,560).
+template <typename T, int V>
+__global__ void __launch_bounds__(512, 4) combine_kernel(const Args a) {
+  const Place pl = place(a);
+  if (!pl.live) return;
   const int packs = a.H / V;
-  const int32_t* slot = a.slots + tok * a.K;
-  for (int p = t; p < packs; p += a.group) {
+  const int32_t* slot = a.slots + pl.tok * a.K;
+  for (int p = pl.t; p < packs; p += a.group) {
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     for (int k = 0; k < a.K; ++k) {
       const int64_t r = __ldg(slot + k);
       if (r < 0) continue;
-      const float w = kWeighted ? weight_of(a.w, a.w_dtype, tok * a.K + k) : 1.f;
+      const float w = weight_of(a, pl, k);
       float v[V];
       vec::load<T, V>(reinterpret_cast<const T*>(a.src) + r * a.H + p * V, v);
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+      vec::axpy<V>(w, v, acc);
     }
-    vec::store<T, V>(reinterpret_cast<T*>(a.dst) + tok * a.H + p * V, acc);
+    vec::store<T, V>(reinterpret_cast<T*>(a.dst) + pl.tok * a.H + p * V, acc);
   }
 }
 
-constexpr int kDots = 8;     // dw terms summed at a time
-
-template <typename T, int V>
-__global__ void __launch_bounds__(256) spread_kernel(const Args a) {
-  __shared__ float red[8][kDots];
-  const int t = threadIdx.x % a.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t tok = (int64_t)blockIdx.x * (blockDim.x / a.group) + threadIdx.x / a.group;
-  const bool live = tok < a.T;
+template <typename T, int V, int KC>
+__global__ void __launch_bounds__(512, 2) collect_kernel(const Args a) {
+  const Place pl = place(a);
+  if (!pl.live) return;
   const int packs = a.H / V;
-  const int32_t* slot = a.slots + (live ? tok : 0) * a.K;
-  for (int k0 = 0; k0 < a.K; k0 += kDots) {
-    const int nk = min(kDots, a.K - k0);
-    float dot[kDots];
+  const T* src = reinterpret_cast<const T*>(a.src);
+  int r[KC];
+  slots_of<KC>(a, pl.tok, 0, r);
+  for (int p = pl.t; p < packs; p += a.group) {
+    float acc[V];
 #pragma unroll
-    for (int k = 0; k < kDots; ++k) dot[k] = 0.f;
-    if (live) {
-      for (int p = t; p < packs; p += a.group) {
-        float g[V];
-        vec::load<T, V>(reinterpret_cast<const T*>(a.src) + tok * a.H + p * V, g);
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int k0 = 0; k0 < a.K; k0 += KC) {
+      if (a.K > KC) slots_of<KC>(a, pl.tok, k0, r);
+      vec::Raw<T, V> raw[KC];
 #pragma unroll
-        for (int k = 0; k < kDots; ++k) {
-          if (k >= nk) continue;
-          const int64_t r = __ldg(slot + k0 + k);
-          if (r < 0) continue;
-          const float w = weight_of(a.w, a.w_dtype, tok * a.K + k0 + k);
-          float v[V], o[V];
-          vec::load<T, V>(reinterpret_cast<const T*>(a.ys) + r * a.H + p * V, v);
+      for (int k = 0; k < KC; ++k)
+        if (r[k] >= 0) raw[k] = vec::load_raw<T, V>(src + (int64_t)r[k] * a.H + p * V);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            dot[k] = fmaf(g[i], v[i], dot[k]);
-            o[i] = w * g[i];
+      for (int k = 0; k < KC; ++k) {
+        if (r[k] < 0) continue;
+        float v[V];
+        vec::unpack<T, V>(raw[k], v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += v[i];
+      }
+    }
+    vec::store<T, V>(reinterpret_cast<T*>(a.dst) + pl.tok * a.H + p * V, acc);
+  }
+}
+
+template <typename T, int V, int KC>
+__global__ void __launch_bounds__(512, 2) spread_kernel(const Args a) {
+  __shared__ float red[16][KC];
+  __shared__ float sw[kMaxTokens * kMaxK];
+  const Place pl = place(a);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = a.group >> 5;
+  const int packs = a.H / V;
+  const int64_t tok = pl.live ? pl.tok : 0;
+  const float* w = sw + pl.slot * a.K;
+  if (pl.t < a.K) sw[pl.slot * a.K + pl.t] = weight_of(a, pl, pl.t);
+  if (pl.t + a.group < a.K)
+    sw[pl.slot * a.K + pl.t + a.group] = weight_of(a, pl, pl.t + a.group);
+  int r[KC];
+  slots_of<KC>(a, tok, 0, r);
+  __syncthreads();
+  for (int k0 = 0; k0 < a.K; k0 += KC) {
+    float dot[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) dot[k] = 0.f;
+    if (pl.live) {
+      if (k0) slots_of<KC>(a, tok, k0, r);
+      for (int p = pl.t; p < packs; p += a.group) {
+        constexpr int B = KC < 4 ? KC : 4;         // of them in flight
+        const vec::Raw<T, V> raw_g =
+            vec::load_raw<T, V>(reinterpret_cast<const T*>(a.src) + tok * a.H + p * V);
+#pragma unroll
+        for (int b = 0; b < KC; b += B) {
+          vec::Raw<T, V> raw[B];
+#pragma unroll
+          for (int k = 0; k < B; ++k)
+            if (r[b + k] >= 0)
+              raw[k] = vec::load_raw<T, V>(reinterpret_cast<const T*>(a.ys) +
+                                           (int64_t)r[b + k] * a.H + p * V);
+          float g[V];
+          vec::unpack<T, V>(raw_g, g);
+#pragma unroll
+          for (int k = 0; k < B; ++k) {
+            if (r[b + k] < 0) continue;
+            const float wk = w[k0 + b + k];
+            float v[V], o[V];
+            vec::unpack<T, V>(raw[k], v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              dot[b + k] = fmaf(g[i], v[i], dot[b + k]);
+              o[i] = wk * g[i];
+            }
+            vec::store<T, V>(reinterpret_cast<T*>(a.dst) + (int64_t)r[b + k] * a.H + p * V, o);
           }
-          vec::store<T, V>(reinterpret_cast<T*>(a.dst) + r * a.H + p * V, o);
         }
       }
     }
 #pragma unroll
-    for (int k = 0; k < kDots; ++k)
+    for (int k = 0; k < KC; ++k)
       for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
-    __syncthreads();
+    if (k0) __syncthreads();            // the sums before have been read
     if (lane == 0) {
 #pragma unroll
-      for (int k = 0; k < kDots; ++k) red[warp][k] = dot[k];
+      for (int k = 0; k < KC; ++k) red[warp][k] = dot[k];
     }
     __syncthreads();
-    if (live && t < nk) {
-      const int nw = a.group >> 5;
+    if (pl.live && pl.t < min(KC, a.K - k0)) {
       float s = 0.f;
-      for (int q = 0; q < nw; ++q) s += red[warp + q][t];
-      const int64_t i = tok * a.K + k0 + t;
+      for (int q = 0; q < nw; ++q) s += red[warp + q][pl.t];
+      const int64_t i = tok * a.K + k0 + pl.t;
       switch (a.w_dtype) {
         case TT_F32: reinterpret_cast<float*>(a.dw)[i] = s; break;
         case TT_BF16: reinterpret_cast<__nv_bfloat16*>(a.dw)[i] = from_f32<__nv_bfloat16>(s); break;
@@ -288,27 +447,37 @@ __global__ void __launch_bounds__(256) spread_kernel(const Args a) {
 
 enum Op { kDispatch, kCollect, kCombine, kSpread };
 
-template <typename T, int V>
+template <typename T, int V, int KC>
 int launch(Op op, Args& a, cudaStream_t st) {
-  // a group of whole warps, 8 warps a block: as many as the row has packs for
+  // a group of whole warps for a token, up to 512 threads, that its packs fill as
+  // evenly as they can; short rows share a block of about 256
   const int packs = a.H / V;
-  a.group = 32;
-  while (a.group < 256 && a.group < packs) a.group *= 2;
-  const int per = 256 / a.group;
+  const int turns = (packs + 511) / 512;
+  a.group = ((packs + turns - 1) / turns + 31) / 32 * 32;
+  const int per = std::max(1, 256 / a.group), threads = a.group * per;
   const int64_t blocks = (a.T + per - 1) / per;
   if (blocks > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)blocks;
   switch (op) {
-    case kDispatch: dispatch_kernel<T, V><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    case kCollect: combine_kernel<T, V, false><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    case kCombine: combine_kernel<T, V, true><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    case kSpread: spread_kernel<T, V><<<(unsigned)blocks, 256, 0, st>>>(a); break;
+    case kDispatch: dispatch_kernel<T, V, KC><<<grid, threads, 0, st>>>(a); break;
+    case kCollect: collect_kernel<T, V, KC><<<grid, threads, 0, st>>>(a); break;
+    case kCombine: combine_kernel<T, V><<<grid, threads, 0, st>>>(a); break;
+    case kSpread: spread_kernel<T, V, KC><<<grid, threads, 0, st>>>(a); break;
   }
   tt_count_launches(1);
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
+template <typename T, int V>
+int launch_k(Op op, Args& a, cudaStream_t st) {
+  a.by_four = a.K % 4 == 0 && reinterpret_cast<uintptr_t>(a.slots) % 16 == 0;
+  if (a.K <= 2) return launch<T, V, 2>(op, a, st);
+  if (a.K <= 4) return launch<T, V, 4>(op, a, st);
+  return launch<T, V, 8>(op, a, st);
+}
+
 int run(Op op, int dtype, Args& a, void* stream) {
-  if (a.T < 0 || a.K < 0 || a.H <= 0 || a.E <= 0 || a.T * a.K > 0x7fffffff)
+  if (a.T < 0 || a.K < 0 || a.K > kMaxK || a.H <= 0 || a.E <= 0 || a.T * a.K > 0x7fffffff)
     return TT_ERR_INVALID_ARG;
   if (a.T == 0) return TT_OK;
   // with K = 0 there are no sorted rows: the side of them may be null
@@ -322,13 +491,9 @@ int run(Op op, int dtype, Args& a, void* stream) {
     constexpr int V = 16 / (int)sizeof(T);
     auto ok = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     if (a.H % V == 0 && ok(a.src) && ok(a.dst) && ok(a.ys))
-      return launch<T, V>(op, a, (cudaStream_t)stream);
-    return launch<T, 1>(op, a, (cudaStream_t)stream);
+      return launch_k<T, V>(op, a, (cudaStream_t)stream);
+    return launch_k<T, 1>(op, a, (cudaStream_t)stream);
   });
-}
-
-int plan_blocks(int64_t n) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>((n + kChunk - 1) / kChunk, vec::kSMs));
 }
 
 }  // namespace
@@ -337,7 +502,8 @@ int plan_blocks(int64_t n) {
 
 extern "C" int64_t tt_moe_plan_workspace_size(int64_t n_entries, int32_t n_experts) {
   if (n_entries < 0 || n_experts <= 0 || n_experts > tt::moe::kMaxExperts) return -1;
-  return (int64_t)tt::moe::plan_blocks(n_entries) * (n_experts + 1) * 4;
+  const int blocks = tt::moe::plan_blocks(n_entries, n_experts);
+  return blocks > 1 ? (int64_t)blocks * (n_experts + 1) * 4 : 0;
 }
 
 extern "C" int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_t n_experts,
@@ -347,22 +513,22 @@ extern "C" int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_
   if (n_entries < 0 || n_entries > 0x7fffffff || n_experts <= 0 || n_experts > kMaxExperts ||
       !offsets || (n_entries > 0 && (!ids || !slots || !entries)))
     return TT_ERR_INVALID_ARG;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int blocks = plan_blocks(n_entries);
-  // a warp's share is a whole number of 32-entry steps
-  const int64_t step = 32 * kPlanWarps;
-  const int64_t chunk = std::max<int64_t>(
-      step, ((n_entries + blocks - 1) / blocks + step - 1) / step * step);
-  const int E = n_experts;
+  const int E = n_experts, blocks = plan_blocks(n_entries, E);
   if (blocks > 1 && (!workspace || workspace_bytes < tt_moe_plan_workspace_size(n_entries, E)))
     return TT_ERR_WORKSPACE;
-  int* counts = blocks > 1 ? (int*)workspace : nullptr;
-  if (counts)
-    plan_count<<<blocks, 32 * kPlanWarps, sizeof(int) * kPlanWarps * (E + 1), st>>>(
-        ids, ids64, n_entries, chunk, E, counts);
-  plan_place<<<blocks, 32 * kPlanWarps, sizeof(int) * (kPlanWarps + 2) * (E + 1), st>>>(
-      ids, ids64, n_entries, chunk, E, counts, slots, entries, offsets);
-  tt_count_launches(counts ? 2 : 1);
+  const int64_t warps = (int64_t)blocks * kPlanWarps;
+  const int64_t run = std::max<int64_t>(32, ((n_entries + warps - 1) / warps + 31) / 32 * 32);
+  const PlanArgs a{ids, ids64, n_entries, run, E, slots, entries, offsets, (int32_t*)workspace};
+  cudaStream_t st = (cudaStream_t)stream;
+  const int threads = 32 * kPlanWarps;
+  const size_t smem = sizeof(int) * kPlanWarps * (E + 1);
+  if (blocks == 1) {
+    plan_rank<true><<<1, threads, smem, st>>>(a);
+  } else {
+    plan_rank<false><<<blocks, threads, smem, st>>>(a);
+    plan_place<<<blocks, threads, sizeof(int) * 2 * (E + 1), st>>>(a);
+  }
+  tt_count_launches(blocks > 1 ? 2 : 1);
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 

@@ -95,6 +95,32 @@ __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   *reinterpret_cast<Raw<T, V>*>(p) = pack<T, V>(v);
 }
 
+// a * b + c on two fp32 values in one instruction (subnormals kept).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+// acc += w v over V elements
+template <int V>
+__device__ __forceinline__ void axpy(float w, const float (&v)[V], float (&acc)[V]) {
+  if constexpr (V == 1) {
+    acc[0] = fmaf(w, v[0], acc[0]);
+  } else {
+    const float2 w2 = make_float2(w, w);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = fma2(w2, make_float2(v[i], v[i + 1]), make_float2(acc[i], acc[i + 1]));
+      acc[i] = r.x, acc[i + 1] = r.y;
+    }
+  }
+}
+
 // Calls f with a value of the C++ type of a TT_* floating dtype.
 template <typename F>
 int dispatch_float(int dtype, F f) {

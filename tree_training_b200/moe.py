@@ -16,6 +16,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, _ops
 
 MAX_EXPERTS = 1024
+MAX_CHOICES = 64
 
 
 class ExpertPlan:
@@ -38,7 +39,7 @@ class ExpertPlan:
 def expert_plan(expert_ids: torch.Tensor, n_experts: int) -> ExpertPlan:
     """Sorts the choices ``expert_ids`` [T, k] (int64/int32) by expert, each
     expert's in token order.  An id outside [0, n_experts) drops the choice.
-    n_experts <= 1024.  CUDA tensors only (no CPU path)."""
+    k <= 64, n_experts <= 1024.  CUDA tensors only (no CPU path)."""
     dev = _ops.check_cuda("expert_plan", expert_ids=expert_ids)
     if expert_ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("expert_plan: int64/int32 expert ids required")
@@ -48,6 +49,8 @@ def expert_plan(expert_ids: torch.Tensor, n_experts: int) -> ExpertPlan:
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"expert_plan: n_experts must be in [1, {MAX_EXPERTS}]")
     T, k = expert_ids.shape
+    if k > MAX_CHOICES:
+        raise ValueError(f"expert_plan: at most {MAX_CHOICES} choices a token")
     n = T * k
     if n > 0x7fffffff:
         raise ValueError("expert_plan: more than 2^31 - 1 choices")
