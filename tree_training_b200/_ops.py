@@ -3,26 +3,42 @@ device, and a call of the library with that device current."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 DTYPES = {torch.float32: _lib.TT_F32, torch.bfloat16: _lib.TT_BF16, torch.float16: _lib.TT_F16}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def stream_ptr(device: torch.device) -> int:
-    return _raw_stream(device.index)
+_current = torch._C._cuda_getDevice
+_functions: dict = {}
 
 
 def call(device: torch.device, name: str, *args) -> None:
     """Calls the library on ``device``'s current stream (appended as the last
     argument); another current device is switched for the call."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _raw_stream(device.index))
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(_lib.lib(), name)
+    i = device.index
+    if i == _current():
+        rc = f(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, _raw_stream(device.index))
+            rc = f(*args, _raw_stream(i))
+    if rc:
+        raise _lib.TTError(name, rc)
+
+
+def once(backward):
+    """A backward whose results carry no graph: differentiating them again is an
+    error, as with ``once_differentiable``, whose cost only calls under
+    ``create_graph`` pay here."""
+    strict = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def check_cuda(op: str, **tensors) -> torch.device:
@@ -43,7 +59,11 @@ def check_cuda(op: str, **tensors) -> torch.device:
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def rows2d(t: torch.Tensor) -> torch.Tensor:

@@ -16,7 +16,6 @@ from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ops
 from .packer import preorder_arrays
@@ -38,11 +37,12 @@ def _forward(x, tokens, k, temperature, keep):
     T, V = x.shape
     M = tokens.shape[1]
     dev = x.device
-    logp = torch.empty((T, M), dtype=torch.float32, device=dev)
-    ent = torch.empty(T, dtype=torch.float32, device=dev)
-    top_lp = torch.empty((T, k), dtype=torch.float32, device=dev)
-    top_tok = torch.empty((T, k), dtype=torch.int64, device=dev)
-    stats = torch.empty((T, 4), dtype=torch.float32, device=dev) if keep else None
+    f32 = torch.float32
+    logp = x.new_empty((T, M), dtype=f32)
+    ent = x.new_empty(T, dtype=f32)
+    top_lp = x.new_empty((T, k), dtype=f32)
+    top_tok = tokens.new_empty((T, k))
+    stats = x.new_empty((T, 4), dtype=f32) if keep else None
     _ops.call(dev, "tt_token_logprobs_fwd", _ops.DTYPES[x.dtype], T, V, x.data_ptr(),
               max(x.stride(0), V), tokens.data_ptr(), M, temperature, k, logp.data_ptr(),
               ent.data_ptr(), top_lp.data_ptr(), top_tok.data_ptr(),
@@ -61,14 +61,14 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, ent, top_lp, top_tok
 
     @staticmethod
-    @once_differentiable
+    @_ops.once
     def backward(ctx, g_logp, g_ent, g_top, _):
         x, tokens, top_tok, stats = ctx.saved_tensors
         if g_logp is None and g_ent is None and g_top is None:
             return None, None, None, None
         T, V = x.shape
         g = [None if t is None else t.float().contiguous() for t in (g_logp, g_ent, g_top)]
-        dx = torch.empty((T, V), dtype=x.dtype, device=x.device)
+        dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty((T, V))
         _ops.call(x.device, "tt_token_logprobs_bwd", _ops.DTYPES[x.dtype], T, V, x.data_ptr(),
                   max(x.stride(0), V), tokens.data_ptr(), tokens.shape[1], ctx.temperature,
                   top_tok.shape[1], top_tok.data_ptr(),

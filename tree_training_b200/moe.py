@@ -11,7 +11,6 @@ Every sum runs in a fixed order in fp32 (no atomics).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _ops
 
@@ -55,9 +54,9 @@ def expert_plan(expert_ids: torch.Tensor, n_experts: int) -> ExpertPlan:
     if n > 0x7fffffff:
         raise ValueError("expert_plan: more than 2^31 - 1 choices")
     ids = expert_ids.contiguous()
-    ws = int(_lib.lib().tt_moe_plan_workspace_size(n, E))
+    ws = _lib.lib().tt_moe_plan_workspace_size(n, E)
     # one array for what a call writes; slots, entries, offsets, workspace
-    buf = torch.empty(2 * n + E + 1 + ws // 4, dtype=torch.int32, device=dev)
+    buf = ids.new_empty(2 * n + E + 1 + ws // 4, dtype=torch.int32)
     slots, entries = buf[:n].view(T, k), buf[n:2 * n]
     offsets = buf[2 * n:2 * n + E + 1]
     p = buf.data_ptr()
@@ -67,7 +66,7 @@ def expert_plan(expert_ids: torch.Tensor, n_experts: int) -> ExpertPlan:
 
 
 def _rows_op(name, src, plan, rows, *more):
-    out = torch.empty((rows, src.shape[1]), dtype=src.dtype, device=src.device)
+    out = src.new_empty((rows, src.shape[1]))
     _ops.call(src.device, name, _ops.DTYPES[src.dtype], *more[:1], plan.n_tokens, plan.k,
               src.shape[1], plan.n_experts, plan.slots.data_ptr(), plan.offsets.data_ptr(),
               src.data_ptr(), *more[1:], out.data_ptr())
@@ -81,7 +80,7 @@ class _Dispatch(torch.autograd.Function):
         return _rows_op("tt_moe_dispatch", x, plan, plan.n_tokens * plan.k)
 
     @staticmethod
-    @once_differentiable
+    @_ops.once
     def backward(ctx, dxs):
         return _rows_op("tt_moe_collect", dxs.contiguous(), ctx.plan, ctx.plan.n_tokens), None
 
@@ -95,7 +94,7 @@ class _Combine(torch.autograd.Function):
                         weights.data_ptr())
 
     @staticmethod
-    @once_differentiable
+    @_ops.once
     def backward(ctx, dy):
         ys, weights = ctx.saved_tensors
         plan = ctx.plan

@@ -8,7 +8,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _ops
 from .attention import _status_word
@@ -21,12 +20,20 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _new(x, dtype):
+    """A contiguous array of x's shape (``empty_like`` keeps an x that is dense in
+    another order as it is)."""
+    if dtype == x.dtype and x.is_contiguous():
+        return torch.empty_like(x)
+    return x.new_empty(x.shape, dtype=dtype)
+
+
 def _forward(x, res, w, post, gate, mode, scale, eps, offset, keep):
     T, D = x.shape
     rt = x.dtype if res is None else res.dtype
-    y = torch.empty((T, D), dtype=x.dtype, device=x.device)
-    r = torch.empty((T, D), dtype=rt, device=x.device)
-    stats = torch.empty((T, 2), dtype=torch.float32, device=x.device) if keep else None
+    y = _new(x, x.dtype)
+    r = _new(x, rt)
+    stats = x.new_empty((T, 2), dtype=torch.float32) if keep else None
     _ops.call(x.device, "tt_residual_norm_fwd", _ops.DTYPES[x.dtype], _ops.DTYPES[rt], T, D,
               x.data_ptr(), x.stride(0), _ptr(res), 0 if res is None else res.stride(0),
               w.data_ptr(), _ptr(post), w.dtype == torch.float32, offset, _ptr(gate),
@@ -45,7 +52,7 @@ class _ResidualNorm(torch.autograd.Function):
         return y, r
 
     @staticmethod
-    @once_differentiable
+    @_ops.once
     def backward(ctx, dy, dr):
         x, res, w, post, gate, stats = ctx.saved_tensors
         mode, scale, offset = ctx.args
@@ -56,16 +63,18 @@ class _ResidualNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         # the same array where nothing stands between the two
         same = post is None and mode == _NONE and scale == 1.0 and rt == x.dtype
-        new = torch.empty if T else torch.zeros
-        dres = new((T, D), dtype=rt, device=dev) if need[1] or (same and need[0]) else None
-        dx = new((T, D), dtype=x.dtype, device=dev) if need[0] and not same else None
-        dw = new(D, dtype=w.dtype, device=dev) if need[2] else None
-        dpost = new(D, dtype=w.dtype, device=dev) if need[3] else None
-        dgate = new(gate.shape, dtype=gate.dtype, device=dev) if need[4] else None
+        new = torch.empty_like if T else torch.zeros_like
+        dres = _new(x, rt) if need[1] or (same and need[0]) else None
+        dx = _new(x, x.dtype) if need[0] and not same else None
+        dw = new(w) if need[2] else None
+        dpost = new(post) if need[3] else None
+        dgate = None
+        if need[4]:
+            dgate = new(gate) if mode == _CHANNEL else gate.new_empty(gate.shape)
         dy = None if dy is None else _ops.rows2d(dy)
         dr = None if dr is None else _ops.rows2d(dr)
-        blocks = int(_lib.lib().tt_residual_norm_bwd_blocks(T, D))
-        part = torch.empty((3, blocks, D), dtype=torch.float32, device=dev)
+        blocks = _lib.lib().tt_residual_norm_bwd_blocks(T, D)
+        part = x.new_empty(3 * blocks * D, dtype=torch.float32)
         _ops.call(dev, "tt_residual_norm_bwd", _ops.DTYPES[x.dtype], _ops.DTYPES[rt], T, D,
                   x.data_ptr(), x.stride(0), _ptr(res), 0 if res is None else res.stride(0),
                   w.data_ptr(), _ptr(post), w.dtype == torch.float32, offset, _ptr(gate),

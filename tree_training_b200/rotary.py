@@ -12,7 +12,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ops
 from .attention import _status_word
@@ -102,10 +101,10 @@ def _turn(q, k, pos, table, interleaved: bool, inverse: bool):
     hk = 0 if k is None else k.shape[1]
     dev = q.device
     q = q if q.stride(2) == 1 else q.contiguous()
-    qo = torch.empty((n, hq, D), dtype=q.dtype, device=dev)
+    qo = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, hq, D))
     if k is not None:
         k = k if k.stride(2) == 1 else k.contiguous()
-        ko = torch.empty((n, hk, D), dtype=q.dtype, device=dev)
+        ko = torch.empty_like(k) if k.is_contiguous() else k.new_empty((n, hk, D))
     else:
         ko = None
     _ops.call(dev, "tt_rotary", _ops.DTYPES[q.dtype], n, hq, hk, D, table.shape[1], interleaved,
@@ -125,7 +124,7 @@ class _Rotary(torch.autograd.Function):
         return (qo, ko) if k is not None else qo
 
     @staticmethod
-    @once_differentiable
+    @_ops.once
     def backward(ctx, dq, dk=None):
         pos, table = ctx.saved_tensors
         gq, gk = _turn(dq, dk if ctx.has_k else None, pos, table, ctx.interleaved, True)
