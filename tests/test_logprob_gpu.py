@@ -286,3 +286,21 @@ def test_refusals():
             f(*a, **kw)
     with pytest.raises(ValueError):
         f(torch.zeros(2, 100, device=DEV), None, top_k=65)
+
+
+def test_differentiating_twice_is_refused():
+    x, tok = logits(4, 30, F32)
+    x.requires_grad_(True)
+    g, = torch.autograd.grad(tt.token_logprobs(x, tok).entropy.sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [x])
+
+
+def test_logits_changed_in_place_are_noticed():
+    x, tok = logits(4, 30, F32)
+    x.requires_grad_(True)
+    y = x * 1.0
+    r = tt.token_logprobs(y, tok)
+    y.detach().mul_(2.0)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(r.entropy.sum(), [x])

@@ -208,3 +208,20 @@ def test_refusals():
               lambda: tt.expert_combine(ys, w[:, :1], plan)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_differentiating_twice_is_refused():
+    plan = tt.expert_plan(torch.zeros(4, 2, dtype=torch.int64, device=DEV), 2)
+    ys = torch.randn(8, 16, device=DEV, requires_grad=True)
+    w = torch.rand(4, 2, device=DEV)
+    g, = torch.autograd.grad(tt.expert_combine(ys, w, plan).sum(), [ys], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [ys])
+
+
+def test_leaf_gradients_add_up():
+    plan = tt.expert_plan(torch.tensor([[0], [1], [0]], device=DEV), 2)
+    x = torch.randn(3, 8, device=DEV, requires_grad=True)
+    for _ in range(2):
+        tt.expert_dispatch(x, plan).sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2.0))

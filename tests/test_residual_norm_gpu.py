@@ -251,3 +251,12 @@ def test_refusals():
     big = torch.zeros(1, 16385, device=DEV)
     with pytest.raises(ValueError):
         ok(big, None, big[0])
+
+
+def test_differentiating_twice_is_refused():
+    v, dy, dr = data(6, 64, F32, F32, False, "none")
+    x = v["x"].requires_grad_(True)
+    y, r = op(v)
+    gs = torch.autograd.grad([y, r], [x], [dy, dr], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gs[0].sum(), [x])

@@ -157,3 +157,11 @@ def test_refusals():
               (q, k, pos, table[:, :7]), (q, k, pos, tt.rotary_table(9, 18, device=DEV))):
         with pytest.raises(ValueError):
             tt.apply_rotary(*a)
+
+
+def test_differentiating_twice_is_refused():
+    q, k, pos, table = data(5, 2, 1, 16, 8, torch.float32)
+    q.requires_grad_(True)
+    g, = torch.autograd.grad(tt.apply_rotary(q, k, pos, table)[0].sum(), [q], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [q])

@@ -8,6 +8,9 @@ arch=compute_100a,code=sm_100a``); the CUDA runtime is linked statically so the
 library does not depend on which libcudart torch happens to load.  Objects go
 to ``_build/`` (git-ignored); the .so lands next to this file so that it
 travels with the repository snapshot.
+
+``csrc/torch/tt_torch.cpp``, the torch bindings of the layer operators, becomes
+the Python module ``_tt_torch.so`` beside it, linked to the library.
 """
 from __future__ import annotations
 
@@ -23,6 +26,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libtt_sm100.so")
+TORCH_SRC = os.path.join(CSRC, "torch", "tt_torch.cpp")
+TORCH_EXT = os.path.join(PKG, "_tt_torch.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -88,7 +93,39 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr[-6000:]}")
         os.replace(tmp, LIB)
+    build_torch_ext(force, verbose)
     return LIB
+
+
+def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the torch bindings if their source, the C ABI's header or torch
+    is newer than they are."""
+    import sysconfig
+
+    import torch
+    home = os.path.dirname(torch.__file__)
+    header = os.path.join(ROOT, "include", "tree_training_b200.h")
+    newest = max(os.path.getmtime(f) for f in (TORCH_SRC, header, torch.version.__file__))
+    if not force and os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= newest:
+        return TORCH_EXT
+    inc = [os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"),
+           os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"),
+           sysconfig.get_paths()["include"]]
+    tmp = TORCH_EXT + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for d in inc:
+        cmd += ["-isystem", d]
+    cmd += [TORCH_SRC, "-o", tmp, f"-L{PKG}", "-l:libtt_sm100.so", "-Wl,-rpath,$ORIGIN",
+            f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {TORCH_SRC}\n{r.stderr[-6000:]}")
+    os.replace(tmp, TORCH_EXT)
+    if verbose:
+        print("compiled tt_torch.cpp", file=sys.stderr)
+    return TORCH_EXT
 
 
 def main():

@@ -33,50 +33,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor
 
 
-def _forward(x, tokens, k, temperature, keep):
-    T, V = x.shape
-    M = tokens.shape[1]
-    dev = x.device
-    f32 = torch.float32
-    logp = x.new_empty((T, M), dtype=f32)
-    ent = x.new_empty(T, dtype=f32)
-    top_lp = x.new_empty((T, k), dtype=f32)
-    top_tok = tokens.new_empty((T, k))
-    stats = x.new_empty((T, 4), dtype=f32) if keep else None
-    _ops.call(dev, "tt_token_logprobs_fwd", _ops.DTYPES[x.dtype], T, V, x.data_ptr(),
-              max(x.stride(0), V), tokens.data_ptr(), M, temperature, k, logp.data_ptr(),
-              ent.data_ptr(), top_lp.data_ptr(), top_tok.data_ptr(),
-              stats.data_ptr() if keep else None)
-    return logp, ent, top_lp, top_tok, stats
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, tokens, k: int, temperature: float):
-        logp, ent, top_lp, top_tok, stats = _forward(x, tokens, k, temperature, True)
-        ctx.save_for_backward(x, tokens, top_tok, stats)
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_tok)
-        return logp, ent, top_lp, top_tok
-
-    @staticmethod
-    @_ops.once
-    def backward(ctx, g_logp, g_ent, g_top, _):
-        x, tokens, top_tok, stats = ctx.saved_tensors
-        if g_logp is None and g_ent is None and g_top is None:
-            return None, None, None, None
-        T, V = x.shape
-        g = [None if t is None else t.float().contiguous() for t in (g_logp, g_ent, g_top)]
-        dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty((T, V))
-        _ops.call(x.device, "tt_token_logprobs_bwd", _ops.DTYPES[x.dtype], T, V, x.data_ptr(),
-                  max(x.stride(0), V), tokens.data_ptr(), tokens.shape[1], ctx.temperature,
-                  top_tok.shape[1], top_tok.data_ptr(),
-                  *(None if t is None else t.data_ptr() for t in g), stats.data_ptr(),
-                  dx.data_ptr())
-        return dx, None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """Log probabilities under softmax(logits / temperature).
@@ -90,34 +46,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 
     Differentiable in ``logits`` through logprobs, entropy and top_logprobs.
     CUDA tensors only (no CPU path)."""
-    dev = _ops.check_cuda("token_logprobs", logits=logits, tokens=tokens)
-    if logits.dtype not in _ops.DTYPES:
-        raise TypeError("token_logprobs: float32/bfloat16/float16 logits required")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError("token_logprobs: logits must be [rows, V]")
-    T, V = logits.shape
-    k, temperature = int(top_k), float(temperature)
-    if not 0 <= k <= min(MAX_TOP_K, V):
-        raise ValueError(f"token_logprobs: top_k must be in [0, {min(MAX_TOP_K, V)}]")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError("token_logprobs: temperature must be positive and finite")
-    if tokens is None:
-        tok = torch.empty((T, 0), dtype=torch.int64, device=dev)
-    else:
-        if tokens.dtype not in (torch.int64, torch.int32):
-            raise TypeError("token_logprobs: int64/int32 tokens required")
-        if tokens.dim() not in (1, 2) or tokens.shape[0] != T:
-            raise ValueError("token_logprobs: tokens must be [rows] or [rows, M]")
-        tok = tokens if tokens.dim() == 2 else tokens[:, None]
-        tok = tok.to(torch.int64).contiguous()
-    x = _ops.rows2d(logits)
-    if _ops.wants_grad(logits):
-        logp, ent, top_lp, top_tok = _TokenLogprobs.apply(x, tok, k, temperature)
-    else:
-        logp, ent, top_lp, top_tok, _ = _forward(x, tok, k, temperature, False)
-    if tokens is not None and tokens.dim() == 1:
-        logp = logp[:, 0]
-    return TokenLogprobs(logp, ent, top_lp, top_tok)
+    return TokenLogprobs(*_ops.ext().token_logprobs(logits, tokens, int(top_k),
+                                                    float(temperature), MAX_TOP_K))
 
 
 def tree_next_tokens(roots: Sequence, ignore: int = IGNORE) -> np.ndarray:

@@ -14,7 +14,6 @@ from typing import Optional, Tuple
 import torch
 
 from . import _ops
-from .attention import _status_word
 
 _SCALINGS = ("default", "linear", "dynamic", "yarn", "llama3", "longrope")
 
@@ -96,41 +95,6 @@ def rotary_table(n_positions: int, dim: int, theta: float = 10000.0,
     return torch.cat([ang.cos() * amp, ang.sin() * amp], 1).float()
 
 
-def _turn(q, k, pos, table, interleaved: bool, inverse: bool):
-    n, hq, D = q.shape
-    hk = 0 if k is None else k.shape[1]
-    dev = q.device
-    q = q if q.stride(2) == 1 else q.contiguous()
-    qo = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, hq, D))
-    if k is not None:
-        k = k if k.stride(2) == 1 else k.contiguous()
-        ko = torch.empty_like(k) if k.is_contiguous() else k.new_empty((n, hk, D))
-    else:
-        ko = None
-    _ops.call(dev, "tt_rotary", _ops.DTYPES[q.dtype], n, hq, hk, D, table.shape[1], interleaved,
-              inverse, q.data_ptr(), q.stride(0), q.stride(1),
-              k.data_ptr() if hk else None, k.stride(0) if hk else 0, k.stride(1) if hk else 0,
-              pos.data_ptr(), pos.dtype == torch.int64, table.data_ptr(), table.shape[0],
-              qo.data_ptr(), ko.data_ptr() if hk else None, _status_word(dev).data_ptr())
-    return qo, ko
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos, table, interleaved: bool):
-        ctx.save_for_backward(pos, table)
-        ctx.interleaved, ctx.has_k = interleaved, k is not None
-        qo, ko = _turn(q, k, pos, table, interleaved, False)
-        return (qo, ko) if k is not None else qo
-
-    @staticmethod
-    @_ops.once
-    def backward(ctx, dq, dk=None):
-        pos, table = ctx.saved_tensors
-        gq, gk = _turn(dq, dk if ctx.has_k else None, pos, table, ctx.interleaved, True)
-        return gq, gk, None, None, None
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  table: torch.Tensor, interleaved: bool = False
                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -144,25 +108,4 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     A position outside the table gives NaN in the turned dims and an error at
     the next ``check_device_status``.  Differentiable in q and k.  CUDA tensors
     only (no CPU path)."""
-    _ops.check_cuda("apply_rotary", q=q, k=k, positions=positions, table=table)
-    if q.dtype not in _ops.DTYPES or (k is not None and k.dtype != q.dtype):
-        raise TypeError("apply_rotary: q and k must share one of float32/bfloat16/float16")
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0]
-                                           or k.shape[2] != q.shape[2])):
-        raise ValueError("apply_rotary: q [N, Hq, D] and k [N, Hk, D] required")
-    if table.dtype != torch.float32 or table.dim() != 2:
-        raise TypeError("apply_rotary: table must be float32 [positions, R] (see rotary_table)")
-    if positions.dtype not in (torch.int64, torch.int32):
-        raise TypeError("apply_rotary: int64/int32 positions required")
-    if positions.dim() != 1 or positions.shape[0] != q.shape[0]:
-        raise ValueError("apply_rotary: positions must be [N]")
-    R = table.shape[1]
-    if R < 2 or R % 2 or R > q.shape[2]:
-        raise ValueError("apply_rotary: the table's width must be even and at most the head dim")
-    if q.shape[1] < 1:
-        raise ValueError("apply_rotary: q has no heads")
-    pos, table = positions.contiguous(), table.contiguous()
-    if _ops.wants_grad(q, k):
-        out = _Rotary.apply(q, k, pos, table, bool(interleaved))
-        return out if k is not None else (out, None)
-    return _turn(q, k, pos, table, bool(interleaved), False)
+    return _ops.ext().apply_rotary(q, k, positions, table, bool(interleaved))
