@@ -110,7 +110,7 @@ def logits(T, V, dtype, seed=0, scale=2.5):
     (1, 1, F32, 1, 1.0), (3, 2, BF, 2, 1.0), (47, 32000, F32, 8, 1.0), (5, 100, F16, 64, 0.7),
     (33, 1000, BF, 5, 1.0), (17, 1001, BF, 5, 1.3), (9, 4099, F16, 20, 1.0),
     (6, 151936, BF, 16, 1.0), (3, 151936, F32, 64, 0.5), (2, 151937, F16, 1, 1.0),
-    (700, 257, BF, 3, 1.0), (1, 50000, BF, 10, 1.0), (2, 300000, BF, 7, 1.0),
+    (700, 257, BF, 3, 1.0), (900, 4097, BF, 64, 1.0), (500, 2050, F32, 33, 1.0), (40, 4104, F16, 64, 1.0), (1, 50000, BF, 10, 1.0), (2, 300000, BF, 7, 1.0),
     (300, 8192, BF, 4, 1.0), (64, 7, F32, 7, 2.0), (1500, 40000, BF, 16, 1.0),
     (1700, 20011, F16, 2, 1.0),
 ])

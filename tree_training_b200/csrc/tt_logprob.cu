@@ -32,8 +32,10 @@ namespace tt {
 namespace logprob {
 namespace {
 
+// Threads of a block: 256, or 64 for short rows, of which an SM then takes more.
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kFewThreads = 64;
+constexpr int kFewPacks = 512;    // 16-byte packs of a row that 64 threads read
 constexpr int kMaxTop = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -215,91 +217,114 @@ __device__ __forceinline__ float logp_of(float x, float m, float ln_s, float inv
 }
 
 constexpr int kUnroll = 4;        // packs in flight a thread
-constexpr int kCandidates = 2048;
 constexpr int kMaxCluster = 8;
 
+template <int TH>
 struct TopShared {
-  uint64_t keys[kWarps * 8];      // the best threads' keys
-  uint64_t found[kCandidates];
+  // (with 64 threads: all of a short row's elements up to 1,024)
+  static constexpr int kCandidates = TH == kThreads ? 2048 : 1024;
+  ulonglong2 keys[TH / 2];        // the threads' largest
+  ulonglong2 found[kCandidates / 2];
   uint64_t list[kMaxTop];         // this block's largest, in order
-  uint64_t lists[kMaxCluster][kMaxTop];   // block 0: every block's
+  uint64_t lists[TH == kThreads ? kMaxCluster : 1][kMaxTop];   // block 0: every block's
   uint64_t bar;                   // the k-th largest of keys: a lower bound
   int n_threads, n_found;
-  int threads[kThreads];
+  int threads[TH];
 };
+
+// How many of the first n keys (n even, or a 0 behind them) are above `mine`.
+__device__ __forceinline__ int count_above(const ulonglong2* keys, int n, uint64_t mine) {
+  int above = 0;
+#pragma unroll 4
+  for (int i = 0; i < (n + 1) / 2; ++i) {
+    const ulonglong2 q = keys[i];
+    above += (q.x > mine) + (q.y > mine);
+  }
+  return above;
+}
 
 // The k largest keys of the block's packs [begin, end) into sh.list, in order
 // (0 where there are fewer).  `best` is this thread's largest logit and
 // `best_pack` the first pack that has it (-1: none); `nan` is set where a sum of
-// the block is NaN, as then `best` may have missed a NaN.  The k-th largest key of
-// any elements is a lower bound of the k-th largest of all, so: take it from the
-// threads' largest (up to 8 of each warp), look once more through the packs of
-// the threads that reach it (about k of them), and rank what is found.  Should
-// more than kCandidates elements reach the bound, or with NaN, the list is made
-// one pass an entry.
-template <typename T>
+// the block is NaN, as then `best` may have missed a NaN.  The k-th largest key
+// of any elements is a lower bound of the k-th largest of all, so: take it from
+// the threads' largest, look once more through the packs of the threads that
+// reach it (about k of them), and rank what is found.  Should more than
+// kCandidates elements reach the bound, or with a NaN, the list is made one pass
+// an entry.
+template <typename T, int TH>
 __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int end, int k,
                                           float best, int best_pack, bool nan,
-                                          TopShared& sh) {
-  constexpr int N = Packs<T>::N;
+                                          TopShared<TH>& sh) {
+  constexpr int N = Packs<T>::N, W = TH / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) sh.bar = 0, sh.n_threads = 0, sh.n_found = 0;
   // a key no larger than that of the thread's largest: its pack's last index
-  const uint32_t best_order = order_of(best);
-  uint32_t order = best_pack < 0 ? 0u : best_order;
-  const uint32_t last = (uint32_t)(row.first(best_pack) + N - 1);
-  // (with fewer keys a warp, a row of equal logits has its bound set by later
-  // warps' and many more candidates)
-  const int rounds = min(8, k);
-  for (int r = 0; r < rounds; ++r) {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, order);
-    const uint32_t at = __reduce_min_sync(0xffffffffu, order == top ? last : 0xffffffffu);
-    if (lane == 0) sh.keys[warp * rounds + r] = top ? key_of(top, at) : 0;
-    if (order == top && last == at) order = 0;
+  const uint32_t order = order_of(best);
+  const uint64_t low = best_pack < 0 ? 0 : key_of(order, row.first(best_pack) + N - 1);
+  // the k-th of them: among all, or, where k is small, among the largest of each
+  // warp (one row: 8 us with k = 1 and 11 with 8, against 10 and 12.5)
+  uint64_t* keys = reinterpret_cast<uint64_t*>(sh.keys);
+  int n_keys = TH;
+  if (k <= 8 || k <= 2 * W) {
+    const int each = min(k, 8);
+    n_keys = W * each;
+    uint32_t hi = (uint32_t)(low >> 32), lo = (uint32_t)low;
+    for (int r = 0; r < each; ++r) {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, hi);
+      const uint32_t at = __reduce_max_sync(0xffffffffu, hi == top ? lo : 0u);
+      if (lane == 0) keys[warp * each + r] = top ? ((uint64_t)top << 32) | at : 0;
+      if (hi == top && lo == at) hi = 0;
+    }
+  } else {
+    keys[threadIdx.x] = low;
   }
   __syncthreads();
-  const int n_keys = kWarps * rounds;
   if ((int)threadIdx.x < n_keys) {
-    const uint64_t mine = sh.keys[threadIdx.x];
-    int above = 0;
-    for (int i = 0; i < n_keys; ++i) above += sh.keys[i] > mine;
-    if (above == k - 1 && mine) sh.bar = mine;    // keys differ unless they are 0
+    const uint64_t mine = keys[threadIdx.x];         // keys differ unless they are 0
+    if (mine && count_above(sh.keys, n_keys, mine) == k - 1) sh.bar = mine;
   }
   __syncthreads();
   const uint64_t bar = sh.bar;
-  if (best_pack >= 0 && key_of(best_order, max((int64_t)0, row.first(best_pack))) >= bar)
+  if (best_pack >= 0 && key_of(order, max((int64_t)0, row.first(best_pack))) >= bar)
     sh.threads[atomicAdd(&sh.n_threads, 1)] = threadIdx.x;
   __syncthreads();
+  uint64_t* found = reinterpret_cast<uint64_t*>(sh.found);
   const int n_threads = nan ? 0 : sh.n_threads;
   const uint32_t bar_order = (uint32_t)(bar >> 32);
-  for (int q = warp; q < n_threads; q += kWarps) {
-    for (int v = begin + sh.threads[q] + lane * kThreads; v < end; v += 32 * kThreads) {
-      const uint4 raw = row.raw(v);
-      if (order_of(pack_max<T>(raw)) < bar_order) continue;
-      float x[N];
-      vec::unpack<T, N>(raw, x);
+  // their packs, one after another, over all threads
+  const int per = (end - begin + TH - 1) / TH;
+  for (int i = threadIdx.x; i < n_threads * per; i += TH) {
+    const int q = i / per, v = begin + sh.threads[q] + (i - q * per) * TH;
+    if (v >= end) continue;
+    const uint4 raw = row.raw(v);
+    if (order_of(pack_max<T>(raw)) < bar_order) continue;
+    float x[N];
+    vec::unpack<T, N>(raw, x);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t e = row.first(v) + i;
-        const uint64_t key = key_of(order_of(x[i]), e);
-        if (key >= bar && e >= 0 && e < row.V) {
-          const int at = atomicAdd(&sh.n_found, 1);
-          if (at < kCandidates) sh.found[at] = key;
-        }
+    for (int i = 0; i < N; ++i) {
+      const int64_t e = row.first(v) + i;
+      const uint64_t key = key_of(order_of(x[i]), e);
+      if (key >= bar && e >= 0 && e < row.V) {
+        const int at = atomicAdd(&sh.n_found, 1);
+        if (at < sh.kCandidates) found[at] = key;
       }
     }
   }
   __syncthreads();
   const int n = sh.n_found;
-  if (n <= kCandidates && !nan) {
-    for (int c = threadIdx.x; c < max(n, k); c += kThreads) {
+  if (n <= sh.kCandidates && !nan) {
+    if (n & 1) {
+      if (threadIdx.x == 0) found[n] = 0;
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < max(n, k); c += TH) {
       if (c >= n) {
         sh.list[c] = 0;
         continue;
       }
-      const uint64_t mine = sh.found[c];
-      int above = 0;
-      for (int i = 0; i < n; ++i) above += sh.found[i] > mine;
+      const uint64_t mine = found[c];
+      const int above = count_above(sh.found, n, mine);
       if (above < k) sh.list[above] = mine;
     }
     __syncthreads();
@@ -308,7 +333,7 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   uint64_t below = ~0ull;
   for (int j = 0; j < k; ++j) {
     uint64_t mine = 0;
-    for (int v = begin + threadIdx.x; v < end; v += kThreads) {
+    for (int v = begin + threadIdx.x; v < end; v += TH) {
       float x[N];
       row.load(v, x);
 #pragma unroll
@@ -324,10 +349,10 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
       mine = other > mine ? other : mine;
     }
     __syncthreads();
-    if (lane == 0) sh.keys[warp] = mine;
+    if (lane == 0) found[warp] = mine;
     __syncthreads();
-    below = sh.keys[0];
-    for (int w = 1; w < kWarps; ++w) below = sh.keys[w] > below ? sh.keys[w] : below;
+    below = found[0];
+    for (int w = 1; w < W; ++w) below = found[w] > below ? found[w] : below;
     if (threadIdx.x == 0) sh.list[j] = below;
   }
   __syncthreads();
@@ -340,14 +365,14 @@ struct Part {
 
 // One row a cluster: its blocks take equal runs of the row's packs and block 0
 // brings their sums and lists together.
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
-  constexpr int N = Packs<T>::N;
-  __shared__ Part warps[kWarps];
+template <typename T, int TH, bool kTop>
+__global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
+  constexpr int W = TH / 32;
+  __shared__ Part warps[W];
   __shared__ Part parts[kMaxCluster];
   __shared__ float st[3];
-  extern __shared__ uint64_t top_raw[];
-  TopShared& sh = *reinterpret_cast<TopShared*>(top_raw);
+  extern __shared__ ulonglong2 top_raw[];
+  TopShared<TH>& sh = *reinterpret_cast<TopShared<TH>*>(top_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -378,14 +403,14 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   };
   int v = begin + threadIdx.x;
   if (v < end) best_pack = v;
-  for (; v + (kUnroll - 1) * kThreads < end; v += kUnroll * kThreads) {
+  for (; v + (kUnroll - 1) * TH < end; v += kUnroll * TH) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) raw[i] = packs.raw(v + i * kThreads);
+    for (int i = 0; i < kUnroll; ++i) raw[i] = packs.raw(v + i * TH);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * kThreads);
+    for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * TH);
   }
-  for (; v < end; v += kThreads) take(packs.raw(v), v);
+  for (; v < end; v += TH) take(packs.raw(v), v);
 
   Sums acc = run.sums();
   const bool nan = acc.s != acc.s;
@@ -397,19 +422,19 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   }
   if (lane == 0) warps[warp] = {acc, wb};
   if constexpr (kTop)
-    block_top<T>(packs, begin, end, a.k, best, best_pack, __syncthreads_or(nan), sh);
+    block_top<T, TH>(packs, begin, end, a.k, best, best_pack, __syncthreads_or(nan), sh);
   else
     __syncthreads();
   if (blocks > 1) {
     cluster.barrier_wait();
     if (threadIdx.x == 0) {
       Part p = warps[0];
-      for (int w = 1; w < kWarps; ++w)
+      for (int w = 1; w < W; ++w)
         p = {merged(p.sums, warps[w].sums, c), fmaxf(p.best, warps[w].best)};
       *cluster.map_shared_rank(&parts[rank], 0) = p;
     }
     if constexpr (kTop)
-      for (int j = threadIdx.x; j < a.k; j += kThreads)
+      for (int j = threadIdx.x; j < a.k; j += TH)
         *cluster.map_shared_rank(&sh.lists[rank][j], 0) = sh.list[j];
     cluster.sync();
     if (rank != 0) return;
@@ -417,7 +442,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   if (threadIdx.x == 0) {
     const Part* from = blocks > 1 ? parts : warps;
     Part p = from[0];
-    for (int i = 1; i < (blocks > 1 ? blocks : kWarps); ++i)
+    for (int i = 1; i < (blocks > 1 ? blocks : W); ++i)
       p = {merged(p.sums, from[i].sums, c), fmaxf(p.best, from[i].best)};
     float ln_s = 0.f, inv_s = 0.f, H = 0.f;
     if (p.sums.s != 0.f) {
@@ -434,18 +459,29 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     if (blocks > 1) {
       // of the blocks' lists, which share no element
       const int n = blocks * a.k;
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t mine = sh.lists[i / a.k][i % a.k];
-        int above = 0;
-        for (int b = 0; b < blocks; ++b)
-          for (int j = 0; j < a.k && sh.lists[b][j] > mine; ++j) ++above;
+      for (int i = threadIdx.x; i < n; i += TH) {
+        const int q = i / a.k;
+        const uint64_t mine = sh.lists[q][i - q * a.k];
+        int above = i - q * a.k;
+        for (int o = 0; o < blocks; ++o) {
+          if (o == q) continue;
+          int lo = 0, hi = a.k;               // entries of o above mine: lo..hi
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (sh.lists[o][mid] > mine)
+              lo = mid + 1;
+            else
+              hi = mid;
+          }
+          above += lo;
+        }
         if (mine && above < a.k) sh.list[above] = mine;
       }
     }
   }
   __syncthreads();
   const float m = st[0], ln_s = st[1], inv_s = st[2];
-  for (int j = threadIdx.x; j < a.M; j += kThreads) {
+  for (int j = threadIdx.x; j < a.M; j += TH) {
     int64_t tok = tok0;
     float xt = x0;
     if (j != (int)threadIdx.x) {
@@ -456,7 +492,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
         (tok < 0 || tok >= a.V) ? 0.f : logp_of(xt, m, ln_s, inv_s, a.temperature);
   }
   if constexpr (kTop)
-    for (int j = threadIdx.x; j < a.k; j += kThreads) {
+    for (int j = threadIdx.x; j < a.k; j += TH) {
       const uint64_t key = sh.list[j];
       a.top_tok[row * a.k + j] = (int64_t)(uint32_t)~(uint32_t)key;
       a.top_logp[row * a.k + j] =
@@ -481,8 +517,8 @@ struct BwdArgs {
 // logp = t ln 2 - ln s:
 //   dx = 2^t (A + B t) + g / temperature at the given tokens,
 //   A = -(G + g_H (H - ln s)) / (s temperature), B = -g_H ln 2 / (s temperature).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
+template <typename T, int TH>
+__global__ void __launch_bounds__(TH) bwd_kernel(const BwdArgs a) {
   constexpr int N = Packs<T>::N;
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x / a.chunks;
@@ -545,18 +581,18 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const BwdArgs a) {
     }
   };
   int v = begin + threadIdx.x;
-  for (; v + (kUnroll - 1) * kThreads < end; v += kUnroll * kThreads) {
+  for (; v + (kUnroll - 1) * TH < end; v += kUnroll * TH) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) raw[i] = fetch(v + i * kThreads);
+    for (int i = 0; i < kUnroll; ++i) raw[i] = fetch(v + i * TH);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) leave(raw[i], v + i * kThreads);
+    for (int i = 0; i < kUnroll; ++i) leave(raw[i], v + i * TH);
   }
-  for (; v < end; v += kThreads) leave(fetch(v), v);
+  for (; v < end; v += TH) leave(fetch(v), v);
   if (empty) return;
   __syncthreads();
   // the given tokens in this block's part: equal ones add up in order
-  for (int j = threadIdx.x; j < n; j += kThreads) {
+  for (int j = threadIdx.x; j < n; j += TH) {
     const int64_t tok = token(j);
     if (tok < 0 || tok >= a.V || tok < to.first(begin) || tok >= to.first(end)) continue;
     float g = 0.f;
@@ -585,14 +621,13 @@ int cluster_of(int64_t rows, int64_t packs) {
   return c;
 }
 
-template <typename T, bool kTop>
-int launch_fwd(const Args& a, cudaStream_t st) {
-  const int c = cluster_of(a.rows, a.V / Packs<T>::N);
+template <typename T, int TH, bool kTop>
+int launch_fwd(const Args& a, int c, cudaStream_t st) {
   if (a.rows * c > 0x7fffffff) return TT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kTop ? sizeof(TopShared) : 0;
+  cfg.blockDim = dim3(TH);
+  cfg.dynamicSmemBytes = kTop ? sizeof(TopShared<TH>) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -600,7 +635,32 @@ int launch_fwd(const Args& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fwd_kernel<T, kTop>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, fwd_kernel<T, TH, kTop>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
+template <typename T>
+int launch_fwd(const Args& a, cudaStream_t st) {
+  const int64_t packs = a.V / Packs<T>::N;
+  // (64 threads' largest are too few to bound many alternatives well)
+  if (packs <= kFewPacks && a.k <= 16)
+    return a.k ? launch_fwd<T, kFewThreads, true>(a, 1, st)
+               : launch_fwd<T, kFewThreads, false>(a, 1, st);
+  const int c = cluster_of(a.rows, packs);
+  return a.k ? launch_fwd<T, kThreads, true>(a, c, st) : launch_fwd<T, kThreads, false>(a, c, st);
+}
+
+template <typename T, int TH>
+int launch_bwd(BwdArgs& a, cudaStream_t st) {
+  // a block takes 4 x kUnroll packs a thread; kUnroll where rows are few
+  const int64_t packs = a.V / Packs<T>::N + 2;
+  const int64_t one = (int64_t)kUnroll * TH;
+  int64_t per = 4 * one;
+  if (a.rows * ((packs + per - 1) / per) < vec::kSMs * 8) per = one;
+  a.per = (int)per;
+  a.chunks = (int)((packs + per - 1) / per);
+  if (a.rows * a.chunks > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+  bwd_kernel<T, TH><<<(unsigned)(a.rows * a.chunks), TH, 0, st>>>(a);
+  return TT_OK;
 }
 
 }  // namespace
@@ -621,9 +681,7 @@ extern "C" int tt_token_logprobs_fwd(int dtype, int64_t n_rows, int32_t vocab, c
   Args a{n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature,
          logprobs, entropy, top_logprobs, top_tokens, stats};
   const int rc = tt::vec::dispatch_float(dtype, [&](auto tag) -> int {
-    using T = decltype(tag);
-    return top_k ? launch_fwd<T, true>(a, (cudaStream_t)stream)
-                 : launch_fwd<T, false>(a, (cudaStream_t)stream);
+    return launch_fwd<decltype(tag)>(a, (cudaStream_t)stream);
   });
   if (rc != TT_OK) return rc;
   tt_count_launches(1);
@@ -645,16 +703,9 @@ extern "C" int tt_token_logprobs_bwd(int dtype, int64_t n_rows, int32_t vocab, c
             g_logprobs, g_entropy, g_top, stats, dlogits, 1, 0};
   const int rc = tt::vec::dispatch_float(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    // a block takes 4 x kUnroll packs a thread; kUnroll where rows are few
-    const int64_t packs = vocab / Packs<T>::N + 2;
-    const int64_t one = (int64_t)kUnroll * kThreads;
-    int64_t per = 4 * one;
-    if (n_rows * ((packs + per - 1) / per) < tt::vec::kSMs * 8) per = one;
-    a.per = (int)per;
-    a.chunks = (int)((packs + per - 1) / per);
-    if (n_rows * a.chunks > 0x7fffffff) return TT_ERR_UNSUPPORTED;
-    bwd_kernel<T><<<(unsigned)(n_rows * a.chunks), kThreads, 0, (cudaStream_t)stream>>>(a);
-    return TT_OK;
+    return vocab / Packs<T>::N <= kFewPacks
+               ? launch_bwd<T, kFewThreads>(a, (cudaStream_t)stream)
+               : launch_bwd<T, kThreads>(a, (cudaStream_t)stream);
   });
   if (rc != TT_OK) return rc;
   tt_count_launches(1);
