@@ -500,6 +500,131 @@ __global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
     }
 }
 
+// Rows of up to 32 P packs: a warp a row, which stays in its registers.  The k-th
+// largest logit is built up bit by bit from counts over the warp; those above
+// it and the first of those equal to it are ranked in shared memory.
+template <typename T, int P, bool kTop>
+__global__ void __launch_bounds__(kThreads) short_kernel(const Args a) {
+  constexpr int N = Packs<T>::N;
+  __shared__ uint64_t lists[kTop ? kThreads / 32 : 1][kMaxTop];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + warp;
+  if (row >= a.rows) return;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  const Packs<T> packs(x, a.V);
+  const float c = kLog2e / a.temperature;
+  uint4 raw[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (lane + 32 * i < packs.n) raw[i] = packs.raw(lane + 32 * i);
+  int64_t tok0 = -1;
+  float x0 = 0.f;
+  if (lane < a.M) {
+    tok0 = a.tokens[row * a.M + lane];
+    if (tok0 >= 0 && tok0 < a.V) x0 = to_f32(x[tok0]);
+  }
+  Running run;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (lane + 32 * i < packs.n) m = fmaxf(m, run.add<T>(raw[i], c));
+  Sums acc = run.sums();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    acc = merged(acc, shfl_xor(acc, o), c);
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
+  float ln_s = 0.f, inv_s = 0.f, H = 0.f;
+  if (acc.s != 0.f) {
+    rebase(acc, m, c);
+    ln_s = logf(acc.s);
+    inv_s = 1.f / acc.s;
+    H = ln_s - kLn2 * (acc.u / acc.s);
+  }
+  if (lane == 0) {
+    a.ent[row] = H;
+    if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(m, ln_s, inv_s, H);
+  }
+  for (int j = lane; j < a.M; j += 32) {
+    int64_t tok = tok0;
+    float xt = x0;
+    if (j != lane) {
+      tok = a.tokens[row * a.M + j];
+      if (tok >= 0 && tok < a.V) xt = to_f32(x[tok]);
+    }
+    a.logp[row * a.M + j] =
+        (tok < 0 || tok >= a.V) ? 0.f : logp_of(xt, m, ln_s, inv_s, a.temperature);
+  }
+  if constexpr (kTop) {
+    const int k = a.k;
+    uint32_t ord[P * N];                 // 0: not of the row
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float f[N];
+      vec::unpack<T, N>(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int64_t e = packs.first(lane + 32 * i) + j;
+        ord[i * N + j] =
+            lane + 32 * i < packs.n && e >= 0 && e < a.V ? order_of(f[j]) : 0u;
+      }
+    }
+    uint32_t tau = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t at = tau | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < P * N; ++i) n += ord[i] >= at;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n >= k) tau = at;
+      if (n == k) break;
+    }
+    int over = 0;
+#pragma unroll
+    for (int i = 0; i < P * N; ++i) over += ord[i] > tau;
+    const int need = k - __reduce_add_sync(0xffffffffu, over);    // of those equal to tau
+    int base_over = 0, base_equal = 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      int mine = 0;                      // above tau, and equal to it << 16
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t o = ord[i * N + j];
+        mine += (o > tau) + ((o == tau && o != 0) << 16);
+      }
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      const int before = upto - mine;
+      int above = base_over + (before & 0xffff), equal = base_equal + (before >> 16);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t o = ord[i * N + j];
+        const bool up = o > tau, eq = o == tau && o != 0;
+        if (up || (eq && equal < need))
+          lists[warp][above + min(equal, need)] = key_of(o, packs.first(lane + 32 * i) + j);
+        above += up;
+        equal += eq;
+      }
+      const int all = __shfl_sync(0xffffffffu, upto, 31);
+      base_over += all & 0xffff;
+      base_equal += all >> 16;
+    }
+    __syncwarp();
+    for (int j = lane; j < k; j += 32) {
+      const uint64_t key = lists[warp][j];
+      int above = 0;
+      for (int i = 0; i < k; ++i) above += lists[warp][i] > key;
+      a.top_tok[row * k + above] = (int64_t)(uint32_t)~(uint32_t)key;
+      a.top_logp[row * k + above] =
+          logp_of(of_order((uint32_t)(key >> 32)), m, ln_s, inv_s, a.temperature);
+    }
+  }
+}
+
 struct BwdArgs {
   int64_t rows;
   int V, M, k;
@@ -638,9 +763,25 @@ int launch_fwd(const Args& a, int c, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, fwd_kernel<T, TH, kTop>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
+template <typename T, int P>
+int launch_short(const Args& a, cudaStream_t st) {
+  constexpr int per = kThreads / 32;
+  const int64_t blocks = (a.rows + per - 1) / per;
+  if (a.k)
+    short_kernel<T, P, true><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  else
+    short_kernel<T, P, false><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  return TT_OK;
+}
+
 template <typename T>
 int launch_fwd(const Args& a, cudaStream_t st) {
   const int64_t packs = a.V / Packs<T>::N;
+  // a row may lie across two packs more than its size asks for
+  if (packs + 2 <= 32) return launch_short<T, 1>(a, st);
+  if (packs + 2 <= 64) return launch_short<T, 2>(a, st);
+  if (packs + 2 <= 128) return launch_short<T, 4>(a, st);
+  if (packs + 2 <= 256) return launch_short<T, 8>(a, st);
   // (64 threads' largest are too few to bound many alternatives well)
   if (packs <= kFewPacks && a.k <= 16)
     return a.k ? launch_fwd<T, kFewThreads, true>(a, 1, st)
