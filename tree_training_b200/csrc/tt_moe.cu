@@ -164,27 +164,35 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_rank(const PlanArgs a) {
   }
 }
 
-__global__ void __launch_bounds__(32 * kPlanWarps) plan_place(const PlanArgs a) {
+constexpr int kPlaceThreads = 512;
+
+__global__ void __launch_bounds__(kPlaceThreads) plan_place(const PlanArgs a, int blocks) {
   extern __shared__ int sm[];
   int* total = sm;                            // [E + 1]
   int* first = sm + a.E + 1;                  // [E + 1]: this block's first rows
-  __shared__ int warp_sum[kPlanWarps];
-  const int E = a.E, blocks = gridDim.x, b0 = blockIdx.x;
-  for (int x = threadIdx.x; x <= E; x += blockDim.x) {
+  __shared__ int warp_sum[kPlaceThreads / 32];
+  const int E = a.E, b0 = blockIdx.x;
+  // an expert's counts are shared out over as many threads as there are
+  const int parts = max(1, (int)blockDim.x / (E + 1)), share = (blocks + parts - 1) / parts;
+  for (int x = threadIdx.x; x < 2 * (E + 1); x += blockDim.x) sm[x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < parts * (E + 1); i += blockDim.x) {
+    const int part = i / (E + 1), x = i - part * (E + 1);
+    const int end = min(blocks, (part + 1) * share);
     int all = 0, before = 0;
-    for (int b = 0; b < blocks; b += 16) {
+    for (int b = part * share; b < end; b += 16) {
       int c[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        c[j] = b + j < blocks ? __ldg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
+        c[j] = b + j < end ? __ldg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         all += c[j];
         before += b + j < b0 ? c[j] : 0;
       }
     }
-    total[x] = all;
-    first[x] = before;
+    atomicAdd(total + x, all);
+    atomicAdd(first + x, before);
   }
   __syncthreads();
   const int per = (E + (int)blockDim.x) / (int)blockDim.x;
@@ -526,7 +534,7 @@ extern "C" int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_
     plan_rank<true><<<1, threads, smem, st>>>(a);
   } else {
     plan_rank<false><<<blocks, threads, smem, st>>>(a);
-    plan_place<<<blocks, threads, sizeof(int) * 2 * (E + 1), st>>>(a);
+    plan_place<<<blocks, kPlaceThreads, sizeof(int) * 2 * (E + 1), st>>>(a, blocks);
   }
   tt_count_launches(blocks > 1 ? 2 : 1);
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
