@@ -51,86 +51,62 @@ struct Args {
   float* part;              // [3][blocks][D]: dw2, dw1, dgate of the channels
 };
 
-// Column of element e of thread t of a row: packs of 8 where rows are aligned,
-// single elements tpr apart otherwise.
-template <bool kVec>
+// Column of element e of thread t of a row: packs of K elements, tpr apart.  K is
+// 8 where rows are aligned, 2 where only their elements' pairs are, else 1.
+template <int K>
 __device__ __forceinline__ int column(int e, int t, int tpr) {
-  return kVec ? (e / 8) * tpr * 8 + t * 8 + (e & 7) : e * tpr + t;
+  return (e / K * tpr + t) * K + e % K;
 }
 
-template <typename T, bool kVec, int E>
+template <typename T, int K, int E>
 struct Row {
   // raw packs as loaded, so that a row can be fetched ahead at its own width
-  static constexpr int P = (int)sizeof(T) / 2;                 // 16-byte loads a pack of 8
-  uint4 raw[kVec ? E / 8 * P : 1];
-  T one[kVec ? 1 : E];
+  static constexpr int L = K * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : K;   // of a load
+  vec::Raw<T, L> raw[E / L];
 
   __device__ __forceinline__ void fetch(const T* row, int t, int tpr, int D, bool live) {
-    if constexpr (kVec) {
 #pragma unroll
-      for (int b = 0; b < E / 8; ++b) {
-        const int c = column<true>(b * 8, t, tpr);
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-          raw[b * P + p] = (live && c < D)
-                               ? __ldg(reinterpret_cast<const uint4*>(row + c) + p)
-                               : make_uint4(0, 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = column<false>(e, t, tpr);
-        one[e] = (live && c < D) ? row[c] : from_f32<T>(0.f);
-      }
+    for (int i = 0; i < E / L; ++i) {
+      const int c = column<K>(i * L, t, tpr);
+      if (live && c < D)
+        raw[i] = vec::load_raw<T, L>(row + c);
+      else
+        raw[i] = vec::Raw<T, L>{};
     }
   }
 
   __device__ __forceinline__ void get(float (&v)[E]) const {
-    if constexpr (kVec) {
 #pragma unroll
-      for (int i = 0; i < E / 8 * P; ++i) {
-        constexpr int W = 16 / (int)sizeof(T);
-        float o[W];
-        vec::unpack<T, W>(raw[i], o);
+    for (int i = 0; i < E / L; ++i) {
+      float o[L];
+      vec::unpack<T, L>(raw[i], o);
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[i * W + j] = o[j];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = to_f32(one[e]);
+      for (int j = 0; j < L; ++j) v[i * L + j] = o[j];
     }
   }
 };
 
-template <typename T, bool kVec, int E>
+template <typename T, int K, int E>
 __device__ __forceinline__ void put(T* row, int t, int tpr, int D, const float (&v)[E]) {
-  if constexpr (kVec) {
-    constexpr int W = 16 / (int)sizeof(T);
+  constexpr int L = Row<T, K, E>::L;
 #pragma unroll
-    for (int i = 0; i < E / W; ++i) {
-      const int c = column<true>(i * W, t, tpr);
-      if (c < D) {
-        float o[W];
+  for (int i = 0; i < E / L; ++i) {
+    const int c = column<K>(i * L, t, tpr);
+    if (c < D) {
+      float o[L];
 #pragma unroll
-        for (int j = 0; j < W; ++j) o[j] = v[i * W + j];
-        vec::store<T, W>(row + c, o);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = column<false>(e, t, tpr);
-      if (c < D) row[c] = from_f32<T>(v[e]);
+      for (int j = 0; j < L; ++j) o[j] = v[i * L + j];
+      vec::store<T, L>(row + c, o);
     }
   }
 }
 
-template <typename T, bool kVec, int E>
+template <typename T, int K, int E>
 __device__ __forceinline__ void weights(const void* w, int f32, float offset, int t, int tpr,
                                         int D, float (&v)[E]) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int c = column<kVec>(e, t, tpr);
+    const int c = column<K>(e, t, tpr);
     v[e] = c >= D ? 0.f
                   : offset + (f32 ? reinterpret_cast<const float*>(w)[c]
                                   : to_f32(reinterpret_cast<const T*>(w)[c]));
@@ -166,7 +142,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* red) {
 
 constexpr int kMaxWarps = 32;
 
-template <typename T, typename R, bool kVec, int E, int kMaxThreads, bool kFullForm>
+template <typename T, typename R, int K, int E, int kMaxThreads, bool kFullForm>
 __global__ void __launch_bounds__(kMaxThreads) fwd_kernel(const Args a) {
   __shared__ float red[2][kMaxWarps];
   const int t = threadIdx.x % a.tpr, slot = threadIdx.x / a.tpr;
@@ -175,16 +151,16 @@ __global__ void __launch_bounds__(kMaxThreads) fwd_kernel(const Args a) {
   const bool post = kFullForm && a.w1 != nullptr;
   const int mode = kFullForm ? a.gate_mode : kNone;
   float w2[E], w1[E], gc[E];
-  weights<T, kVec, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
-  if (post) weights<T, kVec, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
-  if (mode == kChannel) weights<T, kVec, E>(a.gate, 0, 0.f, t, tpr, D, gc);
+  weights<T, K, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
+  if (post) weights<T, K, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
+  if (mode == kChannel) weights<T, K, E>(a.gate, 0, 0.f, t, tpr, D, gc);
   int turn = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
     const int64_t row = row0 + slot;
     const bool live = row < a.rows;
-    Row<T, kVec, E> rx;
-    Row<R, kVec, E> rr;
-    Row<T, kVec, E> rg;
+    Row<T, K, E> rx;
+    Row<R, K, E> rr;
+    Row<T, K, E> rg;
     rx.fetch(reinterpret_cast<const T*>(a.x) + row * a.x_st, t, tpr, D, live);
     rr.fetch(reinterpret_cast<const R*>(a.res) + row * a.res_st, t, tpr, D, live && a.res);
     if (mode == kFull)
@@ -225,10 +201,10 @@ __global__ void __launch_bounds__(kMaxThreads) fwd_kernel(const Args a) {
     turn ^= 1;
     const float i2 = rsqrtf(s[0] / D + a.eps);
     if (live) {
-      put<R, kVec, E>(reinterpret_cast<R*>(a.r) + row * D, t, tpr, D, r);
+      put<R, K, E>(reinterpret_cast<R*>(a.r) + row * D, t, tpr, D, r);
 #pragma unroll
       for (int e = 0; e < E; ++e) r[e] *= i2 * w2[e];
-      put<T, kVec, E>(reinterpret_cast<T*>(a.y) + row * D, t, tpr, D, r);
+      put<T, K, E>(reinterpret_cast<T*>(a.y) + row * D, t, tpr, D, r);
       if (t == 0 && a.stats) {
         a.stats[2 * row] = i1;
         a.stats[2 * row + 1] = i2;
@@ -237,7 +213,7 @@ __global__ void __launch_bounds__(kMaxThreads) fwd_kernel(const Args a) {
   }
 }
 
-template <typename T, typename R, bool kVec, int E, int kMaxThreads, bool kFullForm>
+template <typename T, typename R, int K, int E, int kMaxThreads, bool kFullForm>
 __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
   constexpr int N = kFullForm ? 3 : 1;
   __shared__ float red[2][kMaxWarps * N];
@@ -248,12 +224,12 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
   const bool post = kFullForm && a.w1 != nullptr;
   const int mode = kFullForm ? a.gate_mode : kNone;
   float w2[E], w1[E], gc[E], dw2[E], dw1[E], dgc[E];
-  weights<T, kVec, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
+  weights<T, K, E>(a.w2, a.w_f32, a.offset, t, tpr, D, w2);
   if (kFullForm) {
 #pragma unroll
     for (int e = 0; e < E; ++e) w1[e] = gc[e] = 1.f;
-    if (post) weights<T, kVec, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
-    if (mode == kChannel) weights<T, kVec, E>(a.gate, 0, 0.f, t, tpr, D, gc);
+    if (post) weights<T, K, E>(a.w1, a.w_f32, a.offset, t, tpr, D, w1);
+    if (mode == kChannel) weights<T, K, E>(a.gate, 0, 0.f, t, tpr, D, gc);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) dw2[e] = dw1[e] = dgc[e] = 0.f;
@@ -261,8 +237,8 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
   for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
     const int64_t row = row0 + slot;
     const bool live = row < a.rows;
-    Row<T, kVec, E> rx, ry, rg;
-    Row<R, kVec, E> rr, rd;
+    Row<T, K, E> rx, ry, rg;
+    Row<R, K, E> rr, rd;
     rx.fetch(reinterpret_cast<const T*>(a.x) + row * a.x_st, t, tpr, D, live);
     rr.fetch(reinterpret_cast<const R*>(a.res) + row * a.res_st, t, tpr, D, live && a.res);
     ry.fetch(reinterpret_cast<const T*>(a.dy) + row * a.dy_st, t, tpr, D, live && a.dy);
@@ -305,12 +281,12 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
     const float c = i2 * i2 * i2 * s[0] / D;
 #pragma unroll
     for (int e = 0; e < E; ++e) d[e] = fmaf(-c, r[e], d[e]);
-    if (live && a.dres) put<R, kVec, E>(reinterpret_cast<R*>(a.dres) + row * D, t, tpr, D, d);
+    if (live && a.dres) put<R, K, E>(reinterpret_cast<R*>(a.dres) + row * D, t, tpr, D, d);
     if constexpr (!kFullForm) {
       if (live && a.dx) {
 #pragma unroll
         for (int e = 0; e < E; ++e) d[e] *= k;
-        put<T, kVec, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, d);
+        put<T, K, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, d);
       }
     } else {
       const float dot = s[1] - c * s[2];         // sum of u w1 x d
@@ -327,9 +303,9 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
         dx[e] = fmaf(-back, x[e], i1 * dh * w1[e]);
         d[e] = a.scale * w1[e] * xd;             // gradient of the element's gate
       }
-      if (live && a.dx) put<T, kVec, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, dx);
+      if (live && a.dx) put<T, K, E>(reinterpret_cast<T*>(a.dx) + row * D, t, tpr, D, dx);
       if (mode == kFull && live && a.dgate)
-        put<T, kVec, E>(reinterpret_cast<T*>(a.dgate) + row * D, t, tpr, D, d);
+        put<T, K, E>(reinterpret_cast<T*>(a.dgate) + row * D, t, tpr, D, d);
     }
   }
   // the block's column sums: its rows' slots added in order
@@ -339,7 +315,7 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
     if (per == 1) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int c = column<kVec>(e, t, tpr);
+        const int c = column<K>(e, t, tpr);
         if (c < D) out[c] = v[e];
       }
       return;
@@ -347,7 +323,7 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = column<kVec>(e, t, tpr);
+      const int c = column<K>(e, t, tpr);
       if (c < D) cols[slot * D + c] = v[e];
     }
     __syncthreads();
@@ -461,6 +437,7 @@ __global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring
   const bool in = t * 8 < D;
   const bool post = kFullForm && a.w1, gated = kFullForm && a.gate_mode == kFull;
   const bool by_row = kFullForm && a.gate_mode == kRow;
+  const bool by_channel = kFullForm && a.gate_mode == kChannel;
   const int x_bytes = D * (int)sizeof(T), r_bytes = a.res ? D * (int)sizeof(R) : 0;
   const float inv_D = 1.f / D;
   if (t == 0) {
@@ -486,11 +463,12 @@ __global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring
   };
   if (t == 0)
     for (int i = 0; i < S; ++i) issue(blockIdx.x + (int64_t)i * gridDim.x, i);
-  Raw8<T> w2, w1;
-  w2.zero(), w1.zero();
+  Raw8<T> w2, w1, wg;
+  w2.zero(), w1.zero(), wg.zero();
   if (in) {
     w2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
     if (post) w1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
+    if (by_channel) wg.read(reinterpret_cast<const uint8_t*>(a.gate), t);
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -529,10 +507,11 @@ __global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] *= i1 * (a.offset + w[e]);
     }
+    if (by_channel) wg.get(g);
     float s[1] = {0.f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (gated) h[e] *= g[e];
+      if (gated || by_channel) h[e] *= g[e];
       r[e] = fmaf(k, h[e], r[e]);
       s[0] = fmaf(r[e], r[e], s[0]);
     }
@@ -555,7 +534,7 @@ __global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring
   if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
 }
 
-template <typename T, typename R, bool kFullForm, int kBlocks>
+template <typename T, typename R, bool kFullForm, int kBlocks, bool kByChannel>
 __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Ring ring) {
   constexpr int N = kFullForm ? 3 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -597,15 +576,16 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
   };
   if (t == 0)
     for (int i = 0; i < S; ++i) issue(blockIdx.x + (int64_t)i * gridDim.x, i);
-  Raw8<T> rw2, rw1;
-  rw2.zero(), rw1.zero();
+  Raw8<T> rw2, rw1, rwg;
+  rw2.zero(), rw1.zero(), rwg.zero();
   if (in) {
     rw2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
     if (post) rw1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
+    if (kByChannel) rwg.read(reinterpret_cast<const uint8_t*>(a.gate), t);
   }
-  float dw2[8], dw1[8];
+  float dw2[8], dw1[8], dgc[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw2[e] = dw1[e] = 0.f;
+  for (int e = 0; e < 8; ++e) dw2[e] = dw1[e] = dgc[e] = 0.f;
   int stage = 0, turn = 0;
   uint32_t phase = 0;
   // a row's own values are fetched a row ahead
@@ -660,8 +640,8 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= a.offset + u[e];
         }
-        if (gated) {
-          rg.get(u);
+        if (gated || kByChannel) {
+          (kByChannel ? rwg : rg).get(u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= u[e];
         }
@@ -713,8 +693,8 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = 1.f;
         }
-        if (gated) {
-          rg.get(g);
+        if (gated || kByChannel) {
+          (kByChannel ? rwg : rg).get(g);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) g[e] = 1.f;
@@ -723,6 +703,7 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
         for (int e = 0; e < 8; ++e) {
           const float xd = i1 * x[e] * d[e], kg = k * g[e];
           dw1[e] = fmaf(kg, xd, dw1[e]);
+          if (kByChannel) dgc[e] = fmaf(a.scale * w[e], xd, dgc[e]);
           r[e] = fmaf(-back, x[e], i1 * (kg * d[e]) * w[e]);     // dx
           d[e] = a.scale * w[e] * xd;                            // the element's gate
         }
@@ -736,10 +717,14 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
     float* part = a.part + (int64_t)blockIdx.x * D + t * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) part[e] = dw2[e];
+    const int64_t plane = (int64_t)gridDim.x * D;
     if (post) {
-      part += (int64_t)gridDim.x * D;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[e] = dw1[e];
+      for (int e = 0; e < 8; ++e) part[plane + e] = dw1[e];
+    }
+    if (kByChannel) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[2 * plane + e] = dgc[e];
     }
   }
 }
@@ -797,17 +782,18 @@ Shape shape_of(int D) {
   return s;
 }
 
-bool aligned(const void* p, int64_t stride) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+// Rows of elements of `size` bytes can be read in packs of `pack`.
+bool aligned(const void* p, int64_t stride, int size, int pack) {
+  return reinterpret_cast<uintptr_t>(p) % std::min(16, pack * size) == 0 && stride % pack == 0;
 }
 
 template <typename T, typename R, bool kBwd>
-int launch(const Args& a, bool vec, bool full, Shape s, int blocks, cudaStream_t st) {
+int launch(const Args& a, int pack, bool full, Shape s, int blocks, cudaStream_t st) {
   const int threads = s.tpr * s.per;
   const size_t smem = kBwd && s.per > 1 ? sizeof(float) * s.per * a.D : 0;
   auto go = [&](auto v, auto e, auto m, auto f) {
-    constexpr bool V = decltype(v)::value, F = decltype(f)::value;
-    constexpr int E = decltype(e)::value, M = decltype(m)::value;
+    constexpr bool F = decltype(f)::value;
+    constexpr int V = decltype(v)::value, E = decltype(e)::value, M = decltype(m)::value;
     if constexpr (kBwd)
       bwd_kernel<T, R, V, E, M, F><<<blocks, threads, smem, st>>>(a);
     else
@@ -819,14 +805,19 @@ int launch(const Args& a, bool vec, bool full, Shape s, int blocks, cudaStream_t
   std::integral_constant<int, 16> e16;
   std::integral_constant<int, 512> m512;
   std::integral_constant<int, 1024> m1024;
-  if (!vec) {
-    s.E == 8 ? go(N(), e8, m512, Y()) : go(N(), e16, m1024, Y());
+  std::integral_constant<int, 1> k1;
+  std::integral_constant<int, 2> k2;
+  std::integral_constant<int, 8> k8;
+  if (pack == 1) {
+    s.E == 8 ? go(k1, e8, m512, Y()) : go(k1, e16, m1024, Y());
+  } else if (pack == 2) {
+    s.E == 8 ? go(k2, e8, m512, Y()) : go(k2, e16, m1024, Y());
   } else if (s.E == 8) {
-    full ? go(Y(), e8, m512, Y()) : go(Y(), e8, m512, N());
+    full ? go(k8, e8, m512, Y()) : go(k8, e8, m512, N());
   } else if (threads <= 512) {
-    full ? go(Y(), e16, m512, Y()) : go(Y(), e16, m512, N());
+    full ? go(k8, e16, m512, Y()) : go(k8, e16, m512, N());
   } else {
-    full ? go(Y(), e16, m1024, Y()) : go(Y(), e16, m1024, N());
+    full ? go(k8, e16, m1024, Y()) : go(k8, e16, m1024, N());
   }
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
@@ -840,9 +831,9 @@ struct RingShape {
 
 constexpr int kSharedPerSM = 225 * 1024, kSharedOwn = 2048;   // kSharedOwn: static, reserved
 
-RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes) {
+RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes, int most = 1024) {
   RingShape best{0, 0, stage_bytes, 0};
-  for (int per = 1024 / threads; per > 0; --per) {
+  for (int per = most / threads; per > 0; --per) {
     const int stages = std::min(kMaxStages, (kSharedPerSM / per - kSharedOwn) / stage_bytes);
     if (stages >= 2) {
       best.blocks = (int)std::min<int64_t>(rows, (int64_t)vec::kSMs * per);
@@ -856,7 +847,8 @@ RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes) {
 
 bool rows_by_ring(int D, int dtype, bool vec, const Args& a) {
   return vec && D > 1024 && D <= 4096 && (!a.w_f32 || dtype == TT_F32) &&
-         a.gate_mode != kChannel && reinterpret_cast<uintptr_t>(a.w2) % 16 == 0 &&
+         (a.gate_mode != kChannel || reinterpret_cast<uintptr_t>(a.gate) % 16 == 0) &&
+         reinterpret_cast<uintptr_t>(a.w2) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(a.w1) % 16 == 0;
 }
 
@@ -872,9 +864,10 @@ int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, i
   };
   if constexpr (kBwd)
     // alone on its SM a block of 512 threads may use 128 registers each
-    return !full               ? go(ring_bwd<T, R, false, 2>)
-           : shape.per_sm == 1 ? go(ring_bwd<T, R, true, 1>)
-                               : go(ring_bwd<T, R, true, 2>);
+    return !full                       ? go(ring_bwd<T, R, false, 2, false>)
+           : a.gate_mode == kChannel   ? go(ring_bwd<T, R, true, 1, true>)
+           : shape.per_sm == 1         ? go(ring_bwd<T, R, true, 1, false>)
+                                       : go(ring_bwd<T, R, true, 2, false>);
   else
     return full ? go(ring_fwd<T, R, true>) : go(ring_fwd<T, R, false>);
 }
@@ -895,13 +888,13 @@ int dispatch_ring(int dtype, int res_dtype, const Args& a, int threads, const Ri
 int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
 
 template <bool kBwd>
-int dispatch(int dtype, int res_dtype, const Args& a, bool vec, Shape s, int blocks,
+int dispatch(int dtype, int res_dtype, const Args& a, int pack, Shape s, int blocks,
              cudaStream_t st) {
   const bool full = a.w1 || a.gate_mode != kNone;
   return vec::dispatch_float(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    if (res_dtype == dtype) return launch<T, T, kBwd>(a, vec, full, s, blocks, st);
-    if (res_dtype == TT_F32) return launch<T, float, kBwd>(a, vec, full, s, blocks, st);
+    if (res_dtype == dtype) return launch<T, T, kBwd>(a, pack, full, s, blocks, st);
+    if (res_dtype == TT_F32) return launch<T, float, kBwd>(a, pack, full, s, blocks, st);
     return TT_ERR_UNSUPPORTED;
   });
 }
@@ -936,20 +929,24 @@ extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int3
   a.y = y, a.r = r, a.stats = stats;
   Shape s = shape_of(D);
   a.tpr = s.tpr;
-  const bool vec = D % 8 == 0 && aligned(x, x_st) && aligned(residual, residual ? res_st : 0) &&
-                   aligned(y, D) && aligned(r, D) &&
-                   (gate_mode != kFull || aligned(gate, gate_st));
+  const int xs = size_of(dtype), rs = size_of(res_dtype);
+  auto fits = [&](int k) {
+    return D % k == 0 && aligned(x, x_st, xs, k) && aligned(residual, residual ? res_st : 0, rs, k) &&
+           aligned(y, D, xs, k) && aligned(r, D, rs, k) &&
+           (gate_mode != kFull || aligned(gate, gate_st, xs, k));
+  };
+  const int pack = fits(8) ? 8 : fits(2) ? 2 : 1;
   const int64_t want = (rows + s.per - 1) / s.per;
   const int blocks = (int)std::min<int64_t>(want, tt::vec::kSMs * 16ll);
   RingShape ring{};
-  if (rows_by_ring(D, dtype, vec, a))
+  if (rows_by_ring(D, dtype, pack == 8, a))
     ring = ring_of(rows, D, s.tpr,
                    D * (size_of(dtype) * (gate_mode == kFull ? 2 : 1) +
                         (residual ? size_of(res_dtype) : 0)));
   const int rc = ring.blocks
                      ? dispatch_ring<false>(dtype, res_dtype, a, s.tpr, ring, status,
                                             (cudaStream_t)stream)
-                     : dispatch<false>(dtype, res_dtype, a, vec, s, blocks, (cudaStream_t)stream);
+                     : dispatch<false>(dtype, res_dtype, a, pack, s, blocks, (cudaStream_t)stream);
   if (rc == TT_OK) tt_count_launches(1);
   return rc;
 }
@@ -987,20 +984,25 @@ extern "C" int tt_residual_norm_bwd(
   a.part = part;
   Shape s = shape_of(D);
   a.tpr = s.tpr;
-  const bool vec = D % 8 == 0 && aligned(x, x_st) && aligned(residual, residual ? res_st : 0) &&
-                   aligned(dy, dy ? dy_st : 0) && aligned(dr, dr ? dr_st : 0) && aligned(dx, D) &&
-                   aligned(dres, D) &&
-                   (gate_mode != kFull || (aligned(gate, gate_st) && aligned(dgate, D)));
+  const int xs = size_of(dtype), rs = size_of(res_dtype);
+  auto fits = [&](int k) {
+    return D % k == 0 && aligned(x, x_st, xs, k) && aligned(residual, residual ? res_st : 0, rs, k) &&
+           aligned(dy, dy ? dy_st : 0, xs, k) && aligned(dr, dr ? dr_st : 0, rs, k) &&
+           aligned(dx, D, xs, k) && aligned(dres, D, rs, k) &&
+           (gate_mode != kFull || (aligned(gate, gate_st, xs, k) && aligned(dgate, D, xs, k)));
+  };
+  const int pack = fits(8) ? 8 : fits(2) ? 2 : 1;
   cudaStream_t st = (cudaStream_t)stream;
   RingShape ring{};
-  if (rows_by_ring(D, dtype, vec, a))
+  if (rows_by_ring(D, dtype, pack == 8, a))
     ring = ring_of(rows, D, s.tpr,
                    D * (size_of(dtype) * (1 + (dy ? 1 : 0) + (gate_mode == kFull ? 1 : 0)) +
-                        size_of(res_dtype) * ((residual ? 1 : 0) + (dr ? 1 : 0))));
+                        size_of(res_dtype) * ((residual ? 1 : 0) + (dr ? 1 : 0))),
+                   gate_mode == kChannel ? 512 : 1024);     // 128 registers a thread
   if (ring.blocks) ring.blocks = blocks = std::min(blocks, ring.blocks);
   const int rc = ring.blocks
                      ? dispatch_ring<true>(dtype, res_dtype, a, s.tpr, ring, status, st)
-                     : dispatch<true>(dtype, res_dtype, a, vec, s, blocks, st);
+                     : dispatch<true>(dtype, res_dtype, a, pack, s, blocks, st);
   if (rc != TT_OK) return rc;
   Out out{};
   out.p[0] = dweight;
