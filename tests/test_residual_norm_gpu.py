@@ -100,14 +100,14 @@ def run(T, D, dtype, res, post, gate, scale=1.0, offset=0.0, eps=1e-6, wdtype=No
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("T,D,dtype,res", [
     (47, 256, F32, F32), (130, 2560, BF, BF), (33, 320, F16, F16), (19, 520, BF, F32),
-    (21, 129, BF, BF), (5, 1001, F32, F32), (300, 64, F16, F32), (7, 24, BF, BF),
+    (21, 129, BF, BF), (300, 4608, BF, BF), (31, 1026, F16, F16), (5, 1001, F32, F32), (300, 64, F16, F32), (7, 24, BF, BF),
 ])
 def test_every_form(T, D, dtype, res, post, gate):
     run(T, D, dtype, res, post, gate, scale=0.5, offset=1.0 if post else 0.0)
 
 
 @pytest.mark.parametrize("T,D,dtype", [
-    (1500, 1032, BF), (2000, 2560, F32), (1300, 4096, BF), (1, 1, F32), (3, 2, BF), (1, 4096, BF), (2, 4097, F16), (5, 4104, F32), (6, 8192, BF),
+    (2500, 640, BF), (700, 5120, F16), (40, 6152, F32), (1500, 1032, BF), (2000, 2560, F32), (1300, 4096, BF), (1, 1, F32), (3, 2, BF), (1, 4096, BF), (2, 4097, F16), (5, 4104, F32), (6, 8192, BF),
     (3, 8200, BF), (2, 16384, F32), (2, 16383, BF), (1500, 40, BF), (5000, 128, BF),
 ])
 @pytest.mark.parametrize("full", [False, True])

@@ -497,9 +497,15 @@ int run(Op op, int dtype, Args& a, void* stream) {
   return vec::dispatch_float(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     constexpr int V = 16 / (int)sizeof(T);
-    auto ok = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    if (a.H % V == 0 && ok(a.src) && ok(a.dst) && ok(a.ys))
-      return launch_k<T, V>(op, a, (cudaStream_t)stream);
+    // the widest packs that rows and pointers allow: 16 bytes, pairs, elements
+    auto fits = [&](int v) {
+      auto ok = [&](const void* p) {
+        return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0;
+      };
+      return a.H % v == 0 && ok(a.src) && ok(a.dst) && ok(a.ys);
+    };
+    if (fits(V)) return launch_k<T, V>(op, a, (cudaStream_t)stream);
+    if (fits(2)) return launch_k<T, 2>(op, a, (cudaStream_t)stream);
     return launch_k<T, 1>(op, a, (cudaStream_t)stream);
   });
 }

@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
 
 // ---- rows through shared memory ---------------------------------------------
 //
-// The same for long aligned rows (one a block, weights of x's type): thread 0
+// The same for aligned rows of 520 to 8,192 elements (one a block, weights of x's
+// type): thread 0
 // keeps a ring of `stages` rows filled by bulk copies, so that the next rows
 // arrive while this one is reduced and stored, and raw 16-bit packs instead of
 // fp32 values are what stays in registers across the reduction.  A stage is
@@ -428,7 +429,7 @@ __device__ __forceinline__ void put8(T* row, int t, const float (&v)[8]) {
 }
 
 template <typename T, typename R, bool kFullForm>
-__global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring) {
+__global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][32];
   __shared__ uint64_t full[kMaxStages];
@@ -534,8 +535,8 @@ __global__ void __launch_bounds__(512, 2) ring_fwd(const Args a, const Ring ring
   if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
 }
 
-template <typename T, typename R, bool kFullForm, int kBlocks, bool kByChannel>
-__global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Ring ring) {
+template <typename T, typename R, bool kFullForm, int kThreads, bool kByChannel>
+__global__ void __launch_bounds__(kThreads) ring_bwd(const Args a, const Ring ring) {
   constexpr int N = kFullForm ? 3 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][N * 32];
@@ -729,9 +730,9 @@ __global__ void __launch_bounds__(512, kBlocks) ring_bwd(const Args a, const Rin
   }
 }
 
-// out[c] = sum over the blocks' partials, in a fixed order: 16 threads a
-// column, each over every 16th block.
-constexpr int kSumRows = 16;
+// out[c] = sum over the blocks' partials, in a fixed order: 32 threads a
+// column, each over every 32nd block, four loads in flight.
+constexpr int kSumRows = 32;
 
 struct Out {
   void* p[3];
@@ -745,8 +746,16 @@ sum_partials(int blocks, int D, const float* __restrict__ part, const Out out) {
   const int c = blockIdx.x * 32 + threadIdx.x;
   const float* src = part + (int64_t)blockIdx.y * blocks * D;
   float s = 0.f;
-  if (c < D)
-    for (int b = threadIdx.y; b < blocks; b += kSumRows) s += src[(int64_t)b * D + c];
+  if (c < D) {
+    for (int b = threadIdx.y; b < blocks; b += 4 * kSumRows) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = b + j * kSumRows < blocks ? src[(int64_t)(b + j * kSumRows) * D + c] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += v[j];
+    }
+  }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < D) {
@@ -822,6 +831,8 @@ int launch(const Args& a, int pack, bool full, Shape s, int blocks, cudaStream_t
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
+int ring_threads(int D) { return (D / 8 + 31) / 32 * 32; }
+
 // The ring's shape: as many blocks an SM as threads and registers allow (64 a
 // thread) while each has two stages or more; blocks 0: rows go straight to
 // registers.
@@ -846,7 +857,7 @@ RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes, int most = 
 }
 
 bool rows_by_ring(int D, int dtype, bool vec, const Args& a) {
-  return vec && D > 1024 && D <= 4096 && (!a.w_f32 || dtype == TT_F32) &&
+  return vec && D > 512 && D <= 8192 && (!a.w_f32 || dtype == TT_F32) &&
          (a.gate_mode != kChannel || reinterpret_cast<uintptr_t>(a.gate) % 16 == 0) &&
          reinterpret_cast<uintptr_t>(a.w2) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(a.w1) % 16 == 0;
@@ -862,14 +873,16 @@ int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, i
     kern<<<shape.blocks, threads, smem, st>>>(a, ring);
     return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
   };
-  if constexpr (kBwd)
-    // alone on its SM a block of 512 threads may use 128 registers each
-    return !full                       ? go(ring_bwd<T, R, false, 2, false>)
-           : a.gate_mode == kChannel   ? go(ring_bwd<T, R, true, 1, true>)
-           : shape.per_sm == 1         ? go(ring_bwd<T, R, true, 1, false>)
-                                       : go(ring_bwd<T, R, true, 2, false>);
-  else
+  if constexpr (kBwd) {
+    // with 512 threads or fewer on an SM they may use 128 registers each
+    const bool wide = shape.per_sm * threads <= 512;
+    if (!full) return go(ring_bwd<T, R, false, 1024, false>);
+    if (a.gate_mode == kChannel)
+      return wide ? go(ring_bwd<T, R, true, 512, true>) : go(ring_bwd<T, R, true, 1024, true>);
+    return wide ? go(ring_bwd<T, R, true, 512, false>) : go(ring_bwd<T, R, true, 1024, false>);
+  } else {
     return full ? go(ring_fwd<T, R, true>) : go(ring_fwd<T, R, false>);
+  }
 }
 
 template <bool kBwd>
@@ -940,11 +953,11 @@ extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int3
   const int blocks = (int)std::min<int64_t>(want, tt::vec::kSMs * 16ll);
   RingShape ring{};
   if (rows_by_ring(D, dtype, pack == 8, a))
-    ring = ring_of(rows, D, s.tpr,
+    ring = ring_of(rows, D, ring_threads(D),
                    D * (size_of(dtype) * (gate_mode == kFull ? 2 : 1) +
                         (residual ? size_of(res_dtype) : 0)));
   const int rc = ring.blocks
-                     ? dispatch_ring<false>(dtype, res_dtype, a, s.tpr, ring, status,
+                     ? dispatch_ring<false>(dtype, res_dtype, a, ring_threads(D), ring, status,
                                             (cudaStream_t)stream)
                      : dispatch<false>(dtype, res_dtype, a, pack, s, blocks, (cudaStream_t)stream);
   if (rc == TT_OK) tt_count_launches(1);
@@ -955,9 +968,10 @@ extern "C" int tt_residual_norm_bwd_blocks(int64_t rows, int32_t D) {
   using namespace tt::resnorm;
   if (rows <= 0 || D <= 0 || D > kMaxD) return 1;
   const Shape s = shape_of(D);
-  const int64_t want = (rows + s.per - 1) / s.per;
+  // (the ring's blocks are of one row)
+  const int threads = D > 512 && D <= 8192 ? ring_threads(D) : s.tpr * s.per;
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>(want, tt::vec::kSMs * (int64_t)std::max(1, 1024 / (s.tpr * s.per))));
+      1, std::min<int64_t>(rows, tt::vec::kSMs * (int64_t)std::max(1, 1024 / threads)));
 }
 
 extern "C" int tt_residual_norm_bwd(
@@ -995,13 +1009,18 @@ extern "C" int tt_residual_norm_bwd(
   cudaStream_t st = (cudaStream_t)stream;
   RingShape ring{};
   if (rows_by_ring(D, dtype, pack == 8, a))
-    ring = ring_of(rows, D, s.tpr,
+    ring = ring_of(rows, D, ring_threads(D),
                    D * (size_of(dtype) * (1 + (dy ? 1 : 0) + (gate_mode == kFull ? 1 : 0)) +
                         size_of(res_dtype) * ((residual ? 1 : 0) + (dr ? 1 : 0))),
-                   gate_mode == kChannel ? 512 : 1024);     // 128 registers a thread
-  if (ring.blocks) ring.blocks = blocks = std::min(blocks, ring.blocks);
+                   gate_mode == kChannel && D <= 4096 ? 512 : 1024);   // for 128 registers
+  if (ring.blocks)
+    ring.blocks = blocks = std::min(blocks, ring.blocks);
+  else
+    blocks = (int)std::min<int64_t>(
+        {blocks, (rows + s.per - 1) / s.per,
+         tt::vec::kSMs * (int64_t)std::max(1, 1024 / (s.tpr * s.per))});
   const int rc = ring.blocks
-                     ? dispatch_ring<true>(dtype, res_dtype, a, s.tpr, ring, status, st)
+                     ? dispatch_ring<true>(dtype, res_dtype, a, ring_threads(D), ring, status, st)
                      : dispatch<true>(dtype, res_dtype, a, pack, s, blocks, st);
   if (rc != TT_OK) return rc;
   Out out{};
