@@ -428,8 +428,8 @@ __device__ __forceinline__ void put8(T* row, int t, const float (&v)[8]) {
   }
 }
 
-template <typename T, typename R, bool kFullForm>
-__global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) {
+template <typename T, typename R, bool kFullForm, bool kByChannel>
+__global__ void __launch_bounds__(1024, 1) ring_fwd(const Args a, const Ring ring) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][32];
   __shared__ uint64_t full[kMaxStages];
@@ -438,7 +438,6 @@ __global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) 
   const bool in = t * 8 < D;
   const bool post = kFullForm && a.w1, gated = kFullForm && a.gate_mode == kFull;
   const bool by_row = kFullForm && a.gate_mode == kRow;
-  const bool by_channel = kFullForm && a.gate_mode == kChannel;
   const int x_bytes = D * (int)sizeof(T), r_bytes = a.res ? D * (int)sizeof(R) : 0;
   const float inv_D = 1.f / D;
   if (t == 0) {
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) 
   if (in) {
     w2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
     if (post) w1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
-    if (by_channel) wg.read(reinterpret_cast<const uint8_t*>(a.gate), t);
+    if (kByChannel) wg.read(reinterpret_cast<const uint8_t*>(a.gate), t);
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -508,11 +507,11 @@ __global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) 
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] *= i1 * (a.offset + w[e]);
     }
-    if (by_channel) wg.get(g);
+    if (kByChannel) wg.get(g);
     float s[1] = {0.f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (gated || by_channel) h[e] *= g[e];
+      if (gated || kByChannel) h[e] *= g[e];
       r[e] = fmaf(k, h[e], r[e]);
       s[0] = fmaf(r[e], r[e], s[0]);
     }
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(1024) ring_fwd(const Args a, const Ring ring) 
 }
 
 template <typename T, typename R, bool kFullForm, int kThreads, bool kByChannel>
-__global__ void __launch_bounds__(kThreads) ring_bwd(const Args a, const Ring ring) {
+__global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring ring) {
   constexpr int N = kFullForm ? 3 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][N * 32];
@@ -881,7 +880,9 @@ int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, i
       return wide ? go(ring_bwd<T, R, true, 512, true>) : go(ring_bwd<T, R, true, 1024, true>);
     return wide ? go(ring_bwd<T, R, true, 512, false>) : go(ring_bwd<T, R, true, 1024, false>);
   } else {
-    return full ? go(ring_fwd<T, R, true>) : go(ring_fwd<T, R, false>);
+    if (!full) return go(ring_fwd<T, R, false, false>);
+    return a.gate_mode == kChannel ? go(ring_fwd<T, R, true, true>)
+                                   : go(ring_fwd<T, R, true, false>);
   }
 }
 
