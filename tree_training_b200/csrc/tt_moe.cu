@@ -453,7 +453,126 @@ __global__ void __launch_bounds__(512, 2) spread_kernel(const Args a) {
   zero_tail<T, V>(a);
 }
 
+// ---- rows at any element ---------------------------------------------------------
+//
+// With 16-bit rows whose width is no multiple of 8, every row starts at another
+// place of a 16-byte word.  Threads go by the words of the row that is written
+// (in spread: of the sorted row), and shift what they read into place.
+
+// Elements of a row's first 16-byte word that lie before the row.
+template <typename T>
+__device__ __forceinline__ int lead(const T* row) {
+  return (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) dispatch_any(const Args a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const Place pl = place(a);
+  if (pl.live) {
+    const T *lo = reinterpret_cast<const T*>(a.src), *hi = lo + a.T * a.H;
+    const T* src = lo + pl.tok * a.H;
+    for (int k = 0; k < a.K; ++k) {
+      const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
+      if (r < 0) continue;
+      T* dst = reinterpret_cast<T*>(a.dst) + r * a.H;
+      for (int64_t e = (int64_t)pl.t * N - lead(dst); e < a.H; e += a.group * N)
+        vec::store_part<T>(dst, e, a.H, vec::load_any_of<T>(src, e, a.H, lo, hi));
+    }
+  }
+  zero_tail<T, 1>(a);
+}
+
+template <typename T, bool kWeighted>
+__global__ void __launch_bounds__(512) combine_any(const Args a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const Place pl = place(a);
+  if (!pl.live) return;
+  const T *lo = reinterpret_cast<const T*>(a.src), *hi = lo + a.T * a.K * a.H;
+  T* dst = reinterpret_cast<T*>(a.dst) + pl.tok * a.H;
+  for (int64_t e = (int64_t)pl.t * N - lead(dst); e < a.H; e += a.group * N) {
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int k = 0; k < a.K; ++k) {
+      const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
+      if (r < 0) continue;
+      float v[N];
+      vec::unpack<T, N>(vec::load_any_of<T>(lo + r * a.H, e, a.H, lo, hi), v);
+      vec::axpy<N>(kWeighted ? weight_of(a, pl, k) : 1.f, v, acc);
+    }
+    vec::store_part<T>(dst, e, a.H, vec::pack<T, N>(acc));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) spread_any(const Args a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ float red[16];
+  const Place pl = place(a);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = a.group >> 5;
+  const T *lo = reinterpret_cast<const T*>(a.src), *hi = lo + a.T * a.H;
+  for (int k = 0; k < a.K; ++k) {
+    float dot = 0.f;
+    if (pl.live) {
+      const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
+      if (r >= 0) {
+        const float w = weight_of(a, pl, k);
+        const T* ys = reinterpret_cast<const T*>(a.ys) + r * a.H;
+        T* dst = reinterpret_cast<T*>(a.dst) + r * a.H;
+        const T* yhi = reinterpret_cast<const T*>(a.ys) + a.T * a.K * a.H;
+        for (int64_t e = (int64_t)pl.t * N - lead(dst); e < a.H; e += a.group * N) {
+          float g[N], v[N], o[N];
+          vec::unpack<T, N>(vec::load_any_of<T>(lo + pl.tok * a.H, e, a.H, lo, hi), g);
+          vec::unpack<T, N>(vec::load_any_of<T>(ys, e, a.H, reinterpret_cast<const T*>(a.ys), yhi),
+                            v);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            dot = fmaf(g[i], v[i], dot);
+            o[i] = w * g[i];
+          }
+          vec::store_part<T>(dst, e, a.H, vec::pack<T, N>(o));
+        }
+      }
+    }
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (k) __syncthreads();             // the sums before have been read
+    if (lane == 0) red[warp] = dot;
+    __syncthreads();
+    if (pl.live && pl.t == 0) {
+      float s = 0.f;
+      for (int q = 0; q < nw; ++q) s += red[warp + q];
+      const int64_t i = pl.tok * a.K + k;
+      switch (a.w_dtype) {
+        case TT_F32: reinterpret_cast<float*>(a.dw)[i] = s; break;
+        case TT_BF16: reinterpret_cast<__nv_bfloat16*>(a.dw)[i] = from_f32<__nv_bfloat16>(s); break;
+        default: reinterpret_cast<__half*>(a.dw)[i] = from_f32<__half>(s); break;
+      }
+    }
+  }
+  zero_tail<T, 1>(a);
+}
+
 enum Op { kDispatch, kCollect, kCombine, kSpread };
+
+template <typename T>
+int launch_any(Op op, Args& a, cudaStream_t st) {
+  const int packs = a.H / 8 + 2;
+  const int turns = (packs + 511) / 512;
+  a.group = ((packs + turns - 1) / turns + 31) / 32 * 32;
+  const int per = std::max(1, 256 / a.group), threads = a.group * per;
+  const int64_t blocks = (a.T + per - 1) / per;
+  if (blocks > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)blocks;
+  switch (op) {
+    case kDispatch: dispatch_any<T><<<grid, threads, 0, st>>>(a); break;
+    case kCollect: combine_any<T, false><<<grid, threads, 0, st>>>(a); break;
+    case kCombine: combine_any<T, true><<<grid, threads, 0, st>>>(a); break;
+    case kSpread: spread_any<T><<<grid, threads, 0, st>>>(a); break;
+  }
+  tt_count_launches(1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
 
 template <typename T, int V, int KC>
 int launch(Op op, Args& a, cudaStream_t st) {
@@ -497,7 +616,8 @@ int run(Op op, int dtype, Args& a, void* stream) {
   return vec::dispatch_float(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     constexpr int V = 16 / (int)sizeof(T);
-    // the widest packs that rows and pointers allow: 16 bytes, pairs, elements
+    // 16-byte packs where rows are aligned; 16-bit rows at any element by shifted
+    // words; 32-bit ones in pairs or by elements
     auto fits = [&](int v) {
       auto ok = [&](const void* p) {
         return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0;
@@ -505,8 +625,12 @@ int run(Op op, int dtype, Args& a, void* stream) {
       return a.H % v == 0 && ok(a.src) && ok(a.dst) && ok(a.ys);
     };
     if (fits(V)) return launch_k<T, V>(op, a, (cudaStream_t)stream);
-    if (fits(2)) return launch_k<T, 2>(op, a, (cudaStream_t)stream);
-    return launch_k<T, 1>(op, a, (cudaStream_t)stream);
+    if constexpr (sizeof(T) == 2) {
+      return launch_any<T>(op, a, (cudaStream_t)stream);
+    } else {
+      return fits(2) ? launch_k<T, 2>(op, a, (cudaStream_t)stream)
+                     : launch_k<T, 1>(op, a, (cudaStream_t)stream);
+    }
   });
 }
 

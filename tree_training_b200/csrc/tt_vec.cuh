@@ -121,6 +121,73 @@ __device__ __forceinline__ void axpy(float w, const float (&v)[V], float (&acc)[
   }
 }
 
+// ---- 16 bytes at any element --------------------------------------------------
+
+// Bytes b .. b + 15 of the 32 bytes (a, c), b < 16.
+__device__ __forceinline__ uint4 window(const uint4& a, const uint4& c, int b) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+  if (b & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (b & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = 8 * (b & 3);
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// 16 bytes at p, a multiple of T's size: out of the one or two aligned 16-byte
+// words that hold them, where these lie in [lo, hi); element by element at the
+// ends of a buffer.
+template <typename T>
+__device__ __forceinline__ uint4 load_any(const T* p, const T* lo, const T* hi) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const int b = (int)(at & 15);
+  const uint4* w = reinterpret_cast<const uint4*>(at - b);
+  if (b == 0) return __ldg(w);
+  if (reinterpret_cast<const T*>(w) >= lo && reinterpret_cast<const T*>(w + 2) <= hi)
+    return window(__ldg(w), __ldg(w + 1), b);
+  union U {
+    uint4 raw;
+    T e[16 / sizeof(T)];
+    __device__ U() {}
+  } u;
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) u.e[i] = p[i];
+  return u.raw;
+}
+
+// The same of the elements e0 .. of a row of n elements; those outside it are 0.
+template <typename T>
+__device__ __forceinline__ uint4 load_any_of(const T* row, int64_t e0, int64_t n, const T* lo,
+                                             const T* hi) {
+  constexpr int N = 16 / (int)sizeof(T);
+  if (e0 >= 0 && e0 + N <= n) return load_any<T>(row + e0, lo, hi);
+  float v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(row[e0 + i]) : 0.f;
+  return pack<T, N>(v);
+}
+
+// Stores what lies of a pack at elements e0 .. in a row of n elements; row + e0
+// is on a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_part(T* row, int64_t e0, int64_t n, const uint4& raw) {
+  constexpr int N = 16 / (int)sizeof(T);
+  if (e0 >= 0 && e0 + N <= n) {
+    *reinterpret_cast<uint4*>(row + e0) = raw;
+    return;
+  }
+  float v[N];
+  unpack<T, N>(raw, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = from_f32<T>(v[i]);
+}
+
 // Calls f with a value of the C++ type of a TT_* floating dtype.
 template <typename F>
 int dispatch_float(int dtype, F f) {
