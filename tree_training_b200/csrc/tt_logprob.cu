@@ -109,6 +109,12 @@ __device__ __forceinline__ Sums shfl_xor(const Sums& a, int o) {
           __shfl_xor_sync(0xffffffffu, a.u, o)};
 }
 
+__device__ __forceinline__ void load32(const uint4* p, uint4& a, uint4& b) {
+  asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+      : "l"(p));
+}
+
 // A row as 16-byte packs that start on 16-byte boundaries: pack v holds the
 // elements [v N - shift, (v + 1) N - shift), of which those of the row are
 // loaded and the others are -inf (no probability, and no candidates: their
@@ -140,6 +146,29 @@ struct Packs {
   }
   __device__ __forceinline__ void load(int v, float (&o)[N]) const {
     vec::unpack<T, N>(raw(v), o);
+  }
+  // Whether pack v lies on a 32-byte boundary.
+  __device__ __forceinline__ bool wide(int v) const {
+    return (reinterpret_cast<uintptr_t>(x - shift) + (uint64_t)v * 16) % 32 == 0;
+  }
+  // Packs v to v + G - 1, those below `end` (the others are left alone); `wide`:
+  // 32 bytes a load.
+  template <int G>
+  __device__ __forceinline__ void some(int v, int end, bool wide, uint4 (&r)[G]) const {
+    if (v >= whole0 && v + G - 1 < min(whole1, end)) {
+      const uint4* p = reinterpret_cast<const uint4*>(x - shift) + v;
+      if (G > 1 && wide) {
+#pragma unroll
+        for (int i = 0; i + 1 < G; i += 2) load32(p + i, r[i], r[i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i) r[i] = __ldg(p + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+        if (v + i < end) r[i] = raw(v + i);
+    }
   }
 };
 
@@ -222,13 +251,14 @@ constexpr int kMaxCluster = 8;
 template <int TH>
 struct TopShared {
   // (with 64 threads: all of a short row's elements up to 1,024)
-  static constexpr int kCandidates = TH == kThreads ? 2048 : 1024;
+  static constexpr int kCandidates = TH == kThreads ? 4096 : 1024;
   ulonglong2 keys[TH / 2];        // the threads' largest
   ulonglong2 found[kCandidates / 2];
   uint64_t list[kMaxTop];         // this block's largest, in order
   uint64_t lists[TH == kThreads ? kMaxCluster : 1][kMaxTop];   // block 0: every block's
   uint64_t bar;                   // the k-th largest of keys: a lower bound
-  int n_threads, n_found;
+  int n_threads, n_found, n_kept;
+  int at_least[64];
   int threads[TH];
 };
 
@@ -252,13 +282,15 @@ __device__ __forceinline__ int count_above(const ulonglong2* keys, int n, uint64
 // reach it (about k of them), and rank what is found.  Should more than
 // kCandidates elements reach the bound, or with a NaN, the list is made one pass
 // an entry.
-template <typename T, int TH>
+// G: how many packs in a row a thread reads, every G TH packs.
+template <typename T, int TH, int G>
 __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int end, int k,
                                           float best, int best_pack, bool nan,
                                           TopShared<TH>& sh) {
   constexpr int N = Packs<T>::N, W = TH / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) sh.bar = 0, sh.n_threads = 0, sh.n_found = 0;
+  if (threadIdx.x == 0) sh.bar = 0, sh.n_threads = 0, sh.n_found = 0, sh.n_kept = 0;
+  if (threadIdx.x < 64) sh.at_least[threadIdx.x] = 0;
   // a key no larger than that of the thread's largest: its pack's last index
   const uint32_t order = order_of(best);
   const uint64_t low = best_pack < 0 ? 0 : key_of(order, row.first(best_pack) + N - 1);
@@ -292,27 +324,57 @@ __device__ __forceinline__ void block_top(const Packs<T>& row, int begin, int en
   uint64_t* found = reinterpret_cast<uint64_t*>(sh.found);
   const int n_threads = nan ? 0 : sh.n_threads;
   const uint32_t bar_order = (uint32_t)(bar >> 32);
-  // their packs, one after another, over all threads
-  const int per = (end - begin + TH - 1) / TH;
+  // their packs, over all threads
+  const int per = (end - begin + G * TH - 1) / (G * TH);
+  const bool wide = row.wide(begin);
   for (int i = threadIdx.x; i < n_threads * per; i += TH) {
-    const int q = i / per, v = begin + sh.threads[q] + (i - q * per) * TH;
+    const int q = i / per, v = begin + G * (sh.threads[q] + (i - q * per) * TH);
     if (v >= end) continue;
-    const uint4 raw = row.raw(v);
-    if (order_of(pack_max<T>(raw)) < bar_order) continue;
-    float x[N];
-    vec::unpack<T, N>(raw, x);
+    uint4 raw[G];
+    row.template some<G>(v, end, wide, raw);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t e = row.first(v) + i;
-      const uint64_t key = key_of(order_of(x[i]), e);
-      if (key >= bar && e >= 0 && e < row.V) {
-        const int at = atomicAdd(&sh.n_found, 1);
-        if (at < sh.kCandidates) found[at] = key;
+    for (int u = 0; u < G; ++u) {
+      if (v + u >= end || order_of(pack_max<T>(raw[u])) < bar_order) continue;
+      float x[N];
+      vec::unpack<T, N>(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int64_t e = row.first(v + u) + j;
+        const uint64_t key = key_of(order_of(x[j]), e);
+        if (key >= bar && e >= 0 && e < row.V) {
+          const int at = atomicAdd(&sh.n_found, 1);
+          if (at < sh.kCandidates) found[at] = key;
+        }
       }
     }
   }
   __syncthreads();
   const int n = sh.n_found;
+  if (n <= sh.kCandidates && n > 512 && !nan) {
+    // many equal logits: the k-th key, bit by bit from counts, then those from it on
+    uint64_t kth = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t at = kth | (1ull << bit);
+      int m = 0;
+      for (int i = threadIdx.x; i < n; i += TH) m += found[i] >= at;
+      m = __reduce_add_sync(0xffffffffu, m);
+      if (lane == 0) atomicAdd(&sh.at_least[bit], m);
+      __syncthreads();
+      const int all = sh.at_least[bit];
+      if (all >= k) kth = at;
+      if (all == k) break;
+    }
+    for (int i = threadIdx.x; i < n; i += TH)
+      if (found[i] >= kth) keys[atomicAdd(&sh.n_kept, 1)] = found[i];
+    __syncthreads();
+    if ((int)threadIdx.x < k) {
+      int above = 0;
+      for (int i = 0; i < k; ++i) above += keys[i] > keys[threadIdx.x];
+      sh.list[above] = keys[threadIdx.x];
+    }
+    __syncthreads();
+    return;
+  }
   if (n <= sh.kCandidates && !nan) {
     if (n & 1) {
       if (threadIdx.x == 0) found[n] = 0;
@@ -364,10 +426,15 @@ struct Part {
 };
 
 // One row a cluster: its blocks take equal runs of the row's packs and block 0
-// brings their sums and lists together.
-template <typename T, int TH, bool kTop>
+// brings their sums and lists together.  G is 0 without alternatives, else the
+// packs in a row that a thread reads: 4 in long rows, since the second look's
+// single packs would cost the memory a piece of 64 bytes or more each (4,096 x
+// 151,936 with sixteen: 305 us against 277), 1 where threads have few packs
+// (16,000 x 10,000: 248 against 297).
+template <typename T, int TH, int G>
 __global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
   constexpr int W = TH / 32;
+  constexpr bool kTop = G > 0;
   __shared__ Part warps[W];
   __shared__ Part parts[kMaxCluster];
   __shared__ float st[3];
@@ -401,16 +468,30 @@ __global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
     if (kTop && mx > best) best_pack = v;
     best = fmaxf(best, mx);
   };
-  int v = begin + threadIdx.x;
-  if (v < end) best_pack = v;
-  for (; v + (kUnroll - 1) * TH < end; v += kUnroll * TH) {
-    uint4 raw[kUnroll];
+  if constexpr (G <= 1) {
+    int v = begin + threadIdx.x;
+    if (v < end) best_pack = v;
+    for (; v + (kUnroll - 1) * TH < end; v += kUnroll * TH) {
+      uint4 raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) raw[i] = packs.raw(v + i * TH);
+      for (int i = 0; i < kUnroll; ++i) raw[i] = packs.raw(v + i * TH);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * TH);
+      for (int i = 0; i < kUnroll; ++i) take(raw[i], v + i * TH);
+    }
+    for (; v < end; v += TH) take(packs.raw(v), v);
+  } else {
+    const bool wide = packs.wide(begin);
+    int v = begin + G * (int)threadIdx.x;
+    if (v < end) best_pack = v;
+    for (; v + G - 1 < end; v += G * TH) {
+      uint4 raw[G];
+      packs.template some<G>(v, end, wide, raw);
+#pragma unroll
+      for (int i = 0; i < G; ++i) take(raw[i], v + i);
+    }
+    if (v < end)
+      for (; v < end; ++v) take(packs.raw(v), v);
   }
-  for (; v < end; v += TH) take(packs.raw(v), v);
 
   Sums acc = run.sums();
   const bool nan = acc.s != acc.s;
@@ -422,7 +503,7 @@ __global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
   }
   if (lane == 0) warps[warp] = {acc, wb};
   if constexpr (kTop)
-    block_top<T, TH>(packs, begin, end, a.k, best, best_pack, __syncthreads_or(nan), sh);
+    block_top<T, TH, G>(packs, begin, end, a.k, best, best_pack, __syncthreads_or(nan), sh);
   else
     __syncthreads();
   if (blocks > 1) {
@@ -746,13 +827,13 @@ int cluster_of(int64_t rows, int64_t packs) {
   return c;
 }
 
-template <typename T, int TH, bool kTop>
+template <typename T, int TH, int G>
 int launch_fwd(const Args& a, int c, cudaStream_t st) {
   if (a.rows * c > 0x7fffffff) return TT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));
   cfg.blockDim = dim3(TH);
-  cfg.dynamicSmemBytes = kTop ? sizeof(TopShared<TH>) : 0;
+  cfg.dynamicSmemBytes = G ? sizeof(TopShared<TH>) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -760,7 +841,7 @@ int launch_fwd(const Args& a, int c, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fwd_kernel<T, TH, kTop>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, fwd_kernel<T, TH, G>, a) == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
 template <typename T, int P>
@@ -777,17 +858,22 @@ int launch_short(const Args& a, cudaStream_t st) {
 template <typename T>
 int launch_fwd(const Args& a, cudaStream_t st) {
   const int64_t packs = a.V / Packs<T>::N;
-  // a row may lie across two packs more than its size asks for
-  if (packs + 2 <= 32) return launch_short<T, 1>(a, st);
-  if (packs + 2 <= 64) return launch_short<T, 2>(a, st);
-  if (packs + 2 <= 128) return launch_short<T, 4>(a, st);
-  if (packs + 2 <= 256) return launch_short<T, 8>(a, st);
+  // a row may lie across two packs more than its size asks for; with alternatives,
+  // a few rows are faster with more threads each (47 x 1,000 with 8: 6 us against
+  // 11; 4,096 with 64: 62 against 34)
+  if (a.k == 0 || a.rows >= 1024) {
+    if (packs + 2 <= 32) return launch_short<T, 1>(a, st);
+    if (packs + 2 <= 64) return launch_short<T, 2>(a, st);
+    if (packs + 2 <= 128) return launch_short<T, 4>(a, st);
+    if (packs + 2 <= 256) return launch_short<T, 8>(a, st);
+  }
   // (64 threads' largest are too few to bound many alternatives well)
   if (packs <= kFewPacks && a.k <= 16)
-    return a.k ? launch_fwd<T, kFewThreads, true>(a, 1, st)
-               : launch_fwd<T, kFewThreads, false>(a, 1, st);
+    return a.k ? launch_fwd<T, kFewThreads, 1>(a, 1, st) : launch_fwd<T, kFewThreads, 0>(a, 1, st);
   const int c = cluster_of(a.rows, packs);
-  return a.k ? launch_fwd<T, kThreads, true>(a, c, st) : launch_fwd<T, kThreads, false>(a, c, st);
+  if (a.k == 0) return launch_fwd<T, kThreads, 0>(a, c, st);
+  return packs / c >= 16 * kThreads ? launch_fwd<T, kThreads, 4>(a, c, st)
+                                    : launch_fwd<T, kThreads, 1>(a, c, st);
 }
 
 template <typename T, int TH>
