@@ -431,8 +431,12 @@ struct Part {
 // single packs would cost the memory a piece of 64 bytes or more each (4,096 x
 // 151,936 with sixteen: 305 us against 277), 1 where threads have few packs
 // (16,000 x 10,000: 248 against 297).
+//
+// (0 blocks an SM: left to the compiler, which then takes 48 registers; asked for
+// 1 it takes up to 80, and the loop without alternatives 234 us instead of 218.
+// With G = 4 four blocks are asked for: 277 against 281, 340 with five.)
 template <typename T, int TH, int G>
-__global__ void __launch_bounds__(TH) fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(TH, G == 4 ? 4 : 0) fwd_kernel(const Args a) {
   constexpr int W = TH / 32;
   constexpr bool kTop = G > 0;
   __shared__ Part warps[W];
