@@ -19,6 +19,11 @@
 // logit, from which the alternatives' candidates are found (block_top).  Few
 // rows are split over the blocks of a cluster, which meet in shared memory.
 // Backward: one pass from the four statistics a row that the forward keeps.
+//
+// Measured on a B200 (at the rate of a copy): 2,047 x 151,936 bf16: forward 117 us
+// (97; 101 with the maximum alone), backward 202 (194); 4,096 x 151,936 with sixteen
+// alternatives 283 (194): what they cost is the wait of the second look's loads
+// beside a busy memory.  One row of 151,936: 5.5 us, with eight alternatives 11.
 #include <cooperative_groups.h>
 
 #include <algorithm>

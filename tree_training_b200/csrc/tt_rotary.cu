@@ -10,7 +10,10 @@
 // A unit is V pairs of one head (two V-element packs, 16 bytes each where the
 // sizes allow).  A thread holds the V cosines and sines of its (token, unit)
 // in registers and walks over the heads, so the table is read once per token
-// and head group.
+// and head group.  Bound by HBM.  Measured on a B200, each way: 32,768 tokens, 32 +
+// 8 heads of 128, bf16: 115 us (5.8 TB/s; at the rate of a copy 107); 8,191 tokens,
+// 16 + 2 heads of 256 of which 64 dims turn, interleaved, views of a packed
+// projection: 28 us (24); 47 tokens: 2.2 us.
 #include <algorithm>
 
 #include "tt_vec.cuh"
