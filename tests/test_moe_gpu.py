@@ -225,3 +225,29 @@ def test_leaf_gradients_add_up():
     for _ in range(2):
         tt.expert_dispatch(x, plan).sum().backward()
     assert torch.equal(x.grad, torch.full_like(x, 2.0))
+
+
+@pytest.mark.parametrize("H", [2048, 2047])
+def test_offsets_over_32_bits(H):
+    # 2^31 elements and more of sorted rows; the last expert's rows lie behind them
+    T, k, E = (1 << 31) // (4 * H) + 40, 4, 4
+    ids = torch.arange(4, device=DEV).expand(T, 4).contiguous()
+    plan = tt.expert_plan(ids, E)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.zeros(T, H, dtype=BF, device=DEV)
+    rows = [0, T // 2, T - 1]
+    x[rows] = torch.randn(3, H, generator=g, device=DEV).to(BF)
+    x.requires_grad_(True)
+    w = torch.rand(T, k, generator=g, device=DEV, requires_grad=True)
+    xs = tt.expert_dispatch(x, plan)
+    for e in range(E):
+        assert torch.equal(xs[[e * T + r for r in rows]], x[rows])
+    y = tt.expert_combine(xs, w, plan)
+    wr, xr = w[rows].detach().double(), x[rows].detach().double()
+    check("y", y[rows].detach(), wr.sum(1, keepdim=True) * xr, wr.sum(1, keepdim=True) * xr.abs(), 5)
+    dy = torch.zeros_like(y)
+    dy[rows] = torch.randn(3, H, generator=g, device=DEV).to(BF)
+    dw, = torch.autograd.grad(y, [w], [dy])
+    dot = dy[rows].double() * xr
+    check("dw", dw[rows], dot.sum(1, keepdim=True).expand(3, 4),
+          dot.abs().sum(1, keepdim=True).expand(3, 4), H)

@@ -260,3 +260,30 @@ def test_differentiating_twice_is_refused():
     gs = torch.autograd.grad([y, r], [x], [dy, dr], create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(gs[0].sum(), [x])
+
+
+@pytest.mark.parametrize("D", [4096, 4098])
+def test_offsets_over_32_bits(D):
+    T = (1 << 31) // D + 70
+    rows = [0, 1, T // 2, T - 2, T - 1]
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.ones(T, D, dtype=BF, device=DEV)
+    r = torch.zeros(T, D, dtype=BF, device=DEV)
+    x[rows] = torch.randn(5, D, generator=g, device=DEV).to(BF)
+    r[rows] = torch.randn(5, D, generator=g, device=DEV).to(BF)
+    w = torch.ones(D, dtype=BF, device=DEV)
+    x.requires_grad_(True)
+    y, s = tt.residual_norm(x, r, w, scale=0.5)
+    d = {"x": x[rows].detach().double().requires_grad_(True), "residual": r[rows].double(),
+         "weight": w.double()}
+    yw, rw, mag, f = reference(d, 0.5, 1e-6, 0.0)
+    check("r", s[rows].detach(), rw.detach(), mag.detach(), 96)
+    check("y", y[rows].detach(), yw.detach(), (mag * f.abs()).detach(), 96)
+    dy = torch.zeros_like(y)
+    dy[rows] = torch.randn(5, D, generator=g, device=DEV).to(BF)
+    dx, = torch.autograd.grad(y, [x], [dy])
+    want, = torch.autograd.grad(yw, [d["x"]], [dy[rows].double()])
+    i2 = torch.rsqrt(rw.square().mean(-1, keepdim=True) + 1e-6)
+    an, gy = mag * i2, dy[rows].double().abs()
+    size = 0.5 * i2 * (gy + an * (gy * an).mean(-1, keepdim=True))
+    check("dx", dx[rows], want, size.detach(), 288)

@@ -165,3 +165,18 @@ def test_differentiating_twice_is_refused():
     g, = torch.autograd.grad(tt.apply_rotary(q, k, pos, table)[0].sum(), [q], create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), [q])
+
+
+def test_offsets_over_32_bits():
+    # 2^31 elements and more, read through a strided view
+    N, H, D = (1 << 17) + 3, 128, 128
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q = torch.zeros(N, H, D, dtype=torch.bfloat16, device=DEV)
+    rows = [0, (1 << 17) - 1, 1 << 17, N - 1]
+    q[rows] = torch.randn(4, H, D, generator=g, device=DEV).to(q.dtype)
+    pos = torch.randint(0, 513, (N,), generator=g, device=DEV)
+    table = tt.rotary_table(513, D, 1e4, device=DEV)
+    got, _ = tt.apply_rotary(q, None, pos, table)
+    check("q", got[rows], *turned(q[rows], pos[rows], table, False), 4)
+    k = q.transpose(0, 1).contiguous().transpose(0, 1)          # head-major storage
+    assert torch.equal(tt.apply_rotary(k, None, pos, table)[0][rows], got[rows])
