@@ -594,7 +594,10 @@ __global__ void __launch_bounds__(1024, 1) ring_fwd(const Args a, const Ring rin
   if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
 }
 
-template <typename T, typename R, bool kFullForm, int kThreads, bool kByChannel>
+// Q: packs of 8 elements a thread, a block's threads apart. kShared: the weights'
+// sums lie behind the stages, each read and written by its own thread alone.
+template <typename T, typename R, bool kFullForm, int kThreads, bool kByChannel, int Q,
+          bool kShared>
 __global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring ring) {
   constexpr int N = kFullForm ? 3 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -602,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring
   __shared__ uint64_t full[kMaxStages];
   __shared__ int32_t abort_flag;
   const int D = a.D, t = threadIdx.x, S = ring.stages;
-  const bool in = t * 8 < D;
+  auto index = [&](int q) { return q * (int)blockDim.x + t; };       // of a pack of the row
+  auto in = [&](int q) { return index(q) * 8 < D; };
   const bool post = kFullForm && a.w1, gated = kFullForm && a.gate_mode == kFull;
   const bool by_row = kFullForm && a.gate_mode == kRow;
   const int x_bytes = D * (int)sizeof(T), r_bytes = D * (int)sizeof(R);
@@ -636,16 +640,43 @@ __global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring
   };
   if (t == 0)
     for (int i = 0; i < S; ++i) issue(blockIdx.x + (int64_t)i * gridDim.x, i);
-  Raw8<T> rw2, rw1, rwg;
-  rw2.zero(), rw1.zero(), rwg.zero();
-  if (in) {
-    rw2.read(reinterpret_cast<const uint8_t*>(a.w2), t);
-    if (post) rw1.read(reinterpret_cast<const uint8_t*>(a.w1), t);
-    if (kByChannel) rwg.read(reinterpret_cast<const uint8_t*>(a.gate), t);
-  }
-  float dw2[8], dw1[8], dgc[8];
+  Raw8<T> rw2[Q], rw1[Q], rwg[Q];
+  // the weights' sums over the block's rows, in registers or behind the stages
+  constexpr int kHeld = kShared ? 1 : Q;
+  float dw2[kHeld][8], dw1[kHeld][8], dgc[kHeld][8];
+  float4* sums = reinterpret_cast<float4*>(smem + S * ring.stage_bytes);
+  auto at_sum = [&](int plane, int q, int half) {
+    return sums + ((plane * Q + q) * 2 + half) * (int)blockDim.x + t;
+  };
+  auto held = [&](float (&v)[kHeld][8], int plane, int q) -> float (&)[8] {
+    if constexpr (kShared) {
+      const float4 lo = *at_sum(plane, q, 0), hi = *at_sum(plane, q, 1);
+      v[0][0] = lo.x, v[0][1] = lo.y, v[0][2] = lo.z, v[0][3] = lo.w;
+      v[0][4] = hi.x, v[0][5] = hi.y, v[0][6] = hi.z, v[0][7] = hi.w;
+    }
+    return v[kShared ? 0 : q];
+  };
+  auto keep = [&](float (&v)[8], int plane, int q) {
+    if constexpr (kShared) {
+      *at_sum(plane, q, 0) = make_float4(v[0], v[1], v[2], v[3]);
+      *at_sum(plane, q, 1) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  };
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw2[e] = dw1[e] = dgc[e] = 0.f;
+  for (int q = 0; q < Q; ++q) {
+    rw2[q].zero(), rw1[q].zero(), rwg[q].zero();
+    if (in(q)) {
+      rw2[q].read(reinterpret_cast<const uint8_t*>(a.w2), index(q));
+      if (post) rw1[q].read(reinterpret_cast<const uint8_t*>(a.w1), index(q));
+      if (kByChannel) rwg[q].read(reinterpret_cast<const uint8_t*>(a.gate), index(q));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      dw2[kShared ? 0 : q][e] = dw1[kShared ? 0 : q][e] = dgc[kShared ? 0 : q][e] = 0.f;
+    keep(dw2[kShared ? 0 : q], 0, q);
+    if (post) keep(dw1[kShared ? 0 : q], 1, q);
+    if (kByChannel) keep(dgc[kShared ? 0 : q], 2, q);
+  }
   int stage = 0, turn = 0;
   uint32_t phase = 0;
   // a row's own values are fetched a row ahead
@@ -665,88 +696,95 @@ __global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring
       *(volatile int32_t*)&abort_flag = 1;
     }
     const uint8_t* at = smem + stage * ring.stage_bytes;
-    Raw8<T> rx, rg;
-    float r[8], d[8], s[N];
-    rx.zero(), rg.zero();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = d[e] = 0.f;
+    Raw8<T> rx[Q], rg[Q];
+    float r[Q][8], d[Q][8], s[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = 0.f;
-    if (in) {
-      rx.read(at, t);
-      if (gated) rg.read(at + at_g, t);
+    const float ki = kFullForm ? k * i1 : k;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      rx[q].zero(), rg[q].zero();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[q][e] = d[q][e] = 0.f;
+      if (!in(q)) continue;
+      rx[q].read(at, index(q));
+      if (gated) rg[q].read(at + at_g, index(q));
       if (a.res) {
-        Raw8<R> q;
-        q.read(at + at_r, t);
-        q.get(r);
+        Raw8<R> raw;
+        raw.read(at + at_r, index(q));
+        raw.get(r[q]);
       }
       if (a.dr) {
-        Raw8<R> q;
-        q.read(at + at_dr, t);
-        q.get(d);
+        Raw8<R> raw;
+        raw.read(at + at_dr, index(q));
+        raw.get(d[q]);
       }
       float x[8], u[8], w[8], dy[8];
       Raw8<T> ry;
       if (a.dy)
-        ry.read(at + at_dy, t);
+        ry.read(at + at_dy, index(q));
       else
         ry.zero();
       ry.get(dy);
-      rx.get(x);
+      rx[q].get(x);
       if (kFullForm) {
         // u x: the block's output without scale, row gate and i1
         if (post) {
-          rw1.get(u);
+          rw1[q].get(u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= a.offset + u[e];
         }
         if (gated || kByChannel) {
-          (kByChannel ? rwg : rg).get(u);
+          (kByChannel ? rwg[q] : rg[q]).get(u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= u[e];
         }
       }
-      const float ki = kFullForm ? k * i1 : k;
-      rw2.get(w);
+      rw2[q].get(w);
+      float (&sum2)[8] = held(dw2, 0, q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        r[e] = fmaf(ki, x[e], r[e]);
+        r[q][e] = fmaf(ki, x[e], r[q][e]);
         const float gy = dy[e] * (a.offset + w[e]);
-        dw2[e] = fmaf(dy[e] * i2, r[e], dw2[e]);
-        d[e] = fmaf(i2, gy, d[e]);               // a
-        s[0] = fmaf(gy, r[e], s[0]);
+        sum2[e] = fmaf(dy[e] * i2, r[q][e], sum2[e]);
+        d[q][e] = fmaf(i2, gy, d[q][e]);               // a
+        s[0] = fmaf(gy, r[q][e], s[0]);
         if constexpr (kFullForm) {
-          s[1] = fmaf(x[e], d[e], s[1]);
-          s[2] = fmaf(x[e], r[e], s[2]);
+          s[1] = fmaf(x[e], d[q][e], s[1]);
+          s[2] = fmaf(x[e], r[q][e], s[2]);
         }
       }
+      keep(sum2, 0, q);
     }
     block_sum<N>(s, red[turn]);
     turn ^= 1;
     if (t == 0) issue(row + (int64_t)S * gridDim.x, stage);
     if (++stage == S) stage = 0, phase ^= 1;
     const float c = i2 * i2 * i2 * s[0] * inv_D;
-    if (in) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = fmaf(-c, r[e], d[e]);
-      if (a.dres) put8<R>(reinterpret_cast<R*>(a.dres) + row * D, t, d);
-    }
-    if constexpr (!kFullForm) {
-      if (in && a.dx) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] *= k;
-        put8<T>(reinterpret_cast<T*>(a.dx) + row * D, t, d);
-      }
-    } else {
-      const float dot = s[1] - c * s[2];         // sum of u x d
-      const float back = post ? k * i1 * i1 * i1 * dot * inv_D : 0.f;
+    float dot = 0.f, back = 0.f;
+    if constexpr (kFullForm) {
+      dot = s[1] - c * s[2];                     // sum of u x d
+      back = post ? k * i1 * i1 * i1 * dot * inv_D : 0.f;
       if (by_row && t == 0 && a.dgate)
         reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(a.scale * i1 * dot);
-      if (in) {
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (!in(q)) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[q][e] = fmaf(-c, r[q][e], d[q][e]);
+      if (a.dres) put8<R>(reinterpret_cast<R*>(a.dres) + row * D, index(q), d[q]);
+      if constexpr (!kFullForm) {
+        if (a.dx) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[q][e] *= k;
+          put8<T>(reinterpret_cast<T*>(a.dx) + row * D, index(q), d[q]);
+        }
+      } else {
         float x[8], w[8], g[8];
-        rx.get(x);
+        rx[q].get(x);
         if (post) {
-          rw1.get(w);
+          rw1[q].get(w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] += a.offset;
         } else {
@@ -754,37 +792,42 @@ __global__ void __launch_bounds__(kThreads, 1) ring_bwd(const Args a, const Ring
           for (int e = 0; e < 8; ++e) w[e] = 1.f;
         }
         if (gated || kByChannel) {
-          (kByChannel ? rwg : rg).get(g);
+          (kByChannel ? rwg[q] : rg[q]).get(g);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) g[e] = 1.f;
         }
+        float (&sum1)[8] = held(dw1, post ? 1 : 0, q);
+        float (&sumg)[8] = held(dgc, kByChannel ? 2 : 0, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float xd = i1 * x[e] * d[e], kg = k * g[e];
-          dw1[e] = fmaf(kg, xd, dw1[e]);
-          if (kByChannel) dgc[e] = fmaf(a.scale * w[e], xd, dgc[e]);
-          r[e] = fmaf(-back, x[e], i1 * (kg * d[e]) * w[e]);     // dx
-          d[e] = a.scale * w[e] * xd;                            // the element's gate
+          const float xd = i1 * x[e] * d[q][e], kg = k * g[e];
+          if (post) sum1[e] = fmaf(kg, xd, sum1[e]);
+          if (kByChannel) sumg[e] = fmaf(a.scale * w[e], xd, sumg[e]);
+          r[q][e] = fmaf(-back, x[e], i1 * (kg * d[q][e]) * w[e]);     // dx
+          d[q][e] = a.scale * w[e] * xd;                               // the element's gate
         }
-        if (a.dx) put8<T>(reinterpret_cast<T*>(a.dx) + row * D, t, r);
-        if (gated && a.dgate) put8<T>(reinterpret_cast<T*>(a.dgate) + row * D, t, d);
+        if (post) keep(sum1, 1, q);
+        if (kByChannel) keep(sumg, 2, q);
+        if (a.dx) put8<T>(reinterpret_cast<T*>(a.dx) + row * D, index(q), r[q]);
+        if (gated && a.dgate) put8<T>(reinterpret_cast<T*>(a.dgate) + row * D, index(q), d[q]);
       }
     }
   }
   if (t == 0 && *(volatile int32_t*)&abort_flag) land(full, S, issued);
-  if (in) {
-    float* part = a.part + (int64_t)blockIdx.x * D + t * 8;
+  const int64_t plane = (int64_t)gridDim.x * D;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[e] = dw2[e];
-    const int64_t plane = (int64_t)gridDim.x * D;
-    if (post) {
+  for (int q = 0; q < Q; ++q) {
+    if (!in(q)) continue;
+    float* part = a.part + (int64_t)blockIdx.x * D + index(q) * 8;
+    float (&sum2)[8] = held(dw2, 0, q);
+    float (&sum1)[8] = held(dw1, post ? 1 : 0, q);
+    float (&sumg)[8] = held(dgc, kByChannel ? 2 : 0, q);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[plane + e] = dw1[e];
-    }
-    if (kByChannel) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) part[2 * plane + e] = dgc[e];
+    for (int e = 0; e < 8; ++e) {
+      part[e] = sum2[e];
+      if (post) part[plane + e] = sum1[e];
+      if (kByChannel) part[2 * plane + e] = sumg[e];
     }
   }
 }
@@ -893,21 +936,40 @@ int launch(const Args& a, int pack, bool full, Shape s, int blocks, cudaStream_t
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
-int ring_threads(int D) { return (D / 8 + 31) / 32 * 32; }
+// Threads of a block of the ring: a pack of 8 elements each, or two.
+int ring_threads(int D, bool two) {
+  const int packs = D / 8;
+  return ((two ? (packs + 1) / 2 : packs) + 31) / 32 * 32;
+}
 
-// The ring's shape: as many blocks an SM as threads and registers allow (64 a
-// thread) while each has two stages or more; blocks 0: rows go straight to
-// registers.
+// Whether the backward's threads take two packs each. The full form keeps 128
+// registers a thread, so 512 threads an SM: above 4,096 one row needs two packs.
+// The weights' sums then lie in shared memory behind the stages (in registers
+// they spill, past an L1 that the stages leave no room: 8,000 x 5,120 fully
+// gated 252 us forward and backward, 339 in registers). Below, 16-bit rows
+// gain by it from 1,024 on (20,480 x 2,048 post weight and row gate: 194 us,
+// one pack 210; 40,960 x 1,024 fully gated 226, one pack 217), others do not
+// (10,240 x 4,096, 32-bit residual: 268, one pack 258; 4,000 x 2,560 in 32 bits
+// 159 and 111; a gate by channel, with its third sum, at 10,240 x 4,096 227 and 215).
+bool two_packs(int D, bool full, bool channel, int widest) {
+  return full && (D > 4096 || (D > 1024 && widest == 2 && !channel));
+}
+
+// The ring's shape: as many blocks an SM as `most` threads allow (1,024 with 64
+// registers each, 512 with 128) while each has two stages or more beside its
+// sum_bytes; blocks 0: rows go straight to registers. The full form's backward
+// spills in 64 registers: 40,960 x 1,024 fully gated 267 us with 1,024 threads.
 struct RingShape {
-  int blocks, stages, stage_bytes, per_sm;
+  int blocks, stages, stage_bytes, per_sm, sum_bytes;
 };
 
-constexpr int kSharedPerSM = 225 * 1024, kSharedOwn = 2048;   // kSharedOwn: static, reserved
+constexpr int kSharedPerSM = 228 * 1024, kSharedOwn = 2048;   // kSharedOwn: static, reserved
 
-RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes, int most = 1024) {
-  RingShape best{0, 0, stage_bytes, 0};
+RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes, int most = 1024,
+                  int sum_bytes = 0) {
+  RingShape best{0, 0, stage_bytes, 0, sum_bytes};
   for (int per = most / threads; per > 0; --per) {
-    const int stages = std::min(kMaxStages, (kSharedPerSM / per - kSharedOwn) / stage_bytes);
+    const int stages = std::min(kMaxStages, (kSharedPerSM / per - kSharedOwn - sum_bytes) / stage_bytes);
     if (stages >= 2) {
       best.blocks = (int)std::min<int64_t>(rows, (int64_t)vec::kSMs * per);
       best.stages = stages;
@@ -929,19 +991,23 @@ template <typename T, typename R, bool kBwd>
 int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, int32_t* status,
                 cudaStream_t st) {
   const Ring ring{shape.stages, shape.stage_bytes, status};
-  const int smem = shape.stages * shape.stage_bytes;
+  const int smem = shape.stages * shape.stage_bytes + shape.sum_bytes;
   auto go = [&](auto kern) -> int {
     TT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     kern<<<shape.blocks, threads, smem, st>>>(a, ring);
     return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
   };
   if constexpr (kBwd) {
-    // with 512 threads or fewer on an SM they may use 128 registers each
-    const bool wide = shape.per_sm * threads <= 512;
-    if (!full) return go(ring_bwd<T, R, false, 1024, false>);
-    if (a.gate_mode == kChannel)
-      return wide ? go(ring_bwd<T, R, true, 512, true>) : go(ring_bwd<T, R, true, 1024, true>);
-    return wide ? go(ring_bwd<T, R, true, 512, false>) : go(ring_bwd<T, R, true, 1024, false>);
+    if (!full) return go(ring_bwd<T, R, false, 1024, false, 1, false>);
+    const bool channel = a.gate_mode == kChannel;
+    if (shape.sum_bytes)
+      return channel ? go(ring_bwd<T, R, true, 512, true, 2, true>)
+                     : go(ring_bwd<T, R, true, 512, false, 2, true>);
+    if (threads * 8 < a.D)
+      return channel ? go(ring_bwd<T, R, true, 512, true, 2, false>)
+                     : go(ring_bwd<T, R, true, 512, false, 2, false>);
+    return channel ? go(ring_bwd<T, R, true, 512, true, 1, false>)
+                   : go(ring_bwd<T, R, true, 512, false, 1, false>);
   } else {
     if (!full) return go(ring_fwd<T, R, false, false>);
     return a.gate_mode == kChannel ? go(ring_fwd<T, R, true, true>)
@@ -1017,11 +1083,11 @@ extern "C" int tt_residual_norm_fwd(int dtype, int res_dtype, int64_t rows, int3
   const int blocks = (int)std::min<int64_t>(want, tt::vec::kSMs * 16ll);
   RingShape ring{};
   if (rows_by_ring(D, dtype, pack == kAligned, a))
-    ring = ring_of(rows, D, ring_threads(D),
+    ring = ring_of(rows, D, ring_threads(D, false),
                    D * (size_of(dtype) * (gate_mode == kFull ? 2 : 1) +
                         (residual ? size_of(res_dtype) : 0)));
   const int rc = ring.blocks
-                     ? dispatch_ring<false>(dtype, res_dtype, a, ring_threads(D), ring, status,
+                     ? dispatch_ring<false>(dtype, res_dtype, a, ring_threads(D, false), ring, status,
                                             (cudaStream_t)stream)
                      : dispatch<false>(dtype, res_dtype, a, pack, s, blocks, (cudaStream_t)stream);
   if (rc == TT_OK) tt_count_launches(1);
@@ -1032,8 +1098,8 @@ extern "C" int tt_residual_norm_bwd_blocks(int64_t rows, int32_t D) {
   using namespace tt::resnorm;
   if (rows <= 0 || D <= 0 || D > kMaxD) return 1;
   const Shape s = shape_of(D);
-  // (the ring's blocks are of one row)
-  const int threads = D > 512 && D <= 8192 ? ring_threads(D) : s.tpr * s.per;
+  // (the ring's blocks are of one row; with two packs a thread they are no more)
+  const int threads = D > 512 && D <= 8192 ? ring_threads(D, false) : s.tpr * s.per;
   return (int)std::max<int64_t>(
       1, std::min<int64_t>(rows, tt::vec::kSMs * (int64_t)std::max(1, 1024 / threads)));
 }
@@ -1071,12 +1137,18 @@ extern "C" int tt_residual_norm_bwd(
   };
   const int pack = fits(8) ? kAligned : fits(2) ? kPairs : s.tpr >= 32 ? kShifted : kSingle;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool full = post_weight || gate_mode != kNone, channel = gate_mode == kChannel;
+  const bool two = two_packs(D, full, channel, std::max(xs, rs));
+  const int threads = ring_threads(D, two), most = full ? 512 : 1024;
   RingShape ring{};
-  if (rows_by_ring(D, dtype, pack == kAligned, a))
-    ring = ring_of(rows, D, ring_threads(D),
-                   D * (size_of(dtype) * (1 + (dy ? 1 : 0) + (gate_mode == kFull ? 1 : 0)) +
-                        size_of(res_dtype) * ((residual ? 1 : 0) + (dr ? 1 : 0))),
-                   gate_mode == kChannel && D <= 4096 ? 512 : 1024);   // for 128 registers
+  if (rows_by_ring(D, dtype, pack == kAligned, a)) {
+    const int stage_bytes = D * (xs * (1 + (dy ? 1 : 0) + (gate_mode == kFull ? 1 : 0)) +
+                                 rs * ((residual ? 1 : 0) + (dr ? 1 : 0)));
+    if (two)
+      ring = ring_of(rows, D, threads, stage_bytes, most,
+                     threads * 64 * (channel ? 3 : post_weight ? 2 : 1));
+    if (!ring.blocks) ring = ring_of(rows, D, threads, stage_bytes, most);
+  }
   if (ring.blocks)
     ring.blocks = blocks = std::min(blocks, ring.blocks);
   else
@@ -1084,7 +1156,7 @@ extern "C" int tt_residual_norm_bwd(
         {blocks, (rows + s.per - 1) / s.per,
          tt::vec::kSMs * (int64_t)std::max(1, 1024 / (s.tpr * s.per))});
   const int rc = ring.blocks
-                     ? dispatch_ring<true>(dtype, res_dtype, a, ring_threads(D), ring, status, st)
+                     ? dispatch_ring<true>(dtype, res_dtype, a, threads, ring, status, st)
                      : dispatch<true>(dtype, res_dtype, a, pack, s, blocks, st);
   if (rc != TT_OK) return rc;
   Out out{};
