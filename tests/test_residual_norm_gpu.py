@@ -287,3 +287,14 @@ def test_offsets_over_32_bits(D):
     an, gy = mag * i2, dy[rows].double().abs()
     size = 0.5 * i2 * (gy + an * (gy * an).mean(-1, keepdim=True))
     check("dx", dx[rows], want, size.detach(), 288)
+
+
+@pytest.mark.parametrize("post,gate", [(True, "none"), (True, "row"), (True, "full"),
+                                       (True, "channel"), (False, "channel"), (False, "full")])
+@pytest.mark.parametrize("D,dtype,res", [
+    (1032, BF, BF), (1536, F16, F16), (2576, BF, F32), (4104, BF, BF), (5120, BF, F32),
+    (8192, BF, BF), (4104, F32, F32), (5120, F32, F32),
+])
+def test_many_rows_a_block(D, dtype, res, post, gate):
+    # the weights' sums over rows that pass round the stages several times
+    run(3001, D, dtype, res, post, gate, scale=0.5)
