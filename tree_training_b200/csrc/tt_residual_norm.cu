@@ -950,9 +950,15 @@ int ring_threads(int D, bool two) {
 // gain by it from 1,024 on (20,480 x 2,048 post weight and row gate: 194 us,
 // one pack 210; 40,960 x 1,024 fully gated 226, one pack 217), others do not
 // (10,240 x 4,096, 32-bit residual: 268, one pack 258; 4,000 x 2,560 in 32 bits
-// 159 and 111; a gate by channel, with its third sum, at 10,240 x 4,096 227 and 215).
-bool two_packs(int D, bool full, bool channel, int widest) {
-  return full && (D > 4096 || (D > 1024 && widest == 2 && !channel));
+// 159 and 111; a gate by channel, with its third sum, at 10,240 x 4,096 227 and
+// 215), unless one pack leaves an SM a single block of 5/8 of its threads or less
+// and x is of 16 bits (16,384 x 2,560: gate by channel 228, one pack 253; 32-bit
+// residual 259 and 291; at 2,816, 352 threads, 257 and 244 by channel).
+bool two_packs(int D, bool full, bool channel, int x_size, int res_size) {
+  if (!full) return false;
+  const int one = ring_threads(D, false);
+  return D > 4096 || (D > 1024 && x_size == 2 && res_size == 2 && !channel) ||
+         (x_size == 2 && one > 256 && one <= 320);
 }
 
 // The ring's shape: as many blocks an SM as `most` threads allow (1,024 with 64
@@ -1138,7 +1144,7 @@ extern "C" int tt_residual_norm_bwd(
   const int pack = fits(8) ? kAligned : fits(2) ? kPairs : s.tpr >= 32 ? kShifted : kSingle;
   cudaStream_t st = (cudaStream_t)stream;
   const bool full = post_weight || gate_mode != kNone, channel = gate_mode == kChannel;
-  const bool two = two_packs(D, full, channel, std::max(xs, rs));
+  const bool two = two_packs(D, full, channel, xs, rs);
   const int threads = ring_threads(D, two), most = full ? 512 : 1024;
   RingShape ring{};
   if (rows_by_ring(D, dtype, pack == kAligned, a)) {
