@@ -47,6 +47,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Exponents of 2 are kept from -inf, whose product with a probability of 0
 // would be NaN; 2^-200 is 0 in fp32.
 constexpr float kFloor = -200.f;
+constexpr float kGradFloor = -300.f;
 // The reference moves when the maximum is this far (a factor of 2^12) above it.
 constexpr float kSlack = 12.f;
 
@@ -56,15 +57,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 2^x; the forward's sums do without results under 2^-126 (three instructions
-// less), gradients keep them.
-template <bool kSubnormal = false>
+// 2^x, 0 where that is under 2^-126.
 __device__ __forceinline__ float ex2(float x) {
   float r;
-  if constexpr (kSubnormal)
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  else
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -765,9 +761,14 @@ __global__ void __launch_bounds__(TH) bwd_kernel(const BwdArgs a) {
   const float gH = a.g_ent ? a.g_ent[row] : 0.f;
   const float A = empty ? 0.f : -(G + gH * (st.w - st.y)) * st.z * inv_t;
   const float B = empty ? 0.f : -gH * kLn2 * st.z * inv_t;
+  // Under 2^-126 the exponential is formed 2^100 times as large and the product
+  // scaled back, so that it alone is rounded to a subnormal; the floor still
+  // gives 0.
   auto base = [&](float v) {
-    const float t = max_nan((v - ref) * c, kFloor);
-    return ex2<true>(t) * fmaf(B, t, A);
+    const float t = max_nan((v - ref) * c, kGradFloor);
+    const bool low = t < -126.f;
+    const float r = ex2(low ? t + 100.f : t) * fmaf(B, t, A);
+    return low ? r * 0x1p-100f : r;
   };
   auto fetch = [&](int v) -> uint4 {
     if (same && to.whole(v))
