@@ -240,10 +240,12 @@ struct Args {
   float* stats;              // [rows][4]: m (of x), ln s, 1 / s (0: empty row), H
 };
 
-// log probability of logit x, in the order a softmax takes its steps
+// Log probability of logit x.  The maximum is subtracted before the division, as
+// in the sums: the type's lowest value overflows when it is divided by a
+// temperature under 1.
 __device__ __forceinline__ float logp_of(float x, float m, float ln_s, float inv_s, float temp) {
   if (inv_s == 0.f) return -INFINITY;
-  return (x / temp - m / temp) - ln_s;
+  return (x - m) / temp - ln_s;
 }
 
 constexpr int kUnroll = 4;        // packs in flight a thread
