@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_rank(const PlanArgs a) {
       a.counts[(int64_t)blockIdx.x * (E + 1) + x] = warps_of(x, 0, true);
   }
   __syncthreads();
-  // a warp's atomics on its own counters take effect in the order of its steps
+  // The warp's counters hand out ranks in the order of its steps: each step's
+  // leaders add theirs before the lanes part again for the next step's.
   const bool kept = end - begin <= 32 * kSteps;        // the ids are still in e
   for (int64_t from = begin; from < end; from += 32 * kSteps) {
     if (!kept) fetch(from);
@@ -151,6 +152,7 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_rank(const PlanArgs a) {
       base[s] = 0;
       if (e[s] <= E && lane == __ffs(same[s]) - 1)
         base[s] = atomicAdd(mine + e[s], __popc(same[s]));
+      __syncwarp();
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
