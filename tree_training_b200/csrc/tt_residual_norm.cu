@@ -966,20 +966,19 @@ bool two_packs(int D, bool full, bool channel, int x_size, int res_size) {
 // sum_bytes; blocks 0: rows go straight to registers. The full form's backward
 // spills in 64 registers: 40,960 x 1,024 fully gated 267 us with 1,024 threads.
 struct RingShape {
-  int blocks, stages, stage_bytes, per_sm, sum_bytes;
+  int blocks, stages, stage_bytes, sum_bytes;
 };
 
 constexpr int kSharedPerSM = 228 * 1024, kSharedOwn = 2048;   // kSharedOwn: static, reserved
 
 RingShape ring_of(int64_t rows, int D, int threads, int stage_bytes, int most = 1024,
                   int sum_bytes = 0) {
-  RingShape best{0, 0, stage_bytes, 0, sum_bytes};
+  RingShape best{0, 0, stage_bytes, sum_bytes};
   for (int per = most / threads; per > 0; --per) {
     const int stages = std::min(kMaxStages, (kSharedPerSM / per - kSharedOwn - sum_bytes) / stage_bytes);
     if (stages >= 2) {
       best.blocks = (int)std::min<int64_t>(rows, (int64_t)vec::kSMs * per);
       best.stages = stages;
-      best.per_sm = per;
       break;
     }
   }
@@ -998,8 +997,11 @@ int launch_ring(const Args& a, bool full, int threads, const RingShape& shape, i
                 cudaStream_t st) {
   const Ring ring{shape.stages, shape.stage_bytes, status};
   const int smem = shape.stages * shape.stage_bytes + shape.sum_bytes;
+  // (the limit belongs to the kernel, not to the call: it is the same for every
+  // size, since another thread may set it between here and the launch)
   auto go = [&](auto kern) -> int {
-    TT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    TT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kSharedPerSM - kSharedOwn));
     kern<<<shape.blocks, threads, smem, st>>>(a, ring);
     return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
   };
