@@ -70,6 +70,13 @@ void need_int(const char* op, const char* what, const Tensor& t) {
     type_error(std::string(op) + ": int64/int32 " + what + " required");
 }
 
+// The C ABI's sizes have 32 bits: larger ones are refused, not cut off.
+void need_size(const char* op, const char* what, int64_t n) {
+  if (n > 0x7fffffff)
+    value_error(std::string(op) + ": " + what + " of " + std::to_string(n) +
+                " is over the limit of 2^31 - 1");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -201,6 +208,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
   if (logits.dim() != 2 || logits.size(1) < 1)
     value_error("token_logprobs: logits must be [rows, V]");
   const int64_t T = logits.size(0), V = logits.size(1);
+  need_size(op, "a vocabulary", V);
   if (k < 0 || k > std::min(max_k, V))
     value_error("token_logprobs: top_k must be in [0, " + std::to_string(std::min(max_k, V)) + "]");
   if (!(temperature > 0.0 && temperature < INFINITY))
@@ -211,6 +219,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
     if (tokens.dim() < 1 || tokens.dim() > 2 || tokens.size(0) != T)
       value_error("token_logprobs: tokens must be [rows] or [rows, M]");
     tok = tokens.dim() == 2 ? tokens : tokens.unsqueeze(1);
+    need_size(op, "a number of tokens a row", tok.size(1));
     tok = tok.to(at::kLong).contiguous();
   } else {
     tok = empty({T, 0}, logits, at::kLong);
@@ -301,6 +310,8 @@ std::tuple<Tensor, OptTensor> apply_rotary(const Tensor& q, const OptTensor& k_,
   if (R < 2 || R % 2 || R > q.size(2))
     value_error("apply_rotary: the table's width must be even and at most the head dim");
   if (q.size(1) < 1) value_error("apply_rotary: q has no heads");
+  need_size(op, "a number of heads", q.size(1) + (k.defined() ? k.size(1) : 0));
+  need_size(op, "a head dim", q.size(2));
   const Tensor pos = positions.contiguous(), table = table_.contiguous();
   if (wants_grad({&q, &k})) {
     variable_list v = RotaryFunction::apply(q, k_, pos, table, interleaved);
@@ -587,6 +598,7 @@ void check_rows(const char* op, const char* name, const Tensor& t, int64_t rows,
     type_error(std::string(op) + ": float32/bfloat16/float16 " + name + " required");
   if (t.dim() != 2 || t.size(0) != rows || t.size(1) < 1)
     value_error(std::string(op) + ": " + name + " must be [" + std::to_string(rows) + ", H]");
+  need_size(op, "a row's width", t.size(1));
 }
 
 Tensor expert_dispatch(const Tensor& x_, const Tensor& slots, const Tensor& offsets) {
