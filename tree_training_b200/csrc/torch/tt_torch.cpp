@@ -77,6 +77,14 @@ void need_size(const char* op, const char* what, int64_t n) {
                 " is over the limit of 2^31 - 1");
 }
 
+// There are no forward-mode derivatives: a result without its tangent would be
+// wrong without a word.  (A tangent counts with gradients turned off, too.)
+void no_tangent(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      throw std::runtime_error(std::string(op) + ": forward-mode derivatives are not supported");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -175,6 +183,7 @@ struct LogprobsFunction : Function<LogprobsFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return variable_list(4);
+    no_tangent("token_logprobs", {&g[0], &g[1], &g[2]});
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &tokens = s[1], &top_tok = s[2], &stats = s[3];
     for (int i = 0; i < 3; ++i)
@@ -224,6 +233,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
   } else {
     tok = empty({T, 0}, logits, at::kLong);
   }
+  no_tangent(op, {&logits});
   const Tensor x = rows2d(logits);
   Logprobs r;
   if (wants_grad({&logits})) {
@@ -279,6 +289,7 @@ struct RotaryFunction : Function<RotaryFunction> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor gk = g.size() > 1 ? g[1] : Tensor();
     variable_list grads(5);
+    no_tangent("apply_rotary", {&g[0], &gk});
     if (g[0].defined() || gk.defined()) {
       auto r = turn(g[0], gk, s[0], s[1], ctx->saved_data["interleaved"].toBool(), true);
       grads[0] = r.first, grads[1] = r.second;
@@ -312,6 +323,7 @@ std::tuple<Tensor, OptTensor> apply_rotary(const Tensor& q, const OptTensor& k_,
   if (q.size(1) < 1) value_error("apply_rotary: q has no heads");
   need_size(op, "a number of heads", q.size(1) + (k.defined() ? k.size(1) : 0));
   need_size(op, "a head dim", q.size(2));
+  no_tangent(op, {&q, &k, &table_});
   const Tensor pos = positions.contiguous(), table = table_.contiguous();
   if (wants_grad({&q, &k})) {
     variable_list v = RotaryFunction::apply(q, k_, pos, table, interleaved);
@@ -367,6 +379,7 @@ struct NormFunction : Function<NormFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     variable_list grads(9);
     if (!g[0].defined() && !g[1].defined()) return grads;
+    no_tangent("residual_norm", {&g[0], &g[1]});
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &res = s[1], &w = s[2], &post = s[3], &gate = s[4], &stats = s[5];
     const int64_t mode = ctx->saved_data["mode"].toInt();
@@ -462,6 +475,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& resid
     else
       value_error("residual_norm: gate must be [D], [..., 1] or [..., D]");
   }
+  no_tangent(op, {&x, &residual, &weight, &post, &gate});
   const bool two = x.dim() == 2;
   auto flat = [&](const Tensor& t) {
     if (!t.defined()) return t;
@@ -561,6 +575,7 @@ struct DispatchFunction : Function<DispatchFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    no_tangent("expert_dispatch", {&g[0]});
     return once("expert_dispatch",
                 {collect_rows(g[0].contiguous(), Plan(s[0], s[1])), Tensor(), Tensor()});
   }
@@ -576,6 +591,7 @@ struct CombineFunction : Function<CombineFunction> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &ys = s[0], &w = s[1];
     const Plan p(s[2], s[3]);
+    no_tangent("expert_combine", {&g[0]});
     const Tensor dy = g[0].contiguous();
     Tensor dys = empty(ys.sizes(), ys, ys.scalar_type()), dw = empty(w.sizes(), w, w.scalar_type());
     {
@@ -603,6 +619,7 @@ void check_rows(const char* op, const char* name, const Tensor& t, int64_t rows,
 
 Tensor expert_dispatch(const Tensor& x_, const Tensor& slots, const Tensor& offsets) {
   check_rows("expert_dispatch", "x", x_, slots.size(0), slots);
+  no_tangent("expert_dispatch", {&x_});
   const Tensor x = x_.contiguous();
   if (wants_grad({&x})) return DispatchFunction::apply(x, slots, offsets);
   return dispatch_rows(x, Plan(slots, offsets));
@@ -618,6 +635,7 @@ Tensor expert_combine(const Tensor& ys_, const Tensor& weights, const Tensor& sl
   if (weights.sizes() != slots.sizes())
     value_error("expert_combine: weights must be [" + std::to_string(slots.size(0)) + ", " +
                 std::to_string(slots.size(1)) + "]");
+  no_tangent(op, {&ys_, &weights});
   const Tensor ys = ys_.contiguous(), w = weights.contiguous();
   if (wants_grad({&ys, &w})) return CombineFunction::apply(ys, w, slots, offsets);
   return combine_rows(ys, w, Plan(slots, offsets));
