@@ -532,7 +532,8 @@ int64_t tt_moe_plan_workspace_size(int64_t n_entries, int32_t n_experts);
 int tt_moe_plan(const void* ids, int ids64, int64_t n_entries, int32_t n_experts, int32_t* slots,
                 int32_t* entries, int32_t* offsets, void* workspace, int64_t workspace_bytes,
                 void* stream);
-/* xs[slots[t, j]] = x[t]; rows past the last kept one are zeroed. */
+/* xs[slots[t, j]] = x[t]; rows past the last kept one are zeroed.  Here and below
+ * a slot outside the n_tok * k sorted rows is a dropped choice. */
 int tt_moe_dispatch(int dtype, int64_t n_tok, int32_t k, int32_t H, int32_t n_experts,
                     const int32_t* slots, const int32_t* offsets, const void* x, void* xs,
                     void* stream);

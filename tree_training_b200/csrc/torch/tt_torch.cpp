@@ -606,10 +606,22 @@ struct CombineFunction : Function<CombineFunction> {
   }
 };
 
+// A plan may be the caller's own: what its arrays hold is checked by the kernels,
+// which take a slot outside the sorted rows as a dropped choice.
+void check_plan(const char* op, const Tensor& slots, const Tensor& offsets) {
+  const std::string name = std::string(op) + ": ";
+  if (slots.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt)
+    type_error(name + "the plan's slots and offsets must be int32");
+  if (slots.dim() != 2 || offsets.dim() != 1 || offsets.size(0) < 2)
+    value_error(name + "the plan's slots must be [T, k] and its offsets [experts + 1]");
+  if (slots.numel() > 0x7fffffff) value_error(name + "more than 2^31 - 1 choices");
+}
+
 void check_rows(const char* op, const char* name, const Tensor& t, int64_t rows,
-                const Tensor& slots) {
+                const Tensor& slots, const Tensor& offsets) {
   need_cuda(op, name, t, t);
-  need_cuda(op, "plan", slots, t);
+  need_cuda(op, "plan.slots", slots, t);
+  need_cuda(op, "plan.offsets", offsets, t);
   if (dtype_code(t) < 0)
     type_error(std::string(op) + ": float32/bfloat16/float16 " + name + " required");
   if (t.dim() != 2 || t.size(0) != rows || t.size(1) < 1)
@@ -617,18 +629,22 @@ void check_rows(const char* op, const char* name, const Tensor& t, int64_t rows,
   need_size(op, "a row's width", t.size(1));
 }
 
-Tensor expert_dispatch(const Tensor& x_, const Tensor& slots, const Tensor& offsets) {
-  check_rows("expert_dispatch", "x", x_, slots.size(0), slots);
-  no_tangent("expert_dispatch", {&x_});
-  const Tensor x = x_.contiguous();
+Tensor expert_dispatch(const Tensor& x_, const Tensor& slots_, const Tensor& offsets_) {
+  const char* op = "expert_dispatch";
+  check_plan(op, slots_, offsets_);
+  check_rows(op, "x", x_, slots_.size(0), slots_, offsets_);
+  no_tangent(op, {&x_});
+  const Tensor x = x_.contiguous(), slots = slots_.contiguous(), offsets = offsets_.contiguous();
   if (wants_grad({&x})) return DispatchFunction::apply(x, slots, offsets);
   return dispatch_rows(x, Plan(slots, offsets));
 }
 
-Tensor expert_combine(const Tensor& ys_, const Tensor& weights, const Tensor& slots,
-                      const Tensor& offsets) {
+Tensor expert_combine(const Tensor& ys_, const Tensor& weights, const Tensor& slots_,
+                      const Tensor& offsets_) {
   const char* op = "expert_combine";
-  check_rows(op, "ys", ys_, slots.size(0) * slots.size(1), slots);
+  check_plan(op, slots_, offsets_);
+  const Tensor slots = slots_.contiguous(), offsets = offsets_.contiguous();
+  check_rows(op, "ys", ys_, slots.size(0) * slots.size(1), slots, offsets);
   need_cuda(op, "weights", weights, ys_);
   if (dtype_code(weights) < 0)
     type_error("expert_combine: float32/bfloat16/float16 weights required");

@@ -236,6 +236,7 @@ int plan_blocks(int64_t n, int E) {
 struct Args {
   int64_t T;
   int K, H, E;
+  uint32_t rows;             // sorted ones: T K
   int group;                 // threads of a token
   const int32_t *slots, *offsets;
   const void *src, *ys;      // by token (dispatch, spread) or by row (collect, combine)
@@ -249,7 +250,7 @@ struct Args {
 template <typename T, int V>
 __device__ __forceinline__ void zero_tail(const Args& a) {
   const int64_t n = a.T * a.K;
-  const int64_t kept = a.offsets[a.E];
+  const int64_t kept = max((int64_t)0, (int64_t)a.offsets[a.E]);
   const int packs = a.H / V;
   float z[V];
 #pragma unroll
@@ -276,6 +277,12 @@ __device__ __forceinline__ Place place(const Args& a) {
   p.tok = (int64_t)blockIdx.x * (blockDim.x / a.group) + q;
   p.live = p.tok < a.T;
   return p;
+}
+
+// Whether a slot is a sorted row; else its choice is dropped: -1, and whatever a
+// plan of the caller's may hold.
+__device__ __forceinline__ bool kept(const Args& a, int64_t slot) {
+  return (uint32_t)slot < a.rows;
 }
 
 template <int KC>
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(512) dispatch_kernel(const Args a) {
         const vec::Raw<T, V> v = vec::load_raw<T, V>(src + p * V);
 #pragma unroll
         for (int k = 0; k < KC; ++k)
-          if (r[k] >= 0)
+          if (kept(a, r[k]))
             *reinterpret_cast<vec::Raw<T, V>*>(reinterpret_cast<T*>(a.dst) + (int64_t)r[k] * a.H +
                                                p * V) = v;
       }
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(512, 4) combine_kernel(const Args a) {
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     for (int k = 0; k < a.K; ++k) {
       const int64_t r = __ldg(slot + k);
-      if (r < 0) continue;
+      if (!kept(a, r)) continue;
       const float w = weight_of(a, pl, k);
       float v[V];
       vec::load<T, V>(reinterpret_cast<const T*>(a.src) + r * a.H + p * V, v);
@@ -372,10 +379,10 @@ __global__ void __launch_bounds__(512, 2) collect_kernel(const Args a) {
       vec::Raw<T, V> raw[KC];
 #pragma unroll
       for (int k = 0; k < KC; ++k)
-        if (r[k] >= 0) raw[k] = vec::load_raw<T, V>(src + (int64_t)r[k] * a.H + p * V);
+        if (kept(a, r[k])) raw[k] = vec::load_raw<T, V>(src + (int64_t)r[k] * a.H + p * V);
 #pragma unroll
       for (int k = 0; k < KC; ++k) {
-        if (r[k] < 0) continue;
+        if (!kept(a, r[k])) continue;
         float v[V];
         vec::unpack<T, V>(raw[k], v);
 #pragma unroll
@@ -416,14 +423,14 @@ __global__ void __launch_bounds__(512, 2) spread_kernel(const Args a) {
           vec::Raw<T, V> raw[B];
 #pragma unroll
           for (int k = 0; k < B; ++k)
-            if (r[b + k] >= 0)
+            if (kept(a, r[b + k]))
               raw[k] = vec::load_raw<T, V>(reinterpret_cast<const T*>(a.ys) +
                                            (int64_t)r[b + k] * a.H + p * V);
           float g[V];
           vec::unpack<T, V>(raw_g, g);
 #pragma unroll
           for (int k = 0; k < B; ++k) {
-            if (r[b + k] < 0) continue;
+            if (!kept(a, r[b + k])) continue;
             const float wk = w[k0 + b + k];
             float v[V], o[V];
             vec::unpack<T, V>(raw[k], v);
@@ -481,7 +488,7 @@ __global__ void __launch_bounds__(512) dispatch_any(const Args a) {
     const T* src = lo + pl.tok * a.H;
     for (int k = 0; k < a.K; ++k) {
       const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
-      if (r < 0) continue;
+      if (!kept(a, r)) continue;
       T* dst = reinterpret_cast<T*>(a.dst) + r * a.H;
       for (int64_t e = (int64_t)pl.t * N - lead(dst); e < a.H; e += a.group * N)
         vec::store_part<T>(dst, e, a.H, vec::load_any_of<T>(src, e, a.H, lo, hi));
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(512) combine_any(const Args a) {
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
     for (int k = 0; k < a.K; ++k) {
       const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
-      if (r < 0) continue;
+      if (!kept(a, r)) continue;
       float v[N];
       vec::unpack<T, N>(vec::load_any_of<T>(lo + r * a.H, e, a.H, lo, hi), v);
       vec::axpy<N>(kWeighted ? weight_of(a, pl, k) : 1.f, v, acc);
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(512) spread_any(const Args a) {
     float dot = 0.f;
     if (pl.live) {
       const int64_t r = __ldg(a.slots + pl.tok * a.K + k);
-      if (r >= 0) {
+      if (kept(a, r)) {
         const float w = weight_of(a, pl, k);
         const T* ys = reinterpret_cast<const T*>(a.ys) + r * a.H;
         T* dst = reinterpret_cast<T*>(a.dst) + r * a.H;
@@ -614,6 +621,7 @@ int run(Op op, int dtype, Args& a, void* stream) {
   if (a.T < 0 || a.K < 0 || a.K > kMaxK || a.H <= 0 || a.E <= 0 || a.T * a.K > 0x7fffffff)
     return TT_ERR_INVALID_ARG;
   if (a.T == 0) return TT_OK;
+  a.rows = (uint32_t)(a.T * a.K);
   // with K = 0 there are no sorted rows: the side of them may be null
   const bool by_token = op == kDispatch || op == kSpread;      // src is
   if (!a.offsets || (a.K > 0 && !a.slots) || (!a.src && (by_token || a.K > 0)) ||

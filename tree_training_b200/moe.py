@@ -22,7 +22,10 @@ class ExpertPlan:
     """``slots`` [T, k] int32: the sorted row of each choice, -1 if dropped;
     ``entries`` [T * k] int32: the choice (t * k + j) in each sorted row, -1
     past the kept ones; ``offsets`` [E + 1] int32: the first row of each
-    expert, and the number of kept rows."""
+    expert, and the number of kept rows.
+
+    A plan may be made or changed by the caller: a slot outside the T * k rows
+    drops its choice; rows below offsets[E] that no slot names are not written."""
     __slots__ = ("slots", "entries", "offsets", "n_tokens", "k", "n_experts")
 
     def __init__(self, slots, entries, offsets, n_tokens, k, n_experts):
