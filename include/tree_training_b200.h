@@ -553,7 +553,8 @@ int tt_moe_spread(int dtype, int weight_dtype, int64_t n_tok, int32_t k, int32_t
 
 /* ---- token log probabilities ---------------------------------------------- *
  * For every row of logits [n_rows, vocab] (row stride ld): the log
- * probabilities under softmax(logits / temperature) of n_tokens given tokens
+ * probabilities under softmax(logits / temperature), temperature in [1e-20,
+ * 1e20], of n_tokens given tokens
  * (int64 [n_rows, n_tokens]; outside [0, vocab): ignored, 0), the entropy, and
  * the top_k <= 64 largest logits' tokens (the lowest index first among equals)
  * with their log probabilities.  stats [n_rows][4] fp32 is kept for the

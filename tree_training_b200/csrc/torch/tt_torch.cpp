@@ -220,8 +220,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
   need_size(op, "a vocabulary", V);
   if (k < 0 || k > std::min(max_k, V))
     value_error("token_logprobs: top_k must be in [0, " + std::to_string(std::min(max_k, V)) + "]");
-  if (!(temperature > 0.0 && temperature < INFINITY))
-    value_error("token_logprobs: temperature must be positive and finite");
+  if (!(temperature >= 1e-20 && temperature <= 1e20))
+    value_error("token_logprobs: temperature must be in [1e-20, 1e20]");
   Tensor tok;
   if (tokens.defined()) {
     need_int(op, "tokens", tokens);

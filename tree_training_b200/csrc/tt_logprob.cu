@@ -47,7 +47,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Exponents of 2 are kept from -inf, whose product with a probability of 0
 // would be NaN; 2^-200 is 0 in fp32.
 constexpr float kFloor = -200.f;
-constexpr float kGradFloor = -300.f;
+constexpr float kGradFloor = -300.f;    // where they are 2^100 times as large
+// Between these 1 / temperature and gradients over it are far from the ends of fp32:
+// an infinite or flushed factor would make NaN of a difference of 0 or of -inf.
+constexpr float kMinTemperature = 1e-20f, kMaxTemperature = 1e20f;
 // The reference moves when the maximum is this far (a factor of 2^12) above it.
 constexpr float kSlack = 12.f;
 
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(TH) bwd_kernel(const BwdArgs a) {
 bool bad(int64_t rows, int32_t V, int32_t M, int32_t k, const void* x, int64_t ld,
          const int64_t* tokens, float temperature) {
   return rows < 0 || rows > 0x7fffffff || V <= 0 || M < 0 || k < 0 || k > kMaxTop || k > V ||
-         ld < V || !(temperature > 0.f) || (rows > 0 && (!x || (M > 0 && !tokens)));
+         ld < V || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) || (rows > 0 && (!x || (M > 0 && !tokens)));
 }
 
 // Blocks that share a row: enough that every SM has work, as long as each still

@@ -35,7 +35,8 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
-    """Log probabilities under softmax(logits / temperature).
+    """Log probabilities under softmax(logits / temperature), the temperature in
+    [1e-20, 1e20].
 
     logits [rows, V] (fp32/bf16/fp16, any row stride); tokens [rows] or
     [rows, M] int64/int32, or None.  A token outside [0, V) is ignored: log
