@@ -554,12 +554,12 @@ int tt_moe_spread(int dtype, int weight_dtype, int64_t n_tok, int32_t k, int32_t
 /* ---- token log probabilities ---------------------------------------------- *
  * For every row of logits [n_rows, vocab] (row stride ld): the log
  * probabilities under softmax(logits / temperature), temperature in [1e-20,
- * 1e20], of n_tokens given tokens
- * (int64 [n_rows, n_tokens]; outside [0, vocab): ignored, 0), the entropy, and
- * the top_k <= 64 largest logits' tokens (the lowest index first among equals)
- * with their log probabilities.  stats [n_rows][4] fp32 is kept for the
- * backward (may be null).  A row of nothing but -inf has log probabilities
- * -inf, entropy 0 and no gradient. */
+ * 1e20], of n_tokens given tokens (int64 [n_rows, n_tokens]; outside [0,
+ * vocab): ignored, 0), the entropy, and the top_k <= 64 largest logits' tokens
+ * (the lowest index first among equals) with their log probabilities.  stats
+ * [n_rows][4] fp32, on a 16-byte boundary, is kept for the backward (may be
+ * null).  A row of nothing but -inf has log probabilities -inf, entropy 0 and
+ * no gradient. */
 int tt_token_logprobs_fwd(int dtype, int64_t n_rows, int32_t vocab, const void* logits, int64_t ld,
                           const int64_t* tokens, int32_t n_tokens, float temperature,
                           int32_t top_k, float* logprobs, float* entropy, float* top_logprobs,

@@ -827,10 +827,12 @@ __global__ void __launch_bounds__(TH) bwd_kernel(const BwdArgs a) {
   }
 }
 
+// (statistics are stored and loaded as one 16-byte word a row)
 bool bad(int64_t rows, int32_t V, int32_t M, int32_t k, const void* x, int64_t ld,
-         const int64_t* tokens, float temperature) {
+         const int64_t* tokens, float temperature, const float* stats) {
   return rows < 0 || rows > 0x7fffffff || V <= 0 || M < 0 || k < 0 || k > kMaxTop || k > V ||
-         ld < V || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) || (rows > 0 && (!x || (M > 0 && !tokens)));
+         ld < V || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
+         reinterpret_cast<uintptr_t>(stats) % 16 || (rows > 0 && (!x || (M > 0 && !tokens)));
 }
 
 // Blocks that share a row: enough that every SM has work, as long as each still
@@ -915,7 +917,7 @@ extern "C" int tt_token_logprobs_fwd(int dtype, int64_t n_rows, int32_t vocab, c
                                      float* entropy, float* top_logprobs, int64_t* top_tokens,
                                      float* stats, void* stream) {
   using namespace tt::logprob;
-  if (bad(n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature) ||
+  if (bad(n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature, stats) ||
       (n_rows > 0 && (!entropy || (n_tokens > 0 && !logprobs) ||
                       (top_k > 0 && (!top_logprobs || !top_tokens)))))
     return TT_ERR_INVALID_ARG;
@@ -937,7 +939,7 @@ extern "C" int tt_token_logprobs_bwd(int dtype, int64_t n_rows, int32_t vocab, c
                                      const float* g_top, const float* stats, void* dlogits,
                                      void* stream) {
   using namespace tt::logprob;
-  if (bad(n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature) ||
+  if (bad(n_rows, vocab, n_tokens, top_k, logits, ld, tokens, temperature, stats) ||
       (n_rows > 0 && (!stats || !dlogits || (g_top && top_k > 0 && !top_tokens))))
     return TT_ERR_INVALID_ARG;
   if (n_rows == 0) return TT_OK;
