@@ -812,18 +812,18 @@ __global__ void __launch_bounds__(TH) bwd_kernel(const BwdArgs a) {
   for (; v < end; v += TH) leave(fetch(v), v);
   if (empty) return;
   __syncthreads();
-  // the given tokens in this block's part: equal ones add up in order
+  // the given tokens in this block's part: equal ones add up in order, by the first
+  // of them (the others stop there: few steps where a row has many tokens)
   for (int j = threadIdx.x; j < n; j += TH) {
     const int64_t tok = token(j);
     if (tok < 0 || tok >= a.V || tok < to.first(begin) || tok >= to.first(end)) continue;
-    float g = 0.f;
     bool first = true;
-    for (int i = 0; i < n; ++i) {
-      if (token(i) != tok) continue;
-      if (i < j) first = false;
-      g += grad(i);
-    }
-    if (first) dx[tok] = from_f32<T>(fmaf(g, inv_t, base(to_f32(x[tok]))));
+    for (int i = 0; i < j && first; ++i) first = token(i) != tok;
+    if (!first) continue;
+    float g = grad(j);
+    for (int i = j + 1; i < n; ++i)
+      if (token(i) == tok) g += grad(i);
+    dx[tok] = from_f32<T>(fmaf(g, inv_t, base(to_f32(x[tok]))));
   }
 }
 

@@ -45,6 +45,9 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     the largest).  -inf logits have probability 0; a row of nothing but -inf
     has log probabilities -inf, entropy 0 and no gradient.
 
+    The gradient's time at the given tokens grows with M times the row's different
+    tokens: made for the successors in a tree, not for whole vocabularies.
+
     Differentiable in ``logits`` through logprobs, entropy and top_logprobs.
     CUDA tensors only (no CPU path)."""
     return TokenLogprobs(*_ops.ext().token_logprobs(logits, tokens, int(top_k),
