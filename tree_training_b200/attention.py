@@ -27,8 +27,8 @@ _status: dict = {}
 def _status_word(device: torch.device) -> torch.Tensor:
     s = _status.get(device)
     if s is None:
-        s = torch.zeros(1, dtype=torch.int32, device=device)
-        _status[device] = s
+        # (another thread may be here too: its word or this one, for both)
+        s = _status.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))
     return s
 
 
