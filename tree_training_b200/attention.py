@@ -35,7 +35,9 @@ def _status_word(device: torch.device) -> torch.Tensor:
 def check_device_status(device: Optional[torch.device] = None) -> None:
     """Raise if a kernel on ``device`` recorded an error (e.g. a bounded wait
     that timed out).  Synchronises with the device; call between steps."""
-    dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+    dev = torch.device("cuda" if device is None else device)
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
     s = _status.get(dev)
     if s is not None:
         code = int(s.item())
