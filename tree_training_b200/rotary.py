@@ -80,16 +80,20 @@ def _inverse_frequencies(dim: int, theta: float, scaling: dict, n_positions: int
     return freq * (1.0 - ramp) + freq / factor * ramp, float(amp)
 
 
-def rotary_table(n_positions: int, dim: int, theta: float = 10000.0,
+def rotary_table(n_positions: int, dim: int, theta: Optional[float] = None,
                  scaling: Optional[dict] = None, device=None) -> torch.Tensor:
     """fp32 [n_positions, dim]: dim / 2 cosines, then dim / 2 sines of each
     position.  ``scaling`` is a config's ``rope_scaling`` / ``rope_parameters``
     dict (default, linear, dynamic, yarn, llama3, longrope; ``dynamic`` and
-    ``longrope`` go by ``n_positions``).  Angles are formed in 64 bits: at
+    ``longrope`` go by ``n_positions``).  ``theta`` is the base; None: the
+    ``rope_theta`` of ``scaling``, or 10,000.  Angles are formed in 64 bits: at
     position 40,000 a 32-bit angle is already off by 2e-3."""
     if n_positions < 1 or dim < 2 or dim % 2:
         raise ValueError("rotary_table: n_positions >= 1 and an even dim >= 2 required")
-    freq, amp = _inverse_frequencies(dim, float(theta), dict(scaling or {}), int(n_positions))
+    scaling = dict(scaling or {})
+    if theta is None:
+        theta = scaling.get("rope_theta", 10000.0)
+    freq, amp = _inverse_frequencies(dim, float(theta), scaling, int(n_positions))
     freq = freq.to(device=device)
     ang = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq
     return torch.cat([ang.cos() * amp, ang.sin() * amp], 1).float()
