@@ -1,8 +1,8 @@
 // Torch bindings of the layer operators (token log probabilities, rotary
 // positions, residual norms, tokens sorted by expert): argument checks, outputs
 // and autograd nodes around the C ABI.  A decoder layer makes several of these
-// calls for few tokens, where the host decides: a call is 6 to 8 us here, and
-// was 15 to 18 through Python (forward and backward of a norm 60, not 113).
+// calls for few tokens, where the host decides: a call is 4 to 9 us here, and
+// was 10 to 17 through Python (forward and backward of a norm 64, not 113).
 //
 // No arithmetic is done here.  Every call runs on the current stream of its
 // tensors' device; gradients carry no graph (differentiating them again is an

@@ -26,7 +26,7 @@ struct RawOf<2> { using type = uint16_t; };
 template <typename T, int V>
 using Raw = typename RawOf<(int)sizeof(T) * V>::type;
 
-// Read-only data used once: keeps it out of L1.
+// Data that no kernel writes while it is read (through L1).
 template <typename R>
 __device__ __forceinline__ R ld_stream(const void* p) {
   return __ldg(reinterpret_cast<const R*>(p));

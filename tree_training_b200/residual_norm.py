@@ -1,7 +1,8 @@
-"""The edge between two blocks of a decoder layer in one kernel each way
-(``tt_residual_norm_fwd/bwd``): the norm after a block, its gate, the residual
-sum and the norm before the next block, in place of the layer's chain of
-elementwise ops (``gated_norm.py`` covers the norm inside a delta-net block).
+"""The edge between two blocks of a decoder layer: the norm after a block, its
+gate, the residual sum and the norm before the next block, in place of the
+layer's chain of elementwise ops (``gated_norm.py`` covers the norm inside a
+delta-net block).  One kernel forward, two backward (``tt_residual_norm_fwd/bwd``):
+the second adds up the column sums of the weights' gradients.
 """
 from __future__ import annotations
 
