@@ -571,6 +571,70 @@ int tt_token_logprobs_bwd(int dtype, int64_t n_rows, int32_t vocab, const void* 
                           const float* g_entropy, const float* g_top, const float* stats,
                           void* dlogits, void* stream);
 
+/* ---- embedding ------------------------------------------------------------- *
+ * y[t] = scale * weight[ids[t]]: y [n, H] contiguous, weight [V, H] with row
+ * stride ld, ids int64 (ids64) or int32.  An id outside [0, V) gives a row of NaN
+ * and writes TT_ERR_INVALID_ARG into *status.  n, V < 2^31. */
+int tt_embedding_fwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids, int ids64,
+                     const void* weight, int64_t ld, float scale, void* y, int32_t* status,
+                     void* stream);
+/* dweight [V, H], contiguous: dweight[v] = scale * the sum of dy[t] (row stride
+ * dy_ld) over the t with ids[t] = v, in the order of t; 0 for other rows, for
+ * padding_idx (-1: none), and nothing from ids outside [0, V). */
+int64_t tt_embedding_bwd_workspace_size(int64_t n, int64_t V);
+int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids, int ids64,
+                     const void* dy, int64_t dy_ld, float scale, int64_t padding_idx,
+                     void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- the gated half of a feed-forward block --------------------------------- *
+ * h = act(x wg^T) * (x wu^T): x [T, H], wg and wu [F, H], h [T, F] contiguous; act
+ * 0 silu, 1 gelu, 2 gelu with tanh, 3 relu.  16-bit factors need rows on 16-byte
+ * boundaries (else TT_ERR_UNSUPPORTED).  g and u (fp32, row stride keep_ld; null for
+ * 16-bit inputs: not kept) are the two products, which the backward takes. */
+int64_t tt_gated_linear_fwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F);
+int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x, int64_t x_ld,
+                        const void* wg, int64_t wg_ld, const void* wu, int64_t wu_ld, int act,
+                        void* h, float* g, float* u, int64_t keep_ld, void* workspace,
+                        int64_t workspace_bytes, int32_t* status, void* stream);
+/* dx [T, H], dwg and dwu [F, H], contiguous; null: not wanted. */
+int64_t tt_gated_linear_bwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F);
+int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x, int64_t x_ld,
+                        const void* wg, int64_t wg_ld, const void* wu, int64_t wu_ld, int act,
+                        const float* g, const float* u, int64_t keep_ld, const void* dh,
+                        int64_t dh_ld, void* dx, void* dwg, void* dwu, void* workspace,
+                        int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* ---- cross entropy of an LM head without its logits --------------------------- *
+ * z = scale * x w^T (x [T, H], w [V, H]); lse[t] = log sum exp z[t]; losses[t, m] =
+ * lse[t] - z[t, labels[t, m]], 0 for labels (int64 [T, M]) outside [0, V).  16-bit
+ * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED). */
+int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
+int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
+                     int64_t x_ld, const void* w, int64_t w_ld, const int64_t* labels, float scale,
+                     float* losses, float* lse, void* workspace, int64_t workspace_bytes,
+                     int32_t* status, void* stream);
+/* dx [T, H], dw [V, H], contiguous; null: not wanted.  g_loss [T, M], g_lse [T]
+ * (null: zeros) are the gradients of losses and lse. */
+int64_t tt_linear_ce_bwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
+int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
+                     int64_t x_ld, const void* w, int64_t w_ld, const int64_t* labels, float scale,
+                     const float* lse, const float* g_loss, const float* g_lse, void* dx, void* dw,
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* ---- the norm of many tensors ---------------------------------------------------- *
+ * dtypes, sizes (elements) and tensors are host arrays of `count`.  norm_type 1, 2
+ * or infinity; *norm (device, fp32) is the norm of all elements together. */
+int64_t tt_grad_norm_workspace_size(int32_t count);
+int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
+                 const void* const* tensors, double norm_type, float* norm, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+/* outs[i] = tensors[i] * min(1, max_norm / (norm + eps)); outs[i] may be tensors[i].
+ * given_norm (device; null: computed here) is the norm to go by; *norm gets it. */
+int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
+                      const void* const* tensors, void* const* outs, double norm_type,
+                      const float* given_norm, float max_norm, float eps, float* norm,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,10 @@ from .logprob import TokenLogprobs, token_logprobs, tree_next_tokens  # noqa: F4
 from .rotary import apply_rotary, rotary_table  # noqa: F401
 from .residual_norm import residual_norm  # noqa: F401
 from .moe import ExpertPlan, expert_combine, expert_dispatch, expert_plan  # noqa: F401
+from .embedding import embedding  # noqa: F401
+from .gated_linear import fuse_gated_mlps, gated_linear  # noqa: F401
+from .linear_ce import LinearCE, linear_cross_entropy  # noqa: F401
+from .grad_norm import clip_grad_norm, grad_norm  # noqa: F401
 from ._lib import LIB_PATH, TTError  # noqa: F401
 
 __all__ = [
@@ -22,5 +26,7 @@ __all__ = [
     "register_hf_attention", "tree_mask_placeholder", "meta_from_dense_mask",
     "TokenLogprobs", "token_logprobs", "tree_next_tokens", "apply_rotary", "rotary_table",
     "residual_norm", "ExpertPlan", "expert_plan", "expert_dispatch", "expert_combine",
+    "embedding", "gated_linear", "fuse_gated_mlps", "LinearCE", "linear_cross_entropy",
+    "grad_norm", "clip_grad_norm",
     "check_device_status", "prefetch_tree_meta", "ATTN_IMPL_NAME", "LIB_PATH", "TTError",
 ]

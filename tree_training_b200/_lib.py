@@ -29,6 +29,7 @@ _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _INT = ctypes.c_int
 
 # name -> (restype, argtypes); must match include/tree_training_b200.h
@@ -112,6 +113,25 @@ SIGNATURES = {
                                      _P, _P, _P, _P]),
     "tt_token_logprobs_bwd": (_INT, [_INT, _I64, _I32, _P, _I64, _P, _I32, _F32, _I32, _P, _P,
                                      _P, _P, _P, _P, _P]),
+    "tt_embedding_fwd": (_INT, [_INT, _I64, _I64, _I32, _P, _INT, _P, _I64, _F32, _P, _P, _P]),
+    "tt_embedding_bwd_workspace_size": (_I64, [_I64, _I64]),
+    "tt_embedding_bwd": (_INT, [_INT, _I64, _I64, _I32, _P, _INT, _P, _I64, _F32, _I64, _P, _P,
+                                _I64, _P]),
+    "tt_gated_linear_fwd_workspace_size": (_I64, [_INT, _I64, _I32, _I32]),
+    "tt_gated_linear_fwd": (_INT, [_INT, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _INT, _P,
+                                   _P, _P, _I64, _P, _I64, _P, _P]),
+    "tt_gated_linear_bwd_workspace_size": (_I64, [_INT, _I64, _I32, _I32]),
+    "tt_gated_linear_bwd": (_INT, [_INT, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _INT, _P,
+                                   _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
+    "tt_linear_ce_fwd_workspace_size": (_I64, [_INT, _I64, _I32, _I64, _I64]),
+    "tt_linear_ce_fwd": (_INT, [_INT, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P, _F32, _P,
+                                _P, _P, _I64, _P, _P]),
+    "tt_linear_ce_bwd_workspace_size": (_I64, [_INT, _I64, _I32, _I64, _I64]),
+    "tt_linear_ce_bwd": (_INT, [_INT, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P, _F32, _P,
+                                _P, _P, _P, _P, _P, _I64, _P, _P]),
+    "tt_grad_norm_workspace_size": (_I64, [_I32]),
+    "tt_grad_norm": (_INT, [_I32, _P, _P, _P, _F64, _P, _P, _I64, _P]),
+    "tt_clip_grad_norm": (_INT, [_I32, _P, _P, _P, _P, _F64, _P, _F32, _F32, _P, _P, _I64, _P]),
     "tt_conv_predecessors": (_INT, [_I32, _P, _P, _I32, _P]),
     "tt_conv_successors": (_INT, [_I32, _I32, _P, _P, _P, _P, _I64]),
     "tt_tree_conv_fwd": (_INT, [_INT, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),

@@ -1,0 +1,312 @@
+// The gated half of a feed-forward block and its gradients.
+//
+//   g = x Wg^T,  u = x Wu^T,  h = act(g) * u
+//   dg = dh * u * act'(g),  du = dh * act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// 4 T H F operations forward, 8 T H F backward: bound by the tensor cores for many
+// tokens, by the weights' bytes for few.
+//
+// Forward, 16-bit: one kernel forms both products of a tile side by side in one
+// accumulator (its left half g, its right half u), so that x is read once for both
+// and h leaves from registers.  For the backward g and u are kept in fp32: rounded
+// to 16 bits they would put two more roundings into dg (its own is the one that the
+// tensor cores' operands need), and the eight bytes an element stand against six
+// that g, u and act(g) take in 16 bits.
+//
+// Backward: dg and du leave one elementwise pass in 16 bits, dx is one sum of two
+// products in one accumulator, each weight's gradient one product.
+//
+// fp32: the products on the CUDA cores (see tt_gemm_fp32.cu), h by a pass over g and u.
+#include "tt_gemm_sm100.cuh"
+
+namespace tt {
+namespace gated {
+namespace {
+
+enum Act { kSilu = 0, kGelu = 1, kGeluTanh = 2, kRelu = 3 };
+
+constexpr float kTanhA = 0.7978845608028654f;      // sqrt(2 / pi)
+constexpr float kTanhB = 0.044715f;
+
+template <int A>
+__device__ __forceinline__ float act(float g) {
+  if constexpr (A == kSilu) return g / (1.f + expf(-g));
+  if constexpr (A == kGelu) return g * normcdff(g);
+  if constexpr (A == kGeluTanh)
+    return 0.5f * g * (1.f + tanhf(kTanhA * (g + kTanhB * g * g * g)));
+  return g > 0.f ? g : (g != g ? g : 0.f);
+}
+
+// act(g) and its derivative.
+template <int A>
+__device__ __forceinline__ void act_grad(float g, float& a, float& d) {
+  if constexpr (A == kSilu) {
+    const float q = 1.f / (1.f + expf(-g));
+    a = g * q;
+    // (1 - q loses what little there is of it for large g: q(-g) instead)
+    d = q * (1.f + g * (1.f / (1.f + expf(g))));
+  } else if constexpr (A == kGelu) {
+    const float c = normcdff(g);
+    a = g * c;
+    d = c + g * expf(-0.5f * g * g) * 0.3989422804014327f;
+  } else if constexpr (A == kGeluTanh) {
+    const float t = tanhf(kTanhA * (g + kTanhB * g * g * g));
+    a = 0.5f * g * (1.f + t);
+    d = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * kTanhA * (1.f + 3.f * kTanhB * g * g);
+  } else {
+    a = act<kRelu>(g);
+    d = g > 0.f ? 1.f : (g != g ? g : 0.f);
+  }
+}
+
+template <typename F>
+int dispatch_act(int act, F f) {
+  switch (act) {
+    case kSilu: return f(std::integral_constant<int, kSilu>());
+    case kGelu: return f(std::integral_constant<int, kGelu>());
+    case kGeluTanh: return f(std::integral_constant<int, kGeluTanh>());
+    case kRelu: return f(std::integral_constant<int, kRelu>());
+    default: return TT_ERR_INVALID_ARG;
+  }
+}
+
+template <bool kB, int A>
+struct GatedEpi {
+  static constexpr bool kBf16 = kB;
+  struct Args {
+    void* h;
+    int64_t h_ld;
+    float *g, *u;                          // null: not kept
+    int64_t keep_ld;
+    int F, wide, keep_wide;
+  };
+  static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
+                                              const gemm::TileAt& t, int row, uint32_t acc) {
+    using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
+    const int half = p.bn / 2, n0 = t.n * half, cols = min(half, a.F - n0);
+    const bool live = row < p.M;
+    for (int c = 0; c < cols; c += 32) {
+      float g[32], u[32];
+      __syncwarp();                          // (the loads are the whole warp's)
+      sm100::tmem_ld32x2(acc + c, acc + half + c, g, u);
+      if (!live) continue;
+      const int left = cols - c;
+      if (a.g) {
+        const int64_t at = (int64_t)row * a.keep_ld + n0 + c;
+        gemm::store_row32(a.g + at, g, left, a.keep_wide);
+        gemm::store_row32(a.u + at, u, left, a.keep_wide);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) g[i] = act<A>(g[i]) * u[i];
+      gemm::store_row32(reinterpret_cast<T*>(a.h) + (int64_t)row * a.h_ld + n0 + c, g, left,
+                        a.wide);
+    }
+  }
+};
+
+// h of fp32 g and u.
+template <int A>
+__global__ void __launch_bounds__(256)
+    forward_kernel(const float* g, const float* u, int64_t ld, int64_t rows, int F, float* h) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < F; c += gridDim.x * blockDim.x)
+      h[r * F + c] = act<A>(g[r * ld + c]) * u[r * ld + c];
+}
+
+// dg and du out of g, u (fp32) and dh; columns from F to `ld` are left alone.
+template <typename T, int A, int V>
+__global__ void __launch_bounds__(256)
+    backward_kernel(const float* g, const float* u, int64_t keep_ld, const T* dh, int64_t dh_ld,
+                    int64_t rows, int F, T* dg, T* du, int64_t ld) {
+  const int packs = (F + V - 1) / V;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int p = blockIdx.x * blockDim.x + threadIdx.x; p < packs; p += gridDim.x * blockDim.x) {
+      const int c = p * V;
+      float vg[V], vu[V], vd[V];
+      if constexpr (V > 1) {
+        constexpr int W = 4;
+#pragma unroll
+        for (int i = 0; i < V; i += W) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(g + r * keep_ld + c + i));
+          const float4 y = __ldg(reinterpret_cast<const float4*>(u + r * keep_ld + c + i));
+          vg[i] = x.x, vg[i + 1] = x.y, vg[i + 2] = x.z, vg[i + 3] = x.w;
+          vu[i] = y.x, vu[i + 1] = y.y, vu[i + 2] = y.z, vu[i + 3] = y.w;
+        }
+        vec::load<T, V>(dh + r * dh_ld + c, vd);
+      } else {
+        vg[0] = g[r * keep_ld + c], vu[0] = u[r * keep_ld + c];
+        vd[0] = to_f32(dh[r * dh_ld + c]);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a, d;
+        act_grad<A>(vg[i], a, d);
+        vg[i] = vd[i] * vu[i] * d;
+        vu[i] = vd[i] * a;
+      }
+      vec::store<T, V>(dg + r * ld + c, vg);
+      vec::store<T, V>(du + r * ld + c, vu);
+    }
+}
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+bool sizes_ok(int64_t T, int32_t H, int32_t F) {
+  return T >= 0 && T < ((int64_t)1 << 31) - 256 && H >= 1 && F >= 1;
+}
+
+int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
+
+template <typename T, int A>
+void run_backward(const float* g, const float* u, int64_t keep_ld, const void* dh, int64_t dh_ld,
+                  int64_t rows, int F, void* dg, void* du, int64_t ld, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool wide = F % V == 0 && keep_ld % 4 == 0 && dh_ld % V == 0 && ld % V == 0 &&
+                    ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u) |
+                      reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
+  const int packs = wide ? F / V : F;
+  const dim3 grid((unsigned)std::min((packs + 255) / 256, 64),
+                  (unsigned)std::min<int64_t>(rows, 32768));
+  if (wide)
+    backward_kernel<T, A, V><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F,
+                                                   (T*)dg, (T*)du, ld);
+  else
+    backward_kernel<T, A, 1><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F,
+                                                   (T*)dg, (T*)du, ld);
+  tt_count_launches(1);
+}
+
+template <bool kB>
+int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void* wg,
+               int64_t wg_ld, const void* wu, int64_t wu_ld, int act, void* h, float* g, float* u,
+               int64_t keep_ld, int32_t* status, cudaStream_t st) {
+  return dispatch_act(act, [&](auto a) -> int {
+    using Epi = GatedEpi<kB, decltype(a)::value>;
+    const gemm::Plan plan =
+        gemm::plan_product(T, F, (H + gemm::kBK - 1) / gemm::kBK, 16, true, false);
+    const gemm::Factor fx{x, x_ld, false};
+    const gemm::Term terms[2] = {{fx, {wg, wg_ld, false}, H}, {fx, {wu, wu_ld, false}, H}};
+    gemm::Problem q;
+    if (!gemm::set_up(&q, plan, kB, T, F, terms, 2, true, status)) return TT_ERR_UNSUPPORTED;
+    typename Epi::Args ea{};
+    ea.h = h, ea.h_ld = F, ea.g = g, ea.u = u, ea.keep_ld = keep_ld, ea.F = F;
+    ea.wide = F % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
+    ea.keep_wide = keep_ld % 4 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15) == 0;
+    return gemm::launch<false, false, Epi>(plan, q, ea, st);
+  });
+}
+
+}  // namespace
+}  // namespace gated
+}  // namespace tt
+
+using namespace tt;
+using namespace tt::gated;
+
+extern "C" int64_t tt_gated_linear_fwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F) {
+  if (!sizes_ok(T, H, F) || dtype != TT_F32) return 0;
+  return gemm::fp32_work(T, F, H);
+}
+
+extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x,
+                                   int64_t x_ld, const void* wg, int64_t wg_ld, const void* wu,
+                                   int64_t wu_ld, int act, void* h, float* g, float* u,
+                                   int64_t keep_ld, void* workspace, int64_t workspace_bytes,
+                                   int32_t* status, void* stream) {
+  if (!sizes_ok(T, H, F) || act < kSilu || act > kRelu || x_ld < H || wg_ld < H || wu_ld < H ||
+      !g != !u || (g && keep_ld < F))
+    return TT_ERR_INVALID_ARG;
+  if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
+  if (T == 0) return TT_OK;
+  if (!x || !wg || !wu || !h || (dtype == TT_F32 && !g)) return TT_ERR_INVALID_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == TT_BF16)
+    return forward_16<true>(T, H, F, x, x_ld, wg, wg_ld, wu, wu_ld, act, h, g, u, keep_ld, status,
+                            st);
+  if (dtype == TT_F16)
+    return forward_16<false>(T, H, F, x, x_ld, wg, wg_ld, wu, wu_ld, act, h, g, u, keep_ld, status,
+                             st);
+  if (workspace_bytes < tt_gated_linear_fwd_workspace_size(dtype, T, H, F))
+    return TT_ERR_WORKSPACE;
+  const gemm::Factor fx{x, x_ld, false};
+  const gemm::Term tg{fx, {wg, wg_ld, false}, H}, tu{fx, {wu, wu_ld, false}, H};
+  for (int i = 0; i < 2; ++i) {
+    const gemm::Result r{TT_F32, i ? u : g, keep_ld, nullptr, 0, 1.f, nullptr};
+    if (const int rc = gemm::fp32_product(T, F, i ? &tu : &tg, 1, r, workspace, workspace_bytes, st))
+      return rc;
+  }
+  return dispatch_act(act, [&](auto a) -> int {
+    const dim3 grid((unsigned)std::min((F + 255) / 256, 64),
+                    (unsigned)std::min<int64_t>(T, 32768));
+    forward_kernel<decltype(a)::value><<<grid, 256, 0, st>>>(g, u, keep_ld, T, F, (float*)h);
+    tt_count_launches(1);
+    return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  });
+}
+
+namespace {
+// dg and du, then the parts of a split sum.
+int64_t grad_bytes(int dtype, int64_t T, int32_t F) {
+  return round256(T * round8(F) * size_of(dtype));
+}
+int64_t parts_bytes(int dtype, int64_t T, int32_t H, int32_t F) {
+  if (dtype == TT_F32)
+    return std::max({gemm::fp32_work(T, H, 2 * (int64_t)F), gemm::fp32_work(F, H, T)});
+  return std::max({gemm::tc_work(T, H, 2 * round8(F) + 128, true), gemm::tc_work(F, H, T, true)});
+}
+}  // namespace
+
+extern "C" int64_t tt_gated_linear_bwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F) {
+  if (!sizes_ok(T, H, F) || dtype < TT_F32 || dtype > TT_F16) return 0;
+  return 2 * grad_bytes(dtype, T, F) + parts_bytes(dtype, T, H, F);
+}
+
+extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x,
+                                   int64_t x_ld, const void* wg, int64_t wg_ld, const void* wu,
+                                   int64_t wu_ld, int act, const float* g, const float* u,
+                                   int64_t keep_ld, const void* dh, int64_t dh_ld, void* dx,
+                                   void* dwg, void* dwu, void* workspace, int64_t workspace_bytes,
+                                   int32_t* status, void* stream) {
+  if (!sizes_ok(T, H, F) || act < kSilu || act > kRelu || x_ld < H || wg_ld < H || wu_ld < H ||
+      keep_ld < F || dh_ld < F)
+    return TT_ERR_INVALID_ARG;
+  if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
+  if (T == 0) return TT_OK;
+  if (!x || !wg || !wu || !g || !u || !dh) return TT_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < tt_gated_linear_bwd_workspace_size(dtype, T, H, F))
+    return TT_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int64_t ld = round8(F), bytes = grad_bytes(dtype, T, F);
+  char* ws = (char*)workspace;
+  void *dg = ws, *du = ws + bytes, *work = ws + 2 * bytes;
+  const int64_t work_bytes = workspace_bytes - 2 * bytes;
+  int rc = dispatch_act(act, [&](auto a) -> int {
+    constexpr int A = decltype(a)::value;
+    return vec::dispatch_float(dtype, [&](auto t) -> int {
+      run_backward<decltype(t), A>(g, u, keep_ld, dh, dh_ld, T, F, dg, du, ld, st);
+      return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+    });
+  });
+  if (rc != TT_OK) return rc;
+  auto product = [&](int64_t M, int64_t N, const gemm::Term* terms, int n, void* c) {
+    const gemm::Result r{dtype, c, N, nullptr, 0, 1.f, nullptr};
+    return dtype == TT_F32
+               ? gemm::fp32_product(M, N, terms, n, r, work, work_bytes, st)
+               : gemm::tc_product(dtype == TT_BF16, M, N, terms, n, r, work, work_bytes, status, st);
+  };
+  if (dx) {
+    const gemm::Term terms[2] = {{{dg, ld, false}, {wg, wg_ld, true}, F},
+                                 {{du, ld, false}, {wu, wu_ld, true}, F}};
+    if ((rc = product(T, H, terms, 2, dx))) return rc;
+  }
+  for (int i = 0; i < 2; ++i) {
+    void* dw = i ? dwu : dwg;
+    if (!dw) continue;
+    const gemm::Term term{{i ? du : dg, ld, true}, {x, x_ld, true}, T};
+    if ((rc = product(F, H, &term, 1, dw))) return rc;
+  }
+  return TT_OK;
+}

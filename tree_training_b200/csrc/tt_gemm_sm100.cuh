@@ -1,0 +1,503 @@
+// Matrix products of 16-bit factors on the tensor cores, with the epilogue that
+// the operator wants: the body shared by the feed-forward block and the LM head's
+// loss.
+//
+//   C [M, N] = sum over the terms of A B^T,  A [M, k], B [N, k], fp32 sums
+//
+// Persistent CTAs (pairs of CTAs for tall problems) over tiles of 128 (256) rows by
+// up to 256 columns.  Warp 0 feeds a ring of 64-wide slices of k by TMA, one thread
+// of warp 1 issues `tcgen05.mma` into one of two TMEM accumulators, warps 4 to 7
+// take the other through the epilogue meanwhile.
+//
+// What bounds it.  An SM's tensor core takes bn / 2 clocks for a 128 x bn x 16 step;
+// filling and reading the step's operands takes (128 + bn) * 32 * 2 bytes through a
+// port of 128 bytes a clock: 192 clocks for 128 at bn = 256.  With the rows of a
+// pair (cta_group::2: 256 x 256, each CTA holding half of B) it is 128 for 128.
+//
+// A factor's contiguous index may be k (128-byte rows of 64 k) or its own (64-wide
+// blocks of rows of k); both come by TMA with the 128-byte swizzle, and what lies
+// outside the factor is filled with zeros.
+#pragma once
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "tt_gemm.cuh"
+#include "tt_sm100.cuh"
+#include "tt_vec.cuh"
+
+namespace tt {
+namespace gemm {
+
+using namespace sm100;
+
+constexpr int kBK = 64;                    // k of a slice: 128 bytes
+constexpr int kABytes = 128 * kBK * 2;     // of A in a slice
+constexpr int kMaxStages = 8;
+constexpr int kRingBytes = 196608;         // of shared memory for the ring
+constexpr int kGemmThreads = 256;
+
+struct Problem {
+  CUtensorMap a[2], b[2];
+  int32_t steps[2];                        // slices of k of each term
+  int32_t terms;
+  int32_t M, N;
+  int32_t bn;                              // columns of the accumulator
+  int32_t tiles_m, tiles_n, group;         // group: tiles of m that share an L2 window
+  int32_t parts, part_steps;               // the sum over k split into parts
+  int32_t stages, stage_bytes;
+  int32_t a_bytes;                         // of A that a CTA copies a slice
+  int32_t dual;                            // B's halves are two factors: b[0] and b[1]
+  int32_t* status;
+};
+
+struct TileAt {
+  int part, m, n;
+};
+
+__device__ __forceinline__ TileAt tile_at(const Problem& p, int i) {
+  TileAt t;
+  const int per = p.tiles_m * p.tiles_n;
+  t.part = i / per;
+  i -= t.part * per;
+  // groups of `group` tiles of m, all n within a group, m fastest
+  const int full = p.group * p.tiles_n;
+  const int g = i / full, in = i - g * full;
+  const int rows = min(p.group, p.tiles_m - g * p.group);
+  t.n = in / rows;
+  t.m = g * p.group + in - t.n * rows;
+  return t;
+}
+
+struct Barriers {
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  int32_t abort;
+};
+
+constexpr int kGemmSmem = 1024 + kRingBytes + 1024;   // barriers, ring, its alignment
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The address of CTA 0's copy of a shared-memory address of this CTA.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t a) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                       int c1) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+        "bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    mma_ss(d, a, b, idesc, accumulate);
+}
+
+// Arrives on `bar` of every CTA of the pair once the MMAs so far are done.
+template <int CG>
+__device__ __forceinline__ void commit_all(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    tc_commit(bar);
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_take(uint32_t* slot) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n\t"
+                 "tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::"r"(smem_u32(slot))
+                 : "memory");
+  else
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n\t"
+                 "tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::"r"(smem_u32(slot))
+                 : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_give(uint32_t taddr) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+}
+
+// Epi::tile(args, problem, tile, row, lane address) takes one accumulator out of
+// TMEM: a thread has one row of the tile (row: its index in C, possibly past M) and
+// reads its columns; all 32 lanes of a warp call it.
+template <int CG, bool kAMN, bool kBMN, typename Epi>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    gemm_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epi::Args ea) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Barriers* sh = reinterpret_cast<Barriers*>(smem_raw);
+  const uint32_t ring = (smem_u32(smem_raw) + 1024 + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const volatile int32_t* abort_flag = &sh->abort;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], 4 * CG);
+    mbar_init(&sh->drain, 1);
+    sh->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) tmem_take<CG>(&sh->tmem);
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+  const int items = p.tiles_m * p.tiles_n * p.parts;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const int all_steps = p.steps[0] + (p.terms > 1 ? p.steps[1] : 0);
+  auto fail = [&]() {
+    sh->abort = 1;
+    set_status(p.status, TT_ERR_DEVICE_TIMEOUT);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA
+    if (lane == 0) {
+      const int stages = p.stages;
+      const uint32_t b_bytes = (uint32_t)(p.bn / CG) * 128;
+      const uint32_t tx = (uint32_t)(p.a_bytes + b_bytes) * CG;
+      int s = 0;
+      uint32_t phase = 0;                  // of the ring's current turn
+      int64_t slot = 0;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += stride) {
+        const TileAt t = tile_at(p, i);
+        const int m0 = t.m * 128 * CG + (int)rank * 128;
+        const int begin = t.part * p.part_steps, end = min(all_steps, begin + p.part_steps);
+        for (int k = begin; k < end; ++k, ++slot) {
+          if (slot >= stages && !mbar_wait(&sh->empty[s], phase ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const int term = k >= p.steps[0] && p.terms > 1;
+          const int k0 = (k - (term ? p.steps[0] : 0)) * kBK;
+          const uint32_t sa = ring + s * p.stage_bytes, sb = sa + kABytes;
+          const uint32_t bar =
+              CG == 2 ? leader_addr(smem_u32(&sh->full[s])) : smem_u32(&sh->full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], tx);
+          if constexpr (kAMN) {
+            tma_2d<CG>(sa, &p.a[term], bar, m0, k0);
+            tma_2d<CG>(sa + 8192, &p.a[term], bar, m0 + 64, k0);
+          } else {
+            tma_2d<CG>(sa, &p.a[term], bar, k0, m0);
+          }
+          if (p.dual) {
+            const int half = p.bn / 2;
+            if constexpr (CG == 2) {
+              tma_2d<CG>(sb, &p.b[rank], bar, k0, t.n * half);
+            } else {
+              tma_2d<CG>(sb, &p.b[0], bar, k0, t.n * half);
+              tma_2d<CG>(sb + half * 128, &p.b[1], bar, k0, t.n * half);
+            }
+          } else if constexpr (kBMN) {
+            const int n0 = t.n * p.bn + (int)rank * (p.bn / CG);
+            for (int c = 0; c < p.bn / CG; c += 64)
+              tma_2d<CG>(sb + c * 128, &p.b[term], bar, n0 + c, k0);
+          } else {
+            tma_2d<CG>(sb, &p.b[term], bar, k0, t.n * p.bn + (int)rank * (p.bn / CG));
+          }
+          if (++s == stages) s = 0, phase ^= 1;
+        }
+      }
+      if (ok) {
+        // the last slices' releases have arrived before this CTA may end
+        for (int64_t i = max((int64_t)0, slot - stages); i < slot && ok; ++i)
+          ok = mbar_wait(&sh->empty[i % stages], (uint32_t)(i / stages) & 1, abort_flag);
+      }
+      if (!ok) {
+        fail();
+        // the copies under way land before the CTA ends (the pair's signal here)
+        if (rank == 0)
+          for (int64_t i = max((int64_t)0, slot - stages); i < slot; ++i)
+            mbar_wait(&sh->full[i % stages], (uint32_t)(i / stages) & 1, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_f16_ab(Epi::kBf16, 128 * CG, p.bn, kAMN, kBMN);
+      const int stages = p.stages;
+      // 64-wide blocks of rows of k: 8 KB from block to block, 2 KB a step of 16 k;
+      // rows of 64 k: 32 bytes a step
+      const uint64_t da0 = kAMN ? desc_sw128(ring, 8192, 1024) : desc_sw128(ring, 16, 1024);
+      const uint64_t db0 = kBMN ? desc_sw128(ring + kABytes, 8192, 1024)
+                                : desc_sw128(ring + kABytes, 16, 1024);
+      constexpr uint64_t kStepA = (kAMN ? 2048 : 32) >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;
+      int s = 0, acc = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += stride, ++acc) {
+        const TileAt t = tile_at(p, i);
+        const int buf = acc & 1;
+        if (acc >= 2 && !mbar_wait(&sh->acc_empty[buf], ((acc >> 1) - 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 256;
+        const int begin = t.part * p.part_steps, end = min(all_steps, begin + p.part_steps);
+        for (int k = begin; k < end; ++k) {
+          if (!mbar_wait(&sh->full[s], phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t off = (uint64_t)((uint32_t)(s * p.stage_bytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            mma_f16<CG>(d, da0 + off + kk * kStepA, db0 + off + kk * kStepB, idesc,
+                        k > begin || kk > 0);
+          commit_all<CG>(&sh->empty[s]);
+          if (++s == stages) s = 0, phase ^= 1;
+        }
+        if (ok) commit_all<CG>(&sh->acc_full[buf]);
+      }
+      if (!ok) fail();
+      // every MMA issued is done before the accumulators are given back
+      if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                smem_u32(&sh->drain))
+            : "memory");
+      else
+        tc_commit(&sh->drain);
+      mbar_wait(&sh->drain, 0, nullptr);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int quad = warp & 3;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+    int acc = 0;
+    for (int i = first; i < items; i += stride, ++acc) {
+      const TileAt t = tile_at(p, i);
+      const int buf = acc & 1;
+      const bool ok = mbar_wait(&sh->acc_full[buf], (acc >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        fail();
+        break;
+      }
+      tc_fence_after();
+      const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
+      Epi::tile(ea, p, t, row, lane_addr + buf * 256);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                           leader_addr(smem_u32(&sh->acc_empty[buf])))
+                       : "memory");
+        else
+          mbar_arrive(&sh->acc_empty[buf]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();
+  tc_fence_after();
+  if (warp == 2) tmem_give<CG>(tmem);
+}
+
+// ---- host -----------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encoder() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// What TMA asks of a factor.
+inline bool copyable(const Factor& f) {
+  return (reinterpret_cast<uintptr_t>(f.p) & 15) == 0 && f.ld % 8 == 0;
+}
+
+// The map of a factor of `n` rows and k columns: boxes of 64 k by `rows`, or of 64
+// rows by 64 k where the rows are contiguous.
+inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_t k, int rows) {
+  const EncodeTiledFn fn = encoder();
+  if (!fn || !copyable(f)) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)(f.mn ? n : k), (cuuint64_t)(f.mn ? k : n)};
+  const cuuint64_t strides[1] = {(cuuint64_t)f.ld * 2};
+  const cuuint32_t box[2] = {64u, (cuuint32_t)(f.mn ? 64 : rows)};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            const_cast<void*>(f.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a product is cut up.
+struct Plan {
+  int cg, bn, parts;
+};
+
+// Clocks of a slice of 64 k in a tile: the tensor core's, or the shared-memory
+// port's where that is more (see the top).
+inline int64_t slice_clocks(int cg, int bn) {
+  return cg == 1 ? 256 + 2 * bn : std::max(256 + bn, 2 * bn);
+}
+
+// The cheapest of the forms by the tiles' waves.  `n_step`: what widths of the
+// accumulator are a multiple of; `width`: columns of C that a column of the
+// accumulator stands for (1, or 2 halves of one: dual).
+inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool dual, bool split) {
+  Plan best{1, n_step, 1};
+  double least = 1e300;
+  for (int cg = 1; cg <= 1; ++cg) {
+    const int step = std::max(n_step * cg, dual ? 16 * cg : 16 * cg);
+    const int64_t slots = vec::kSMs / cg;
+    for (int bn = 256; bn >= step; bn -= step) {
+      const int64_t cols = dual ? bn / 2 : bn;
+      const int64_t tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + cols - 1) / cols);
+      const int64_t most = split ? std::max<int64_t>(1, std::min(slots / tiles, steps / 8)) : 1;
+      for (int64_t parts = 1; parts <= most; ++parts) {
+        const int64_t waves = (tiles * parts + slots - 1) / slots;
+        // a tile's start and end that nothing hides, and the parts' way through L2
+        double clocks = (double)waves * (double)(((steps + parts - 1) / parts) *
+                                                 slice_clocks(cg, bn) + 600) + 1500;
+        if (parts > 1) clocks += 3000 + (double)(parts + 1) * M * N * 4 / 3000;
+        if (clocks < least * 0.999) least = clocks, best = Plan{cg, bn, (int)parts};
+      }
+    }
+  }
+  return best;
+}
+
+// Fills the problem (maps, tiles, ring) for up to two terms; false where a factor
+// cannot be copied by TMA.
+inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N, const Term* terms,
+                   int n_terms, bool dual, int32_t* status) {
+  const int cg = plan.cg, bn = plan.bn;
+  const int a_rows = cg == 1 ? (int)std::min<int64_t>(128, (M + 7) / 8 * 8) : 128;
+  const int b_rows = dual ? bn / 2 : bn / cg;
+  q->terms = dual ? 1 : n_terms;
+  int64_t steps = 0;
+  for (int i = 0; i < 2; ++i) {
+    const Term& t = terms[i < n_terms ? i : 0];
+    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows) || !encode(&q->b[i], bf16, t.b, N, t.k, b_rows))
+      return false;
+    q->steps[i] = (int32_t)((t.k + kBK - 1) / kBK);
+    if (i < q->terms) steps += q->steps[i];
+  }
+  q->M = (int32_t)M, q->N = (int32_t)N, q->bn = bn, q->dual = dual;
+  const int64_t cols = dual ? bn / 2 : bn;
+  q->tiles_m = (int32_t)((M + 128 * cg - 1) / (128 * cg));
+  q->tiles_n = (int32_t)((N + cols - 1) / cols);
+  q->group = std::min(q->tiles_m, 32 / cg);
+  q->part_steps = (int32_t)((steps + plan.parts - 1) / plan.parts);
+  q->parts = (int32_t)((steps + q->part_steps - 1) / q->part_steps);
+  q->stage_bytes = kABytes + bn / cg * 128;
+  q->stages = std::min(kMaxStages, kRingBytes / q->stage_bytes);
+  q->a_bytes = terms[0].a.mn ? kABytes : a_rows * 128;
+  q->status = status;
+  return (int64_t)q->tiles_m * q->tiles_n * q->parts < ((int64_t)1 << 31);
+}
+
+template <int CG, bool kAMN, bool kBMN, typename Epi>
+int launch(const Problem& q, const typename Epi::Args& ea, cudaStream_t st) {
+  auto* kernel = gemm_kernel<CG, kAMN, kBMN, Epi>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) !=
+      cudaSuccess)
+    return TT_ERR_CUDA;
+  const int64_t items = (int64_t)q.tiles_m * q.tiles_n * q.parts;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)(std::min<int64_t>(items, vec::kSMs / CG) * CG));
+  c.blockDim = dim3(kGemmThreads);
+  c.dynamicSmemBytes = kGemmSmem;
+  c.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {CG, 1, 1};
+  c.attrs = attr;
+  c.numAttrs = CG == 2 ? 1 : 0;
+  if (cudaLaunchKernelEx(&c, kernel, q, ea) != cudaSuccess) return TT_ERR_CUDA;
+  tt_count_launches(1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
+template <bool kAMN, bool kBMN, typename Epi>
+int launch(const Plan& plan, const Problem& q, const typename Epi::Args& ea, cudaStream_t st) {
+  return plan.cg == 2 ? launch<2, kAMN, kBMN, Epi>(q, ea, st)
+                      : launch<1, kAMN, kBMN, Epi>(q, ea, st);
+}
+
+// 32 values of a row at columns col .. of n: 16-byte stores where `wide` allows.
+template <typename T>
+__device__ __forceinline__ void store_row32(T* p, const float (&v)[32], int left, bool wide) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (wide && left >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += V) {
+      float w[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = v[i + j];
+      vec::store<T, V>(p + i, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < left) p[i] = from_f32<T>(v[i]);
+  }
+}
+
+// A product of 16-bit factors into C (tensor cores).  `work` as in fp32_product.
+int tc_product(bool bf16, int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r,
+               void* work, int64_t work_bytes, int32_t* status, cudaStream_t st);
+int64_t tc_work(int64_t M, int64_t N, int64_t k, bool b_mn);
+
+}  // namespace gemm
+}  // namespace tt

@@ -37,6 +37,7 @@ import torch.nn.functional as F
 from .attention import ATTN_IMPL_NAME, register_hf_attention, tree_mask_placeholder
 from .packer import TreeNode, build_dfs_tree_info  # noqa: F401  (TreeNode re-export)
 from .ce import fused_linear_cross_entropy
+from .linear_ce import linear_cross_entropy
 from .ssm import SSMPartitionState, has_ssm_layers, patch_ssm_layers
 
 
@@ -193,7 +194,7 @@ def _loss_leaf_spans(info, p: SubtreePartition):
 
 def _subtree_forward(model, p: SubtreePartition, gw: Optional[SubtreeGateway], dev, gateway_mask,
                      leaf_logits_only: bool = False, cut_nodes=(), ssm_exact: bool = False,
-                     fused_loss: Optional[TreeLeafLoss] = None):
+                     fused_loss: Optional[TreeLeafLoss] = None, fused_ce=True):
     """Forward of one partition.  Returns (logits, info, full_kv, spans, ssm):
     with ``leaf_logits_only`` the LM head runs only on the loss leaves' tokens
     (HF ``logits_to_keep`` with an index tensor) and spans maps each loss leaf
@@ -249,8 +250,8 @@ def _subtree_forward(model, p: SubtreePartition, gw: Optional[SubtreeGateway], d
     full_kv = {l: cache._full_kv[l] for l in sorted(cache._full_kv)}
     if fused_loss is None:
         return out.logits, info, full_kv, spans, ssm
-    return _fused_leaf_loss(model, out.last_hidden_state[0], info, leaves, fused_loss), info, \
-        full_kv, spans, ssm
+    loss = _fused_leaf_loss(model, out.last_hidden_state[0], info, leaves, fused_loss, fused_ce)
+    return loss, info, full_kv, spans, ssm
 
 
 def _base_model(model):
@@ -261,9 +262,10 @@ def _base_model(model):
     return base
 
 
-def _fused_leaf_loss(model, hidden, info, leaves, loss: TreeLeafLoss) -> torch.Tensor:
+def _fused_leaf_loss(model, hidden, info, leaves, loss: TreeLeafLoss, fused_ce) -> torch.Tensor:
     """sum over the partition's loss leaves of CE(leaf logits) / n_leaves from
-    the final hidden states [N, H], without materialising the logits."""
+    the final hidden states [N, H], without materialising the logits (by chunks
+    of tokens, or with ``fused_ce="pieces"`` by pieces of the vocabulary)."""
     if not leaves:
         return hidden.sum() * 0.0
     idx = np.concatenate([np.arange(s, e) for _, s, e in leaves])
@@ -273,7 +275,11 @@ def _fused_leaf_loss(model, hidden, info, leaves, loss: TreeLeafLoss) -> torch.T
         labs.append(lab)
         wts.append(loss.token_weights(lab))
     h = hidden.index_select(0, torch.as_tensor(idx, dtype=torch.long, device=hidden.device))
-    return fused_linear_cross_entropy(h, model.lm_head.weight, torch.cat(labs), torch.cat(wts),
+    labels, weights = torch.cat(labs), torch.cat(wts)
+    if fused_ce == "pieces":
+        labels = torch.where(labels == loss.ignore_index, -1, labels)
+        return (linear_cross_entropy(h, model.lm_head.weight, labels).losses * weights).sum()
+    return fused_linear_cross_entropy(h, model.lm_head.weight, labels, weights,
                                       ignore_index=loss.ignore_index)
 
 
@@ -396,7 +402,7 @@ def _ensure_tree_attention(model):
 def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
                      gateway_mask: str = "tree", backward: str = "fused",
                      leaf_logits_only: bool = True, ssm_exact_inverse: bool = False,
-                     fused_ce: bool = False,
+                     fused_ce=False,
                      before_last_backward: Optional[Callable[[], None]] = None) -> torch.Tensor:
     """Partitioned tree forward/backward (tree_grad_hybrid.py:434-539):
     partitions run top-down, each with the gateway K/V of its cut node; then
@@ -408,7 +414,8 @@ def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
     gradients through ONE autograd traversal of the partition graph;
     with ``fused_ce`` (a ``make_tree_loss_fn`` loss, ``backward="fused"``) the
     leaf losses come from the final hidden states through the chunked LM-head
-    cross-entropy of ``ce`` and no logits are formed;
+    cross-entropy of ``ce`` and no logits are formed (``fused_ce="pieces"``:
+    through ``linear_cross_entropy``, by pieces of the vocabulary);
     ``"per_leaf"`` calls backward once per leaf loss and once per gateway with
     retain_graph, as the reference does (tree_grad_hybrid.py:521-539).  Both
     accumulate the same sum of gradients; every per-leaf call traverses the
@@ -437,6 +444,8 @@ def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
         raise ValueError("gateway_mask must be 'tree' or 'reference'")
     if backward not in ("fused", "per_leaf"):
         raise ValueError("backward must be 'fused' or 'per_leaf'")
+    if fused_ce not in (False, True, "pieces"):
+        raise ValueError("fused_ce must be False, True or 'pieces'")
     if fused_ce and (backward != "fused" or not isinstance(leaf_loss_fn, TreeLeafLoss)):
         raise ValueError("fused_ce needs backward='fused' and a make_tree_loss_fn loss")
     _ensure_tree_attention(model)
@@ -459,7 +468,7 @@ def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
                 cuts.append(cn)
         logits, info, full_kv, spans, ssm = _subtree_forward(
             model, p, gw, dev, gateway_mask, leaf_logits_only, cuts, ssm_exact_inverse,
-            leaf_loss_fn if fused_ce else None)
+            leaf_loss_fn if fused_ce else None, fused_ce)
         fwd[id(p)] = (logits, info, spans)
         if cuts:
             child = _make_child_gateways(full_kv, info, p, gw, cuts, gateway_mask, ssm)
