@@ -581,7 +581,7 @@ int tt_embedding_fwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids
 /* dweight [V, H], contiguous: dweight[v] = scale * the sum of dy[t] (row stride
  * dy_ld) over the t with ids[t] = v, in the order of t; 0 for other rows, for
  * padding_idx (-1: none), and nothing from ids outside [0, V). */
-int64_t tt_embedding_bwd_workspace_size(int64_t n, int64_t V);
+int64_t tt_embedding_bwd_workspace_size(int64_t n, int64_t V, int32_t H);
 int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids, int ids64,
                      const void* dy, int64_t dy_ld, float scale, int64_t padding_idx,
                      void* dweight, void* workspace, int64_t workspace_bytes, void* stream);

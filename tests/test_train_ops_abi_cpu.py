@@ -41,9 +41,9 @@ def test_embedding_gradient(bad):
 def test_embedding_types_and_workspace():
     assert embed(dtype=U8) == UNSUPPORTED and embed_bwd(dtype=U8) == UNSUPPORTED
     assert embed(n=0, ids=None, w=None, y=None) == _lib.TT_OK
-    need = status("tt_embedding_bwd_workspace_size", 4, 10)
+    need = status("tt_embedding_bwd_workspace_size", 4, 10, 8)
     assert embed_bwd(size=need - 1) == WORKSPACE and embed_bwd(ws=None) == WORKSPACE
-    assert status("tt_embedding_bwd_workspace_size", -1, 10) == 0
+    assert status("tt_embedding_bwd_workspace_size", -1, 10, 8) == 0
 
 
 def gated(dtype=BF16, T=4, H=16, F=8, x=P, x_ld=16, wg=P, wg_ld=16, wu=P, wu_ld=16, act=0, h=P,

@@ -114,7 +114,7 @@ SIGNATURES = {
     "tt_token_logprobs_bwd": (_INT, [_INT, _I64, _I32, _P, _I64, _P, _I32, _F32, _I32, _P, _P,
                                      _P, _P, _P, _P, _P]),
     "tt_embedding_fwd": (_INT, [_INT, _I64, _I64, _I32, _P, _INT, _P, _I64, _F32, _P, _P, _P]),
-    "tt_embedding_bwd_workspace_size": (_I64, [_I64, _I64]),
+    "tt_embedding_bwd_workspace_size": (_I64, [_I64, _I64, _I32]),
     "tt_embedding_bwd": (_INT, [_INT, _I64, _I64, _I32, _P, _INT, _P, _I64, _F32, _I64, _P, _P,
                                 _I64, _P]),
     "tt_gated_linear_fwd_workspace_size": (_I64, [_INT, _I64, _I32, _I32]),

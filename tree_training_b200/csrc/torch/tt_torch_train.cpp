@@ -67,7 +67,7 @@ struct EmbeddingFunction : Function<EmbeddingFunction> {
     Tensor dw = empty({V, H}, dy, dy.scalar_type());
     {
       On on(dy);
-      const int64_t size = tt_embedding_bwd_workspace_size(n, V);
+      const int64_t size = tt_embedding_bwd_workspace_size(n, V, (int32_t)H);
       const Tensor ws = bytes(size, dy);
       check_status("tt_embedding_bwd",
                    tt_embedding_bwd(dtype_code(dy), n, V, (int32_t)H, ptr(ids),

@@ -5,9 +5,16 @@
 //
 // Bound by HBM.  Forward: a token's row is read and written once.  Backward: every
 // row of dW is written (the words of no token as zeros), which is most of its
-// traffic, and dy is read once.  The sum goes by sorted tokens: two or three stable
-// counting sorts by ten bits of the id each (the sort of the experts' plan), so
-// that a word's rows stand next to one another in the order of the tokens.
+// traffic, and dy is read once.
+//
+// The gradient's sum goes by sorted tokens: stable counting sorts by up to ten bits of
+// the id each, two launches a sort (as the experts' plan), so that a word's rows stand
+// next to one another in the order of the tokens.  The sorted rows are cut into chunks
+// of 32, whatever words they hold, so that a word of half the text is summed by as many
+// blocks as its rows are; sums of words that reach over a chunk's end leave as fp32
+// parts and are added up in order by a last launch.  The sorts are bound by latency
+// (20 us for 32,768 tokens): the rows of words without tokens, which a bitmap of the
+// first launch tells, are zeroed by further blocks of the launches after it.
 #include <algorithm>
 
 #include "tt_vec.cuh"
@@ -16,8 +23,7 @@ namespace tt {
 namespace embed {
 namespace {
 
-constexpr int kDigits = 1024;          // of a counting sort
-constexpr int kBits = 10;
+constexpr int kBits = 10;              // of a counting sort, at most
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t t) {
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[t]
@@ -73,74 +79,363 @@ __global__ void __launch_bounds__(256) rows_kernel(const Rows a) {
 
 // ---- the gradient -------------------------------------------------------------
 
-// The digit of each entry's id in the order given (null: as they are); -1 for an
-// entry without a row.
-__global__ void __launch_bounds__(256)
-    digits_kernel(const void* ids, int ids64, int64_t n, int64_t V, int64_t padding,
-                  const int32_t* order, int shift, int32_t* digits) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t t = order ? order[i] : i;
-  int32_t d = -1;
-  if (t >= 0) {
-    const int64_t id = id_at(ids, ids64, t);
-    if (id >= 0 && id < V && id != padding) d = (int32_t)((id >> shift) & (kDigits - 1));
-  }
-  digits[i] = d;
-}
+constexpr int kWarps = 8;              // of a sorting block
+constexpr int kSteps = 8;              // of 32 entries, fetched together
+constexpr int kPlaceThreads = 512;
+constexpr int kChunk = 32;             // sorted rows a group of threads adds up
 
-// The entries sorted by one more digit.
-__global__ void __launch_bounds__(256)
-    follow_kernel(const int32_t* order, const int32_t* entries, int64_t n, int32_t* next) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int32_t e = entries[i];
-  next[i] = e < 0 ? -1 : order[e];
-}
-
-// Where each word's entries begin in the sorted order; -1 (as cleared) for others.
-__global__ void __launch_bounds__(256)
-    heads_kernel(const void* ids, int ids64, int64_t n, const int32_t* order, int32_t* first) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n || order[i] < 0) return;
-  const int64_t id = id_at(ids, ids64, order[i]);
-  if (i == 0 || id_at(ids, ids64, order[i - 1]) != id) first[id] = (int32_t)i;
-}
-
-struct Sum {
+struct Grad {
   const void* ids;
   int ids64;
-  int64_t n, V;
+  int64_t n, V, padding;
   int H;
-  const int32_t *order, *first;
   const void* dy;
   int64_t ld;
   float scale;
   void* dw;
+  uint32_t* used;                      // [V / 32]: words with tokens
+  int32_t *slots, *counts;             // of the sorts
+  float* parts;                        // [chunks][2][part_ld]
+  int64_t part_ld, chunks;
 };
 
-// A block a word.
+// The entry's word, -1 where it has no gradient.
+__device__ __forceinline__ int32_t word_of(const Grad& a, int64_t t) {
+  if (t < 0) return -1;
+  const int64_t id = id_at(a.ids, a.ids64, t);
+  return id >= 0 && id < a.V && id != a.padding ? (int32_t)id : -1;
+}
+
+// Zeroes the rows of the words without tokens: share `part` of `parts`, by the blocks
+// `block` of `blocks`, a warp a row.
 template <typename T>
-__global__ void __launch_bounds__(128) sum_kernel(const Sum a) {
-  for (int64_t v = blockIdx.x; v < a.V; v += gridDim.x) {
-    const int32_t first = a.first[v];
-    for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
-      float s = 0.f;
-      if (first >= 0)
-        for (int64_t i = first; i < a.n && a.order[i] >= 0; ++i) {
-          const int64_t t = a.order[i];
-          if (id_at(a.ids, a.ids64, t) != v) break;
-          s += to_f32(reinterpret_cast<const T*>(a.dy)[t * a.ld + c]);
-        }
-      reinterpret_cast<T*>(a.dw)[v * a.H + c] = from_f32<T>(s * a.scale);
+__device__ __forceinline__ void zero_rows(const Grad& a, int part, int parts, int block,
+                                          int blocks) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  const int64_t per = (a.V + parts - 1) / parts;
+  const int64_t end = min(a.V, (part + 1) * per);
+  for (int64_t v = part * per + (int64_t)block * warps + threadIdx.x / 32; v < end;
+       v += (int64_t)blocks * warps) {
+    if ((a.used[v >> 5] >> (v & 31)) & 1) continue;
+    T* row = reinterpret_cast<T*>(a.dw) + v * a.H;
+    const int ahead = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
+    for (int e0 = lane * N - ahead; e0 < a.H; e0 += 32 * N)
+      vec::store_part<T>(row, e0, a.H, make_uint4(0, 0, 0, 0));
+  }
+}
+
+// One counting sort of the entries (order: as the sort before left them; null: as
+// they are) by the digit at `shift`; entries without a word go last.
+struct Sort {
+  const int32_t* order;
+  int32_t* next;
+  int shift, digits;                   // digits: how many; that one is "no word"
+  int64_t run;                         // entries of a warp
+  int blocks;                          // that sort; further ones zero rows
+  int part, parts;                     // the share of rows (parts 0: none)
+};
+
+__device__ __forceinline__ int digit_of(const Sort& s, int32_t word) {
+  return word < 0 ? s.digits : (word >> s.shift) & (s.digits - 1);
+}
+
+// The lanes whose e is this lane's, by one vote a bit.
+__device__ __forceinline__ unsigned same_as(int e, int bits) {
+  unsigned m = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (e >> b) & 1;
+    const unsigned v = __ballot_sync(0xffffffffu, one);
+    m &= one ? v : ~v;
+  }
+  return m;
+}
+
+// Each entry's rank among its block's entries of the same digit, the blocks' counts,
+// and (first sort) the bitmap of words.
+template <typename T, bool kFirst>
+__global__ void __launch_bounds__(32 * kWarps) rank_kernel(const Grad a, const Sort s) {
+  extern __shared__ int hist[];               // [warps][digits + 1]: counts, then ranks
+  if ((int)blockIdx.x >= s.blocks) {
+    zero_rows<T>(a, s.part, s.parts, blockIdx.x - s.blocks, gridDim.x - s.blocks);
+    return;
+  }
+  const int E = s.digits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t begin = min(a.n, ((int64_t)blockIdx.x * kWarps + warp) * s.run);
+  const int64_t end = min(a.n, begin + s.run);
+  for (int i = threadIdx.x; i < kWarps * (E + 1); i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  int* mine = hist + warp * (E + 1);
+  const int bits = 32 - __clz(E + 1);
+  int e[kSteps];
+  unsigned same[kSteps];
+  auto fetch = [&](int64_t from, bool mark) {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int64_t i = from + j * 32 + lane;
+      e[j] = E + 1;
+      if (i < end) {
+        const int32_t w = word_of(a, s.order ? s.order[i] : i);
+        e[j] = digit_of(s, w);
+        if (kFirst && mark && w >= 0) atomicOr(a.used + (w >> 5), 1u << (w & 31));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+      if (from + j * 32 < end) same[j] = same_as(e[j], bits);
+  };
+  for (int64_t from = begin; from < end; from += 32 * kSteps) {
+    fetch(from, true);
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+      if (e[j] <= E && lane == __ffs(same[j]) - 1) atomicAdd(mine + e[j], __popc(same[j]));
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x <= E; x += blockDim.x) {
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = hist[w * (E + 1) + x];
+      hist[w * (E + 1) + x] = all;
+      all += c;
+    }
+    a.counts[(int64_t)blockIdx.x * (E + 1) + x] = all;
+  }
+  __syncthreads();
+  // (each step's leaders add theirs before the lanes part again for the next step's)
+  const bool kept = end - begin <= 32 * kSteps;        // the digits are still in e
+  for (int64_t from = begin; from < end; from += 32 * kSteps) {
+    if (!kept) fetch(from, false);
+    int base[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      base[j] = 0;
+      if (e[j] <= E && lane == __ffs(same[j]) - 1)
+        base[j] = atomicAdd(mine + e[j], __popc(same[j]));
+      __syncwarp();
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int64_t i = from + j * 32 + lane;
+      if (from + j * 32 >= end) continue;
+      const int rank = __shfl_sync(0xffffffffu, base[j], __ffs(same[j]) - 1) +
+                       __popc(same[j] & ((1u << lane) - 1));
+      if (e[j] <= E) a.slots[i] = rank;
     }
   }
 }
 
-int digits_of(int64_t V) {
-  int d = 1;
-  while (d < 4 && ((int64_t)1 << (kBits * d)) < V) ++d;
-  return d;
+// The entries in their places: the blocks' counts added up, then the ranks.
+template <typename T>
+__global__ void __launch_bounds__(kPlaceThreads) place_kernel(const Grad a, const Sort s) {
+  extern __shared__ int sm[];
+  if ((int)blockIdx.x >= s.blocks) {
+    zero_rows<T>(a, s.part, s.parts, blockIdx.x - s.blocks, gridDim.x - s.blocks);
+    return;
+  }
+  const int E = s.digits, b0 = blockIdx.x;
+  int* total = sm;                            // [E + 1]
+  int* first = sm + E + 1;                    // [E + 1]: this block's first rows
+  __shared__ int warp_sum[kPlaceThreads / 32];
+  const int parts = max(1, (int)blockDim.x / (E + 1)), share = (s.blocks + parts - 1) / parts;
+  for (int x = threadIdx.x; x < 2 * (E + 1); x += blockDim.x) sm[x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < parts * (E + 1); i += blockDim.x) {
+    const int part = i / (E + 1), x = i - part * (E + 1);
+    const int end = min(s.blocks, (part + 1) * share);
+    int all = 0, before = 0;
+    for (int b = part * share; b < end; b += 16) {
+      int c[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        c[j] = b + j < end ? __ldg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        all += c[j];
+        before += b + j < b0 ? c[j] : 0;
+      }
+    }
+    atomicAdd(total + x, all);
+    atomicAdd(first + x, before);
+  }
+  __syncthreads();
+  const int per = (E + (int)blockDim.x) / (int)blockDim.x;
+  const int x0 = min((int)threadIdx.x * per, E + 1), x1 = min(x0 + per, E + 1);
+  int sum = 0;
+  for (int x = x0; x < x1; ++x) sum += total[x];
+  int scan = sum;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += up;
+  }
+  if (lane == 31) warp_sum[warp] = scan;
+  __syncthreads();
+  int at = scan - sum;
+  for (int w = 0; w < warp; ++w) at += warp_sum[w];
+  for (int x = x0; x < x1; ++x) {
+    first[x] += at;
+    at += total[x];
+  }
+  __syncthreads();
+  const int64_t begin = min(a.n, (int64_t)b0 * kWarps * s.run);
+  const int64_t end = min(a.n, begin + kWarps * s.run);
+  for (int64_t i = begin + threadIdx.x; i < end; i += blockDim.x) {
+    const int64_t t = s.order ? s.order[i] : i;
+    const int32_t w = word_of(a, t);
+    s.next[first[digit_of(s, w)] + a.slots[i]] = w < 0 ? -1 : (int32_t)t;
+  }
+}
+
+// Adds up the sorted rows: a group of threads (whole warps) a chunk, a thread the
+// elements e0 .. of its word's row, on 16-byte boundaries of dW; columns beyond the
+// group's by gridDim.y.  Further blocks zero rows.
+template <typename T, bool kAligned>
+__global__ void __launch_bounds__(512)
+    sum_kernel(const Grad a, const int32_t* order, int group, int sum_blocks, int part,
+               int parts_of_rows) {
+  constexpr int N = 16 / (int)sizeof(T);
+  constexpr int kAhead = 4;                   // rows fetched together
+  if ((int)blockIdx.x >= sum_blocks) {
+    if (blockIdx.y == 0)
+      zero_rows<T>(a, part, parts_of_rows, blockIdx.x - sum_blocks, gridDim.x - sum_blocks);
+    return;
+  }
+  const int g = threadIdx.x / group, tid = threadIdx.x - g * group, lane = threadIdx.x & 31;
+  const int64_t chunk = (int64_t)blockIdx.x * (blockDim.x / group) + g;
+  if (chunk >= a.chunks) return;
+  const int64_t r0 = chunk * kChunk;
+  const int rows = (int)min((int64_t)kChunk, a.n - r0);
+  const int32_t my_t = lane < rows ? order[r0 + lane] : -1;
+  const int32_t my_w = word_of(a, my_t);
+  const int32_t before = r0 > 0 ? word_of(a, order[r0 - 1]) : -1;
+  const int32_t after = r0 + rows < a.n ? word_of(a, order[r0 + rows]) : -1;
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+  const T* lo = dy;
+  const T* hi = dy + (a.n - 1) * a.ld + a.H;
+  const int64_t col = ((int64_t)blockIdx.y * group + tid) * N;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  // elements of dW before a row's 16-byte boundary (the packs begin there)
+  auto ahead_of = [&](int32_t w) {
+    return kAligned ? 0
+                    : (int)(reinterpret_cast<uintptr_t>(reinterpret_cast<T*>(a.dw) +
+                                                        (int64_t)w * a.H) & 15) / (int)sizeof(T);
+  };
+  int from = 0;                               // where the word's rows begin in the chunk
+  for (int r = 0; r < rows; r += kAhead) {
+    uint4 raw[kAhead];
+    int32_t w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int at = min(r + j, kChunk - 1);
+      const int32_t t = __shfl_sync(0xffffffffu, my_t, at);
+      w[j] = r + j < rows ? __shfl_sync(0xffffffffu, my_w, at) : -1;
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (w[j] >= 0) {
+        if constexpr (kAligned) {
+          if (col < a.H) raw[j] = __ldg(reinterpret_cast<const uint4*>(dy + t * a.ld + col));
+        } else {
+          const int64_t e0 = col - ahead_of(w[j]);
+          if (e0 < a.H) raw[j] = vec::load_any_of<T>(dy + t * a.ld, e0, a.H, lo, hi);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (w[j] < 0) continue;                 // (past the last word, too: they are sorted last)
+      float v[N];
+      vec::unpack<T, N>(raw[j], v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += v[i];
+      const int here = r + j;
+      const int32_t next = here + 1 < rows ? __shfl_sync(0xffffffffu, my_w, here + 1) : after;
+      if (next == w[j]) continue;
+      // the word's last row: whole, or the end of a sum that began before
+      const bool whole = from > 0 || before != w[j];
+      if (whole) {
+        const int64_t e0 = col - ahead_of(w[j]);
+        if (e0 < a.H) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] *= a.scale;
+          T* row = reinterpret_cast<T*>(a.dw) + (int64_t)w[j] * a.H;
+          if constexpr (kAligned) vec::store<T, N>(row + col, acc);
+          else vec::store_part<T>(row, e0, a.H, vec::pack<T, N>(acc));
+        }
+      } else if (col < a.part_ld) {
+        float* p = a.parts + (chunk * 2) * a.part_ld + col;
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = acc[i];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      from = here + 1;
+    }
+  }
+  // a word that goes on in the next chunk (after whole chunks of it: from == 0)
+  const int32_t last = __shfl_sync(0xffffffffu, my_w, rows - 1);
+  if (last >= 0 && last == after && col < a.part_ld) {
+    const bool began = from > 0 || before != last;
+    float* p = a.parts + (chunk * 2 + (began ? 1 : 0)) * a.part_ld + col;
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = acc[i];
+  }
+}
+
+// The sums that reach over chunks: a block for each chunk in which such a word begins
+// (blockIdx.y: columns).
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const Grad a, const int32_t* order) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int64_t chunk = blockIdx.x, next = (chunk + 1) * kChunk;
+  if (next >= a.n) return;
+  const int32_t w = word_of(a, order[next - 1]);
+  if (w < 0 || word_of(a, order[next]) != w) return;
+  const int64_t r0 = chunk * kChunk;
+  // (it began here, not before)
+  if (r0 > 0 && word_of(a, order[r0 - 1]) == w) return;
+  // its last row, by bisection: words are sorted, those without one last
+  int64_t lo = next, hi = a.n - 1;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) / 2;
+    if (word_of(a, order[mid]) == w) lo = mid; else hi = mid - 1;
+  }
+  const int64_t last = lo / kChunk;
+  const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * N;
+  T* row = reinterpret_cast<T*>(a.dw) + (int64_t)w * a.H;
+  const int64_t e0 = col - (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
+  if (col >= a.part_ld || e0 >= a.H) return;
+  float acc[N];
+  const float* p = a.parts + (chunk * 2 + 1) * a.part_ld + col;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = p[i];
+#pragma unroll 4
+  for (int64_t c = chunk + 1; c <= last; ++c) {
+    const float* q = a.parts + (c * 2) * a.part_ld + col;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += q[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= a.scale;
+  vec::store_part<T>(row, e0, a.H, vec::pack<T, N>(acc));
+}
+
+// ---- host ---------------------------------------------------------------------
+
+// Sorts, and the bits of each one's digit.
+int sorts_of(int64_t V, int* bits) {
+  int all = 1;
+  while (((int64_t)1 << all) < V) ++all;
+  const int sorts = (all + kBits - 1) / kBits;
+  *bits = (all + sorts - 1) / sorts;
+  return sorts;
+}
+
+// Blocks of a sort (each adds up `blocks` counts a digit).
+int sort_blocks(int64_t n, int digits) {
+  const int64_t most = std::max<int64_t>(8, std::min<int64_t>(64, 32768 / (digits + 1)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, (n + 32 * kWarps - 1) / (32 * kWarps)));
 }
 
 int64_t round16(int64_t b) { return (b + 15) / 16 * 16; }
@@ -153,6 +448,7 @@ bool ok_sizes(int64_t n, int64_t V, int H) {
 }  // namespace embed
 }  // namespace tt
 
+using namespace tt;
 using namespace tt::embed;
 
 extern "C" int tt_embedding_fwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids,
@@ -171,11 +467,84 @@ extern "C" int tt_embedding_fwd(int dtype, int64_t n, int64_t V, int32_t H, cons
   });
 }
 
-extern "C" int64_t tt_embedding_bwd_workspace_size(int64_t n, int64_t V) {
-  if (!ok_sizes(n, V, 1)) return 0;
-  // digits, slots, entries, two orders; first rows; the sort's offsets and counts
-  return 5 * round16(4 * n) + round16(4 * V) + round16(4 * (kDigits + 1)) +
-         round16(tt_moe_plan_workspace_size(n, kDigits));
+namespace {
+
+// (the packs of a row of dW that begins off a 16-byte boundary: one more)
+int64_t part_ld(int32_t H) { return (H + 7) / 8 * 8 + 8; }
+
+struct Layout {
+  int64_t used, slots, order, counts, parts, all;
+  Layout(int64_t n, int64_t V, int32_t H) {
+    int bits;
+    sorts_of(V, &bits);
+    used = round16((V + 31) / 32 * 4);
+    slots = round16(4 * n);
+    order = round16(4 * n);
+    counts = round16((int64_t)sort_blocks(n, 1 << bits) * ((1 << bits) + 1) * 4);
+    parts = (n + kChunk - 1) / kChunk * 2 * part_ld(H) * 4;
+    all = used + slots + 2 * order + counts + parts;
+  }
+};
+
+template <typename T>
+int gradient(Grad a, int32_t* const* orders, cudaStream_t st) {
+  int bits;
+  const int sorts = sorts_of(a.V, &bits), digits = 1 << bits;
+  const int blocks = sort_blocks(a.n, digits);
+  const int64_t warps = (int64_t)blocks * kWarps;
+  // every launch but the first zeroes a share of the rows
+  const int shares = 2 * sorts;
+  const int64_t bytes = a.V * a.H * (int64_t)sizeof(T) / shares;
+  const int zero_blocks = (int)std::max<int64_t>(1, std::min<int64_t>(4 * vec::kSMs, bytes >> 13));
+  Sort s{};
+  s.digits = digits, s.blocks = blocks, s.parts = shares;
+  s.run = std::max<int64_t>(32, ((a.n + warps - 1) / warps + 31) / 32 * 32);
+  const size_t rank_smem = sizeof(int) * kWarps * (digits + 1);
+  const size_t place_smem = sizeof(int) * 2 * (digits + 1);
+  const int32_t* order = nullptr;
+  for (int d = 0; d < sorts; ++d) {
+    s.order = order, s.next = orders[d & 1], s.shift = bits * d;
+    if (d == 0) {
+      rank_kernel<T, true><<<blocks, 32 * kWarps, rank_smem, st>>>(a, s);
+    } else {
+      rank_kernel<T, false><<<blocks + zero_blocks, 32 * kWarps, rank_smem, st>>>(a, s);
+      ++s.part;
+    }
+    place_kernel<T><<<blocks + zero_blocks, kPlaceThreads, place_smem, st>>>(a, s);
+    ++s.part;
+    tt_count_launches(2);
+    order = s.next;
+  }
+  constexpr int N = 16 / (int)sizeof(T);
+  const bool aligned = a.H % N == 0 && a.ld % N == 0 &&
+                       ((reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dw)) &
+                        15) == 0;
+  const int packs = (int)((a.H + N - 1) / N) + (aligned ? 0 : 1);
+  const int group = std::min(512, (packs + 31) / 32 * 32);
+  const int groups = std::max(1, 256 / group);
+  const unsigned cols = (unsigned)((packs + group - 1) / group);
+  const int64_t sum_blocks = (a.chunks + groups - 1) / groups;
+  const dim3 grid((unsigned)(sum_blocks + zero_blocks), cols);
+  if (aligned)
+    sum_kernel<T, true><<<grid, group * groups, 0, st>>>(a, order, group, (int)sum_blocks, s.part,
+                                                         shares);
+  else
+    sum_kernel<T, false><<<grid, group * groups, 0, st>>>(a, order, group, (int)sum_blocks, s.part,
+                                                          shares);
+  tt_count_launches(1);
+  if (a.chunks > 1) {
+    join_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)((a.part_ld / N + 127) / 128)), 128, 0,
+                     st>>>(a, order);
+    tt_count_launches(1);
+  }
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" int64_t tt_embedding_bwd_workspace_size(int64_t n, int64_t V, int32_t H) {
+  if (!ok_sizes(n, V, H)) return 0;
+  return Layout(n, V, H).all;
 }
 
 extern "C" int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids,
@@ -184,46 +553,20 @@ extern "C" int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, cons
                                 int64_t workspace_bytes, void* stream) {
   if (!ok_sizes(n, V, H) || (n > 1 && dy_ld < H)) return TT_ERR_INVALID_ARG;
   if (!dweight || (n > 0 && (!ids || !dy))) return TT_ERR_INVALID_ARG;
-  if (workspace_bytes < tt_embedding_bwd_workspace_size(n, V) || !workspace)
-    return TT_ERR_WORKSPACE;
+  if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
+  const Layout l(n, V, H);
+  if (workspace_bytes < l.all || !workspace) return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   char* p = (char*)workspace;
-  auto take = [&](int64_t bytes) {
-    char* q = p;
-    p += round16(bytes);
-    return q;
-  };
-  int32_t* digits = (int32_t*)take(4 * n);
-  int32_t* slots = (int32_t*)take(4 * n);
-  int32_t* entries = (int32_t*)take(4 * n);
-  int32_t* orders[2] = {(int32_t*)take(4 * n), (int32_t*)take(4 * n)};
-  int32_t* first = (int32_t*)take(4 * V);
-  int32_t* offsets = (int32_t*)take(4 * (kDigits + 1));
-  const int64_t plan_bytes = tt_moe_plan_workspace_size(n, kDigits);
+  Grad a{ids, ids64, n, V, padding_idx, H, dy, dy_ld, scale, dweight};
+  a.used = (uint32_t*)p, p += l.used;
+  a.slots = (int32_t*)p, p += l.slots;
+  int32_t* orders[2] = {(int32_t*)p, (int32_t*)(p + l.order)};
+  p += 2 * l.order;
+  a.counts = (int32_t*)p, p += l.counts;
+  a.parts = (float*)p, a.part_ld = part_ld(H), a.chunks = (n + kChunk - 1) / kChunk;
+  if (cudaMemsetAsync(a.used, 0, l.used, st) != cudaSuccess) return TT_ERR_CUDA;
   return tt::vec::dispatch_float(dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    const unsigned blocks = (unsigned)((n + 255) / 256);
-    const int32_t* order = nullptr;
-    if (cudaMemsetAsync(first, 0xff, 4 * V, st) != cudaSuccess) return TT_ERR_CUDA;
-    if (n > 0) {
-      for (int d = 0; d < digits_of(V); ++d) {
-        digits_kernel<<<blocks, 256, 0, st>>>(ids, ids64, n, V, padding_idx, order, kBits * d,
-                                              digits);
-        int32_t* next = orders[d & 1];
-        int32_t* to = d == 0 ? next : entries;
-        if (const int rc = tt_moe_plan(digits, 0, n, kDigits, slots, to, offsets, p, plan_bytes,
-                                       st))
-          return rc;
-        if (d > 0) follow_kernel<<<blocks, 256, 0, st>>>(order, entries, n, next);
-        order = next;
-        tt_count_launches(d > 0 ? 2 : 1);
-      }
-      heads_kernel<<<blocks, 256, 0, st>>>(ids, ids64, n, order, first);
-      tt_count_launches(1);
-    }
-    const Sum a{ids, ids64, n, V, H, order, first, dy, dy_ld, scale, dweight};
-    sum_kernel<T><<<(unsigned)std::min<int64_t>(V, 16 * tt::vec::kSMs), 128, 0, st>>>(a);
-    tt_count_launches(1);
-    return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+    return gradient<decltype(t)>(a, orders, st);
   });
 }
