@@ -10,7 +10,7 @@
 // The gradient's sum goes by sorted tokens: stable counting sorts by up to ten bits of
 // the id each, two launches a sort (as the experts' plan), so that a word's rows stand
 // next to one another in the order of the tokens.  The sorted rows are cut into chunks
-// of 32, whatever words they hold, so that a word of half the text is summed by as many
+// of up to 32, whatever words they hold, so that a word of half the text is summed by as many
 // blocks as its rows are; sums of words that reach over a chunk's end leave as fp32
 // parts and are added up in order by a last launch.  The sorts are bound by latency
 // (20 us for 32,768 tokens): the rows of words without tokens, which a bitmap of the
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Rows a) {
 constexpr int kWarps = 8;              // of a sorting block
 constexpr int kSteps = 8;              // of 32 entries, fetched together
 constexpr int kPlaceThreads = 512;
-constexpr int kChunk = 32;             // sorted rows a group of threads adds up
+constexpr int kMaxChunk = 32;
 
 struct Grad {
   const void* ids;
@@ -97,7 +97,12 @@ struct Grad {
   int32_t *slots, *counts;             // of the sorts
   float* parts;                        // [chunks][2][part_ld]
   int64_t part_ld, chunks;
+  int chunk;                           // sorted rows of a group of threads
+  int2* ends;                          // [chunks]: kBegins, kThrough; the word
 };
+
+enum { kBegins = 1, kThrough = 2 };    // a word begins in the chunk and goes on behind it;
+                                       // fills it and goes on on both sides
 
 // The entry's word, -1 where it has no gradient.
 __device__ __forceinline__ int32_t word_of(const Grad& a, int64_t t) {
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(512)
     sum_kernel(const Grad a, const int32_t* order, int group, int sum_blocks, int part,
                int parts_of_rows) {
   constexpr int N = 16 / (int)sizeof(T);
-  constexpr int kAhead = 4;                   // rows fetched together
+  constexpr int kAhead = kAligned ? 8 : 4;    // rows fetched together
   if ((int)blockIdx.x >= sum_blocks) {
     if (blockIdx.y == 0)
       zero_rows<T>(a, part, parts_of_rows, blockIdx.x - sum_blocks, gridDim.x - sum_blocks);
@@ -304,8 +309,8 @@ __global__ void __launch_bounds__(512)
   const int g = threadIdx.x / group, tid = threadIdx.x - g * group, lane = threadIdx.x & 31;
   const int64_t chunk = (int64_t)blockIdx.x * (blockDim.x / group) + g;
   if (chunk >= a.chunks) return;
-  const int64_t r0 = chunk * kChunk;
-  const int rows = (int)min((int64_t)kChunk, a.n - r0);
+  const int64_t r0 = chunk * a.chunk;
+  const int rows = (int)min((int64_t)a.chunk, a.n - r0);
   const int32_t my_t = lane < rows ? order[r0 + lane] : -1;
   const int32_t my_w = word_of(a, my_t);
   const int32_t before = r0 > 0 ? word_of(a, order[r0 - 1]) : -1;
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(512)
     int32_t w[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const int at = min(r + j, kChunk - 1);
+      const int at = min(r + j, kMaxChunk - 1);
       const int32_t t = __shfl_sync(0xffffffffu, my_t, at);
       w[j] = r + j < rows ? __shfl_sync(0xffffffffu, my_w, at) : -1;
       raw[j] = make_uint4(0, 0, 0, 0);
@@ -375,50 +380,106 @@ __global__ void __launch_bounds__(512)
   }
   // a word that goes on in the next chunk (after whole chunks of it: from == 0)
   const int32_t last = __shfl_sync(0xffffffffu, my_w, rows - 1);
-  if (last >= 0 && last == after && col < a.part_ld) {
-    const bool began = from > 0 || before != last;
+  const bool goes_on = last >= 0 && last == after, began = from > 0 || before != last;
+  if (tid == 0 && blockIdx.y == 0)
+    a.ends[chunk] = make_int2(!goes_on ? 0 : began ? kBegins : kThrough, last);
+  if (goes_on && col < a.part_ld) {
     float* p = a.parts + (chunk * 2 + (began ? 1 : 0)) * a.part_ld + col;
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = acc[i];
   }
 }
 
-// The sums that reach over chunks: a block for each chunk in which such a word begins
-// (blockIdx.y: columns).
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const Grad a, const int32_t* order) {
-  constexpr int N = 16 / (int)sizeof(T);
-  const int64_t chunk = blockIdx.x, next = (chunk + 1) * kChunk;
-  if (next >= a.n) return;
-  const int32_t w = word_of(a, order[next - 1]);
-  if (w < 0 || word_of(a, order[next]) != w) return;
-  const int64_t r0 = chunk * kChunk;
-  // (it began here, not before)
-  if (r0 > 0 && word_of(a, order[r0 - 1]) == w) return;
-  // its last row, by bisection: words are sorted, those without one last
-  int64_t lo = next, hi = a.n - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) / 2;
-    if (word_of(a, order[mid]) == w) lo = mid; else hi = mid - 1;
+constexpr int kJoinWarps = 16;
+
+constexpr int kShort = 8;              // parts that one warp adds up
+
+// The chunk in which the word ends that begins in `chunk` and goes on behind it: the
+// first that it does not go through.
+__device__ __forceinline__ int64_t ends_in(const Grad& a, int64_t chunk) {
+  for (int64_t last = chunk + 1;; last += 32) {
+    const int64_t c = last + (threadIdx.x & 31);
+    const unsigned stop = __ballot_sync(0xffffffffu, c >= a.chunks || a.ends[c].x != kThrough);
+    if (stop) return last + __ffs(stop) - 1;
   }
-  const int64_t last = lo / kChunk;
-  const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * N;
+}
+
+// Parts begin .. end of a word's (slot 1 of the chunk it begins in, slot 0 of those
+// after it), at columns col ...
+template <int N>
+__device__ __forceinline__ void add_parts(const Grad& a, int64_t chunk, int64_t begin, int64_t end,
+                                          int64_t col, float (&acc)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  if (col >= a.part_ld) return;
+#pragma unroll 8
+  for (int64_t k = begin; k < end; ++k) {
+    const float4* q = reinterpret_cast<const float4*>(
+        a.parts + ((chunk + k) * 2 + (k == 0 ? 1 : 0)) * a.part_ld + col);
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(q + i / 4);
+      acc[i] += x.x, acc[i + 1] += x.y, acc[i + 2] += x.z, acc[i + 3] += x.w;
+    }
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_sum(const Grad& a, int32_t w, int64_t col, float (&acc)[N]) {
   T* row = reinterpret_cast<T*>(a.dw) + (int64_t)w * a.H;
   const int64_t e0 = col - (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
   if (col >= a.part_ld || e0 >= a.H) return;
-  float acc[N];
-  const float* p = a.parts + (chunk * 2 + 1) * a.part_ld + col;
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = p[i];
-#pragma unroll 4
-  for (int64_t c = chunk + 1; c <= last; ++c) {
-    const float* q = a.parts + (c * 2) * a.part_ld + col;
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += q[i];
-  }
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] *= a.scale;
   vec::store_part<T>(row, e0, a.H, vec::pack<T, N>(acc));
+}
+
+// The sums that reach over chunks (blockIdx.y: columns): the chunks in which such a
+// word begins are shared out over the blocks, which look for theirs first. A word of
+// few parts is one warp's; of a longer one the warps add up runs of the parts, and the
+// first warp the runs' sums, in order.
+template <typename T>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Grad a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  constexpr int kThreads = 32 * kJoinWarps;
+  __shared__ float sm[kJoinWarps][32][N + 1];
+  __shared__ int64_t mine[kThreads], longer[kThreads];
+  __shared__ int count, longer_count;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col = ((int64_t)blockIdx.y * 32 + lane) * N;
+  float acc[N];
+  for (int64_t base = blockIdx.x; base < a.chunks; base += (int64_t)kThreads * gridDim.x) {
+    if (threadIdx.x == 0) count = longer_count = 0;
+    __syncthreads();
+    const int64_t c = base + (int64_t)threadIdx.x * gridDim.x;
+    if (c < a.chunks && a.ends[c].x == kBegins) mine[atomicAdd(&count, 1)] = c;
+    __syncthreads();
+    for (int i = warp; i < count; i += kJoinWarps) {
+      const int64_t chunk = mine[i], n = ends_in(a, chunk) - chunk + 1;
+      if (n > kShort) {
+        if (lane == 0) longer[atomicAdd(&longer_count, 1)] = chunk;
+        continue;
+      }
+      add_parts<N>(a, chunk, 0, n, col, acc);
+      store_sum<T, N>(a, a.ends[chunk].y, col, acc);
+    }
+    __syncthreads();
+    for (int i = 0; i < longer_count; ++i) {
+      const int64_t chunk = longer[i], n = ends_in(a, chunk) - chunk + 1;
+      const int64_t run = (n + kJoinWarps - 1) / kJoinWarps;
+      add_parts<N>(a, chunk, warp * run, min(n, (warp + 1) * run), col, acc);
+#pragma unroll
+      for (int x = 0; x < N; ++x) sm[warp][lane][x] = acc[x];
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+          for (int x = 0; x < N; ++x) acc[x] += sm[w][lane][x];
+        store_sum<T, N>(a, a.ends[chunk].y, col, acc);
+      }
+      __syncthreads();
+    }
+  }
 }
 
 // ---- host ---------------------------------------------------------------------
@@ -473,7 +534,8 @@ namespace {
 int64_t part_ld(int32_t H) { return (H + 7) / 8 * 8 + 8; }
 
 struct Layout {
-  int64_t used, slots, order, counts, parts, all;
+  int64_t used, slots, order, counts, parts, ends, all;
+  int chunk;
   Layout(int64_t n, int64_t V, int32_t H) {
     int bits;
     sorts_of(V, &bits);
@@ -481,8 +543,13 @@ struct Layout {
     slots = round16(4 * n);
     order = round16(4 * n);
     counts = round16((int64_t)sort_blocks(n, 1 << bits) * ((1 << bits) + 1) * 4);
-    parts = (n + kChunk - 1) / kChunk * 2 * part_ld(H) * 4;
-    all = used + slots + 2 * order + counts + parts;
+    // smaller chunks where there are few rows: about a thousand threads an SM
+    chunk = kMaxChunk;
+    while (chunk > 4 && n / chunk * ((H + 255) / 256 * 32) < (int64_t)1024 * vec::kSMs) chunk /= 2;
+    const int64_t chunks = (n + chunk - 1) / chunk;
+    parts = chunks * 2 * part_ld(H) * 4;
+    ends = round16(chunks * 8);
+    all = used + slots + 2 * order + counts + parts + ends;
   }
 };
 
@@ -533,8 +600,9 @@ int gradient(Grad a, int32_t* const* orders, cudaStream_t st) {
                                                           shares);
   tt_count_launches(1);
   if (a.chunks > 1) {
-    join_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)((a.part_ld / N + 127) / 128)), 128, 0,
-                     st>>>(a, order);
+    const int64_t cols = (a.part_ld / N + 31) / 32;
+    const int64_t blocks = std::max<int64_t>(1, std::min(a.chunks, 4 * vec::kSMs / cols));
+    join_kernel<T><<<dim3((unsigned)blocks, (unsigned)cols), 32 * kJoinWarps, 0, st>>>(a);
     tt_count_launches(1);
   }
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
@@ -564,7 +632,9 @@ extern "C" int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, cons
   int32_t* orders[2] = {(int32_t*)p, (int32_t*)(p + l.order)};
   p += 2 * l.order;
   a.counts = (int32_t*)p, p += l.counts;
-  a.parts = (float*)p, a.part_ld = part_ld(H), a.chunks = (n + kChunk - 1) / kChunk;
+  a.ends = (int2*)p, p += l.ends;
+  a.parts = (float*)p, a.part_ld = part_ld(H);
+  a.chunk = l.chunk, a.chunks = (n + l.chunk - 1) / l.chunk;
   if (cudaMemsetAsync(a.used, 0, l.used, st) != cudaSuccess) return TT_ERR_CUDA;
   return tt::vec::dispatch_float(dtype, [&](auto t) -> int {
     return gradient<decltype(t)>(a, orders, st);

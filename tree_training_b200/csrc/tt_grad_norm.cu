@@ -6,8 +6,9 @@
 // Bound by HBM: the norm reads every element, the scaling reads it again and
 // writes it (3 n b bytes for what could do with 2 if it all stayed on the chip).
 // The tensors' addresses and sizes travel in the launch's parameters, a table of
-// up to kMaxTensors of them a launch; a chunk of 32 KB is a block's unit of work,
-// found in the table by bisection.
+// up to kMaxTensors of them a launch; a chunk of them is a block's unit of work,
+// found in the table by bisection: of 32 KB, or of 128 KB where there are enough of
+// those for every block.
 //
 // Sums.  A pack's 16 bytes are added up in fp32 and the packs in fp64, so that
 // neither the number of elements nor their size matters: a pack whose sum of
@@ -25,8 +26,9 @@ namespace {
 
 constexpr int kMaxTensors = 512;       // of a launch: a table of 20 KB
 constexpr int kThreads = 512;
-constexpr int kChunkBytes = 32768;
-constexpr int kBlocks = 4 * vec::kSMs; // at most, of a launch
+constexpr int64_t kChunkBytes = 32768, kLargeChunkBytes = 131072;
+constexpr int kBlocks = 2 * vec::kSMs; // at most, of a launch: all that are resident
+constexpr int kAhead = 4;              // packs of a thread that are fetched together
 
 struct Table {
   const void* src[kMaxTensors];
@@ -34,7 +36,7 @@ struct Table {
   int64_t n[kMaxTensors];              // elements
   int32_t first[kMaxTensors + 1];      // first chunk
   int8_t dtype[kMaxTensors];
-  int32_t count;
+  int32_t count, chunk_bytes;
 };
 
 enum Kind { kTwo = 0, kOne = 1, kInf = 2 };
@@ -48,10 +50,10 @@ __device__ __forceinline__ double join(double a, double b, int kind) {
 }
 
 // What a pack's V values add to the sum (the maximum).
-template <int V>
-__device__ __forceinline__ double pack_sum(const float (&v)[V], int kind) {
+template <int kind, int V>
+__device__ __forceinline__ double pack_sum(const float (&v)[V]) {
   float s = 0.f;
-  if (kind == kTwo) {
+  if constexpr (kind == kTwo) {
 #pragma unroll
     for (int i = 0; i < V; ++i) s = fmaf(v[i], v[i], s);
     if (s >= 0x1p-100f && s <= 0x1p120f) return (double)s;
@@ -64,7 +66,7 @@ __device__ __forceinline__ double pack_sum(const float (&v)[V], int kind) {
     for (int i = 0; i < V; ++i) d = fma((double)v[i], (double)v[i], d);
     return d;
   }
-  if (kind == kOne) {
+  if constexpr (kind == kOne) {
 #pragma unroll
     for (int i = 0; i < V; ++i) s += fabsf(v[i]);
     if (s <= 0x1p120f) return (double)s;
@@ -88,8 +90,8 @@ __device__ __forceinline__ int tensor_of(const Table& t, int chunk) {
 }
 
 // The chunk's sum over this thread's elements.
-template <typename T>
-__device__ __forceinline__ double chunk_sum(const T* p, int64_t n, int kind) {
+template <int kind, typename T>
+__device__ __forceinline__ double chunk_sum(const T* p, int64_t n) {
   constexpr int V = pack_of<T>();
   double sum = 0.0;
   // elements before the first 16-byte boundary, whole packs, the rest
@@ -98,21 +100,21 @@ __device__ __forceinline__ double chunk_sum(const T* p, int64_t n, int kind) {
   const int64_t packs = (n - lead) / V;
   auto one = [&](int64_t i) {
     const float v[1] = {to_f32(p[i])};
-    sum = join(sum, pack_sum<1>(v, kind), kind);
+    sum = join(sum, pack_sum<kind, 1>(v), kind);
   };
   if ((int64_t)threadIdx.x < lead) one(threadIdx.x);
   const T* body = p + lead;
-  for (int64_t i = threadIdx.x; i < packs; i += kThreads * 4) {
-    vec::Raw<T, V> raw[4];
+  for (int64_t i = threadIdx.x; i < packs; i += kThreads * kAhead) {
+    vec::Raw<T, V> raw[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAhead; ++j)
       if (i + j * kThreads < packs) raw[j] = vec::load_raw<T, V>(body + (i + j * kThreads) * V);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAhead; ++j)
       if (i + j * kThreads < packs) {
         float v[V];
         vec::unpack<T, V>(raw[j], v);
-        sum = join(sum, pack_sum<V>(v, kind), kind);
+        sum = join(sum, pack_sum<kind, V>(v), kind);
       }
   }
   const int64_t at = lead + packs * V + threadIdx.x;
@@ -133,8 +135,9 @@ __device__ __forceinline__ double block_join(double v, int kind, double* sm) {
   return sm[0];
 }
 
+template <int kind>
 __global__ void __launch_bounds__(kThreads, 2)
-    norm_kernel(const __grid_constant__ Table t, int kind, double* part) {
+    norm_kernel(const __grid_constant__ Table t, double* part) {
   __shared__ double sm[kThreads / 32];
   double sum = 0.0;
   for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
@@ -142,19 +145,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t at = c - t.first[i];
     switch (t.dtype[i]) {
       case TT_F32: {
-        const int64_t e = kChunkBytes / 4, n = min(e, t.n[i] - at * e);
-        sum = join(sum, chunk_sum(reinterpret_cast<const float*>(t.src[i]) + at * e, n, kind), kind);
+        const int64_t e = t.chunk_bytes / 4, n = min(e, t.n[i] - at * e);
+        sum = join(sum, chunk_sum<kind>(reinterpret_cast<const float*>(t.src[i]) + at * e, n),
+                   kind);
         break;
       }
       case TT_BF16: {
-        const int64_t e = kChunkBytes / 2, n = min(e, t.n[i] - at * e);
-        sum = join(sum, chunk_sum(reinterpret_cast<const __nv_bfloat16*>(t.src[i]) + at * e, n,
-                                  kind), kind);
+        const int64_t e = t.chunk_bytes / 2, n = min(e, t.n[i] - at * e);
+        sum = join(sum, chunk_sum<kind>(reinterpret_cast<const __nv_bfloat16*>(t.src[i]) + at * e, n),
+                   kind);
         break;
       }
       default: {
-        const int64_t e = kChunkBytes / 2, n = min(e, t.n[i] - at * e);
-        sum = join(sum, chunk_sum(reinterpret_cast<const __half*>(t.src[i]) + at * e, n, kind),
+        const int64_t e = t.chunk_bytes / 2, n = min(e, t.n[i] - at * e);
+        sum = join(sum, chunk_sum<kind>(reinterpret_cast<const __half*>(t.src[i]) + at * e, n),
                    kind);
       }
     }
@@ -190,15 +194,15 @@ __device__ __forceinline__ void scale_chunk(const T* p, T* q, int64_t n, float c
   const int64_t packs = (n - lead) / V;
   auto one = [&](int64_t i) { q[i] = from_f32<T>(to_f32(p[i]) * c); };
   if ((int64_t)threadIdx.x < lead) one(threadIdx.x);
-  for (int64_t i = threadIdx.x; i < packs; i += kThreads * 4) {
+  for (int64_t i = threadIdx.x; i < packs; i += kThreads * kAhead) {
     // (p and q may be one array: no read-only loads)
-    uint4 raw[4];
+    uint4 raw[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAhead; ++j)
       if (i + j * kThreads < packs)
         raw[j] = *reinterpret_cast<const uint4*>(p + lead + (i + j * kThreads) * V);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAhead; ++j)
       if (i + j * kThreads < packs) {
         float v[V];
         vec::unpack<T, V>(raw[j], v);
@@ -227,19 +231,19 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t at = k - t.first[i];
     switch (t.dtype[i]) {
       case TT_F32: {
-        const int64_t e = kChunkBytes / 4, n = min(e, t.n[i] - at * e);
+        const int64_t e = t.chunk_bytes / 4, n = min(e, t.n[i] - at * e);
         scale_chunk(reinterpret_cast<const float*>(t.src[i]) + at * e,
                     reinterpret_cast<float*>(t.dst[i]) + at * e, n, c);
         break;
       }
       case TT_BF16: {
-        const int64_t e = kChunkBytes / 2, n = min(e, t.n[i] - at * e);
+        const int64_t e = t.chunk_bytes / 2, n = min(e, t.n[i] - at * e);
         scale_chunk(reinterpret_cast<const __nv_bfloat16*>(t.src[i]) + at * e,
                     reinterpret_cast<__nv_bfloat16*>(t.dst[i]) + at * e, n, c);
         break;
       }
       default: {
-        const int64_t e = kChunkBytes / 2, n = min(e, t.n[i] - at * e);
+        const int64_t e = t.chunk_bytes / 2, n = min(e, t.n[i] - at * e);
         scale_chunk(reinterpret_cast<const __half*>(t.src[i]) + at * e,
                     reinterpret_cast<__half*>(t.dst[i]) + at * e, n, c);
       }
@@ -247,19 +251,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-int64_t chunks_of(int dtype, int64_t n) {
-  const int64_t e = kChunkBytes / (dtype == TT_F32 ? 4 : 2);
-  return (n + e - 1) / e;
+int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
+
+int64_t chunk_bytes_of(int32_t count, const int32_t* dtypes, const int64_t* sizes) {
+  int64_t all = 0;
+  for (int32_t i = 0; i < count; ++i) all += sizes[i] * size_of(dtypes[i]);
+  return all >= 8 * kBlocks * kLargeChunkBytes ? kLargeChunkBytes : kChunkBytes;
 }
 
 // Fills the table with tensors from `at` on, as many as fit: the next one.
 int32_t fill(Table* t, int32_t at, int32_t count, const int32_t* dtypes, const int64_t* sizes,
-             const void* const* src, void* const* dst) {
+             const void* const* src, void* const* dst, int64_t chunk_bytes) {
   t->count = 0;
+  t->chunk_bytes = (int32_t)chunk_bytes;
   int64_t chunks = 0;
   for (; at < count && t->count < kMaxTensors; ++at) {
     if (sizes[at] == 0) continue;
-    const int64_t c = chunks_of(dtypes[at], sizes[at]);
+    const int64_t e = chunk_bytes / size_of(dtypes[at]), c = (sizes[at] + e - 1) / e;
     if (chunks + c > 0x7fffffff) break;
     t->src[t->count] = src[at];
     t->dst[t->count] = dst ? dst[at] : nullptr;
@@ -297,13 +305,16 @@ int kind_of(double p) {
 int norm_passes(int32_t count, const int32_t* dtypes, const int64_t* sizes, const void* const* src,
                 int kind, double* part, int64_t room, int* parts, cudaStream_t st) {
   Table t;
+  const int64_t chunk = chunk_bytes_of(count, dtypes, sizes);
   *parts = 0;
   for (int32_t at = 0; at < count;) {
-    at = fill(&t, at, count, dtypes, sizes, src, nullptr);
+    at = fill(&t, at, count, dtypes, sizes, src, nullptr, chunk);
     if (t.count == 0) continue;
     const int blocks = blocks_of(t);
     if (*parts + blocks > room) return TT_ERR_WORKSPACE;
-    norm_kernel<<<blocks, kThreads, 0, st>>>(t, kind, part + *parts);
+    if (kind == kTwo) norm_kernel<kTwo><<<blocks, kThreads, 0, st>>>(t, part + *parts);
+    else if (kind == kOne) norm_kernel<kOne><<<blocks, kThreads, 0, st>>>(t, part + *parts);
+    else norm_kernel<kInf><<<blocks, kThreads, 0, st>>>(t, part + *parts);
     tt_count_launches(1);
     *parts += blocks;
   }
@@ -358,10 +369,11 @@ extern "C" int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int
   int in_place = 1;
   for (int32_t i = 0; i < count; ++i) in_place &= tensors[i] == outs[i];
   Table t;
+  const int64_t chunk = kChunkBytes;
   bool first = true;
   int32_t at = 0;
   do {
-    at = fill(&t, at, count, dtypes, sizes, tensors, outs);
+    at = fill(&t, at, count, dtypes, sizes, tensors, outs, chunk);
     if (t.count == 0 && !first) break;
     scale_kernel<<<std::max(1, blocks_of(t)), kThreads, 0, st>>>(
         t, part, parts, kind, given_norm, max_norm, eps, first ? norm : nullptr, in_place);
