@@ -397,7 +397,7 @@ inline int64_t slice_clocks(int cg, int bn) {
 inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool dual, bool split) {
   Plan best{1, n_step, 1};
   double least = 1e300;
-  for (int cg = 1; cg <= 1; ++cg) {
+  for (int cg = 1; cg <= 2; ++cg) {
     const int step = std::max(n_step * cg, dual ? 16 * cg : 16 * cg);
     const int64_t slots = vec::kSMs / cg;
     for (int bn = 256; bn >= step; bn -= step) {
