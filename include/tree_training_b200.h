@@ -586,11 +586,19 @@ int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids
                      const void* dy, int64_t dy_ld, float scale, int64_t padding_idx,
                      void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* 16-bit rows of any stride (elements) and alignment copied to rows on 16-byte
+ * boundaries (dst_ld a multiple of 8), for the products below; the columns up to the
+ * next multiple of 8 are zeroed. */
+int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
+                  int64_t dst_ld, void* stream);
+
 /* ---- the gated half of a feed-forward block --------------------------------- *
  * h = act(x wg^T) * (x wu^T): x [T, H], wg and wu [F, H], h [T, F] contiguous; act
  * 0 silu, 1 gelu, 2 gelu with tanh, 3 relu.  16-bit factors need rows on 16-byte
- * boundaries (else TT_ERR_UNSUPPORTED).  g and u (fp32, row stride keep_ld; null for
- * 16-bit inputs: not kept) are the two products, which the backward takes. */
+ * boundaries (else TT_ERR_UNSUPPORTED).  g and u (fp32; null for 16-bit inputs: not
+ * kept) are the two products, which the backward takes: on 16-byte boundaries, their
+ * row stride keep_ld a multiple of 4 and at least round_up(F, 8).  What stands past
+ * column F is not read as a value. */
 int64_t tt_gated_linear_fwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F);
 int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x, int64_t x_ld,
                         const void* wg, int64_t wg_ld, const void* wu, int64_t wu_ld, int act,

@@ -46,6 +46,18 @@ def test_embedding_types_and_workspace():
     assert status("tt_embedding_bwd_workspace_size", -1, 10, 8) == 0
 
 
+def align(rows=4, cols=9, src=P, ld=9, dst=P, dst_ld=16):
+    return status("tt_align_rows", rows, cols, src, ld, dst, dst_ld, None)
+
+
+@pytest.mark.parametrize("bad", [dict(rows=-1), dict(cols=0), dict(ld=8), dict(dst_ld=8),
+                                 dict(dst_ld=17), dict(src=None), dict(dst=None), dict(dst=P + 8),
+                                 dict(src=P + 1)])
+def test_align_rows(bad):
+    assert align(**bad) == INVALID
+    assert align(rows=0, src=None, dst=None) == _lib.TT_OK
+
+
 def gated(dtype=BF16, T=4, H=16, F=8, x=P, x_ld=16, wg=P, wg_ld=16, wu=P, wu_ld=16, act=0, h=P,
           g=None, u=None, ld=8, ws=P, size=BIG):
     return status("tt_gated_linear_fwd", dtype, T, H, F, x, x_ld, wg, wg_ld, wu, wu_ld, act, h, g, u,
@@ -63,12 +75,14 @@ BAD_GATED = [dict(T=-1), dict(T=1 << 31), dict(H=0), dict(F=0), dict(x_ld=15), d
 
 
 @pytest.mark.parametrize("bad", BAD_GATED + [dict(h=None), dict(g=P), dict(u=P),
-                                             dict(g=P, u=P, ld=7), dict(dtype=F32)])
+                                             dict(g=P, u=P, ld=7), dict(g=P, u=P, ld=10),
+                                             dict(g=P + 8, u=P), dict(dtype=F32)])
 def test_gated_linear(bad):
     assert gated(**bad) == INVALID
 
 
-@pytest.mark.parametrize("bad", BAD_GATED + [dict(g=None), dict(u=None), dict(ld=7), dict(dh=None),
+@pytest.mark.parametrize("bad", BAD_GATED + [dict(g=None), dict(u=None), dict(ld=7), dict(ld=10),
+                                             dict(u=P + 4), dict(dh=None),
                                              dict(dh_ld=7)])
 def test_gated_linear_gradient(bad):
     assert gated_bwd(**bad) == INVALID

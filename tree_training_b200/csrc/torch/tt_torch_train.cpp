@@ -24,9 +24,14 @@ Tensor rows16(const Tensor& t_) {
   if (t.size(0) == 1 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 &&
       t.size(1) % 8 == 0)
     return t;
-  Tensor c = empty({t.size(0), pad8(t.size(1))}, t, t.scalar_type()).narrow(1, 0, t.size(1));
-  c.copy_(t.detach());
-  return c;
+  const int64_t ld = pad8(t.size(1));
+  Tensor c = empty({t.size(0), ld}, t, t.scalar_type());
+  On on(t);
+  check_status("tt_align_rows", tt_align_rows(t.size(0), t.size(1), ptr(t),
+                                              std::max(t.stride(0), t.size(1)), out(c), ld,
+                                              on.stream));
+  at::NoGradGuard no_grad;
+  return c.narrow(1, 0, t.size(1));
 }
 
 // The stride of rows (of one row: its own width, rounded up).
@@ -138,16 +143,15 @@ struct GatedFunction : Function<GatedFunction> {
                         int64_t act) {
     const Tensor x2 = rows16(x), g2 = rows16(wg), u2 = rows16(wu);
     Gated r = gated_forward(x2, g2, u2, act, true);
-    // (the padded copies of a call with odd widths are made again)
-    ctx->save_for_backward({x, wg, wu, r.g, r.u});
+    // (with odd widths the copies that were made)
+    ctx->save_for_backward({x2, g2, u2, r.g, r.u});
     ctx->saved_data["act"] = act;
     return r.h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     no_tangent("gated_linear", {&grad[0]});
     const variable_list s = ctx->get_saved_variables();
-    const Tensor x = rows16(s[0]), wg = rows16(s[1]), wu = rows16(s[2]);
-    const Tensor &g = s[3], &u = s[4];
+    const Tensor &x = s[0], &wg = s[1], &wu = s[2], &g = s[3], &u = s[4];
     const int64_t T = x.size(0), H = x.size(1), F = wg.size(0);
     const Tensor dh = rows2d(grad[0]);
     Tensor dx, dwg, dwu;
@@ -227,8 +231,10 @@ std::pair<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Ten
 struct LinearCEFunction : Function<LinearCEFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
                                const Tensor& labels, double scale) {
-    auto r = ce_forward(rows16(x), rows16(w), labels, scale);
-    ctx->save_for_backward({x, w, labels, r.second});
+    const Tensor x2 = rows16(x), w2 = rows16(w);
+    auto r = ce_forward(x2, w2, labels, scale);
+    // (with odd widths the copies that were made)
+    ctx->save_for_backward({x2, w2, labels, r.second});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return {r.first, r.second};
@@ -238,8 +244,7 @@ struct LinearCEFunction : Function<LinearCEFunction> {
     if (!g[0].defined() && !g[1].defined()) return grads;
     no_tangent("linear_cross_entropy", {&g[0], &g[1]});
     const variable_list s = ctx->get_saved_variables();
-    const Tensor x = rows16(s[0]), w = rows16(s[1]);
-    const Tensor &labels = s[2], &lse = s[3];
+    const Tensor &x = s[0], &w = s[1], &labels = s[2], &lse = s[3];
     const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
     for (int i = 0; i < 2; ++i)
       if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();

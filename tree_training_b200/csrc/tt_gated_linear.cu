@@ -79,10 +79,10 @@ struct GatedEpi {
     int64_t h_ld;
     float *g, *u;                          // null: not kept
     int64_t keep_ld;
-    int F, wide, keep_wide;
+    int F, wide;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc) {
+                                              const gemm::TileAt& t, int row, uint32_t acc, float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const int half = p.bn / 2, n0 = t.n * half, cols = min(half, a.F - n0);
     const bool live = row < p.M;
@@ -90,17 +90,16 @@ struct GatedEpi {
       float g[32], u[32];
       __syncwarp();                          // (the loads are the whole warp's)
       sm100::tmem_ld32x2(acc + c, acc + half + c, g, u);
-      if (!live) continue;
       const int left = cols - c;
       if (a.g) {
         const int64_t at = (int64_t)row * a.keep_ld + n0 + c;
-        gemm::store_row32(a.g + at, g, left, a.keep_wide);
-        gemm::store_row32(a.u + at, u, left, a.keep_wide);
+        gemm::store_block(live ? a.g + at : nullptr, g, left, true, block);
+        gemm::store_block(live ? a.u + at : nullptr, u, left, true, block);
       }
 #pragma unroll
       for (int i = 0; i < 32; ++i) g[i] = act<A>(g[i]) * u[i];
-      gemm::store_row32(reinterpret_cast<T*>(a.h) + (int64_t)row * a.h_ld + n0 + c, g, left,
-                        a.wide);
+      T* h = reinterpret_cast<T*>(a.h) + (int64_t)row * a.h_ld + n0 + c;
+      gemm::store_block(live ? h : nullptr, g, left, a.wide, block);
     }
   }
 };
@@ -114,36 +113,34 @@ __global__ void __launch_bounds__(256)
       h[r * F + c] = act<A>(g[r * ld + c]) * u[r * ld + c];
 }
 
-// dg and du out of g, u (fp32) and dh; columns from F to `ld` are left alone.
-template <typename T, int A, int V>
+// dg and du out of g, u (fp32) and dh, in packs of 16 bytes: g, u, dg and du have rows
+// of whole packs (columns from F on are zeroed), rows of dh may begin anywhere.
+template <typename T, int A>
 __global__ void __launch_bounds__(256)
     backward_kernel(const float* g, const float* u, int64_t keep_ld, const T* dh, int64_t dh_ld,
                     int64_t rows, int F, T* dg, T* du, int64_t ld) {
+  constexpr int V = 16 / (int)sizeof(T);
   const int packs = (F + V - 1) / V;
+  const T* hi = dh + (rows - 1) * dh_ld + F;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
     for (int p = blockIdx.x * blockDim.x + threadIdx.x; p < packs; p += gridDim.x * blockDim.x) {
       const int c = p * V;
       float vg[V], vu[V], vd[V];
-      if constexpr (V > 1) {
-        constexpr int W = 4;
 #pragma unroll
-        for (int i = 0; i < V; i += W) {
-          const float4 x = __ldg(reinterpret_cast<const float4*>(g + r * keep_ld + c + i));
-          const float4 y = __ldg(reinterpret_cast<const float4*>(u + r * keep_ld + c + i));
-          vg[i] = x.x, vg[i + 1] = x.y, vg[i + 2] = x.z, vg[i + 3] = x.w;
-          vu[i] = y.x, vu[i + 1] = y.y, vu[i + 2] = y.z, vu[i + 3] = y.w;
-        }
-        vec::load<T, V>(dh + r * dh_ld + c, vd);
-      } else {
-        vg[0] = g[r * keep_ld + c], vu[0] = u[r * keep_ld + c];
-        vd[0] = to_f32(dh[r * dh_ld + c]);
+      for (int i = 0; i < V; i += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(g + r * keep_ld + c + i));
+        const float4 y = __ldg(reinterpret_cast<const float4*>(u + r * keep_ld + c + i));
+        vg[i] = x.x, vg[i + 1] = x.y, vg[i + 2] = x.z, vg[i + 3] = x.w;
+        vu[i] = y.x, vu[i + 1] = y.y, vu[i + 2] = y.z, vu[i + 3] = y.w;
       }
+      vec::unpack<T, V>(vec::load_any_of<T>(dh + r * dh_ld, c, F, dh, hi), vd);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float a, d;
         act_grad<A>(vg[i], a, d);
-        vg[i] = vd[i] * vu[i] * d;
-        vu[i] = vd[i] * a;
+        const bool in = c + i < F;             // (what is kept past F is not written)
+        vg[i] = in ? vd[i] * vu[i] * d : 0.f;
+        vu[i] = in ? vd[i] * a : 0.f;
       }
       vec::store<T, V>(dg + r * ld + c, vg);
       vec::store<T, V>(du + r * ld + c, vu);
@@ -162,19 +159,11 @@ int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
 template <typename T, int A>
 void run_backward(const float* g, const float* u, int64_t keep_ld, const void* dh, int64_t dh_ld,
                   int64_t rows, int F, void* dg, void* du, int64_t ld, cudaStream_t st) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool wide = F % V == 0 && keep_ld % 4 == 0 && dh_ld % V == 0 && ld % V == 0 &&
-                    ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u) |
-                      reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
-  const int packs = wide ? F / V : F;
+  const int packs = (F * (int)sizeof(T) + 15) / 16;
   const dim3 grid((unsigned)std::min((packs + 255) / 256, 64),
                   (unsigned)std::min<int64_t>(rows, 32768));
-  if (wide)
-    backward_kernel<T, A, V><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F,
-                                                   (T*)dg, (T*)du, ld);
-  else
-    backward_kernel<T, A, 1><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F,
-                                                   (T*)dg, (T*)du, ld);
+  backward_kernel<T, A><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F, (T*)dg,
+                                              (T*)du, ld);
   tt_count_launches(1);
 }
 
@@ -193,8 +182,6 @@ int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void*
     typename Epi::Args ea{};
     ea.h = h, ea.h_ld = F, ea.g = g, ea.u = u, ea.keep_ld = keep_ld, ea.F = F;
     ea.wide = F % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
-    ea.keep_wide = keep_ld % 4 == 0 &&
-                   ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15) == 0;
     return gemm::launch<false, false, Epi>(plan, q, ea, st);
   });
 }
@@ -217,7 +204,9 @@ extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, c
                                    int64_t keep_ld, void* workspace, int64_t workspace_bytes,
                                    int32_t* status, void* stream) {
   if (!sizes_ok(T, H, F) || act < kSilu || act > kRelu || x_ld < H || wg_ld < H || wu_ld < H ||
-      !g != !u || (g && keep_ld < F))
+      !g != !u ||
+      (g && (keep_ld < round8(F) || keep_ld % 4 ||
+             ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15))))
     return TT_ERR_INVALID_ARG;
   if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
   if (T == 0) return TT_OK;
@@ -248,20 +237,23 @@ extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, c
 }
 
 namespace {
-// dg and du, then the parts of a split sum.
+// dg and du side by side, du from column round8(F) on; then the parts of a split sum.
 int64_t grad_bytes(int dtype, int64_t T, int32_t F) {
-  return round256(T * round8(F) * size_of(dtype));
+  return round256(T * 2 * round8(F) * size_of(dtype));
 }
+int64_t slices(int64_t k) { return (k + gemm::kBK - 1) / gemm::kBK; }
 int64_t parts_bytes(int dtype, int64_t T, int32_t H, int32_t F) {
+  const int64_t both = round8(F) + F;
   if (dtype == TT_F32)
-    return std::max({gemm::fp32_work(T, H, 2 * (int64_t)F), gemm::fp32_work(F, H, T)});
-  return std::max({gemm::tc_work(T, H, 2 * round8(F) + 128, true), gemm::tc_work(F, H, T, true)});
+    return std::max(gemm::fp32_work(T, H, 2 * (int64_t)F), gemm::fp32_work(F, H, T));
+  return std::max({gemm::tc_work(T, H, 2 * slices(F), true), gemm::tc_work(F, H, slices(T), true),
+                   gemm::tc_work(both, H, slices(T), true)});
 }
 }  // namespace
 
 extern "C" int64_t tt_gated_linear_bwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F) {
   if (!sizes_ok(T, H, F) || dtype < TT_F32 || dtype > TT_F16) return 0;
-  return 2 * grad_bytes(dtype, T, F) + parts_bytes(dtype, T, H, F);
+  return grad_bytes(dtype, T, F) + parts_bytes(dtype, T, H, F);
 }
 
 extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x,
@@ -276,13 +268,16 @@ extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, c
   if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
   if (T == 0) return TT_OK;
   if (!x || !wg || !wu || !g || !u || !dh) return TT_ERR_INVALID_ARG;
+  if (keep_ld < round8(F) || keep_ld % 4 ||
+      ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15))
+    return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_gated_linear_bwd_workspace_size(dtype, T, H, F))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t ld = round8(F), bytes = grad_bytes(dtype, T, F);
+  const int64_t F8 = round8(F), ld = 2 * F8, bytes = grad_bytes(dtype, T, F);
   char* ws = (char*)workspace;
-  void *dg = ws, *du = ws + bytes, *work = ws + 2 * bytes;
-  const int64_t work_bytes = workspace_bytes - 2 * bytes;
+  void *dg = ws, *du = ws + F8 * size_of(dtype), *work = ws + bytes;
+  const int64_t work_bytes = workspace_bytes - bytes;
   int rc = dispatch_act(act, [&](auto a) -> int {
     constexpr int A = decltype(a)::value;
     return vec::dispatch_float(dtype, [&](auto t) -> int {
@@ -301,6 +296,13 @@ extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, c
     const gemm::Term terms[2] = {{{dg, ld, false}, {wg, wg_ld, true}, F},
                                  {{du, ld, false}, {wu, wu_ld, true}, F}};
     if ((rc = product(T, H, terms, 2, dx))) return rc;
+  }
+  if (dwg && dwu && dtype != TT_F32) {
+    // one product for both: its last wave of tiles comes once
+    const gemm::Term term{{dg, ld, true}, {x, x_ld, true}, T};
+    gemm::Result r{dtype, dwg, H, nullptr, 0, 1.f, nullptr};
+    r.p2 = dwu, r.gap = F, r.second = F8;
+    return gemm::tc_product(dtype == TT_BF16, F8 + F, H, &term, 1, r, work, work_bytes, status, st);
   }
   for (int i = 0; i < 2; ++i) {
     void* dw = i ? dwu : dwg;

@@ -30,6 +30,10 @@ struct Result {
   int64_t cin_ld;
   float alpha;
   const float* alpha_dev;
+  // (tensor cores) rows from `second` on are those of another array, from its first
+  // row; rows from `gap` to there are none.  0: no such rows.
+  void* p2 = nullptr;
+  int64_t gap = 0, second = 0;
 };
 
 // fp32 products on the CUDA cores: sums in fp32, in the order of k.  Up to two

@@ -9,8 +9,10 @@ template <bool kB>
 struct StoreEpi {
   static constexpr bool kBf16 = kB;
   struct Args {
-    void* c;
-    int64_t ld, part;                      // part: elements from one part to the next
+    void *c, *c2;
+    int64_t ld;
+    int gap, second;                       // c2's rows (see Result)
+    float* parts;                          // [units][128 CG][bn]
     const float* cin;
     int64_t cin_ld;
     float alpha;
@@ -18,20 +20,31 @@ struct StoreEpi {
     int f32, wide, cin_wide;
   };
   static __device__ __forceinline__ void tile(const Args& a, const Problem& p, const TileAt& t,
-                                              int row, uint32_t acc) {
+                                              int row, uint32_t acc, float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const float alpha = a.alpha * (a.alpha_dev ? __ldg(a.alpha_dev) : 1.f);
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
     const bool live = row < p.M;
+    if (t.unit >= 0) {                     // a part of a sum: the tile as it is
+      // (a warp's rows of the tile, whichever CTA of the pair it is in)
+      const int64_t tile_rows = p.tile_rows;
+      float* q = a.parts + ((int64_t)t.unit * tile_rows + (row - t.m * tile_rows)) * p.bn;
+      for (int c = 0; c < cols; c += 32) {
+        float v[32];
+        __syncwarp();
+        tmem_ld32(acc + c, v);
+        store_block(live ? q + c : nullptr, v, p.bn - c, true, block);
+      }
+      return;
+    }
     for (int c = 0; c < cols; c += 32) {
       float v[32];
       __syncwarp();                          // (the load is the whole warp's)
       tmem_ld32(acc + c, v);
-      if (!live) continue;
       const int left = cols - c;
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= alpha;
-      if (a.cin) {
+      if (a.cin && live) {
         const float* q = a.cin + (int64_t)row * a.cin_ld + n0 + c;
         if (a.cin_wide && left >= 32) {
 #pragma unroll
@@ -45,12 +58,51 @@ struct StoreEpi {
             if (i < left) v[i] += q[i];
         }
       }
-      const int64_t at = t.part * a.part + (int64_t)row * a.ld + n0 + c;
-      if (a.f32) store_row32(reinterpret_cast<float*>(a.c) + at, v, left, a.wide);
-      else store_row32(reinterpret_cast<T*>(a.c) + at, v, left, a.wide);
+      const bool none = !live || (row >= a.gap && row < a.second);
+      const bool two = a.second && row >= a.second;
+      void* base = two ? a.c2 : a.c;
+      const int64_t at = (int64_t)(two ? row - a.second : row) * a.ld + n0 + c;
+      if (a.f32)
+        store_block(none ? nullptr : reinterpret_cast<float*>(base) + at, v, left, a.wide, block);
+      else
+        store_block(none ? nullptr : reinterpret_cast<T*>(base) + at, v, left, a.wide, block);
     }
   }
 };
+
+// The tiles that were summed in parts, into C.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    join_tiles_kernel(const __grid_constant__ Problem p, const float* parts, T* c, T* c2,
+                      int gap, int second, int64_t ld, const float* cin, int64_t cin_ld, float alpha, const float* alpha_dev) {
+  const TileAt t = tile_at(p, p.whole + blockIdx.x * p.parts);
+  const int64_t size = (int64_t)p.tile_rows * p.bn;
+  const float* q = parts + (int64_t)t.unit * size;
+  const int cols = min(p.bn, p.N - t.n * p.bn);
+  if (alpha_dev) alpha *= *alpha_dev;
+  // a thread four columns; rows by the others (bn is a multiple of 16)
+  const int quads = p.bn / 4, rows = blockDim.x / quads;
+  const int col = (int)(threadIdx.x % quads) * 4;
+  if ((int)threadIdx.x >= quads * rows || col >= cols) return;
+  for (int r = blockIdx.y * rows + threadIdx.x / quads; r < p.tile_rows; r += gridDim.y * rows) {
+    const int64_t row = (int64_t)t.m * p.tile_rows + r;
+    if (row >= p.M) break;
+    if (row >= gap && row < second) continue;
+    const float* at = q + (int64_t)r * p.bn + col;
+    float4 s = __ldg(reinterpret_cast<const float4*>(at));
+#pragma unroll 4
+    for (int k = 1; k < p.parts; ++k) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(at + k * size));
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    const float v[4] = {s.x * alpha, s.y * alpha, s.z * alpha, s.w * alpha};
+    const int64_t n = (int64_t)t.n * p.bn + col;
+    T* to = (second && row >= second ? c2 + (row - second) * ld : c + row * ld) + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < cols) to[j] = from_f32<T>(cin ? v[j] + cin[row * cin_ld + n + j] : v[j]);
+  }
+}
 
 template <bool kB>
 int product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r, void* work,
@@ -59,35 +111,50 @@ int product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& 
   int64_t steps = 0;
   for (int i = 0; i < n_terms; ++i) steps += (terms[i].k + kBK - 1) / kBK;
   const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
-  Plan plan = plan_product(M, N, steps, bmn ? 64 : 16, false, work != nullptr);
-  while (plan.parts > 1 && plan.parts * M * N * 4 > work_bytes) --plan.parts;
+  Plan plan = plan_product(M, N, steps, bmn ? 64 : 16, false, true);
+  if (plan.work > work_bytes || !work) plan = plan_product(M, N, steps, bmn ? 64 : 16, false, false);
   Problem q;
   if (!set_up(&q, plan, kB, M, N, terms, n_terms, false, status)) return TT_ERR_UNSUPPORTED;
   typename Epi::Args a{};
-  a.alpha = r.alpha, a.alpha_dev = r.alpha_dev;
-  if (q.parts > 1) {
-    a.c = work, a.ld = N, a.part = M * N, a.f32 = 1;
-  } else {
-    a.c = r.p, a.ld = r.ld, a.cin = r.cin, a.cin_ld = r.cin_ld, a.f32 = r.dtype == TT_F32;
-  }
-  const int size = a.f32 ? 4 : 2;
-  a.wide = (reinterpret_cast<uintptr_t>(a.c) & 15) == 0 && a.ld * size % 16 == 0 &&
-           a.part * size % 16 == 0;
+  a.alpha = r.alpha, a.alpha_dev = r.alpha_dev, a.parts = (float*)work;
+  a.c = r.p, a.c2 = r.p2, a.gap = (int)r.gap, a.second = (int)r.second, a.ld = r.ld;
+  a.cin = r.cin, a.cin_ld = r.cin_ld, a.f32 = r.dtype == TT_F32;
+  a.wide = ((reinterpret_cast<uintptr_t>(a.c) | reinterpret_cast<uintptr_t>(a.c2)) & 15) == 0 && a.ld * (a.f32 ? 4 : 2) % 16 == 0;
   a.cin_wide = (reinterpret_cast<uintptr_t>(a.cin) & 15) == 0 && a.cin_ld % 4 == 0;
   int rc;
   if (amn && bmn) rc = launch<true, true, Epi>(plan, q, a, st);
   else if (!amn && bmn) rc = launch<false, true, Epi>(plan, q, a, st);
   else return TT_ERR_INVALID_ARG;          // (no operator has this form)
-  if (rc != TT_OK || q.parts == 1) return rc;
-  return join_parts((const float*)work, q.parts, M, N, r, st);
+  const int64_t split = (int64_t)q.tiles_m * q.tiles_n - q.whole;
+  if (rc != TT_OK || split == 0) return rc;
+  return vec::dispatch_float(r.dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const dim3 grid((unsigned)split, (unsigned)std::min<int64_t>(64, std::max<int64_t>(1, 8 * vec::kSMs / split)));
+    join_tiles_kernel<T><<<grid, 256, 0, st>>>(q, a.parts, (T*)r.p, (T*)r.p2, a.gap, a.second, r.ld,
+                                               r.cin, r.cin_ld, r.alpha, r.alpha_dev);
+    tt_count_launches(1);
+    return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  });
+}
+
+// 16-bit rows onto 16-byte boundaries, in packs of 8; columns past the last are zero.
+__global__ void __launch_bounds__(256)
+    align_rows_kernel(const __nv_bfloat16* src, int64_t ld, int64_t rows, int64_t cols,
+                      __nv_bfloat16* dst, int64_t dst_ld) {
+  const __nv_bfloat16* hi = src + (rows - 1) * ld + cols;
+  const int64_t packs = (cols + 7) / 8;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int64_t p = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; p < packs;
+         p += (int64_t)gridDim.x * blockDim.x)
+      *reinterpret_cast<uint4*>(dst + r * dst_ld + p * 8) =
+          vec::load_any_of<__nv_bfloat16>(src + r * ld, p * 8, cols, src, hi);
 }
 
 }  // namespace
 
-int64_t tc_work(int64_t M, int64_t N, int64_t k, bool b_mn) {
+int64_t tc_work(int64_t M, int64_t N, int64_t steps, bool b_mn) {
   if (M <= 0 || N <= 0) return 0;
-  const Plan p = plan_product(M, N, (k + kBK - 1) / kBK, b_mn ? 64 : 16, false, true);
-  return p.parts > 1 ? p.parts * M * N * 4 : 0;
+  return plan_product(M, N, steps, b_mn ? 64 : 16, false, true).work;
 }
 
 int tc_product(bool bf16, int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r,
@@ -101,3 +168,20 @@ int tc_product(bool bf16, int64_t M, int64_t N, const Term* terms, int n_terms, 
 
 }  // namespace gemm
 }  // namespace tt
+
+extern "C" int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
+                             int64_t dst_ld, void* stream) {
+  if (rows < 0 || cols < 1 || (rows > 1 && ld < cols) || dst_ld < cols || dst_ld % 8 != 0)
+    return TT_ERR_INVALID_ARG;
+  if (rows == 0) return TT_OK;
+  if (!src || !dst || (reinterpret_cast<uintptr_t>(dst) & 15) ||
+      (reinterpret_cast<uintptr_t>(src) & 1))
+    return TT_ERR_INVALID_ARG;
+  const int64_t packs = (cols + 7) / 8;
+  const dim3 grid((unsigned)std::min<int64_t>((packs + 255) / 256, 64),
+                  (unsigned)std::min<int64_t>(rows, 65535));
+  tt::gemm::align_rows_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
+      (const __nv_bfloat16*)src, ld, rows, cols, (__nv_bfloat16*)dst, dst_ld);
+  tt_count_launches(1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}

@@ -45,8 +45,9 @@ struct Problem {
   int32_t terms;
   int32_t M, N;
   int32_t bn;                              // columns of the accumulator
-  int32_t tiles_m, tiles_n, group;         // group: tiles of m that share an L2 window
-  int32_t parts, part_steps;               // the sum over k split into parts
+  int32_t tile_rows, tiles_m, tiles_n, group;         // group: tiles of m that share an L2 window
+  int32_t whole;                           // tiles whose sum over k is one CTA's; those
+  int32_t parts, part_steps;               // behind them are summed in parts
   int32_t stages, stage_bytes;
   int32_t a_bytes;                         // of A that a CTA copies a slice
   int32_t dual;                            // B's halves are two factors: b[0] and b[1]
@@ -54,18 +55,24 @@ struct Problem {
 };
 
 struct TileAt {
-  int part, m, n;
+  int unit, begin, end, m, n;              // unit: of a sum in parts (else -1)
 };
 
-__device__ __forceinline__ TileAt tile_at(const Problem& p, int i) {
+// Item i: a whole tile, or a part of one of the last ones.
+__host__ __device__ __forceinline__ TileAt tile_at(const Problem& p, int i) {
   TileAt t;
-  const int per = p.tiles_m * p.tiles_n;
-  t.part = i / per;
-  i -= t.part * per;
+  t.unit = i - p.whole;
+  t.begin = 0;
+  t.end = p.steps[0] + (p.terms > 1 ? p.steps[1] : 0);
+  if (t.unit >= 0) {
+    i = p.whole + t.unit / p.parts;
+    t.begin = (t.unit % p.parts) * p.part_steps;
+    t.end = t.end < t.begin + p.part_steps ? t.end : t.begin + p.part_steps;
+  }
   // groups of `group` tiles of m, all n within a group, m fastest
   const int full = p.group * p.tiles_n;
   const int g = i / full, in = i - g * full;
-  const int rows = min(p.group, p.tiles_m - g * p.group);
+  const int left = p.tiles_m - g * p.group, rows = left < p.group ? left : p.group;
   t.n = in / rows;
   t.m = g * p.group + in - t.n * rows;
   return t;
@@ -77,7 +84,10 @@ struct Barriers {
   int32_t abort;
 };
 
-constexpr int kGemmSmem = 1024 + kRingBytes + 1024;   // barriers, ring, its alignment
+constexpr int kStageRow = 33;              // floats of a row of a warp's 32 x 32 block
+constexpr int kStageBytes = 4 * 32 * kStageRow * 4;
+// barriers, ring, its alignment, the epilogue's blocks
+constexpr int kGemmSmem = 1024 + kRingBytes + 1024 + kStageBytes;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -157,9 +167,10 @@ __device__ __forceinline__ void tmem_give(uint32_t taddr) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
 }
 
-// Epi::tile(args, problem, tile, row, lane address) takes one accumulator out of
+// Epi::tile(args, problem, tile, row, lane address, block) takes one accumulator out of
 // TMEM: a thread has one row of the tile (row: its index in C, possibly past M) and
-// reads its columns; all 32 lanes of a warp call it.
+// reads its columns; all 32 lanes of a warp call it.  block: 32 x 33 floats of shared
+// memory of the warp's own.
 template <int CG, bool kAMN, bool kBMN, typename Epi>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epi::Args ea) {
@@ -182,9 +193,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   if constexpr (CG == 2) cluster_barrier();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
-  const int items = p.tiles_m * p.tiles_n * p.parts;
+  const int items = p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.parts;
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
-  const int all_steps = p.steps[0] + (p.terms > 1 ? p.steps[1] : 0);
   auto fail = [&]() {
     sh->abort = 1;
     set_status(p.status, TT_ERR_DEVICE_TIMEOUT);
@@ -203,8 +213,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int i = first; i < items && ok; i += stride) {
         const TileAt t = tile_at(p, i);
         const int m0 = t.m * 128 * CG + (int)rank * 128;
-        const int begin = t.part * p.part_steps, end = min(all_steps, begin + p.part_steps);
-        for (int k = begin; k < end; ++k, ++slot) {
+        for (int k = t.begin; k < t.end; ++k, ++slot) {
           if (slot >= stages && !mbar_wait(&sh->empty[s], phase ^ 1, abort_flag)) {
             ok = false;
             break;
@@ -275,8 +284,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
-        const int begin = t.part * p.part_steps, end = min(all_steps, begin + p.part_steps);
-        for (int k = begin; k < end; ++k) {
+        for (int k = t.begin; k < t.end; ++k) {
           if (!mbar_wait(&sh->full[s], phase, abort_flag)) {
             ok = false;
             break;
@@ -286,7 +294,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk)
             mma_f16<CG>(d, da0 + off + kk * kStepA, db0 + off + kk * kStepB, idesc,
-                        k > begin || kk > 0);
+                        k > t.begin || kk > 0);
           commit_all<CG>(&sh->empty[s]);
           if (++s == stages) s = 0, phase ^= 1;
         }
@@ -307,6 +315,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int quad = warp & 3;
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+    float* block = reinterpret_cast<float*>(smem_raw + 2048 + kRingBytes) + quad * 32 * kStageRow;
     int acc = 0;
     for (int i = first; i < items; i += stride, ++acc) {
       const TileAt t = tile_at(p, i);
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       tc_fence_after();
       const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
-      Epi::tile(ea, p, t, row, lane_addr + buf * 256);
+      Epi::tile(ea, p, t, row, lane_addr + buf * 256, block);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -380,9 +389,13 @@ inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a product is cut up.
+// How a product is cut up: columns of the accumulator, tiles that are summed whole,
+// and the parts of the sums of the others.
 struct Plan {
-  int cg, bn, parts;
+  int cg, bn;
+  int64_t whole;
+  int parts;
+  int64_t work;                            // bytes of the parts
 };
 
 // Clocks of a slice of 64 k in a tile: the tensor core's, or the shared-memory
@@ -392,25 +405,32 @@ inline int64_t slice_clocks(int cg, int bn) {
 }
 
 // The cheapest of the forms by the tiles' waves.  `n_step`: what widths of the
-// accumulator are a multiple of; `width`: columns of C that a column of the
-// accumulator stands for (1, or 2 halves of one: dual).
+// accumulator are a multiple of; `dual`: its halves stand for one column of C each.
+// With `split` the tiles of the last wave, where they leave half of the SMs idle, are
+// summed in parts (8,192 x 2,560 over k = 19,456: 320 tiles on 74 pairs of SMs, 5 waves
+// or 4 and a third).
 inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool dual, bool split) {
-  Plan best{1, n_step, 1};
+  Plan best{};
   double least = 1e300;
   for (int cg = 1; cg <= 2; ++cg) {
-    const int step = std::max(n_step * cg, dual ? 16 * cg : 16 * cg);
+    const int step = std::max(n_step, 16) * cg;
     const int64_t slots = vec::kSMs / cg;
     for (int bn = 256; bn >= step; bn -= step) {
       const int64_t cols = dual ? bn / 2 : bn;
       const int64_t tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + cols - 1) / cols);
-      const int64_t most = split ? std::max<int64_t>(1, std::min(slots / tiles, steps / 8)) : 1;
-      for (int64_t parts = 1; parts <= most; ++parts) {
-        const int64_t waves = (tiles * parts + slots - 1) / slots;
-        // a tile's start and end that nothing hides, and the parts' way through L2
-        double clocks = (double)waves * (double)(((steps + parts - 1) / parts) *
-                                                 slice_clocks(cg, bn) + 600) + 1500;
-        if (parts > 1) clocks += 3000 + (double)(parts + 1) * M * N * 4 / 3000;
-        if (clocks < least * 0.999) least = clocks, best = Plan{cg, bn, (int)parts};
+      const int64_t rest = tiles % slots, most = rest && split ? std::min(slots / rest, steps / 8) : 1;
+      const double clocks = (double)slice_clocks(cg, bn);
+      for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); ++parts) {
+        // (a tile's start and end, which nothing hides: 600 clocks; the parts' way
+        // through L2 and the launch that adds them up)
+        const int64_t whole = parts > 1 ? tiles - rest : tiles;
+        double t = (double)((whole + slots - 1) / slots) * (steps * clocks + 600) + 1500;
+        const int64_t unit = (int64_t)128 * cg * bn * 4;
+        if (parts > 1)
+          t += (double)((steps + parts - 1) / parts) * clocks + 600 + 5000 +
+               (double)(rest * (parts + 1) * unit) / 3000;
+        if (t < least * 0.999)
+          least = t, best = Plan{cg, bn, whole, (int)parts, parts > 1 ? rest * parts * unit : 0};
       }
     }
   }
@@ -435,16 +455,19 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   }
   q->M = (int32_t)M, q->N = (int32_t)N, q->bn = bn, q->dual = dual;
   const int64_t cols = dual ? bn / 2 : bn;
+  q->tile_rows = 128 * cg;
   q->tiles_m = (int32_t)((M + 128 * cg - 1) / (128 * cg));
   q->tiles_n = (int32_t)((N + cols - 1) / cols);
-  q->group = std::min(q->tiles_m, 32 / cg);
+  // (a wave's tiles about as many of m as of n)
+  q->group = std::min(q->tiles_m, cg == 2 ? 8 : 12);
+  q->whole = (int32_t)plan.whole;
   q->part_steps = (int32_t)((steps + plan.parts - 1) / plan.parts);
   q->parts = (int32_t)((steps + q->part_steps - 1) / q->part_steps);
   q->stage_bytes = kABytes + bn / cg * 128;
   q->stages = std::min(kMaxStages, kRingBytes / q->stage_bytes);
   q->a_bytes = terms[0].a.mn ? kABytes : a_rows * 128;
   q->status = status;
-  return (int64_t)q->tiles_m * q->tiles_n * q->parts < ((int64_t)1 << 31);
+  return (int64_t)q->tiles_m * q->tiles_n < ((int64_t)1 << 30);
 }
 
 template <int CG, bool kAMN, bool kBMN, typename Epi>
@@ -453,7 +476,7 @@ int launch(const Problem& q, const typename Epi::Args& ea, cudaStream_t st) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) !=
       cudaSuccess)
     return TT_ERR_CUDA;
-  const int64_t items = (int64_t)q.tiles_m * q.tiles_n * q.parts;
+  const int64_t items = q.whole + ((int64_t)q.tiles_m * q.tiles_n - q.whole) * q.parts;
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)(std::min<int64_t>(items, vec::kSMs / CG) * CG));
   c.blockDim = dim3(kGemmThreads);
@@ -475,11 +498,16 @@ int launch(const Plan& plan, const Problem& q, const typename Epi::Args& ea, cud
                       : launch<1, kAMN, kBMN, Epi>(q, ea, st);
 }
 
-// 32 values of a row at columns col .. of n: 16-byte stores where `wide` allows.
+// A 32 x 32 block of C: each lane 32 values of a row of its own at `p` (null: none), of
+// which `left` are in C.  Where rows are on 16-byte boundaries (wide) a lane stores its
+// own; else the warp stores row after row out of shared memory, 32 elements next to
+// one another (elements of 32 rows at a time cost an odd width three times the rest).
 template <typename T>
-__device__ __forceinline__ void store_row32(T* p, const float (&v)[32], int left, bool wide) {
+__device__ __forceinline__ void store_block(T* p, const float (&v)[32], int left, bool wide,
+                                            float* block) {
   constexpr int V = 16 / (int)sizeof(T);
   if (wide && left >= 32) {
+    if (!p) return;
 #pragma unroll
     for (int i = 0; i < 32; i += V) {
       float w[V];
@@ -487,17 +515,25 @@ __device__ __forceinline__ void store_row32(T* p, const float (&v)[32], int left
       for (int j = 0; j < V; ++j) w[j] = v[i + j];
       vec::store<T, V>(p + i, w);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < left) p[i] = from_f32<T>(v[i]);
+    return;
   }
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) block[lane * kStageRow + i] = v[i];
+  __syncwarp();
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r) {
+    T* row = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), r));
+    if (row && lane < left) row[lane] = from_f32<T>(block[r * kStageRow + lane]);
+  }
+  __syncwarp();
 }
 
-// A product of 16-bit factors into C (tensor cores).  `work` as in fp32_product.
+// A product of 16-bit factors into C (tensor cores).  `work` as in fp32_product;
+// steps: slices of 64 of k, of all terms.
 int tc_product(bool bf16, int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r,
                void* work, int64_t work_bytes, int32_t* status, cudaStream_t st);
-int64_t tc_work(int64_t M, int64_t N, int64_t k, bool b_mn);
+int64_t tc_work(int64_t M, int64_t N, int64_t steps, bool b_mn);
 
 }  // namespace gemm
 }  // namespace tt

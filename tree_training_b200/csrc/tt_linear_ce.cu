@@ -18,7 +18,10 @@
 // The pieces are as wide as a quarter of a gigabyte of dz allows, and at least
 // 4,096: every piece reads and writes dx's fp32 sum once.
 //
-// dz is rounded to 16 bits once, as the tensor cores' operands need.  In fp16 it is
+// dz is rounded to 16 bits once, as the tensor cores' operands need.  A row's label
+// dominates its dz, so that over few rows that one rounding (2^-9 in bf16) would show
+// in dx and dW beside their own: up to 256 rows, where W's bytes bound the products
+// anyway, dz is two 16-bit terms, and each product a sum of two.  In fp16 it is
 // multiplied by a power of two first that brings the largest weight of a row to
 // about 2^14 (and divided out of the sums): softmax probabilities times weights of
 // 1 / T lie below fp16's smallest number.
@@ -91,7 +94,8 @@ struct LseEpi {
     float scale;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc) {
+                                              const gemm::TileAt& t, int row, uint32_t acc,
+                                              float* block) {
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
     const bool live = row < p.M;
     const int count = live ? a.labels.count[row] : 0;
@@ -218,11 +222,12 @@ struct GradEpi {
   static constexpr bool kBf16 = kB;
   struct Args {
     Grad g;
-    void* dz;
+    void *dz, *rest;                       // rest: what rounding took off dz, or null
     int64_t ld;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc) {
+                                              const gemm::TileAt& t, int row, uint32_t acc,
+                                              float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
     const bool live = row < p.M;
@@ -236,12 +241,17 @@ struct GradEpi {
       float z[32];
       __syncwarp();                          // (the load is the whole warp's)
       sm100::tmem_ld32(acc + c, z);
-      if (!live) continue;
 #pragma unroll
       for (int i = 0; i < 32; ++i) z[i] *= a.g.scale;
       gradient<32>(a.g, row, count, (mask >> (c >> 5)) & 1, lse, w, f, v0 + c, z);
-      gemm::store_row32(reinterpret_cast<T*>(a.dz) + (int64_t)row * a.ld + n0 + c, z, cols - c,
-                        true);
+      const int64_t at = (int64_t)row * a.ld + n0 + c;
+      gemm::store_block(live ? reinterpret_cast<T*>(a.dz) + at : nullptr, z, cols - c, true, block);
+      if (a.rest) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] -= to_f32(from_f32<T>(z[i]));
+        gemm::store_block(live ? reinterpret_cast<T*>(a.rest) + at : nullptr, z, cols - c, true,
+                          block);
+      }
     }
   }
 };
@@ -304,10 +314,16 @@ bool sizes_ok(int64_t T, int32_t H, int64_t V, int64_t M) {
          V < ((int64_t)1 << 31) - 256 && M >= 0 && M <= 0x7fffffff;
 }
 
-// Columns of a piece of the vocabulary: a quarter of a gigabyte of dz (of fp32
-// logits), at least 4,096.
+constexpr int64_t kTwoTermRows = 256;      // see the top
+
+bool two_terms(int dtype, int64_t T) { return dtype != TT_F32 && T <= kTwoTermRows; }
+
+// Bytes of dz (of fp32 logits) an element.
+int64_t dz_size(int dtype, int64_t T) { return dtype == TT_F32 || two_terms(dtype, T) ? 4 : 2; }
+
+// Columns of a piece of the vocabulary: a quarter of a gigabyte of dz, at least 4,096.
 int64_t piece_of(int dtype, int64_t T, int64_t V) {
-  const int64_t wide = ((int64_t)1 << 28) / ((dtype == TT_F32 ? 4 : 2) * std::max<int64_t>(T, 1));
+  const int64_t wide = ((int64_t)1 << 28) / (dz_size(dtype, T) * std::max<int64_t>(T, 1));
   return std::min((V + 255) / 256 * 256, std::max<int64_t>(4096, wide / 256 * 256));
 }
 
@@ -362,14 +378,14 @@ int forward_16(const Shape& s, const void* x, int64_t x_ld, const void* w, int64
 
 template <bool kB>
 int gradient_16(const Shape& s, const void* x, int64_t x_ld, const void* w, int64_t w_ld, int64_t n,
-                const Grad& g, void* dz, int64_t ld, int32_t* status, cudaStream_t st) {
+                const Grad& g, void* dz, void* rest, int64_t ld, int32_t* status, cudaStream_t st) {
   using Epi = GradEpi<kB>;
   const gemm::Plan plan = gemm::plan_product(s.T, n, (s.H + gemm::kBK - 1) / gemm::kBK, 16, false,
                                              false);
   const gemm::Term term{{x, x_ld, false}, {w, w_ld, false}, s.H};
   gemm::Problem q;
   if (!gemm::set_up(&q, plan, kB, s.T, n, &term, 1, false, status)) return TT_ERR_UNSUPPORTED;
-  typename Epi::Args ea{g, dz, ld};
+  typename Epi::Args ea{g, dz, rest, ld};
   return gemm::launch<false, false, Epi>(plan, q, ea, st);
 }
 
@@ -451,10 +467,13 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
 }
 
 namespace {
+int64_t slices(int64_t k) { return (k + gemm::kBK - 1) / gemm::kBK; }
+int terms_of(int dtype, int64_t T) { return two_terms(dtype, T) ? 2 : 1; }
 int64_t product_work(int dtype, int64_t T, int32_t H, int64_t P) {
   return dtype == TT_F32 ? std::max({gemm::fp32_work(T, P, H), gemm::fp32_work(T, H, P),
                                      gemm::fp32_work(P, H, T)})
-                         : std::max(gemm::tc_work(T, H, P, true), gemm::tc_work(P, H, T, true));
+                         : std::max(gemm::tc_work(T, H, terms_of(dtype, T) * slices(P), true),
+                                    gemm::tc_work(P, H, terms_of(dtype, T) * slices(T), true));
 }
 }  // namespace
 
@@ -462,8 +481,8 @@ extern "C" int64_t tt_linear_ce_bwd_workspace_size(int dtype, int64_t T, int32_t
                                                    int64_t M) {
   if (!sizes_ok(T, H, V, M) || dtype < TT_F32 || dtype > TT_F16) return 0;
   if (T == 0) return 0;
-  const int64_t P = piece_of(dtype, T, V), size = dtype == TT_F32 ? 4 : 2;
-  return labels_bytes(T, M) + round256(4 * T) + 2 * 256 + round256(size * T * P) +
+  const int64_t P = piece_of(dtype, T, V);
+  return labels_bytes(T, M) + round256(4 * T) + 2 * 256 + round256(dz_size(dtype, T) * T * P) +
          (P < V ? round256(4 * T * H) : 0) + product_work(dtype, T, H, P);
 }
 
@@ -488,7 +507,9 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   float* weight = ws.take<float>(4 * T);
   uint32_t* largest = ws.take<uint32_t>(4);
   float* factor = ws.take<float>(8);
-  void* dz = ws.take<char>(size * T * P);
+  const int n_terms = terms_of(dtype, T);
+  char* dz = ws.take<char>(dz_size(dtype, T) * T * P);
+  char* rest = n_terms == 2 ? dz + 2 * T * P : nullptr;
   float* sum = P < V ? ws.take<float>(4 * T * H) : nullptr;
   void* work = ws.p;
   const int64_t work_bytes = product_work(dtype, T, H, P);
@@ -504,9 +525,11 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   }
   g.weight = weight, g.lse = lse, g.g_loss = g_loss, g.scale = scale;
   auto product = [&](int64_t m, int64_t n, const gemm::Term& term, const gemm::Result& r) {
-    return f32 ? gemm::fp32_product(m, n, &term, 1, r, work, work_bytes, st)
-               : gemm::tc_product(dtype == TT_BF16, m, n, &term, 1, r, work, work_bytes, status,
-                                  st);
+    if (f32) return gemm::fp32_product(m, n, &term, 1, r, work, work_bytes, st);
+    gemm::Term terms[2] = {term, term};
+    terms[1].a.p = rest;
+    return gemm::tc_product(dtype == TT_BF16, m, n, terms, n_terms, r, work, work_bytes, status,
+                            st);
   };
   int rc = TT_OK;
   for (int64_t v0 = 0; v0 < V; v0 += P) {
@@ -520,8 +543,8 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
       grad_kernel<<<row_blocks(T), 256, 0, st>>>((float*)dz, T, (int)n, P, g);
       tt_count_launches(1);
     } else {
-      rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, P, status, st)
-                            : gradient_16<false>(s, x, x_ld, wp, w_ld, n, g, dz, P, status, st);
+      rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st)
+                            : gradient_16<false>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st);
       if (rc) return rc;
     }
     if (dx) {
