@@ -17,6 +17,11 @@
 // Backward: dg and du leave one elementwise pass in 16 bits, dx is one sum of two
 // products in one accumulator, each weight's gradient one product.
 //
+// Up to kFewRows tokens (a rollout's single ones) no tensor core is needed: a warp a
+// feature reads its two rows once, 16 bytes a lane, and multiplies by fma (2,560 x
+// 9,728 bf16: 21 us a token, 25 two; the tensor cores take 29 for 3 to 128 tokens, fma
+// 33 for three).
+//
 // fp32: the products on the CUDA cores (see tt_gemm_fp32.cu), h by a pass over g and u.
 #include "tt_gemm_sm100.cuh"
 
@@ -96,13 +101,100 @@ struct GatedEpi {
         gemm::store_block(live ? a.g + at : nullptr, g, left, true, block);
         gemm::store_block(live ? a.u + at : nullptr, u, left, true, block);
       }
+      // (not of rows past the last: what stands there may be anything, and the division's
+      // way through NaN and infinities took 14 us of 43 for 64 tokens)
+      if (live) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) g[i] = act<A>(g[i]) * u[i];
+        for (int i = 0; i < 32; ++i) g[i] = act<A>(g[i]) * u[i];
+      }
       T* h = reinterpret_cast<T*>(a.h) + (int64_t)row * a.h_ld + n0 + c;
       gemm::store_block(live ? h : nullptr, g, left, a.wide, block);
     }
   }
 };
+
+constexpr int kFewRows = 2;
+constexpr int kFewBytes = 40960;           // of x in shared memory
+
+// A warp a feature, N rows of x.
+template <typename T, int A, int N>
+__global__ void __launch_bounds__(256)
+    few_rows_kernel(const T* x, int64_t x_ld, const T* wg, int64_t wg_ld, const T* wu,
+                    int64_t wu_ld, int rows, int H, int F, T* h, float* g_out, float* u_out,
+                    int64_t keep_ld) {
+  constexpr int kAhead = 5;                // packs of a row that are fetched together
+  extern __shared__ uint4 xs[];            // [N][packs]
+  const int packs = (H + 7) / 8, lane = threadIdx.x & 31;
+  const int f = blockIdx.x * 8 + threadIdx.x / 32;
+  const T* rg = wg + (int64_t)min(f, F - 1) * wg_ld;
+  const T* ru = wu + (int64_t)min(f, F - 1) * wu_ld;
+  // (a row's last pack may be a part of one: element by element, then)
+  auto pack_of = [&](const T* row, int p) {
+    return (p + 1) * 8 <= H ? __ldg(reinterpret_cast<const uint4*>(row) + p)
+                            : vec::load_any_of<T>(row, p * 8, H, row, row);
+  };
+  uint4 a[kAhead], b[kAhead];
+  auto fetch = [&](int p0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int p = p0 + j * 32 + lane;
+      a[j] = b[j] = make_uint4(0, 0, 0, 0);
+      if (p < packs) a[j] = pack_of(rg, p), b[j] = pack_of(ru, p);
+    }
+  };
+  fetch(0);
+  for (int i = threadIdx.x; i < N * packs; i += blockDim.x) {
+    const int t = i / packs, p = i - t * packs;
+    xs[i] = t < rows ? pack_of(x + t * x_ld, p) : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  float g[N], u[N];
+#pragma unroll
+  for (int t = 0; t < N; ++t) g[t] = u[t] = 0.f;
+  for (int p0 = 0; p0 < packs; p0 += 32 * kAhead) {
+    if (p0) fetch(p0);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int p = p0 + j * 32 + lane;
+      if (p >= packs) continue;
+      float vg[8], vu[8];
+      vec::unpack<T, 8>(a[j], vg);
+      vec::unpack<T, 8>(b[j], vu);
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        float vx[8];
+        vec::unpack<T, 8>(xs[t * packs + p], vx);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[t] = fmaf(vg[i], vx[i], g[t]), u[t] = fmaf(vu[i], vx[i], u[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      g[t] += __shfl_xor_sync(0xffffffffu, g[t], o);
+      u[t] += __shfl_xor_sync(0xffffffffu, u[t], o);
+    }
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+    if (lane == t && t < rows && f < F) {
+      h[(int64_t)t * F + f] = from_f32<T>(act<A>(g[t]) * u[t]);
+      if (g_out) g_out[t * keep_ld + f] = g[t], u_out[t * keep_ld + f] = u[t];
+    }
+}
+
+template <typename T, int A>
+int few_rows(const void* x, int64_t x_ld, const void* wg, int64_t wg_ld, const void* wu,
+             int64_t wu_ld, int rows, int H, int F, void* h, float* g, float* u, int64_t keep_ld,
+             cudaStream_t st) {
+  auto* kernel = rows == 1 ? few_rows_kernel<T, A, 1> : few_rows_kernel<T, A, 2>;
+  kernel<<<(F + 7) / 8, 256, rows * ((H + 7) / 8) * 16, st>>>(
+      (const T*)x, x_ld, (const T*)wg, wg_ld, (const T*)wu, wu_ld, rows, H, F, (T*)h, g, u,
+      keep_ld);
+  tt_count_launches(1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
 
 // h of fp32 g and u.
 template <int A>
@@ -172,6 +264,13 @@ int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void*
                int64_t wg_ld, const void* wu, int64_t wu_ld, int act, void* h, float* g, float* u,
                int64_t keep_ld, int32_t* status, cudaStream_t st) {
   return dispatch_act(act, [&](auto a) -> int {
+    const gemm::Factor all[3] = {{x, x_ld, false}, {wg, wg_ld, false}, {wu, wu_ld, false}};
+    for (const gemm::Factor& f : all)
+      if (!gemm::copyable(f)) return TT_ERR_UNSUPPORTED;
+    if (T <= kFewRows && T * ((H + 7) / 8) * 16 <= kFewBytes)
+      return few_rows<typename std::conditional<kB, __nv_bfloat16, __half>::type,
+                      decltype(a)::value>(x, x_ld, wg, wg_ld, wu, wu_ld, (int)T, H, F, h, g, u,
+                                          keep_ld, st);
     using Epi = GatedEpi<kB, decltype(a)::value>;
     const gemm::Plan plan =
         gemm::plan_product(T, F, (H + gemm::kBK - 1) / gemm::kBK, 16, true, false);
@@ -195,7 +294,7 @@ using namespace tt::gated;
 
 extern "C" int64_t tt_gated_linear_fwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F) {
   if (!sizes_ok(T, H, F) || dtype != TT_F32) return 0;
-  return gemm::fp32_work(T, F, H);
+  return gemm::fp32_work(T, F, H, 2);
 }
 
 extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x,
@@ -221,12 +320,10 @@ extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, c
   if (workspace_bytes < tt_gated_linear_fwd_workspace_size(dtype, T, H, F))
     return TT_ERR_WORKSPACE;
   const gemm::Factor fx{x, x_ld, false};
-  const gemm::Term tg{fx, {wg, wg_ld, false}, H}, tu{fx, {wu, wu_ld, false}, H};
-  for (int i = 0; i < 2; ++i) {
-    const gemm::Result r{TT_F32, i ? u : g, keep_ld, nullptr, 0, 1.f, nullptr};
-    if (const int rc = gemm::fp32_product(T, F, i ? &tu : &tg, 1, r, workspace, workspace_bytes, st))
-      return rc;
-  }
+  const gemm::Term terms[2] = {{fx, {wg, wg_ld, false}, H}, {fx, {wu, wu_ld, false}, H}};
+  const gemm::Result r[2] = {{TT_F32, g, keep_ld, nullptr, 0, 1.f, nullptr},
+                             {TT_F32, u, keep_ld, nullptr, 0, 1.f, nullptr}};
+  if (const int rc = gemm::fp32_products(T, F, terms, r, workspace, workspace_bytes, st)) return rc;
   return dispatch_act(act, [&](auto a) -> int {
     const dim3 grid((unsigned)std::min((F + 255) / 256, 64),
                     (unsigned)std::min<int64_t>(T, 32768));
@@ -245,7 +342,8 @@ int64_t slices(int64_t k) { return (k + gemm::kBK - 1) / gemm::kBK; }
 int64_t parts_bytes(int dtype, int64_t T, int32_t H, int32_t F) {
   const int64_t both = round8(F) + F;
   if (dtype == TT_F32)
-    return std::max(gemm::fp32_work(T, H, 2 * (int64_t)F), gemm::fp32_work(F, H, T));
+    return std::max({gemm::fp32_work(T, H, 2 * (int64_t)F), gemm::fp32_work(F, H, T),
+                     gemm::fp32_work(F, H, T, 2)});
   return std::max({gemm::tc_work(T, H, 2 * slices(F), true), gemm::tc_work(F, H, slices(T), true),
                    gemm::tc_work(both, H, slices(T), true)});
 }
@@ -297,7 +395,14 @@ extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, c
                                  {{du, ld, false}, {wu, wu_ld, true}, F}};
     if ((rc = product(T, H, terms, 2, dx))) return rc;
   }
-  if (dwg && dwu && dtype != TT_F32) {
+  if (dwg && dwu && dtype == TT_F32) {
+    const gemm::Factor fx{x, x_ld, true};
+    const gemm::Term terms[2] = {{{dg, ld, true}, fx, T}, {{du, ld, true}, fx, T}};
+    const gemm::Result r[2] = {{dtype, dwg, H, nullptr, 0, 1.f, nullptr},
+                               {dtype, dwu, H, nullptr, 0, 1.f, nullptr}};
+    return gemm::fp32_products(F, H, terms, r, work, work_bytes, st);
+  }
+  if (dwg && dwu) {
     // one product for both: its last wave of tiles comes once
     const gemm::Term term{{dg, ld, true}, {x, x_ld, true}, T};
     gemm::Result r{dtype, dwg, H, nullptr, 0, 1.f, nullptr};

@@ -41,11 +41,11 @@ struct Result {
 // make room for any split; with less the sum is split less).
 int fp32_product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r, void* work,
                  int64_t work_bytes, cudaStream_t st);
-int64_t fp32_work(int64_t M, int64_t N, int64_t k);
+int64_t fp32_work(int64_t M, int64_t N, int64_t k, int batch = 1);
 
-// C = the parts [n_parts][M][N], added up in order, + cin.
-int join_parts(const float* parts, int n_parts, int64_t M, int64_t N, const Result& r,
-               cudaStream_t st);
+// Two products of the same shape in one launch, a term and a result each.
+int fp32_products(int64_t M, int64_t N, const Term* terms, const Result* r, void* work,
+                  int64_t work_bytes, cudaStream_t st);
 
 }  // namespace gemm
 }  // namespace tt

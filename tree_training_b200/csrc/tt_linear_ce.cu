@@ -258,51 +258,62 @@ struct GradEpi {
 
 // ---- fp32: passes over the logits of a piece --------------------------------------------
 
-// A block a row: the piece's (m, s) joined to the row's, its labels' logits.
+// (m, s) of a row's columns of a piece, by segments (blockIdx.y) of them, and its
+// labels' logits.
 __global__ void __launch_bounds__(256)
-    lse_kernel(const float* z, int64_t T, int64_t v0, int n, int64_t ld, const Labels l,
-               float2* part, int first, float* picked) {
+    lse_kernel(const float* z, int64_t T, int64_t v0, int n, int64_t ld, int segment,
+               const Labels l, float2* part, float* picked) {
   __shared__ float2 sm[256];
+  const int c0 = blockIdx.y * segment, c1 = min(n, c0 + segment);
   for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
     const float* row = z + t * ld;
     float m = -INFINITY, s = 0.f;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) m = fmaxf(m, row[c]);
+    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) m = fmaxf(m, row[c]);
     const float ref = m == -INFINITY ? 0.f : m;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) s += expf(row[c] - ref);
+    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) s += expf(row[c] - ref);
     sm[threadIdx.x] = make_float2(m, s);
     __syncthreads();
     for (int o = 128; o; o >>= 1) {
       if (threadIdx.x < o) sm[threadIdx.x] = join(sm[threadIdx.x], sm[threadIdx.x + o]);
       __syncthreads();
     }
-    if (threadIdx.x == 0) part[t] = first ? sm[0] : join(part[t], sm[0]);
+    if (threadIdx.x == 0) part[(int64_t)blockIdx.y * T + t] = sm[0];
     for (int i = threadIdx.x; i < l.count[t]; i += blockDim.x) {
       const int2 y = l.list[t * l.M + i];
-      if (y.x >= v0 && y.x < v0 + n) picked[t * l.M + y.y] = row[y.x - v0];
+      if (y.x >= v0 + c0 && y.x < v0 + c1) picked[t * l.M + y.y] = row[y.x - v0];
     }
     __syncthreads();
   }
 }
 
+// dz in place of the logits of a piece.
 __global__ void __launch_bounds__(256)
-    grad_kernel(float* z, int64_t T, int n, int64_t ld, const Grad g) {
+    grad_kernel(float* z, int64_t T, int n, int64_t ld, int segment, const Grad g) {
+  const int c0 = blockIdx.y * segment, c1 = min(n, c0 + segment);
   for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
     const int count = g.labels.count[t];
+    const float w = g.weight[t], lse = g.lse[t];
     float* row = z + t * ld;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) {
-      const float v = g.weight[t] * expf(row[c] - g.lse[t]);
-      row[c] = v;
-    }
+    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) row[c] = w * expf(row[c] - lse);
     __syncthreads();
     // (one thread: a label may be given twice)
     if (threadIdx.x == 0 && g.g_loss)
       for (int k = 0; k < count; ++k) {
         const int2 l = g.labels.list[t * g.labels.M + k];
         const int64_t at = l.x - g.v0;
-        if (at >= 0 && at < n) row[at] -= g.g_loss[t * g.labels.M + l.y] * g.scale;
+        if (at >= c0 && at < c1) row[at] -= g.g_loss[t * g.labels.M + l.y] * g.scale;
       }
     __syncthreads();
   }
+}
+
+// Columns of a segment: four blocks an SM where there are few rows.
+int segment_of(int64_t T, int64_t n) {
+  const int64_t want = std::max<int64_t>(1, 4 * vec::kSMs / T);
+  return (int)std::max<int64_t>(512, (n + want - 1) / want);
+}
+int64_t segments_of(int64_t T, int64_t n) {
+  return (n + segment_of(T, n) - 1) / segment_of(T, n);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -415,7 +426,8 @@ extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t
   if (T == 0) return base;
   if (dtype == TT_F32) {
     const int64_t P = piece_of(dtype, T, V);
-    return base + round256(8 * T) + round256(4 * T * P) + gemm::fp32_work(T, P, H);
+    return base + round256(8 * T * segments_of(T, P) * ((V + P - 1) / P)) +
+           round256(4 * T * P) + gemm::fp32_work(T, P, H);
   }
   const gemm::Plan p = forward_plan(T, H, V);
   return base + round256(8 * T * ((V + p.bn - 1) / p.bn));
@@ -439,8 +451,9 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   int parts = 1, rc = TT_OK;
   float2* part;
   if (dtype == TT_F32) {
-    part = ws.take<float2>(8 * T);
-    const int64_t P = piece_of(dtype, T, V);
+    const int64_t P = piece_of(dtype, T, V), segments = segments_of(T, P);
+    part = ws.take<float2>(8 * T * segments * ((V + P - 1) / P));
+    parts = 0;
     float* z = ws.take<float>(4 * T * P);
     for (int64_t v0 = 0; v0 < V; v0 += P) {
       const int64_t n = std::min(P, V - v0);
@@ -448,7 +461,11 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
       const gemm::Result r{TT_F32, z, P, nullptr, 0, scale, nullptr};
       if ((rc = gemm::fp32_product(T, n, &term, 1, r, ws.p, gemm::fp32_work(T, P, H), st)))
         return rc;
-      lse_kernel<<<row_blocks(T), 256, 0, st>>>(z, T, v0, (int)n, P, l, part, v0 == 0, picked);
+      // (the last piece may have fewer of them)
+      const int segment = segment_of(T, P), here = (int)((n + segment - 1) / segment);
+      lse_kernel<<<dim3(row_blocks(T), here), 256, 0, st>>>(z, T, v0, (int)n, P, segment, l,
+                                                            part + (int64_t)parts * T, picked);
+      parts += here;
       tt_count_launches(1);
     }
   } else {
@@ -540,7 +557,9 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
       const gemm::Term term{{x, x_ld, false}, {wp, w_ld, false}, H};
       if ((rc = product(T, n, term, gemm::Result{TT_F32, dz, P, nullptr, 0, scale, nullptr})))
         return rc;
-      grad_kernel<<<row_blocks(T), 256, 0, st>>>((float*)dz, T, (int)n, P, g);
+      const int segment = segment_of(T, P);
+      grad_kernel<<<dim3(row_blocks(T), (unsigned)((n + segment - 1) / segment)), 256, 0, st>>>(
+          (float*)dz, T, (int)n, P, segment, g);
       tt_count_launches(1);
     } else {
       rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st)
