@@ -161,6 +161,8 @@ __device__ __forceinline__ unsigned same_as(int e, int bits) {
 template <typename T, bool kFirst>
 __global__ void __launch_bounds__(32 * kWarps) rank_kernel(const Grad a, const Sort s) {
   extern __shared__ int hist[];               // [warps][digits + 1]: counts, then ranks
+  vec::let_next_begin();
+  if (!kFirst) vec::wait_previous();
   if ((int)blockIdx.x >= s.blocks) {
     zero_rows<T>(a, s.part, s.parts, blockIdx.x - s.blocks, gridDim.x - s.blocks);
     return;
@@ -234,6 +236,8 @@ __global__ void __launch_bounds__(32 * kWarps) rank_kernel(const Grad a, const S
 template <typename T>
 __global__ void __launch_bounds__(kPlaceThreads) place_kernel(const Grad a, const Sort s) {
   extern __shared__ int sm[];
+  vec::let_next_begin();
+  vec::wait_previous();
   if ((int)blockIdx.x >= s.blocks) {
     zero_rows<T>(a, s.part, s.parts, blockIdx.x - s.blocks, gridDim.x - s.blocks);
     return;
@@ -301,6 +305,8 @@ __global__ void __launch_bounds__(512)
                int parts_of_rows) {
   constexpr int N = 16 / (int)sizeof(T);
   constexpr int kAhead = kAligned ? 8 : 4;    // rows fetched together
+  vec::let_next_begin();
+  vec::wait_previous();
   if ((int)blockIdx.x >= sum_blocks) {
     if (blockIdx.y == 0)
       zero_rows<T>(a, part, parts_of_rows, blockIdx.x - sum_blocks, gridDim.x - sum_blocks);
@@ -448,6 +454,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Grad a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t col = ((int64_t)blockIdx.y * 32 + lane) * N;
   float acc[N];
+  vec::wait_previous();
   for (int64_t base = blockIdx.x; base < a.chunks; base += (int64_t)kThreads * gridDim.x) {
     if (threadIdx.x == 0) count = longer_count = 0;
     __syncthreads();
@@ -574,10 +581,14 @@ int gradient(Grad a, int32_t* const* orders, cudaStream_t st) {
     if (d == 0) {
       rank_kernel<T, true><<<blocks, 32 * kWarps, rank_smem, st>>>(a, s);
     } else {
-      rank_kernel<T, false><<<blocks + zero_blocks, 32 * kWarps, rank_smem, st>>>(a, s);
+      if (vec::launch_next(rank_kernel<T, false>, blocks + zero_blocks, 32 * kWarps, rank_smem, st,
+                           a, s) != cudaSuccess)
+        return TT_ERR_CUDA;
       ++s.part;
     }
-    place_kernel<T><<<blocks + zero_blocks, kPlaceThreads, place_smem, st>>>(a, s);
+    if (vec::launch_next(place_kernel<T>, blocks + zero_blocks, kPlaceThreads, place_smem, st, a,
+                         s) != cudaSuccess)
+      return TT_ERR_CUDA;
     ++s.part;
     tt_count_launches(2);
     order = s.next;
@@ -592,17 +603,16 @@ int gradient(Grad a, int32_t* const* orders, cudaStream_t st) {
   const unsigned cols = (unsigned)((packs + group - 1) / group);
   const int64_t sum_blocks = (a.chunks + groups - 1) / groups;
   const dim3 grid((unsigned)(sum_blocks + zero_blocks), cols);
-  if (aligned)
-    sum_kernel<T, true><<<grid, group * groups, 0, st>>>(a, order, group, (int)sum_blocks, s.part,
-                                                         shares);
-  else
-    sum_kernel<T, false><<<grid, group * groups, 0, st>>>(a, order, group, (int)sum_blocks, s.part,
-                                                          shares);
+  if (vec::launch_next(aligned ? sum_kernel<T, true> : sum_kernel<T, false>, grid, group * groups,
+                       0, st, a, order, group, (int)sum_blocks, s.part, shares) != cudaSuccess)
+    return TT_ERR_CUDA;
   tt_count_launches(1);
   if (a.chunks > 1) {
     const int64_t cols = (a.part_ld / N + 31) / 32;
     const int64_t blocks = std::max<int64_t>(1, std::min(a.chunks, 4 * vec::kSMs / cols));
-    join_kernel<T><<<dim3((unsigned)blocks, (unsigned)cols), 32 * kJoinWarps, 0, st>>>(a);
+    if (vec::launch_next(join_kernel<T>, dim3((unsigned)blocks, (unsigned)cols), 32 * kJoinWarps, 0,
+                         st, a) != cudaSuccess)
+      return TT_ERR_CUDA;
     tt_count_launches(1);
   }
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;

@@ -139,6 +139,7 @@ template <int kind>
 __global__ void __launch_bounds__(kThreads, 2)
     norm_kernel(const __grid_constant__ Table t, double* part) {
   __shared__ double sm[kThreads / 32];
+  vec::let_next_begin();
   double sum = 0.0;
   for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
     const int i = tensor_of(t, c);
@@ -178,6 +179,7 @@ __device__ __forceinline__ double norm_of(const double* part, int n, int kind, d
 __global__ void __launch_bounds__(kThreads) finish_kernel(const double* part, int n, int kind,
                                                            float* norm) {
   __shared__ double sm[kThreads / 32];
+  vec::wait_previous();
   const double v = norm_of(part, n, kind, sm);
   if (threadIdx.x == 0) *norm = (float)v;
 }
@@ -221,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     scale_kernel(const __grid_constant__ Table t, const double* part, int parts, int kind,
                  const float* given, float max_norm, float eps, float* norm, int in_place) {
   __shared__ double sm[kThreads / 32];
+  vec::wait_previous();
   const float v = given ? *given : (float)norm_of(part, parts, kind, sm);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   const float q = max_norm / (v + eps);
@@ -345,9 +348,11 @@ extern "C" int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t*
   if (const int rc = norm_passes(count, dtypes, sizes, tensors, kind, part, workspace_bytes / 8,
                                  &parts, st))
     return rc;
-  finish_kernel<<<1, kThreads, 0, st>>>(part, parts, kind, norm);
+  if (tt::vec::launch_next(finish_kernel, 1, kThreads, 0, st, part, parts, kind, norm) !=
+      cudaSuccess)
+    return TT_ERR_CUDA;
   tt_count_launches(1);
-  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+  return TT_OK;
 }
 
 extern "C" int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
@@ -375,8 +380,10 @@ extern "C" int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int
   do {
     at = fill(&t, at, count, dtypes, sizes, tensors, outs, chunk);
     if (t.count == 0 && !first) break;
-    scale_kernel<<<std::max(1, blocks_of(t)), kThreads, 0, st>>>(
-        t, part, parts, kind, given_norm, max_norm, eps, first ? norm : nullptr, in_place);
+    if (tt::vec::launch_next(scale_kernel, std::max(1, blocks_of(t)), kThreads, 0, st, t, part,
+                             parts, kind, given_norm, max_norm, eps, first ? norm : nullptr,
+                             in_place) != cudaSuccess)
+      return TT_ERR_CUDA;
     tt_count_launches(1);
     first = false;
   } while (at < count);

@@ -188,6 +188,36 @@ __device__ __forceinline__ void store_part(T* row, int64_t e0, int64_t n, const 
     if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = from_f32<T>(v[i]);
 }
 
+// ---- launches that follow one another closely ------------------------------------
+
+// A kernel launched by launch_next may begin while the one before it in its stream
+// ends: it waits here, before it touches memory, until that one has finished.
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Lets the next kernel begin as soon as every block of this one has come here (or
+// ended).
+__device__ __forceinline__ void let_next_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launches a kernel that calls wait_previous first.
+template <typename... P, typename... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                        cudaStream_t st, A... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+
 // Calls f with a value of the C++ type of a TT_* floating dtype.
 template <typename F>
 int dispatch_float(int dtype, F f) {
