@@ -43,6 +43,17 @@ __device__ __forceinline__ float act(float g) {
   return g > 0.f ? g : (g != g ? g : 0.f);
 }
 
+// The same for results of 16 bits, where 2^-20 of a value does not show: the epilogue
+// of the products has no time for the exact quotient.
+template <int A>
+__device__ __forceinline__ float act_16(float g) {
+  if constexpr (A == kSilu) return __fdividef(g, 1.f + __expf(-g));
+  // (1 + tanh y) / 2 = 1 / (1 + exp(-2 y))
+  if constexpr (A == kGeluTanh)
+    return __fdividef(g, 1.f + __expf(-2.f * kTanhA * (g + kTanhB * g * g * g)));
+  return act<A>(g);
+}
+
 // act(g) and its derivative.
 template <int A>
 __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
@@ -87,11 +98,12 @@ struct GatedEpi {
     int F, wide;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc, float* block) {
+                                              const gemm::TileAt& t, int row, uint32_t acc, int c0,
+                                              float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const int half = p.bn / 2, n0 = t.n * half, cols = min(half, a.F - n0);
     const bool live = row < p.M;
-    for (int c = 0; c < cols; c += 32) {
+    for (int c = c0; c < cols; c += 64) {
       float g[32], u[32];
       __syncwarp();                          // (the loads are the whole warp's)
       sm100::tmem_ld32x2(acc + c, acc + half + c, g, u);
@@ -101,11 +113,11 @@ struct GatedEpi {
         gemm::store_block(live ? a.g + at : nullptr, g, left, true, block);
         gemm::store_block(live ? a.u + at : nullptr, u, left, true, block);
       }
-      // (not of rows past the last: what stands there may be anything, and the division's
-      // way through NaN and infinities took 14 us of 43 for 64 tokens)
+      // (not of rows past the last: what stands there may be anything, and the exact
+      // division's way through NaN and infinities took 14 us of 43 for 64 tokens)
       if (live) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = act<A>(g[i]) * u[i];
+        for (int i = 0; i < 32; ++i) g[i] = act_16<A>(g[i]) * u[i];
       }
       T* h = reinterpret_cast<T*>(a.h) + (int64_t)row * a.h_ld + n0 + c;
       gemm::store_block(live ? h : nullptr, g, left, a.wide, block);

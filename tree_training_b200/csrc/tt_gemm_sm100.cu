@@ -20,7 +20,7 @@ struct StoreEpi {
     int f32, wide, cin_wide;
   };
   static __device__ __forceinline__ void tile(const Args& a, const Problem& p, const TileAt& t,
-                                              int row, uint32_t acc, float* block) {
+                                              int row, uint32_t acc, int c0, float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const float alpha = a.alpha * (a.alpha_dev ? __ldg(a.alpha_dev) : 1.f);
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
@@ -29,7 +29,7 @@ struct StoreEpi {
       // (a warp's rows of the tile, whichever CTA of the pair it is in)
       const int64_t tile_rows = p.tile_rows;
       float* q = a.parts + ((int64_t)t.unit * tile_rows + (row - t.m * tile_rows)) * p.bn;
-      for (int c = 0; c < cols; c += 32) {
+      for (int c = c0; c < cols; c += 64) {
         float v[32];
         __syncwarp();
         tmem_ld32(acc + c, v);
@@ -37,7 +37,7 @@ struct StoreEpi {
       }
       return;
     }
-    for (int c = 0; c < cols; c += 32) {
+    for (int c = c0; c < cols; c += 64) {
       float v[32];
       __syncwarp();                          // (the load is the whole warp's)
       tmem_ld32(acc + c, v);

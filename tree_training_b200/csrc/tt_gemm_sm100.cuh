@@ -6,8 +6,9 @@
 //
 // Persistent CTAs (pairs of CTAs for tall problems) over tiles of 128 (256) rows by
 // up to 256 columns.  Warp 0 feeds a ring of 64-wide slices of k by TMA, one thread
-// of warp 1 issues `tcgen05.mma` into one of two TMEM accumulators, warps 4 to 7
-// take the other through the epilogue meanwhile.
+// of warp 1 issues `tcgen05.mma` into one of two TMEM accumulators, warps 4 to 11
+// take the other through the epilogue meanwhile (with four of them the epilogue of the
+// gated product took longer than sums over 1,000 of k).
 //
 // What bounds it.  An SM's tensor core takes bn / 2 clocks for a 128 x bn x 16 step;
 // filling and reading the step's operands takes (128 + bn) * 32 * 2 bytes through a
@@ -37,7 +38,8 @@ constexpr int kBK = 64;                    // k of a slice: 128 bytes
 constexpr int kABytes = 128 * kBK * 2;     // of A in a slice
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 196608;         // of shared memory for the ring
-constexpr int kGemmThreads = 256;
+constexpr int kEpiWarps = 8;               // warps 4 to 11: two for each quarter of the lanes
+constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
 
 struct Problem {
   CUtensorMap a[2], b[2];
@@ -85,7 +87,7 @@ struct Barriers {
 };
 
 constexpr int kStageRow = 33;              // floats of a row of a warp's 32 x 32 block
-constexpr int kStageBytes = 4 * 32 * kStageRow * 4;
+constexpr int kStageBytes = kEpiWarps * 32 * kStageRow * 4;
 // barriers, ring, its alignment, the epilogue's blocks
 constexpr int kGemmSmem = 1024 + kRingBytes + 1024 + kStageBytes;
 
@@ -167,10 +169,11 @@ __device__ __forceinline__ void tmem_give(uint32_t taddr) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
 }
 
-// Epi::tile(args, problem, tile, row, lane address, block) takes one accumulator out of
-// TMEM: a thread has one row of the tile (row: its index in C, possibly past M) and
-// reads its columns; all 32 lanes of a warp call it.  block: 32 x 33 floats of shared
-// memory of the warp's own.
+// Epi::tile(args, problem, tile, row, lane address, c0, block) takes one accumulator out
+// of TMEM: a thread has one row of the tile (row: its index in C, possibly past M) and
+// reads its columns c0 .. c0 + 31, c0 + 64 .. (c0: 0 or 32, another warp has the other
+// half); all 32 lanes of a warp call it.  block: 32 x 33 floats of shared memory of the
+// warp's own.
 template <int CG, bool kAMN, bool kBMN, typename Epi>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epi::Args ea) {
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const volatile int32_t* abort_flag = &sh->abort;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], 4 * CG);
+    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kEpiWarps * CG);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -315,7 +318,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int quad = warp & 3;
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-    float* block = reinterpret_cast<float*>(smem_raw + 2048 + kRingBytes) + quad * 32 * kStageRow;
+    float* block =
+        reinterpret_cast<float*>(smem_raw + 2048 + kRingBytes) + (warp - 4) * 32 * kStageRow;
     int acc = 0;
     for (int i = first; i < items; i += stride, ++acc) {
       const TileAt t = tile_at(p, i);
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       tc_fence_after();
       const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
-      Epi::tile(ea, p, t, row, lane_addr + buf * 256, block);
+      Epi::tile(ea, p, t, row, lane_addr + buf * 256, warp < 8 ? 0 : 32, block);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -498,6 +502,13 @@ int launch(const Plan& plan, const Problem& q, const typename Epi::Args& ea, cud
                       : launch<1, kAMN, kBMN, Epi>(q, ea, st);
 }
 
+// 32 bytes, on their boundary.
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x),
+               "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 // A 32 x 32 block of C: each lane 32 values of a row of its own at `p` (null: none), of
 // which `left` are in C.  Where rows are on 16-byte boundaries (wide) a lane stores its
 // own; else the warp stores row after row out of shared memory, 32 elements next to
@@ -508,12 +519,20 @@ __device__ __forceinline__ void store_block(T* p, const float (&v)[32], int left
   constexpr int V = 16 / (int)sizeof(T);
   if (wide && left >= 32) {
     if (!p) return;
+    // (whole sectors of 32 bytes where rows allow: two stores of 16 would each go to L2)
+    const bool sectors = (reinterpret_cast<uintptr_t>(p) & 31) == 0;
 #pragma unroll
-    for (int i = 0; i < 32; i += V) {
-      float w[V];
+    for (int i = 0; i < 32; i += 2 * V) {
+      float w[2][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) w[j] = v[i + j];
-      vec::store<T, V>(p + i, w);
+      for (int j = 0; j < V; ++j) w[0][j] = v[i + j], w[1][j] = v[i + V + j];
+      const uint4 a = vec::pack<T, V>(w[0]), b = vec::pack<T, V>(w[1]);
+      if (sectors) {
+        store32(p + i, a, b);
+      } else {
+        *reinterpret_cast<uint4*>(p + i) = a;
+        *reinterpret_cast<uint4*>(p + i + V) = b;
+      }
     }
     return;
   }

@@ -11,7 +11,7 @@
 // bound by the tensor cores, for few tokens by W's bytes.
 //
 // Forward, 16-bit: the product's epilogue reduces each row of a tile of logits to its
-// maximum and the sum of exp above it (8 bytes for 256 logits) and picks out the
+// maximum and the sum of exp above it (16 bytes for 256 logits) and picks out the
 // labels' logits; a second kernel joins the tiles in order.  Backward: by pieces of
 // the vocabulary, each formed again, turned into 16-bit dz by the epilogue, and
 // multiplied twice: dW's rows of the piece are complete, dx is summed up in fp32.
@@ -88,20 +88,20 @@ template <bool kB>
 struct LseEpi {
   static constexpr bool kBf16 = kB;
   struct Args {
-    float2* part;                          // [tiles of n][T]
+    float2* part;                          // [tiles of n][2][T]
     Labels labels;
     float* picked;                         // [T][M]
     float scale;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc,
+                                              const gemm::TileAt& t, int row, uint32_t acc, int c0,
                                               float* block) {
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
     const bool live = row < p.M;
     const int count = live ? a.labels.count[row] : 0;
     const uint32_t mask = chunks_with_labels(a.labels, row, count, n0, cols);
     float m = -INFINITY, s = 0.f;
-    for (int c = 0; c < cols; c += 32) {
+    for (int c = c0; c < cols; c += 64) {
       float z[32];
       __syncwarp();                          // (the load is the whole warp's)
       sm100::tmem_ld32(acc + c, z);
@@ -120,7 +120,7 @@ struct LseEpi {
           a.picked[(int64_t)row * a.labels.M + l.y] = v;
         }
     }
-    if (live) a.part[(int64_t)t.n * p.M + row] = make_float2(m, s);
+    if (live) a.part[(int64_t)(2 * t.n + (c0 > 0)) * p.M + row] = make_float2(m, s);
   }
 };
 
@@ -226,7 +226,7 @@ struct GradEpi {
     int64_t ld;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc,
+                                              const gemm::TileAt& t, int row, uint32_t acc, int c0,
                                               float* block) {
     using T = typename std::conditional<kB, __nv_bfloat16, __half>::type;
     const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
@@ -237,7 +237,7 @@ struct GradEpi {
     const float lse = live ? a.g.lse[row] : 0.f;
     const float f = a.g.factor ? *a.g.factor : 1.f;
     const float w = live ? a.g.weight[row] * f : 0.f;
-    for (int c = 0; c < cols; c += 32) {
+    for (int c = c0; c < cols; c += 64) {
       float z[32];
       __syncwarp();                          // (the load is the whole warp's)
       sm100::tmem_ld32(acc + c, z);
@@ -382,7 +382,7 @@ int forward_16(const Shape& s, const void* x, int64_t x_ld, const void* w, int64
   const gemm::Term term{{x, x_ld, false}, {w, w_ld, false}, s.H};
   gemm::Problem q;
   if (!gemm::set_up(&q, plan, kB, s.T, s.V, &term, 1, false, status)) return TT_ERR_UNSUPPORTED;
-  *parts = q.tiles_n;
+  *parts = 2 * q.tiles_n;
   typename Epi::Args ea{part, l, picked, scale};
   return gemm::launch<false, false, Epi>(plan, q, ea, st);
 }
@@ -430,7 +430,7 @@ extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t
            round256(4 * T * P) + gemm::fp32_work(T, P, H);
   }
   const gemm::Plan p = forward_plan(T, H, V);
-  return base + round256(8 * T * ((V + p.bn - 1) / p.bn));
+  return base + round256(16 * T * ((V + p.bn - 1) / p.bn));
 }
 
 extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M,
