@@ -52,6 +52,7 @@ struct Problem {
   int32_t parts, part_steps;               // behind them are summed in parts
   int32_t stages, stage_bytes;
   int32_t a_bytes;                         // of A that a CTA copies a slice
+  int32_t a_blocks, b_blocks;              // whole blocks of 64: copied together
   int32_t dual;                            // B's halves are two factors: b[0] and b[1]
   int32_t* status;
 };
@@ -121,6 +122,24 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+// The blocks of 64 of a factor's own index that a slice has, in one copy.
+template <int CG>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c1,
+                                       int c2) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+        "bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(c1), "r"(c2)
         : "memory");
 }
 
@@ -227,7 +246,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t bar =
               CG == 2 ? leader_addr(smem_u32(&sh->full[s])) : smem_u32(&sh->full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], tx);
-          if constexpr (kAMN) {
+          if (kAMN && p.a_blocks) {
+            tma_3d<CG>(sa, &p.a[term], bar, k0, m0 / 64);
+          } else if constexpr (kAMN) {
             tma_2d<CG>(sa, &p.a[term], bar, m0, k0);
             tma_2d<CG>(sa + 8192, &p.a[term], bar, m0 + 64, k0);
           } else {
@@ -243,7 +264,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
           } else if constexpr (kBMN) {
             const int n0 = t.n * p.bn + (int)rank * (p.bn / CG);
-            for (int c = 0; c < p.bn / CG; c += 64)
+            if (p.b_blocks) tma_3d<CG>(sb, &p.b[term], bar, k0, n0 / 64);
+            else for (int c = 0; c < p.bn / CG; c += 64)
               tma_2d<CG>(sb + c * 128, &p.b[term], bar, n0 + c, k0);
           } else {
             tma_2d<CG>(sb, &p.b[term], bar, k0, t.n * p.bn + (int)rank * (p.bn / CG));
@@ -378,11 +400,22 @@ inline bool copyable(const Factor& f) {
   return (reinterpret_cast<uintptr_t>(f.p) & 15) == 0 && f.ld % 8 == 0;
 }
 
-// The map of a factor of `n` rows and k columns: boxes of 64 k by `rows`, or of 64
-// rows by 64 k where the rows are contiguous.
-inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_t k, int rows) {
+// The map of a factor of `n` rows and k columns: boxes of 64 k by `rows`; where the
+// rows are contiguous, of 64 rows by 64 k, or (blocks) `rows` / 64 of these in one box.
+inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_t k, int rows,
+                   bool blocks) {
   const EncodeTiledFn fn = encoder();
   if (!fn || !copyable(f)) return false;
+  if (blocks) {
+    const cuuint64_t dims[3] = {64u, (cuuint64_t)k, (cuuint64_t)(n / 64)};
+    const cuuint64_t strides[2] = {(cuuint64_t)f.ld * 2, 128u};
+    const cuuint32_t box[3] = {64u, 64u, (cuuint32_t)(rows / 64)};
+    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+              const_cast<void*>(f.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
   const cuuint64_t dims[2] = {(cuuint64_t)(f.mn ? n : k), (cuuint64_t)(f.mn ? k : n)};
   const cuuint64_t strides[1] = {(cuuint64_t)f.ld * 2};
   const cuuint32_t box[2] = {64u, (cuuint32_t)(f.mn ? 64 : rows)};
@@ -446,13 +479,16 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool d
 inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N, const Term* terms,
                    int n_terms, bool dual, int32_t* status) {
   const int cg = plan.cg, bn = plan.bn;
-  const int a_rows = cg == 1 ? (int)std::min<int64_t>(128, (M + 7) / 8 * 8) : 128;
+  const int a_rows =
+      cg == 1 && !terms[0].a.mn ? (int)std::min<int64_t>(128, (M + 7) / 8 * 8) : 128;
   const int b_rows = dual ? bn / 2 : bn / cg;
   q->terms = dual ? 1 : n_terms;
   int64_t steps = 0;
+  q->a_blocks = terms[0].a.mn && M % 64 == 0, q->b_blocks = terms[0].b.mn && N % 64 == 0;
   for (int i = 0; i < 2; ++i) {
     const Term& t = terms[i < n_terms ? i : 0];
-    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows) || !encode(&q->b[i], bf16, t.b, N, t.k, b_rows))
+    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks) ||
+        !encode(&q->b[i], bf16, t.b, N, t.k, b_rows, q->b_blocks))
       return false;
     q->steps[i] = (int32_t)((t.k + kBK - 1) / kBK);
     if (i < q->terms) steps += q->steps[i];
