@@ -52,6 +52,7 @@ struct Problem {
   int32_t parts, part_steps;               // behind them are summed in parts
   int32_t stages, stage_bytes;
   int32_t a_bytes;                         // of A that a CTA copies a slice
+  int32_t kb;                              // a slice is kb * 64 wide
   int32_t a_blocks, b_blocks;              // whole blocks of 64: copied together
   int32_t dual;                            // B's halves are two factors: b[0] and b[1]
   int32_t* status;
@@ -125,7 +126,8 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
         : "memory");
 }
 
-// The blocks of 64 of a factor's own index that a slice has, in one copy.
+// The blocks of 64 of a factor's own index that a slice has, in one copy
+// (k contiguous: the slice's blocks of 64 k).
 template <int CG>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c1,
                                        int c2) {
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) {
       const int stages = p.stages;
       const uint32_t b_bytes = (uint32_t)(p.bn / CG) * 128;
-      const uint32_t tx = (uint32_t)(p.a_bytes + b_bytes) * CG;
+      const uint32_t tx = (uint32_t)(p.a_bytes + b_bytes) * CG * p.kb;
       int s = 0;
       uint32_t phase = 0;                  // of the ring's current turn
       int64_t slot = 0;
@@ -241,8 +243,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             break;
           }
           const int term = k >= p.steps[0] && p.terms > 1;
-          const int k0 = (k - (term ? p.steps[0] : 0)) * kBK;
-          const uint32_t sa = ring + s * p.stage_bytes, sb = sa + kABytes;
+          const int k0 = (k - (term ? p.steps[0] : 0)) * kBK * p.kb;
+          const uint32_t sa = ring + s * p.stage_bytes, sb = sa + kABytes * p.kb;
           const uint32_t bar =
               CG == 2 ? leader_addr(smem_u32(&sh->full[s])) : smem_u32(&sh->full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], tx);
@@ -251,13 +253,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           } else if constexpr (kAMN) {
             tma_2d<CG>(sa, &p.a[term], bar, m0, k0);
             tma_2d<CG>(sa + 8192, &p.a[term], bar, m0 + 64, k0);
+          } else if (p.a_blocks) {
+            tma_3d<CG>(sa, &p.a[term], bar, m0, k0 / 64);
           } else {
             tma_2d<CG>(sa, &p.a[term], bar, k0, m0);
           }
           if (p.dual) {
             const int half = p.bn / 2;
             if constexpr (CG == 2) {
-              tma_2d<CG>(sb, &p.b[rank], bar, k0, t.n * half);
+              if (p.b_blocks) tma_3d<CG>(sb, &p.b[rank], bar, t.n * half, k0 / 64);
+              else tma_2d<CG>(sb, &p.b[rank], bar, k0, t.n * half);
             } else {
               tma_2d<CG>(sb, &p.b[0], bar, k0, t.n * half);
               tma_2d<CG>(sb + half * 128, &p.b[1], bar, k0, t.n * half);
@@ -268,7 +273,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             else for (int c = 0; c < p.bn / CG; c += 64)
               tma_2d<CG>(sb + c * 128, &p.b[term], bar, n0 + c, k0);
           } else {
-            tma_2d<CG>(sb, &p.b[term], bar, k0, t.n * p.bn + (int)rank * (p.bn / CG));
+            const int n0 = t.n * p.bn + (int)rank * (p.bn / CG);
+            if (p.b_blocks) tma_3d<CG>(sb, &p.b[term], bar, n0, k0 / 64);
+            else tma_2d<CG>(sb, &p.b[term], bar, k0, n0);
           }
           if (++s == stages) s = 0, phase ^= 1;
         }
@@ -291,12 +298,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16_ab(Epi::kBf16, 128 * CG, p.bn, kAMN, kBMN);
       const int stages = p.stages;
-      // 64-wide blocks of rows of k: 8 KB from block to block, 2 KB a step of 16 k;
-      // rows of 64 k: 32 bytes a step
-      const uint64_t da0 = kAMN ? desc_sw128(ring, 8192, 1024) : desc_sw128(ring, 16, 1024);
-      const uint64_t db0 = kBMN ? desc_sw128(ring + kABytes, 8192, 1024)
-                                : desc_sw128(ring + kABytes, 16, 1024);
+      // 64-wide blocks of rows of k: 8 KB (kb times) from block to block, 2 KB a step of
+      // 16 k; rows of 64 k: 32 bytes a step, kb times all rows
+      const uint32_t rb = ring + kABytes * p.kb;
+      const uint64_t da0 = kAMN ? desc_sw128(ring, 8192 * p.kb, 1024) : desc_sw128(ring, 16, 1024);
+      const uint64_t db0 = kBMN ? desc_sw128(rb, 8192 * p.kb, 1024) : desc_sw128(rb, 16, 1024);
       constexpr uint64_t kStepA = (kAMN ? 2048 : 32) >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;
+      const uint64_t sub_a = (kAMN ? 8192 : kABytes) >> 4;
+      const uint64_t sub_b = (uint64_t)(kBMN ? 8192 : p.bn / CG * 128) >> 4;
       int s = 0, acc = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -316,10 +325,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           tc_fence_after();
           const uint64_t off = (uint64_t)((uint32_t)(s * p.stage_bytes) >> 4);
+          for (int sub = 0; sub < p.kb; ++sub) {
+            const uint64_t a = da0 + off + sub * sub_a, b = db0 + off + sub * sub_b;
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk)
-            mma_f16<CG>(d, da0 + off + kk * kStepA, db0 + off + kk * kStepB, idesc,
-                        k > t.begin || kk > 0);
+            for (int kk = 0; kk < kBK / 16; ++kk)
+              mma_f16<CG>(d, a + kk * kStepA, b + kk * kStepB, idesc,
+                          k > t.begin || sub > 0 || kk > 0);
+          }
           commit_all<CG>(&sh->empty[s]);
           if (++s == stages) s = 0, phase ^= 1;
         }
@@ -400,16 +412,19 @@ inline bool copyable(const Factor& f) {
   return (reinterpret_cast<uintptr_t>(f.p) & 15) == 0 && f.ld % 8 == 0;
 }
 
-// The map of a factor of `n` rows and k columns: boxes of 64 k by `rows`; where the
-// rows are contiguous, of 64 rows by 64 k, or (blocks) `rows` / 64 of these in one box.
+// The map of a factor of `n` rows and k columns: boxes of 64 k by `rows`, or (blocks) kb
+// of these in one box; where the rows are contiguous, of 64 rows by 64 k, or (blocks)
+// `rows` / 64 of 64 rows by kb * 64 k.  Only whole blocks can be copied together: what
+// lies outside is told by the first index otherwise.
 inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_t k, int rows,
-                   bool blocks) {
+                   bool blocks, int kb) {
   const EncodeTiledFn fn = encoder();
   if (!fn || !copyable(f)) return false;
   if (blocks) {
-    const cuuint64_t dims[3] = {64u, (cuuint64_t)k, (cuuint64_t)(n / 64)};
+    const cuuint64_t dims[3] = {64u, (cuuint64_t)(f.mn ? k : n), (cuuint64_t)((f.mn ? n : k) / 64)};
     const cuuint64_t strides[2] = {(cuuint64_t)f.ld * 2, 128u};
-    const cuuint32_t box[3] = {64u, 64u, (cuuint32_t)(rows / 64)};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)(f.mn ? 64 * kb : rows),
+                               (cuuint32_t)(f.mn ? rows / 64 : kb)};
     const cuuint32_t estr[3] = {1u, 1u, 1u};
     return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
               const_cast<void*>(f.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -484,13 +499,18 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   const int b_rows = dual ? bn / 2 : bn / cg;
   q->terms = dual ? 1 : n_terms;
   int64_t steps = 0;
-  q->a_blocks = terms[0].a.mn && M % 64 == 0, q->b_blocks = terms[0].b.mn && N % 64 == 0;
+  const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
+  bool k64 = true;                          // whole blocks of 64 k
+  for (int i = 0; i < n_terms; ++i) k64 &= terms[i].k % 64 == 0;
+  q->a_blocks = amn ? M % 64 == 0 : k64 && cg == 2, q->b_blocks = bmn ? N % 64 == 0 : k64 && cg == 2;
+  // slices of 128 where they can be copied at once: half the barriers and copies
+  q->kb = cg == 2 && q->a_blocks && q->b_blocks ? 2 : 1;
   for (int i = 0; i < 2; ++i) {
     const Term& t = terms[i < n_terms ? i : 0];
-    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks) ||
-        !encode(&q->b[i], bf16, t.b, N, t.k, b_rows, q->b_blocks))
+    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks, q->kb) ||
+        !encode(&q->b[i], bf16, t.b, N, t.k, b_rows, q->b_blocks, q->kb))
       return false;
-    q->steps[i] = (int32_t)((t.k + kBK - 1) / kBK);
+    q->steps[i] = (int32_t)((t.k + kBK * q->kb - 1) / (kBK * q->kb));
     if (i < q->terms) steps += q->steps[i];
   }
   q->M = (int32_t)M, q->N = (int32_t)N, q->bn = bn, q->dual = dual;
@@ -503,7 +523,7 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   q->whole = (int32_t)plan.whole;
   q->part_steps = (int32_t)((steps + plan.parts - 1) / plan.parts);
   q->parts = (int32_t)((steps + q->part_steps - 1) / q->part_steps);
-  q->stage_bytes = kABytes + bn / cg * 128;
+  q->stage_bytes = (kABytes + bn / cg * 128) * q->kb;
   q->stages = std::min(kMaxStages, kRingBytes / q->stage_bytes);
   q->a_bytes = terms[0].a.mn ? kABytes : a_rows * 128;
   q->status = status;
