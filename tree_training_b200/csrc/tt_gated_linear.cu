@@ -76,6 +76,22 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
   }
 }
 
+// The same for gradients of 16 bits (with exact quotients this pass is bound by their
+// instructions, not by its bytes).
+template <int A>
+__device__ __forceinline__ void act_grad_16(float g, float& a, float& d) {
+  if constexpr (A == kSilu || A == kGeluTanh) {
+    // s = 1 / (1 + exp(-z)), 1 - s = exp(-z) s; past -80 both are nothing beside 1
+    const float z = A == kSilu ? g : 2.f * kTanhA * (g + kTanhB * g * g * g);
+    const float e = __expf(-fmaxf(z, -80.f)), s = __fdividef(1.f, 1.f + e);
+    const float dz = A == kSilu ? 1.f : 2.f * kTanhA * (1.f + 3.f * kTanhB * g * g);
+    a = g * s;
+    d = s * (1.f + g * dz * (e * s));
+  } else {
+    act_grad<A>(g, a, d);
+  }
+}
+
 template <typename F>
 int dispatch_act(int act, F f) {
   switch (act) {
@@ -241,7 +257,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float a, d;
-        act_grad<A>(vg[i], a, d);
+        if constexpr (sizeof(T) == 4) act_grad<A>(vg[i], a, d);
+        else act_grad_16<A>(vg[i], a, d);
         const bool in = c + i < F;             // (what is kept past F is not written)
         vg[i] = in ? vd[i] * vu[i] * d : 0.f;
         vu[i] = in ? vd[i] * a : 0.f;
