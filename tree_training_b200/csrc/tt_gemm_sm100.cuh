@@ -248,34 +248,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t bar =
               CG == 2 ? leader_addr(smem_u32(&sh->full[s])) : smem_u32(&sh->full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], tx);
-          if (kAMN && p.a_blocks) {
-            tma_3d<CG>(sa, &p.a[term], bar, k0, m0 / 64);
+          // (blocks that cannot be copied together: one after another)
+          if (p.a_blocks) {
+            tma_3d<CG>(sa, &p.a[term], bar, kAMN ? k0 : m0, (kAMN ? m0 : k0) / 64);
           } else if constexpr (kAMN) {
-            tma_2d<CG>(sa, &p.a[term], bar, m0, k0);
-            tma_2d<CG>(sa + 8192, &p.a[term], bar, m0 + 64, k0);
-          } else if (p.a_blocks) {
-            tma_3d<CG>(sa, &p.a[term], bar, m0, k0 / 64);
+            for (int c = 0; c < 2; ++c)
+              tma_2d<CG>(sa + c * 8192 * p.kb, &p.a[term], bar, m0 + 64 * c, k0);
           } else {
-            tma_2d<CG>(sa, &p.a[term], bar, k0, m0);
+            for (int c = 0; c < p.kb; ++c)
+              tma_2d<CG>(sa + c * kABytes, &p.a[term], bar, k0 + 64 * c, m0);
           }
-          if (p.dual) {
-            const int half = p.bn / 2;
-            if constexpr (CG == 2) {
-              if (p.b_blocks) tma_3d<CG>(sb, &p.b[rank], bar, t.n * half, k0 / 64);
-              else tma_2d<CG>(sb, &p.b[rank], bar, k0, t.n * half);
-            } else {
-              tma_2d<CG>(sb, &p.b[0], bar, k0, t.n * half);
-              tma_2d<CG>(sb + half * 128, &p.b[1], bar, k0, t.n * half);
-            }
-          } else if constexpr (kBMN) {
-            const int n0 = t.n * p.bn + (int)rank * (p.bn / CG);
-            if (p.b_blocks) tma_3d<CG>(sb, &p.b[term], bar, k0, n0 / 64);
-            else for (int c = 0; c < p.bn / CG; c += 64)
-              tma_2d<CG>(sb + c * 128, &p.b[term], bar, n0 + c, k0);
+          const int n0 = p.dual ? t.n * (p.bn / 2) : t.n * p.bn + (int)rank * (p.bn / CG);
+          const int b_rows = p.bn / CG;
+          if (CG == 1 && p.dual) {
+            tma_2d<CG>(sb, &p.b[0], bar, k0, n0);
+            tma_2d<CG>(sb + b_rows / 2 * 128, &p.b[1], bar, k0, n0);
           } else {
-            const int n0 = t.n * p.bn + (int)rank * (p.bn / CG);
-            if (p.b_blocks) tma_3d<CG>(sb, &p.b[term], bar, n0, k0 / 64);
-            else tma_2d<CG>(sb, &p.b[term], bar, k0, n0);
+            const CUtensorMap* map = &p.b[p.dual ? rank : term];
+            if (p.b_blocks) {
+              tma_3d<CG>(sb, map, bar, kBMN ? k0 : n0, (kBMN ? n0 : k0) / 64);
+            } else if constexpr (kBMN) {
+              for (int c = 0; c < b_rows; c += 64)
+                tma_2d<CG>(sb + c * 128 * p.kb, map, bar, n0 + c, k0);
+            } else {
+              for (int c = 0; c < p.kb; ++c)
+                tma_2d<CG>(sb + c * b_rows * 128, map, bar, k0 + 64 * c, n0);
+            }
           }
           if (++s == stages) s = 0, phase ^= 1;
         }
@@ -433,7 +431,7 @@ inline bool encode(CUtensorMap* m, bool bf16, const Factor& f, int64_t n, int64_
   }
   const cuuint64_t dims[2] = {(cuuint64_t)(f.mn ? n : k), (cuuint64_t)(f.mn ? k : n)};
   const cuuint64_t strides[1] = {(cuuint64_t)f.ld * 2};
-  const cuuint32_t box[2] = {64u, (cuuint32_t)(f.mn ? 64 : rows)};
+  const cuuint32_t box[2] = {64u, (cuuint32_t)(f.mn ? 64 * kb : rows)};
   const cuuint32_t estr[2] = {1u, 1u};
   return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
             const_cast<void*>(f.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -503,8 +501,8 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   bool k64 = true;                          // whole blocks of 64 k
   for (int i = 0; i < n_terms; ++i) k64 &= terms[i].k % 64 == 0;
   q->a_blocks = amn ? M % 64 == 0 : k64 && cg == 2, q->b_blocks = bmn ? N % 64 == 0 : k64 && cg == 2;
-  // slices of 128 where they can be copied at once: half the barriers and copies
-  q->kb = cg == 2 && q->a_blocks && q->b_blocks ? 2 : 1;
+  // slices of 128 on pairs: half the barriers, and fewer copies where blocks go together
+  q->kb = cg == 2 ? 2 : 1;
   for (int i = 0; i < 2; ++i) {
     const Term& t = terms[i < n_terms ? i : 0];
     if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks, q->kb) ||
