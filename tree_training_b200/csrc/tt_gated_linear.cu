@@ -105,7 +105,7 @@ int dispatch_act(int act, F f) {
 
 template <bool kB, int A>
 struct GatedEpi {
-  static constexpr bool kBf16 = kB;
+  static constexpr bool kBf16 = kB, kChunks = false;
   struct Args {
     void* h;
     int64_t h_ld;

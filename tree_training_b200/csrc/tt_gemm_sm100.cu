@@ -7,7 +7,7 @@ namespace {
 
 template <bool kB>
 struct StoreEpi {
-  static constexpr bool kBf16 = kB;
+  static constexpr bool kBf16 = kB, kChunks = false;
   struct Args {
     void *c, *c2;
     int64_t ld;

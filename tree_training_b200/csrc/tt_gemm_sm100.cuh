@@ -6,7 +6,7 @@
 //
 // Persistent CTAs (pairs of CTAs for tall problems) over tiles of 128 (256) rows by
 // up to 256 columns.  Warp 0 feeds a ring of 64-wide slices of k by TMA, one thread
-// of warp 1 issues `tcgen05.mma` into one of two TMEM accumulators, warps 4 to 11
+// of warp 1 issues `tcgen05.mma` into one of two TMEM accumulators, warps 2 to 9
 // take the other through the epilogue meanwhile (with four of them the epilogue of the
 // gated product took longer than sums over 1,000 of k).
 //
@@ -38,8 +38,9 @@ constexpr int kBK = 64;                    // k of a slice: 128 bytes
 constexpr int kABytes = 128 * kBK * 2;     // of A in a slice
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 196608;         // of shared memory for the ring
-constexpr int kEpiWarps = 8;               // warps 4 to 11: two for each quarter of the lanes
-constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
+constexpr int kEpiWarps = 8;               // warps 2 to 9: two for each quarter of the lanes
+constexpr int kSumWarps = 16;              // of epilogues that sum in chunks
+constexpr int kChunk = 640;                // of k, a chunk
 
 struct Problem {
   CUtensorMap a[2], b[2];
@@ -195,8 +196,20 @@ __device__ __forceinline__ void tmem_give(uint32_t taddr) {
 // reads its columns c0 .. c0 + 31, c0 + 64 .. (c0: 0 or 32, another warp has the other
 // half); all 32 lanes of a warp call it.  block: 32 x 33 floats of shared memory of the
 // warp's own.
+//
+// An epilogue that sums in chunks (Epi::kChunks) adds up the accumulators of kChunk of k
+// each in registers instead: the tensor cores cut off what falls below an accumulator's
+// last bit at every 16 of k, always towards zero, and a logit over k = 2,560 comes out
+// 5e-7 of itself too small (loss off by 1.4e-6 of itself, 3.5e-7 in chunks).  Sixteen
+// warps have a row and 64 columns a thread: Epi::finish(args, problem, tile, row, c0,
+// values).
+template <typename Epi>
+constexpr int warps_of() { return Epi::kChunks ? kSumWarps : kEpiWarps; }
+template <typename Epi>
+constexpr int threads_of() { return 64 + 32 * warps_of<Epi>(); }
+
 template <int CG, bool kAMN, bool kBMN, typename Epi>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(threads_of<Epi>(), 1)
     gemm_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epi::Args ea) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Barriers* sh = reinterpret_cast<Barriers*>(smem_raw);
@@ -206,12 +219,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const volatile int32_t* abort_flag = &sh->abort;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kEpiWarps * CG);
+    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], warps_of<Epi>() * CG);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
   }
-  if (warp == 2) tmem_take<CG>(&sh->tmem);
+  if (warp == 1) tmem_take<CG>(&sh->tmem);
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_barrier();
@@ -307,33 +320,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       int s = 0, acc = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int i = first; i < items && ok; i += stride, ++acc) {
+      const int chunk = kChunk / (kBK * p.kb);
+      for (int i = first; i < items && ok; i += stride) {
         const TileAt t = tile_at(p, i);
-        const int buf = acc & 1;
-        if (acc >= 2 && !mbar_wait(&sh->acc_empty[buf], ((acc >> 1) - 1) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + buf * 256;
-        for (int k = t.begin; k < t.end; ++k) {
-          if (!mbar_wait(&sh->full[s], phase, abort_flag)) {
+        for (int from = t.begin, to; from < t.end && ok; from = to, ++acc) {
+          to = Epi::kChunks ? min(t.end, from + chunk) : t.end;
+          const int buf = acc & 1;
+          if (acc >= 2 && !mbar_wait(&sh->acc_empty[buf], ((acc >> 1) - 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t off = (uint64_t)((uint32_t)(s * p.stage_bytes) >> 4);
-          for (int sub = 0; sub < p.kb; ++sub) {
-            const uint64_t a = da0 + off + sub * sub_a, b = db0 + off + sub * sub_b;
+          const uint32_t d = tmem + buf * 256;
+          for (int k = from; k < to; ++k) {
+            if (!mbar_wait(&sh->full[s], phase, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t off = (uint64_t)((uint32_t)(s * p.stage_bytes) >> 4);
+            for (int sub = 0; sub < p.kb; ++sub) {
+              const uint64_t a = da0 + off + sub * sub_a, b = db0 + off + sub * sub_b;
 #pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk)
-              mma_f16<CG>(d, a + kk * kStepA, b + kk * kStepB, idesc,
-                          k > t.begin || sub > 0 || kk > 0);
+              for (int kk = 0; kk < kBK / 16; ++kk)
+                mma_f16<CG>(d, a + kk * kStepA, b + kk * kStepB, idesc,
+                            k > from || sub > 0 || kk > 0);
+            }
+            commit_all<CG>(&sh->empty[s]);
+            if (++s == stages) s = 0, phase ^= 1;
           }
-          commit_all<CG>(&sh->empty[s]);
-          if (++s == stages) s = 0, phase ^= 1;
+          if (ok) commit_all<CG>(&sh->acc_full[buf]);
         }
-        if (ok) commit_all<CG>(&sh->acc_full[buf]);
       }
       if (!ok) fail();
       // every MMA issued is done before the accumulators are given back
@@ -346,33 +363,62 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tc_commit(&sh->drain);
       mbar_wait(&sh->drain, 0, nullptr);
     }
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------ epilogue
     const int quad = warp & 3;
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-    float* block =
-        reinterpret_cast<float*>(smem_raw + 2048 + kRingBytes) + (warp - 4) * 32 * kStageRow;
     int acc = 0;
-    for (int i = first; i < items; i += stride, ++acc) {
-      const TileAt t = tile_at(p, i);
-      const int buf = acc & 1;
-      const bool ok = mbar_wait(&sh->acc_full[buf], (acc >> 1) & 1, abort_flag);
+    // the accumulator's turn: true once it is there, and back to the MMAs
+    auto take = [&]() {
+      const bool ok = mbar_wait(&sh->acc_full[acc & 1], (acc >> 1) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         fail();
-        break;
+        return false;
       }
       tc_fence_after();
-      const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
-      Epi::tile(ea, p, t, row, lane_addr + buf * 256, warp < 8 ? 0 : 32, block);
+      return true;
+    };
+    auto give = [&]() {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if constexpr (CG == 2)
           asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                           leader_addr(smem_u32(&sh->acc_empty[buf])))
+                           leader_addr(smem_u32(&sh->acc_empty[acc & 1])))
                        : "memory");
         else
-          mbar_arrive(&sh->acc_empty[buf]);
+          mbar_arrive(&sh->acc_empty[acc & 1]);
+      }
+      ++acc;
+    };
+    bool ok = true;
+    for (int i = first; i < items && ok; i += stride) {
+      const TileAt t = tile_at(p, i);
+      const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
+      if constexpr (Epi::kChunks) {
+        const int c0 = (warp - 2) / 4 * 64, chunk = kChunk / (kBK * p.kb);
+        float v[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = 0.f;
+#pragma unroll 1
+        for (int k = t.begin; k < t.end; k += chunk) {
+          if (!(ok = take())) break;
+#pragma unroll
+          for (int h = 0; h < 64; h += 16) {       // (as many as registers are left for)
+            float x[16];
+            tmem_ld16(lane_addr + (acc & 1) * 256 + c0 + h, x);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h + j] += x[j];
+          }
+          give();
+        }
+        if (ok) Epi::finish(ea, p, t, row, c0, v);
+      } else {
+        float* block =
+            reinterpret_cast<float*>(smem_raw + 2048 + kRingBytes) + (warp - 2) * 32 * kStageRow;
+        if (!(ok = take())) break;
+        Epi::tile(ea, p, t, row, lane_addr + (acc & 1) * 256, warp < 6 ? 0 : 32, block);
+        give();
       }
     }
   }
@@ -381,7 +427,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   __syncthreads();
   if constexpr (CG == 2) cluster_barrier();
   tc_fence_after();
-  if (warp == 2) tmem_give<CG>(tmem);
+  if (warp == 1) tmem_give<CG>(tmem);
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -537,7 +583,7 @@ int launch(const Problem& q, const typename Epi::Args& ea, cudaStream_t st) {
   const int64_t items = q.whole + ((int64_t)q.tiles_m * q.tiles_n - q.whole) * q.parts;
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)(std::min<int64_t>(items, vec::kSMs / CG) * CG));
-  c.blockDim = dim3(kGemmThreads);
+  c.blockDim = dim3(threads_of<Epi>());
   c.dynamicSmemBytes = kGemmSmem;
   c.stream = st;
   cudaLaunchAttribute attr[1];

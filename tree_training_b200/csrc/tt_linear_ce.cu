@@ -11,7 +11,7 @@
 // bound by the tensor cores, for few tokens by W's bytes.
 //
 // Forward, 16-bit: the product's epilogue reduces each row of a tile of logits to its
-// maximum and the sum of exp above it (16 bytes for 256 logits) and picks out the
+// maximum and the sum of exp above it (8 bytes for 64 logits) and picks out the
 // labels' logits; a second kernel joins the tiles in order.  Backward: by pieces of
 // the vocabulary, each formed again, turned into 16-bit dz by the epilogue, and
 // multiplied twice: dW's rows of the piece are complete, dx is summed up in fp32.
@@ -86,41 +86,34 @@ __device__ __forceinline__ void take(const float (&z)[N], float& m, float& s) {
 
 template <bool kB>
 struct LseEpi {
-  static constexpr bool kBf16 = kB;
+  static constexpr bool kBf16 = kB, kChunks = true;
   struct Args {
-    float2* part;                          // [tiles of n][2][T]
+    float2* part;                          // [tiles of n][4][T]
     Labels labels;
     float* picked;                         // [T][M]
     float scale;
   };
-  static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
-                                              const gemm::TileAt& t, int row, uint32_t acc, int c0,
-                                              float* block) {
-    const int n0 = t.n * p.bn, cols = min(p.bn, p.N - n0);
-    const bool live = row < p.M;
-    const int count = live ? a.labels.count[row] : 0;
-    const uint32_t mask = chunks_with_labels(a.labels, row, count, n0, cols);
+  static __device__ __forceinline__ void finish(const Args& a, const gemm::Problem& p,
+                                                const gemm::TileAt& t, int row, int c0,
+                                                float (&z)[64]) {
+    const int n0 = t.n * p.bn + c0, cols = min(64, min(p.bn, p.N - t.n * p.bn) - c0);
+    if (row >= p.M) return;
     float m = -INFINITY, s = 0.f;
-    for (int c = c0; c < cols; c += 64) {
-      float z[32];
-      __syncwarp();                          // (the load is the whole warp's)
-      sm100::tmem_ld32(acc + c, z);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) z[i] = c + i < cols ? z[i] * a.scale : -INFINITY;
-      take<32>(z, m, s);
-      if ((mask >> (c >> 5)) & 1)
-        for (int k = 0; k < count; ++k) {
-          const int2 l = a.labels.list[(int64_t)row * a.labels.M + k];
-          const int at = l.x - n0 - c;                 // (the tile may end in this chunk)
-          if (at < 0 || at >= min(32, cols - c)) continue;
-          float v = 0.f;
+    for (int i = 0; i < 64; ++i) z[i] = i < cols ? z[i] * a.scale : -INFINITY;
+    take<64>(z, m, s);
+    a.part[(int64_t)(4 * t.n + c0 / 64) * p.M + row] = make_float2(m, s);
+    const int count = a.labels.count[row];
+    for (int k = 0; k < count; ++k) {
+      const int2 l = a.labels.list[(int64_t)row * a.labels.M + k];
+      const int at = l.x - n0;
+      if (at < 0 || at >= cols) continue;
+      float v = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (at == i) v = z[i];
-          a.picked[(int64_t)row * a.labels.M + l.y] = v;
-        }
+      for (int i = 0; i < 64; ++i)
+        if (at == i) v = z[i];
+      a.picked[(int64_t)row * a.labels.M + l.y] = v;
     }
-    if (live) a.part[(int64_t)(2 * t.n + (c0 > 0)) * p.M + row] = make_float2(m, s);
   }
 };
 
@@ -219,7 +212,7 @@ __device__ __forceinline__ void gradient(const Grad& a, int64_t row, int count, 
 
 template <bool kB>
 struct GradEpi {
-  static constexpr bool kBf16 = kB;
+  static constexpr bool kBf16 = kB, kChunks = false;
   struct Args {
     Grad g;
     void *dz, *rest;                       // rest: what rounding took off dz, or null
@@ -382,7 +375,7 @@ int forward_16(const Shape& s, const void* x, int64_t x_ld, const void* w, int64
   const gemm::Term term{{x, x_ld, false}, {w, w_ld, false}, s.H};
   gemm::Problem q;
   if (!gemm::set_up(&q, plan, kB, s.T, s.V, &term, 1, false, status)) return TT_ERR_UNSUPPORTED;
-  *parts = 2 * q.tiles_n;
+  *parts = 4 * q.tiles_n;
   typename Epi::Args ea{part, l, picked, scale};
   return gemm::launch<false, false, Epi>(plan, q, ea, st);
 }
@@ -430,7 +423,7 @@ extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t
            round256(4 * T * P) + gemm::fp32_work(T, P, H);
   }
   const gemm::Plan p = forward_plan(T, H, V);
-  return base + round256(16 * T * ((V + p.bn - 1) / p.bn));
+  return base + round256(32 * T * ((V + p.bn - 1) / p.bn));
 }
 
 extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M,
