@@ -53,11 +53,14 @@ struct Problem {
   int32_t parts, part_steps;               // behind them are summed in parts
   int32_t stages, stage_bytes;
   int32_t a_bytes;                         // of A that a CTA copies a slice
-  int32_t kb;                              // a slice is kb * 64 wide
   int32_t a_blocks, b_blocks;              // whole blocks of 64: copied together
   int32_t dual;                            // B's halves are two factors: b[0] and b[1]
   int32_t* status;
 };
+
+// A slice is 64 of k wide, on pairs of CTAs 128: half the barriers, and fewer copies
+// where blocks of 64 go together (8,192 x 2,560 over k = 19,456: 535 us, 509).
+__host__ __device__ constexpr int blocks_of_k(int cg) { return cg; }
 
 struct TileAt {
   int unit, begin, end, m, n;              // unit: of a sum in parts (else -1)
@@ -146,6 +149,12 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uin
         : "memory");
 }
 
+__device__ __forceinline__ uint64_t low_plus(uint64_t desc, uint32_t n) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"((uint32_t)desc + n), "r"((uint32_t)(desc >> 32)));
+  return r;
+}
+
 template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -212,6 +221,7 @@ template <int CG, bool kAMN, bool kBMN, typename Epi>
 __global__ void __launch_bounds__(threads_of<Epi>(), 1)
     gemm_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epi::Args ea) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
+  constexpr int kKb = blocks_of_k(CG);
   Barriers* sh = reinterpret_cast<Barriers*>(smem_raw);
   const uint32_t ring = (smem_u32(smem_raw) + 1024 + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -242,7 +252,9 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
     if (lane == 0) {
       const int stages = p.stages;
       const uint32_t b_bytes = (uint32_t)(p.bn / CG) * 128;
-      const uint32_t tx = (uint32_t)(p.a_bytes + b_bytes) * CG * p.kb;
+      const uint32_t tx = (uint32_t)(p.a_bytes + b_bytes) * CG * kKb;
+      const uint32_t full0 = smem_u32(&sh->full[0]);
+      const uint32_t bar0 = CG == 2 ? leader_addr(full0) : full0;
       int s = 0;
       uint32_t phase = 0;                  // of the ring's current turn
       int64_t slot = 0;
@@ -256,19 +268,18 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
             break;
           }
           const int term = k >= p.steps[0] && p.terms > 1;
-          const int k0 = (k - (term ? p.steps[0] : 0)) * kBK * p.kb;
-          const uint32_t sa = ring + s * p.stage_bytes, sb = sa + kABytes * p.kb;
-          const uint32_t bar =
-              CG == 2 ? leader_addr(smem_u32(&sh->full[s])) : smem_u32(&sh->full[s]);
+          const int k0 = (k - (term ? p.steps[0] : 0)) * kBK * kKb;
+          const uint32_t sa = ring + s * p.stage_bytes, sb = sa + kABytes * kKb;
+          const uint32_t bar = bar0 + 8 * s;
           if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], tx);
           // (blocks that cannot be copied together: one after another)
           if (p.a_blocks) {
             tma_3d<CG>(sa, &p.a[term], bar, kAMN ? k0 : m0, (kAMN ? m0 : k0) / 64);
           } else if constexpr (kAMN) {
             for (int c = 0; c < 2; ++c)
-              tma_2d<CG>(sa + c * 8192 * p.kb, &p.a[term], bar, m0 + 64 * c, k0);
+              tma_2d<CG>(sa + c * 8192 * kKb, &p.a[term], bar, m0 + 64 * c, k0);
           } else {
-            for (int c = 0; c < p.kb; ++c)
+            for (int c = 0; c < kKb; ++c)
               tma_2d<CG>(sa + c * kABytes, &p.a[term], bar, k0 + 64 * c, m0);
           }
           const int n0 = p.dual ? t.n * (p.bn / 2) : t.n * p.bn + (int)rank * (p.bn / CG);
@@ -282,9 +293,9 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
               tma_3d<CG>(sb, map, bar, kBMN ? k0 : n0, (kBMN ? n0 : k0) / 64);
             } else if constexpr (kBMN) {
               for (int c = 0; c < b_rows; c += 64)
-                tma_2d<CG>(sb + c * 128 * p.kb, map, bar, n0 + c, k0);
+                tma_2d<CG>(sb + c * 128 * kKb, map, bar, n0 + c, k0);
             } else {
-              for (int c = 0; c < p.kb; ++c)
+              for (int c = 0; c < kKb; ++c)
                 tma_2d<CG>(sb + c * b_rows * 128, map, bar, k0 + 64 * c, n0);
             }
           }
@@ -309,18 +320,18 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16_ab(Epi::kBf16, 128 * CG, p.bn, kAMN, kBMN);
       const int stages = p.stages;
-      // 64-wide blocks of rows of k: 8 KB (kb times) from block to block, 2 KB a step of
-      // 16 k; rows of 64 k: 32 bytes a step, kb times all rows
-      const uint32_t rb = ring + kABytes * p.kb;
-      const uint64_t da0 = kAMN ? desc_sw128(ring, 8192 * p.kb, 1024) : desc_sw128(ring, 16, 1024);
-      const uint64_t db0 = kBMN ? desc_sw128(rb, 8192 * p.kb, 1024) : desc_sw128(rb, 16, 1024);
-      constexpr uint64_t kStepA = (kAMN ? 2048 : 32) >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;
-      const uint64_t sub_a = (kAMN ? 8192 : kABytes) >> 4;
-      const uint64_t sub_b = (uint64_t)(kBMN ? 8192 : p.bn / CG * 128) >> 4;
+      // 64-wide blocks of rows of k: 8 KB (kKb times) from block to block, 2 KB a step of
+      // 16 k; rows of 64 k: 32 bytes a step, kKb times all rows
+      const uint32_t rb = ring + kABytes * kKb;
+      const uint64_t da0 = kAMN ? desc_sw128(ring, 8192 * kKb, 1024) : desc_sw128(ring, 16, 1024);
+      const uint64_t db0 = kBMN ? desc_sw128(rb, 8192 * kKb, 1024) : desc_sw128(rb, 16, 1024);
+      constexpr uint32_t kStepA = (kAMN ? 2048 : 32) >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;
+      constexpr uint32_t sub_a = (kAMN ? 8192 : kABytes) >> 4;
+      const uint32_t sub_b = (uint32_t)(kBMN ? 8192 : p.bn / CG * 128) >> 4;
       int s = 0, acc = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const int chunk = kChunk / (kBK * p.kb);
+      const int chunk = kChunk / (kBK * kKb);
       for (int i = first; i < items && ok; i += stride) {
         const TileAt t = tile_at(p, i);
         for (int from = t.begin, to; from < t.end && ok; from = to, ++acc) {
@@ -338,14 +349,15 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
               break;
             }
             tc_fence_after();
-            const uint64_t off = (uint64_t)((uint32_t)(s * p.stage_bytes) >> 4);
-            for (int sub = 0; sub < p.kb; ++sub) {
-              const uint64_t a = da0 + off + sub * sub_a, b = db0 + off + sub * sub_b;
+            // (a descriptor's address is in its low word)
+            const uint32_t off = (uint32_t)(s * p.stage_bytes) >> 4;
+#pragma unroll
+            for (int sub = 0; sub < kKb; ++sub)
 #pragma unroll
               for (int kk = 0; kk < kBK / 16; ++kk)
-                mma_f16<CG>(d, a + kk * kStepA, b + kk * kStepB, idesc,
-                            k > from || sub > 0 || kk > 0);
-            }
+                mma_f16<CG>(d, low_plus(da0, off + sub * sub_a + kk * kStepA),
+                            low_plus(db0, off + sub * sub_b + kk * kStepB), idesc,
+                            sub > 0 || kk > 0 ? 1u : (uint32_t)(k > from));
             commit_all<CG>(&sh->empty[s]);
             if (++s == stages) s = 0, phase ^= 1;
           }
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
       const TileAt t = tile_at(p, i);
       const int row = t.m * 128 * CG + (int)rank * 128 + quad * 32 + lane;
       if constexpr (Epi::kChunks) {
-        const int c0 = (warp - 2) / 4 * 64, chunk = kChunk / (kBK * p.kb);
+        const int c0 = (warp - 2) / 4 * 64, chunk = kChunk / (kBK * kKb);
         float v[64];
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] = 0.f;
@@ -547,14 +559,13 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   bool k64 = true;                          // whole blocks of 64 k
   for (int i = 0; i < n_terms; ++i) k64 &= terms[i].k % 64 == 0;
   q->a_blocks = amn ? M % 64 == 0 : k64 && cg == 2, q->b_blocks = bmn ? N % 64 == 0 : k64 && cg == 2;
-  // slices of 128 on pairs: half the barriers, and fewer copies where blocks go together
-  q->kb = cg == 2 ? 2 : 1;
+  const int kb = blocks_of_k(cg);
   for (int i = 0; i < 2; ++i) {
     const Term& t = terms[i < n_terms ? i : 0];
-    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks, q->kb) ||
-        !encode(&q->b[i], bf16, t.b, N, t.k, b_rows, q->b_blocks, q->kb))
+    if (!encode(&q->a[i], bf16, t.a, M, t.k, a_rows, q->a_blocks, kb) ||
+        !encode(&q->b[i], bf16, t.b, N, t.k, b_rows, q->b_blocks, kb))
       return false;
-    q->steps[i] = (int32_t)((t.k + kBK * q->kb - 1) / (kBK * q->kb));
+    q->steps[i] = (int32_t)((t.k + kBK * kb - 1) / (kBK * kb));
     if (i < q->terms) steps += q->steps[i];
   }
   q->M = (int32_t)M, q->N = (int32_t)N, q->bn = bn, q->dual = dual;
@@ -567,7 +578,7 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   q->whole = (int32_t)plan.whole;
   q->part_steps = (int32_t)((steps + plan.parts - 1) / plan.parts);
   q->parts = (int32_t)((steps + q->part_steps - 1) / q->part_steps);
-  q->stage_bytes = (kABytes + bn / cg * 128) * q->kb;
+  q->stage_bytes = (kABytes + bn / cg * 128) * kb;
   q->stages = std::min(kMaxStages, kRingBytes / q->stage_bytes);
   q->a_bytes = terms[0].a.mn ? kABytes : a_rows * 128;
   q->status = status;
