@@ -226,3 +226,27 @@ def test_hf_modules():
     got = [mlp[0](x), *torch.autograd.grad(mlp[0](x), [x, *ps], dy)]
     for a, b in zip(got, want):          # fp32 on both sides: sums of up to 264 terms
         assert float((a - b).norm() / b.norm()) < 264 * EPS
+
+
+def test_modules_that_do_more_keep_their_forward():
+    class Block(torch.nn.Module):
+        def __init__(self, act, limit=None, bias=False):
+            super().__init__()
+            self.gate_proj = torch.nn.Linear(32, 48, bias=bias)
+            self.up_proj = torch.nn.Linear(32, 48, bias=False)
+            self.down_proj = torch.nn.Linear(48, 32)
+            self.act_fn, self.limit = act, limit
+
+        def forward(self, x):
+            h = self.act_fn(self.gate_proj(x)) * self.up_proj(x)
+            return self.down_proj(h if self.limit is None else h.clamp(max=self.limit))
+    torch.manual_seed(1)
+    m = torch.nn.ModuleList([Block(torch.nn.SiLU()), Block(torch.nn.SiLU(), 0.01),
+                             Block(torch.nn.Tanh()), Block(torch.nn.SiLU(), bias=True),
+                             Block(torch.nn.GELU(approximate="tanh")), Block(torch.nn.GELU()),
+                             Block(torch.nn.ReLU())]).to(DEV)
+    x = torch.randn(5, 32, device=DEV)
+    want = [b(x) for b in m]
+    assert tt.fuse_gated_mlps(m) == 4
+    for b, w in zip(m, want):
+        assert float((b(x) - w).norm() / w.norm()) < 100 * EPS

@@ -412,6 +412,9 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, double 
       type_error("clip_grad_norm: norm must be one float32");
     given = *norm_;
   }
+  // what is written has a new version: autograd refuses what it saved of it (and
+  // inference tensors are not written outside inference mode)
+  for (const Tensor& t : outs) t.unsafeGetTensorImpl()->bump_version();
   On on(grads[0]);
   const int64_t size = tt_grad_norm_workspace_size(src.count());
   const Tensor ws = bytes(size, grads[0]);
@@ -420,8 +423,6 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, double 
                                  src.data.data(), dst.data.data(), norm_type,
                                  (const float*)ptr(given), (float)max_norm, (float)eps,
                                  (float*)out(norm), out(ws), size, on.stream));
-  // what was written has a new version: autograd refuses what it saved of it
-  for (const Tensor& t : outs) t.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

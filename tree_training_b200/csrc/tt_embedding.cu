@@ -509,7 +509,7 @@ int sort_blocks(int64_t n, int digits) {
 int64_t round16(int64_t b) { return (b + 15) / 16 * 16; }
 
 bool ok_sizes(int64_t n, int64_t V, int H) {
-  return n >= 0 && n <= 0x7fffffff && V >= 1 && V <= 0x7fffffff && H >= 1;
+  return n >= 0 && n <= 0x7fffffff && V >= 1 && V <= 0x7fffffff && H >= 1 && H <= (1 << 30);
 }
 
 }  // namespace

@@ -25,6 +25,7 @@ struct Args {
   int64_t a_ld[2], b_ld[2], k[2];
   int M, N, terms;                         // terms of one sum, or (batch) of one each
   int batch;
+  uint32_t tiles_n;
   int vec_a, vec_b, vec_c;                 // 16-byte loads and stores allowed
   int parts;
   int64_t k_part;                          // of k, a block's share (all: the sum of k)
@@ -89,9 +90,10 @@ __global__ void __launch_bounds__(kThreads, 2) product_kernel(const Args a) {
   constexpr int EM = SM / 16, EN = SN / 16, RA = SM + 4, RB = SN + 4;
   __shared__ __align__(16) float sa[2][kK * RA];
   __shared__ __align__(16) float sb[2][kK * RB];
-  const int64_t i0 = (int64_t)blockIdx.y * SM, j0 = (int64_t)blockIdx.x * SN;
+  const int64_t i0 = (int64_t)(blockIdx.x / a.tiles_n) * SM;
+  const int64_t j0 = (int64_t)(blockIdx.x % a.tiles_n) * SN;
   const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
-  const int part = blockIdx.z % a.parts, which = blockIdx.z / a.parts;
+  const int part = blockIdx.y % a.parts, which = blockIdx.y / a.parts;
   float2 acc[EM][EN / 2];
 #pragma unroll
   for (int i = 0; i < EM; ++i)
@@ -269,8 +271,9 @@ int run(int64_t M, int64_t N, const Term* terms, int n_terms, const Result* r, i
   a.vec_c = a.c_ld % 4 == 0 && a.c_part % 4 == 0;
   for (int i = 0; i < batch; ++i) a.vec_c &= (reinterpret_cast<uintptr_t>(a.c[i]) & 15) == 0;
   const int64_t rows = (M + f.rows - 1) / f.rows, cols = (N + f.cols - 1) / f.cols;
-  if (rows > 65535) return TT_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)cols, (unsigned)rows, (unsigned)(a.parts * batch));
+  if (rows * cols > 0x7fffffff) return TT_ERR_UNSUPPORTED;
+  a.tiles_n = (uint32_t)cols;
+  const dim3 grid((unsigned)(rows * cols), (unsigned)(a.parts * batch));
   const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
   const int rc = f.rows == 128   ? launch_product<128, 128>(a, grid, amn, bmn, st)
                  : f.cols == 128 ? launch_product<64, 128>(a, grid, amn, bmn, st)

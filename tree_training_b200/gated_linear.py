@@ -35,13 +35,23 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
 
 def _activation_of(fn):
     """The name of a module's activation, None where it is not one of these."""
-    if isinstance(fn, torch.nn.SiLU) or type(fn).__name__ == "SiLUActivation":
-        return "silu"
-    if isinstance(fn, torch.nn.ReLU):
-        return "relu"
     if isinstance(fn, torch.nn.GELU):
         return "gelu_tanh" if fn.approximate == "tanh" else "gelu"
-    return None
+    return {"SiLU": "silu", "SiLUActivation": "silu", "ReLU": "relu", "GELUActivation": "gelu",
+            "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"}.get(type(fn).__name__)
+
+
+@torch.no_grad()
+def _is_plain(mod) -> bool:
+    """Whether the module's forward is down(act(gate(x)) * up(x)) and nothing else
+    (no dropout, sparsity or clamp), by what it gives for a few rows."""
+    w = mod.gate_proj.weight
+    x = torch.linspace(-3, 3, 4 * w.shape[1], dtype=torch.float32).view(4, -1).sin()
+    x = x.to(w.device, w.dtype)
+    y = mod.forward(x)
+    want = mod.down_proj(mod.act_fn(mod.gate_proj(x)) * mod.up_proj(x))
+    return isinstance(y, torch.Tensor) and y.shape == want.shape and \
+        torch.allclose(y.float(), want.float(), rtol=2e-2, atol=1e-3 * float(want.abs().max()))
 
 
 def _gated_mlp_forward(self, x):
@@ -53,14 +63,15 @@ def fuse_gated_mlps(model) -> int:
     """Routes every gated feed-forward module of an HF model (``gate_proj``,
     ``up_proj`` and ``down_proj`` without biases, ``act_fn`` one of the activations)
     through :func:`gated_linear`.  Returns how many modules were patched; modules
-    of another form keep their own forward."""
+    of another form (or whose forward does more than that) keep their own forward."""
     n = 0
     for mod in model.modules():
         parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
         if not all(type(p) is torch.nn.Linear for p in parts) or not hasattr(mod, "act_fn"):
             continue
         name = _activation_of(mod.act_fn)
-        if name is None or parts[0].bias is not None or parts[1].bias is not None:
+        if name is None or parts[0].bias is not None or parts[1].bias is not None \
+                or not _is_plain(mod):
             continue
         mod._tt_activation = name
         mod.forward = types.MethodType(_gated_mlp_forward, mod)
