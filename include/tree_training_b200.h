@@ -615,19 +615,23 @@ int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* 
 /* ---- cross entropy of an LM head without its logits --------------------------- *
  * z = scale * x w^T (x [T, H], w [V, H]); lse[t] = log sum exp z[t]; losses[t, m] =
  * lse[t] - z[t, labels[t, m]], 0 for labels (int64 [T, M]) outside [0, V).  16-bit
- * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED). */
+ * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED).  kept (null, or
+ * [T][tt_linear_ce_kept_ld] fp32 where that is not 0) takes the logits for the
+ * backward, which forms them again without it. */
+int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int64_t V);
 int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
 int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
                      int64_t x_ld, const void* w, int64_t w_ld, const int64_t* labels, float scale,
-                     float* losses, float* lse, void* workspace, int64_t workspace_bytes,
-                     int32_t* status, void* stream);
+                     float* losses, float* lse, float* kept, void* workspace,
+                     int64_t workspace_bytes, int32_t* status, void* stream);
 /* dx [T, H], dw [V, H], contiguous; null: not wanted.  g_loss [T, M], g_lse [T]
  * (null: zeros) are the gradients of losses and lse. */
 int64_t tt_linear_ce_bwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
 int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
                      int64_t x_ld, const void* w, int64_t w_ld, const int64_t* labels, float scale,
-                     const float* lse, const float* g_loss, const float* g_lse, void* dx, void* dw,
-                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+                     const float* lse, const float* kept, const float* g_loss, const float* g_lse,
+                     void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                     int32_t* status, void* stream);
 
 /* ---- the norm of many tensors ---------------------------------------------------- *
  * dtypes, sizes (elements) and tensors are host arrays of `count`.  norm_type 1, 2

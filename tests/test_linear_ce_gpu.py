@@ -208,6 +208,16 @@ def test_same_bits_another_stream_and_replay():
     assert all(torch.equal(a, b) for a, b in zip(step(), got))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_backward_twice(dtype):
+    x, w, labels, gl, ge = make(70, 64, 500, 2, dtype, 12)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    r = tt.linear_cross_entropy(*leaves, labels)
+    one = torch.autograd.grad([r.losses, r.lse], leaves, [gl, ge], retain_graph=True)
+    two = torch.autograd.grad([r.losses, r.lse], leaves, [gl, ge])
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
 def test_refusals():
     x, w, labels, _, _ = make(4, 16, 24, 1, BF)
     for bad in ((x[0], w, labels), (x, w[:, :8], labels), (x, w, labels[:3]),

@@ -104,20 +104,20 @@ def test_gated_linear_types_and_workspace():
 
 
 def ce(dtype=BF16, T=4, H=16, V=100, M=1, x=P, x_ld=16, w=P, w_ld=16, labels=P, losses=P, lse=P,
-       ws=P, size=BIG):
+       kept=None, ws=P, size=BIG):
     return status("tt_linear_ce_fwd", dtype, T, H, V, M, x, x_ld, w, w_ld, labels, 1.0, losses, lse,
-                  ws, size, None, None)
+                  kept, ws, size, None, None)
 
 
-def ce_bwd(dtype=BF16, T=4, H=16, V=100, M=1, x=P, x_ld=16, w=P, w_ld=16, labels=P, lse=P, ws=P,
-           size=BIG):
-    return status("tt_linear_ce_bwd", dtype, T, H, V, M, x, x_ld, w, w_ld, labels, 1.0, lse, P, P, P,
-                  P, ws, size, None, None)
+def ce_bwd(dtype=BF16, T=4, H=16, V=100, M=1, x=P, x_ld=16, w=P, w_ld=16, labels=P, lse=P,
+           kept=None, ws=P, size=BIG):
+    return status("tt_linear_ce_bwd", dtype, T, H, V, M, x, x_ld, w, w_ld, labels, 1.0, lse, kept, P,
+                  P, P, P, ws, size, None, None)
 
 
 BAD_CE = [dict(T=-1), dict(T=1 << 31), dict(H=0), dict(V=0), dict(V=1 << 31), dict(M=-1),
           dict(M=1 << 31), dict(x_ld=15), dict(w_ld=15), dict(x=None), dict(w=None),
-          dict(labels=None), dict(lse=None)]
+          dict(labels=None), dict(lse=None), dict(kept=P)]
 
 
 @pytest.mark.parametrize("bad", BAD_CE + [dict(losses=None)])
@@ -128,6 +128,13 @@ def test_linear_ce(bad):
 @pytest.mark.parametrize("bad", BAD_CE)
 def test_linear_ce_gradient(bad):
     assert ce_bwd(**bad) == INVALID
+
+
+def test_linear_ce_kept_logits():
+    f = lambda *a: status("tt_linear_ce_kept_ld", *a)
+    assert f(F32, 47, 1001) == 1008 and f(BF16, 47, 1001) == 0 and f(F32, 0, 1001) == 0
+    assert f(F32, 1 << 20, 4096) == 0 and f(F32, 4096, 16384) == 16384 and f(F32, 4097, 16384) == 0
+    assert f(F32, -1, 10) == 0 and f(F32, 10, 0) == 0
 
 
 def test_linear_ce_types_and_workspace():

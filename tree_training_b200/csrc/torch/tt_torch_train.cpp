@@ -212,10 +212,15 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
 
 // ---- the LM head's loss ------------------------------------------------------------------
 
-std::pair<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels,
-                                     double scale) {
+struct CE {
+  Tensor losses, lse, kept;
+};
+
+CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double scale, bool keep) {
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
-  Tensor losses = empty({T, M}, x, at::kFloat), lse = empty({T}, x, at::kFloat);
+  CE r{empty({T, M}, x, at::kFloat), empty({T}, x, at::kFloat), Tensor()};
+  const int64_t ld = keep ? tt_linear_ce_kept_ld(dtype_code(x), T, V) : 0;
+  if (ld) r.kept = empty({T, ld}, x, at::kFloat);
   int32_t* status = status_of(x);
   On on(x);
   const int64_t size = tt_linear_ce_fwd_workspace_size(dtype_code(x), T, (int32_t)H, V, M);
@@ -223,28 +228,28 @@ std::pair<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Ten
   check_status("tt_linear_ce_fwd",
                tt_linear_ce_fwd(dtype_code(x), T, (int32_t)H, V, M, ptr(x), ld_of(x), ptr(w),
                                 ld_of(w), (const int64_t*)ptr(labels), (float)scale,
-                                (float*)out(losses), (float*)out(lse), out(ws), size, status,
-                                on.stream));
-  return {losses, lse};
+                                (float*)out(r.losses), (float*)out(r.lse), (float*)out(r.kept),
+                                out(ws), size, status, on.stream));
+  return r;
 }
 
 struct LinearCEFunction : Function<LinearCEFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
                                const Tensor& labels, double scale) {
     const Tensor x2 = rows16(x), w2 = rows16(w);
-    auto r = ce_forward(x2, w2, labels, scale);
+    CE r = ce_forward(x2, w2, labels, scale, true);
     // (with odd widths the copies that were made)
-    ctx->save_for_backward({x2, w2, labels, r.second});
+    ctx->save_for_backward({x2, w2, labels, r.lse, r.kept});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
-    return {r.first, r.second};
+    return {r.losses, r.lse};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     variable_list grads(4);
     if (!g[0].defined() && !g[1].defined()) return grads;
     no_tangent("linear_cross_entropy", {&g[0], &g[1]});
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &labels = s[2], &lse = s[3];
+    const Tensor &x = s[0], &w = s[1], &labels = s[2], &lse = s[3], &kept = s[4];
     const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
     for (int i = 0; i < 2; ++i)
       if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();
@@ -264,8 +269,8 @@ struct LinearCEFunction : Function<LinearCEFunction> {
                    tt_linear_ce_bwd(dtype_code(x), T, (int32_t)H, V, M, ptr(x), ld_of(x), ptr(w),
                                     ld_of(w), (const int64_t*)ptr(labels),
                                     (float)ctx->saved_data["scale"].toDouble(),
-                                    (const float*)ptr(lse), (const float*)ptr(g[0]),
-                                    (const float*)ptr(g[1]), out(dx), out(dw), out(ws), size,
+                                    (const float*)ptr(lse), (const float*)ptr(kept),
+                                    (const float*)ptr(g[0]), (const float*)ptr(g[1]), out(dx), out(dw), out(ws), size,
                                     status, on.stream));
     }
     return once("linear_cross_entropy", {dx, dw, Tensor(), Tensor()});
@@ -301,8 +306,8 @@ std::tuple<Tensor, Tensor> linear_cross_entropy(const Tensor& x_, const Tensor& 
     variable_list v = LinearCEFunction::apply(x_, w, labels, scale);
     losses = v[0], lse = v[1];
   } else {
-    auto r = ce_forward(rows16(x_), rows16(w), labels, scale);
-    losses = r.first, lse = r.second;
+    CE r = ce_forward(rows16(x_), rows16(w), labels, scale, false);
+    losses = r.losses, lse = r.lse;
   }
   if (labels_.dim() == 1) losses = losses.squeeze(1);
   return {losses, lse};

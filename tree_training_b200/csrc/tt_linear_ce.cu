@@ -27,7 +27,8 @@
 // 1 / T lie below fp16's smallest number.
 //
 // fp32: the same steps with products on the CUDA cores and passes over the logits
-// of a piece.
+// of a piece.  Where one piece holds all logits (a quarter of a gigabyte at most) the
+// forward leaves them for the backward, whose fourth product would cost a third more.
 #include <cfloat>
 
 #include "tt_gemm_sm100.cuh"
@@ -279,15 +280,17 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dz in place of the logits of a piece.
+// dz out of the logits of a piece (which it may replace).
 __global__ void __launch_bounds__(256)
-    grad_kernel(float* z, int64_t T, int n, int64_t ld, int segment, const Grad g) {
+    grad_kernel(const float* z, int64_t z_ld, float* dz, int64_t T, int n, int64_t ld, int segment,
+                const Grad g) {
   const int c0 = blockIdx.y * segment, c1 = min(n, c0 + segment);
   for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
     const int count = g.labels.count[t];
     const float w = g.weight[t], lse = g.lse[t];
-    float* row = z + t * ld;
-    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) row[c] = w * expf(row[c] - lse);
+    const float* from = z + t * z_ld;
+    float* row = dz + t * ld;
+    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) row[c] = w * expf(from[c] - lse);
     __syncthreads();
     // (one thread: a label may be given twice)
     if (threadIdx.x == 0 && g.g_loss)
@@ -322,13 +325,22 @@ constexpr int64_t kTwoTermRows = 256;      // see the top
 
 bool two_terms(int dtype, int64_t T) { return dtype != TT_F32 && T <= kTwoTermRows; }
 
+constexpr int64_t kPieceBytes = (int64_t)1 << 28;
+
 // Bytes of dz (of fp32 logits) an element.
 int64_t dz_size(int dtype, int64_t T) { return dtype == TT_F32 || two_terms(dtype, T) ? 4 : 2; }
 
 // Columns of a piece of the vocabulary: a quarter of a gigabyte of dz, at least 4,096.
 int64_t piece_of(int dtype, int64_t T, int64_t V) {
-  const int64_t wide = ((int64_t)1 << 28) / (dz_size(dtype, T) * std::max<int64_t>(T, 1));
+  const int64_t wide = kPieceBytes / (dz_size(dtype, T) * std::max<int64_t>(T, 1));
   return std::min((V + 255) / 256 * 256, std::max<int64_t>(4096, wide / 256 * 256));
+}
+
+// The row stride of the logits that the forward leaves for the backward; 0: none.
+int64_t kept_ld(int dtype, int64_t T, int64_t V) {
+  const int64_t ld = (V + 7) / 8 * 8;
+  return dtype == TT_F32 && T > 0 && T * ld * 4 <= kPieceBytes && piece_of(dtype, T, V) >= V ? ld
+                                                                                             : 0;
 }
 
 int64_t labels_bytes(int64_t T, int64_t M) { return round256(4 * T) + round256(8 * T * M); }
@@ -412,6 +424,10 @@ const char* row_of(const Shape& s, const void* w, int64_t w_ld, int64_t v) {
 using namespace tt;
 using namespace tt::linear_ce;
 
+extern "C" int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int64_t V) {
+  return sizes_ok(T, 1, V, 0) ? kept_ld(dtype, T, V) : 0;
+}
+
 extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V,
                                                    int64_t M) {
   if (!sizes_ok(T, H, V, M) || dtype < TT_F32 || dtype > TT_F16) return 0;
@@ -429,12 +445,12 @@ extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t
 extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M,
                                 const void* x, int64_t x_ld, const void* w, int64_t w_ld,
                                 const int64_t* labels, float scale, float* losses, float* lse,
-                                void* workspace, int64_t workspace_bytes, int32_t* status,
-                                void* stream) {
+                                float* kept, void* workspace, int64_t workspace_bytes,
+                                int32_t* status, void* stream) {
   const Shape s{dtype, T, H, V, M};
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
-  if (!lse || (M > 0 && !losses)) return TT_ERR_INVALID_ARG;
+  if (!lse || (M > 0 && !losses) || (kept && !kept_ld(dtype, T, V))) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_fwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -447,16 +463,18 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
     const int64_t P = piece_of(dtype, T, V), segments = segments_of(T, P);
     part = ws.take<float2>(8 * T * segments * ((V + P - 1) / P));
     parts = 0;
-    float* z = ws.take<float>(4 * T * P);
+    float* room = ws.take<float>(4 * T * P);
+    float* z = kept ? kept : room;
+    const int64_t ld = kept ? kept_ld(dtype, T, V) : P;
     for (int64_t v0 = 0; v0 < V; v0 += P) {
       const int64_t n = std::min(P, V - v0);
       const gemm::Term term{{x, x_ld, false}, {row_of(s, w, w_ld, v0), w_ld, false}, H};
-      const gemm::Result r{TT_F32, z, P, nullptr, 0, scale, nullptr};
+      const gemm::Result r{TT_F32, z, ld, nullptr, 0, scale, nullptr};
       if ((rc = gemm::fp32_product(T, n, &term, 1, r, ws.p, gemm::fp32_work(T, P, H), st)))
         return rc;
       // (the last piece may have fewer of them)
       const int segment = segment_of(T, P), here = (int)((n + segment - 1) / segment);
-      lse_kernel<<<dim3(row_blocks(T), here), 256, 0, st>>>(z, T, v0, (int)n, P, segment, l,
+      lse_kernel<<<dim3(row_blocks(T), here), 256, 0, st>>>(z, T, v0, (int)n, ld, segment, l,
                                                             part + (int64_t)parts * T, picked);
       parts += here;
       tt_count_launches(1);
@@ -499,13 +517,13 @@ extern "C" int64_t tt_linear_ce_bwd_workspace_size(int dtype, int64_t T, int32_t
 extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M,
                                 const void* x, int64_t x_ld, const void* w, int64_t w_ld,
                                 const int64_t* labels, float scale, const float* lse,
-                                const float* g_loss, const float* g_lse, void* dx, void* dw,
+                                const float* kept, const float* g_loss, const float* g_lse, void* dx, void* dw,
                                 void* workspace, int64_t workspace_bytes, int32_t* status,
                                 void* stream) {
   const Shape s{dtype, T, H, V, M};
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
-  if (!lse) return TT_ERR_INVALID_ARG;
+  if (!lse || (kept && !kept_ld(dtype, T, V))) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_bwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -548,11 +566,13 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
     g.v0 = v0;
     if (f32) {
       const gemm::Term term{{x, x_ld, false}, {wp, w_ld, false}, H};
-      if ((rc = product(T, n, term, gemm::Result{TT_F32, dz, P, nullptr, 0, scale, nullptr})))
+      if (!kept &&
+          (rc = product(T, n, term, gemm::Result{TT_F32, dz, P, nullptr, 0, scale, nullptr})))
         return rc;
       const int segment = segment_of(T, P);
       grad_kernel<<<dim3(row_blocks(T), (unsigned)((n + segment - 1) / segment)), 256, 0, st>>>(
-          (float*)dz, T, (int)n, P, segment, g);
+          kept ? kept : (const float*)dz, kept ? kept_ld(dtype, T, V) : P, (float*)dz, T, (int)n, P,
+          segment, g);
       tt_count_launches(1);
     } else {
       rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st)
