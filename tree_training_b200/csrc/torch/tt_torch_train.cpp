@@ -216,9 +216,12 @@ struct CE {
   Tensor losses, lse, kept;
 };
 
-CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double scale, bool keep) {
+// (flat: losses [T] of one label a row)
+CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double scale, bool flat,
+              bool keep) {
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
-  CE r{empty({T, M}, x, at::kFloat), empty({T}, x, at::kFloat), Tensor()};
+  CE r{flat ? empty({T}, x, at::kFloat) : empty({T, M}, x, at::kFloat),
+       empty({T}, x, at::kFloat), Tensor()};
   const int64_t ld = keep ? tt_linear_ce_kept_ld(dtype_code(x), T, V) : 0;
   if (ld) r.kept = empty({T, ld}, x, at::kFloat);
   int32_t* status = status_of(x);
@@ -235,9 +238,9 @@ CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double sca
 
 struct LinearCEFunction : Function<LinearCEFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
-                               const Tensor& labels, double scale) {
+                               const Tensor& labels, double scale, bool flat) {
     const Tensor x2 = rows16(x), w2 = rows16(w);
-    CE r = ce_forward(x2, w2, labels, scale, true);
+    CE r = ce_forward(x2, w2, labels, scale, flat, true);
     // (with odd widths the copies that were made)
     ctx->save_for_backward({x2, w2, labels, r.lse, r.kept});
     ctx->saved_data["scale"] = scale;
@@ -245,7 +248,7 @@ struct LinearCEFunction : Function<LinearCEFunction> {
     return {r.losses, r.lse};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list grads(4);
+    variable_list grads(5);
     if (!g[0].defined() && !g[1].defined()) return grads;
     no_tangent("linear_cross_entropy", {&g[0], &g[1]});
     const variable_list s = ctx->get_saved_variables();
@@ -273,7 +276,7 @@ struct LinearCEFunction : Function<LinearCEFunction> {
                                     (const float*)ptr(g[0]), (const float*)ptr(g[1]), out(dx), out(dw), out(ws), size,
                                     status, on.stream));
     }
-    return once("linear_cross_entropy", {dx, dw, Tensor(), Tensor()});
+    return once("linear_cross_entropy", {dx, dw, Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -303,13 +306,12 @@ std::tuple<Tensor, Tensor> linear_cross_entropy(const Tensor& x_, const Tensor& 
   no_tangent(op, {&x_, &w});
   Tensor losses, lse;
   if (wants_grad({&x_, &w})) {
-    variable_list v = LinearCEFunction::apply(x_, w, labels, scale);
+    variable_list v = LinearCEFunction::apply(x_, w, labels, scale, labels_.dim() == 1);
     losses = v[0], lse = v[1];
   } else {
-    CE r = ce_forward(rows16(x_), rows16(w), labels, scale, false);
+    CE r = ce_forward(rows16(x_), rows16(w), labels, scale, labels_.dim() == 1, false);
     losses = r.losses, lse = r.lse;
   }
-  if (labels_.dim() == 1) losses = losses.squeeze(1);
   return {losses, lse};
 }
 

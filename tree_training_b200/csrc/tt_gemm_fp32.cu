@@ -217,7 +217,7 @@ Form form_of(int64_t M, int64_t N, int64_t k, int batch, bool split) {
     const int64_t tiles = ((M + f[0] - 1) / f[0]) * ((N + f[1] - 1) / f[1]) * batch;
     const int64_t most =
         split ? std::max<int64_t>(1, std::min<int64_t>(k / 64, 4 * vec::kSMs / tiles)) : 1;
-    for (int64_t parts = 1; parts <= most; ++parts) {
+    for (int64_t parts = 1; parts <= most; parts = next_parts(parts, most)) {
       const double slices = (double)((k + parts - 1) / parts + kK - 1) / kK;
       double t = (double)((tiles * parts + vec::kSMs - 1) / vec::kSMs) * slices * f[2] + 1500;
       if (parts > 1) t += 5000 + (double)(parts + 1) * batch * M * N * 4 / 1500;

@@ -528,7 +528,7 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool d
       const int64_t tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + cols - 1) / cols);
       const int64_t rest = tiles % slots, most = rest && split ? std::min(slots / rest, steps / 8) : 1;
       const double clocks = (double)slice_clocks(cg, bn);
-      for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); ++parts) {
+      for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); parts = next_parts(parts, most)) {
         // (a tile's start and end, which nothing hides: 600 clocks; the parts' way
         // through L2 and the launch that adds them up)
         const int64_t whole = parts > 1 ? tiles - rest : tiles;

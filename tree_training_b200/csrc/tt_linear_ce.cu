@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 
 // ---- backward ------------------------------------------------------------------------
 
-// The weight of a row's probabilities, and the largest weight of all (as bits).
+// The weight of a row's probabilities, and (fp16) the largest weight of all, as bits.
 __global__ void __launch_bounds__(256)
     weights_kernel(const Labels l, int64_t T, const float* g_loss, const float* g_lse, float scale,
                    float* weight, uint32_t* largest) {
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256)
     most *= fabsf(scale);
   }
   for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if ((threadIdx.x & 31) == 0 && most > 0.f) atomicMax(largest, __float_as_uint(most));
+  if (largest && (threadIdx.x & 31) == 0 && most > 0.f) atomicMax(largest, __float_as_uint(most));
 }
 
 // The power of two that fp16's dz is multiplied by, and one over it.
@@ -541,12 +541,13 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   float* sum = P < V ? ws.take<float>(4 * T * H) : nullptr;
   void* work = ws.p;
   const int64_t work_bytes = product_work(dtype, T, H, P);
-  if (cudaMemsetAsync(largest, 0, 4, st) != cudaSuccess) return TT_ERR_CUDA;
+  const bool f16 = dtype == TT_F16;
+  if (f16 && cudaMemsetAsync(largest, 0, 4, st) != cudaSuccess) return TT_ERR_CUDA;
   weights_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(g.labels, T, g_loss, g_lse, scale,
-                                                              weight, largest);
+                                                              weight, f16 ? largest : nullptr);
   tt_count_launches(1);
   const float* back = nullptr;
-  if (dtype == TT_F16) {
+  if (f16) {
     factor_kernel<<<1, 1, 0, st>>>(largest, factor);
     tt_count_launches(1);
     g.factor = factor, back = factor + 1;
