@@ -61,9 +61,12 @@ def parse():
     ap.add_argument("--fused-prologue", type=int, default=1,
                     help="e2e5: q/k RMSNorm + rotary in one fused kernel (1) or the model's "
                          "own ops (0)")
-    ap.add_argument("--fused-ce", type=int, default=1,
-                    help="e2e5: leaf losses by the chunked fused LM-head cross-entropy (1) "
-                         "or from leaf-only logits (0)")
+    ap.add_argument("--fused-ce", type=int, default=1, choices=(0, 1, 2),
+                    help="e2e5: leaf losses by the chunked fused LM-head cross-entropy (1), by "
+                         "pieces of the vocabulary (2), or from leaf-only logits (0)")
+    ap.add_argument("--fused-mlp", type=int, default=0,
+                    help="e2e5: gate, up, activation and product of the MLPs in one kernel (1) "
+                         "or the model's own ops (0)")
     ap.add_argument("--gdn-keep", type=int, default=1,
                     help="gdn: keep the forward's intermediates for the backward (1) or "
                          "recompute them (0)")
@@ -1202,6 +1205,8 @@ def run_e2e5(args):
         model = Qwen3ForCausalLM(cfg)
     torch.set_default_dtype(prev)
     model.train()
+    if args.fused_mlp:
+        tt.fuse_gated_mlps(model)
     if args.ckpt_mlp:
         from tree_training_b200.hybrid import checkpoint_mlps
         checkpoint_mlps(model)
@@ -1235,7 +1240,8 @@ def run_e2e5(args):
         c0.record()
         opt.zero_grad(set_to_none=True)
         loss = tree_grad_hybrid(model, roots, loss_fn, max_tokens=8192,
-                                fused_ce=bool(args.fused_ce), before_last_backward=avg.arm)
+                                fused_ce=(False, True, "pieces")[args.fused_ce],
+                                before_last_backward=avg.arm)
         ar_issued.append(avg.issued_during_backward())
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
@@ -1326,8 +1332,12 @@ def run_e2e5(args):
                        "parallelism": f"dp{world} (NCCL bucketed all-reduce)",
                        "peak_mem_gb_rank0": peak_mem / 1e9,
                        "mlp_recompute": bool(args.ckpt_mlp),
-                       "leaf_loss": ("fused chunked LM head + CE (no logits)" if args.fused_ce
-                                     else "leaf-only logits + CE"),
+                       "leaf_loss": ("leaf-only logits + CE",
+                                     "fused chunked LM head + CE (no logits)",
+                                     "LM head + CE by pieces of the vocabulary (no logits)"
+                                     )[args.fused_ce],
+                       "mlp": ("gate, up, activation and product in one kernel"
+                               if args.fused_mlp else "model's own ops"),
                        "qk_prologue": ("fused q/k RMSNorm + rotary kernel" if args.fused_prologue
                                        else "model's own ops")},
             "e2e": {"value": tokens_all / t_step, "unit": "tokens/s",
