@@ -184,7 +184,10 @@ __global__ void __launch_bounds__(32 * kWarps) rank_kernel(const Grad a, const S
       if (i < end) {
         const int32_t w = word_of(a, s.order ? s.order[i] : i);
         e[j] = digit_of(s, w);
-        if (kFirst && mark && w >= 0) atomicOr(a.used + (w >> 5), 1u << (w & 31));
+        // (most tokens are of words that are marked already: a third of a text's, and all
+        // its atomics, may be on one address)
+        if (kFirst && mark && w >= 0 && !((__ldcg(a.used + (w >> 5)) >> (w & 31)) & 1))
+          atomicOr(a.used + (w >> 5), 1u << (w & 31));
       }
     }
 #pragma unroll

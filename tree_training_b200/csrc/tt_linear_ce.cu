@@ -125,29 +125,51 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   return make_float2(m, a.y * expf(a.x - ref) + b.y * expf(b.x - ref));
 }
 
-constexpr int kJoinWarps = 16;
+constexpr int kJoinThreads = 512;
 
-// lse and losses of 32 rows a block: each warp joins a run of the parts.
-__global__ void __launch_bounds__(32 * kJoinWarps)
-    finish_kernel(const float2* part, int parts, int64_t T, const int64_t* labels, int M, int64_t V,
-                  const float* picked, float* lse, float* losses) {
-  __shared__ float2 sm[kJoinWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
-  const int run = (parts + kJoinWarps - 1) / kJoinWarps;
-  float2 v = make_float2(-INFINITY, 0.f);
-  if (row < T)
-    for (int i = warp * run; i < min(parts, (warp + 1) * run); ++i)
-      v = join(v, part[(int64_t)i * T + row]);
-  sm[warp][lane] = v;
+// lse and losses of R rows a block (a power of two): its threads share out the parts,
+// twice over: the maximum of all, then the sums above it.
+__global__ void __launch_bounds__(kJoinThreads)
+    finish_kernel(const float2* part, int parts, int64_t T, int R, const int64_t* labels, int M,
+                  int64_t V, const float* picked, float* lse, float* losses) {
+  __shared__ float sm[kJoinThreads];
+  const int r = threadIdx.x % R, lanes = kJoinThreads / R, mine = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
+  const float2* p = part + row;
+  float m = -INFINITY;
+  if (row < T) {
+#pragma unroll 4
+    for (int i = mine; i < parts; i += lanes) m = fmaxf(m, p[(int64_t)i * T].x);
+  }
+  sm[threadIdx.x] = m;
+  for (int o = lanes / 2; o; o >>= 1) {
+    __syncthreads();
+    if (mine < o) sm[threadIdx.x] = fmaxf(sm[threadIdx.x], sm[threadIdx.x + o * R]);
+  }
   __syncthreads();
-  for (int w = 0; w < kJoinWarps; ++w) v = w ? join(v, sm[w][lane]) : sm[0][lane];
+  m = sm[r];
+  __syncthreads();
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  if (row < T) {
+#pragma unroll 4
+    for (int i = mine; i < parts; i += lanes) {
+      const float2 v = p[(int64_t)i * T];
+      s += v.y * expf(v.x - ref);
+    }
+  }
+  sm[threadIdx.x] = s;
+  for (int o = lanes / 2; o; o >>= 1) {
+    __syncthreads();
+    if (mine < o) sm[threadIdx.x] += sm[threadIdx.x + o * R];
+  }
+  __syncthreads();
+  s = sm[r];
   if (row >= T) return;
-  const float l = v.x + logf(v.y);
-  if (warp == 0) lse[row] = l;
-  for (int m = warp; m < M; m += kJoinWarps) {
-    const int64_t i = row * M + m, y = labels[i];
-    losses[i] = y >= 0 && y < V ? (v.x - picked[i]) + logf(v.y) : 0.f;
+  if (mine == 0) lse[row] = m + logf(s);
+  for (int k = mine; k < M; k += lanes) {
+    const int64_t i = row * M + k, y = labels[i];
+    losses[i] = y >= 0 && y < V ? (m - picked[i]) + logf(s) : 0.f;
   }
 }
 
@@ -487,9 +509,11 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
                                               status, st);
     if (rc) return rc;
   }
-  finish_kernel<<<(unsigned)((T + 31) / 32), 32 * kJoinWarps, 0, st>>>(part, parts, T, labels,
-                                                                       (int)M, V, picked, lse,
-                                                                       losses);
+  // 32 rows a block read whole lines of the parts; with few rows there are more blocks
+  int R = 32;
+  while (R > 1 && T / R < 2 * vec::kSMs) R /= 2;
+  finish_kernel<<<(unsigned)((T + R - 1) / R), kJoinThreads, 0, st>>>(
+      part, parts, T, R, labels, (int)M, V, picked, lse, losses);
   tt_count_launches(1);
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
