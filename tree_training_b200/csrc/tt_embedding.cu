@@ -14,7 +14,12 @@
 // blocks as its rows are; sums of words that reach over a chunk's end leave as fp32
 // parts and are added up in order by a last launch.  The sorts are bound by latency
 // (20 us for 32,768 tokens): the rows of words without tokens, which a bitmap of the
-// first launch tells, are zeroed by further blocks of the launches after it.
+// first launch tells, are zeroed by further blocks of the launches after it.  The
+// launches begin while the one before ends (so what that one writes is not read through
+// the read-only path).
+//
+// Measured on a B200, bf16, forward and backward: 32,768 tokens of 151,936 x 2,560 259 us
+// (48 forward; 1.05 GB backward: 5.0 TB/s), 32,768 of 32,000 x 1,024 about 150.
 #include <algorithm>
 
 #include "tt_vec.cuh"
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(kPlaceThreads) place_kernel(const Grad a, cons
       int c[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        c[j] = b + j < end ? __ldg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
+        c[j] = b + j < end ? __ldcg(a.counts + (int64_t)(b + j) * (E + 1) + x) : 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         all += c[j];
@@ -427,7 +432,7 @@ __device__ __forceinline__ void add_parts(const Grad& a, int64_t chunk, int64_t 
         a.parts + ((chunk + k) * 2 + (k == 0 ? 1 : 0)) * a.part_ld + col);
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const float4 x = __ldg(q + i / 4);
+      const float4 x = __ldcg(q + i / 4);
       acc[i] += x.x, acc[i + 1] += x.y, acc[i + 2] += x.z, acc[i + 3] += x.w;
     }
   }

