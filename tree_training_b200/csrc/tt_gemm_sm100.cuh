@@ -518,6 +518,14 @@ inline int64_t slice_clocks(int cg, int bn) {
   return cg == 1 ? 256 + 2 * bn : std::max(256 + bn, 2 * bn);
 }
 
+// Clocks of a tile's epilogue, which sums shorter than it cannot hide: a pair's has as
+// many rows a CTA, and waits for the other CTA (both weights' gradients of 2,560 x 9,728
+// over 64 tokens: 39 us by pairs, 29 by single CTAs; over 512: 52 and 48).  The gated
+// product's is longer than that wait (8,192 x 256 x 1,024: 31 us by pairs, 39).
+inline int64_t epilogue_clocks(int cg, int bn, bool dual) {
+  return (dual ? 8000 : cg == 1 ? 5000 : 8000) * bn / 256;
+}
+
 // The cheapest of the forms by the tiles' waves.  `n_step`: what widths of the
 // accumulator are a multiple of; `dual`: its halves stand for one column of C each.
 // With `split` the tiles of the last wave, where they leave half of the SMs idle, are
@@ -533,17 +541,18 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool d
       const int64_t cols = dual ? bn / 2 : bn;
       const int64_t tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + cols - 1) / cols);
       const int64_t rest = tiles % slots, most = rest && split ? std::min(slots / rest, steps / 8) : 1;
-      const double clocks = (double)slice_clocks(cg, bn);
+      const double clocks = (double)slice_clocks(cg, bn), end = (double)epilogue_clocks(cg, bn, dual);
+      auto tile = [&](int64_t n) { return std::max((double)n * clocks, end) + 600; };
       for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); parts = next_parts(parts, most)) {
         // (a tile's start and end, which nothing hides: 600 clocks; the parts' way
         // through L2 and the launch that adds them up)
         const int64_t whole = parts > 1 ? tiles - rest : tiles;
-        double t = (double)((whole + slots - 1) / slots) * (steps * clocks + 600) + 1500;
+        double t = (double)((whole + slots - 1) / slots) * tile(steps) + 1500;
         const int64_t unit = (int64_t)128 * cg * bn * 4;
         if (parts > 1)
-          t += (double)((steps + parts - 1) / parts) * clocks + 600 + 5000 +
+          t += tile((steps + parts - 1) / parts) + 5000 +
                (double)(rest * (parts + 1) * unit) / 3000;
-        if (t < least * 0.999)
+        if (t < least * 0.999 || (parts == 1 && cg > best.cg && t <= least))
           least = t, best = Plan{cg, bn, whole, (int)parts, parts > 1 ? rest * parts * unit : 0};
       }
     }
