@@ -618,7 +618,7 @@ int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* 
  * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED).  kept (null, or
  * [T][tt_linear_ce_kept_ld] fp32 where that is not 0) takes the logits for the
  * backward, which forms them again without it. */
-int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int64_t V);
+int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int32_t H, int64_t V);
 int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
 int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
                      int64_t x_ld, const void* w, int64_t w_ld, const int64_t* labels, float scale,

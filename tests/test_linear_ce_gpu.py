@@ -232,3 +232,14 @@ def test_refusals():
         tt.linear_cross_entropy(x, w, labels.float())
     with pytest.raises(RuntimeError):
         tt.linear_cross_entropy(x, w, labels.cpu())
+
+
+@pytest.mark.parametrize("dtype,T,H,V,M", [(BF, 15, 72, 1001, 3), (F16, 9, 130, 777, 2),
+                                           (BF, 300, 1024, 2050, 2), (F16, 260, 1032, 515, 9),
+                                           (BF, 1, 2560, 40001, 300)])
+def test_16_bit_logits_that_are_left_for_the_backward(dtype, T, H, V, M):
+    from tree_training_b200 import _lib
+    assert _lib.lib().tt_linear_ce_kept_ld({BF: 1, F16: 2}[dtype], T, H, V)
+    compare(*make(T, H, V, M, dtype, T))
+    x, w, _, gl, ge = make(T, H, V, M, dtype, T)
+    compare(x, w, torch.full((T, M), V - 1, device=DEV), gl, ge)        # one label for all

@@ -117,7 +117,7 @@ def ce_bwd(dtype=BF16, T=4, H=16, V=100, M=1, x=P, x_ld=16, w=P, w_ld=16, labels
 
 BAD_CE = [dict(T=-1), dict(T=1 << 31), dict(H=0), dict(V=0), dict(V=1 << 31), dict(M=-1),
           dict(M=1 << 31), dict(x_ld=15), dict(w_ld=15), dict(x=None), dict(w=None),
-          dict(labels=None), dict(lse=None), dict(kept=P)]
+          dict(labels=None), dict(lse=None), dict(kept=P, T=100)]
 
 
 @pytest.mark.parametrize("bad", BAD_CE + [dict(losses=None)])
@@ -132,9 +132,13 @@ def test_linear_ce_gradient(bad):
 
 def test_linear_ce_kept_logits():
     f = lambda *a: status("tt_linear_ce_kept_ld", *a)
-    assert f(F32, 47, 1001) == 1008 and f(BF16, 47, 1001) == 0 and f(F32, 0, 1001) == 0
-    assert f(F32, 1 << 20, 4096) == 0 and f(F32, 4096, 16384) == 16384 and f(F32, 4097, 16384) == 0
-    assert f(F32, -1, 10) == 0 and f(F32, 10, 0) == 0
+    assert f(F32, 47, 64, 1001) == 1008 and f(F32, 0, 64, 1001) == 0 and f(U8, 47, 64, 1001) == 0
+    assert f(F32, 1 << 20, 64, 4096) == 0
+    assert f(F32, 4096, 64, 16384) == 16384 and f(F32, 4097, 64, 16384) == 0
+    # 16 bits: where forming them again takes longer
+    assert f(BF16, 47, 64, 1001) == 0 and f(BF16, 15, 64, 1001) == 1008
+    assert f(F16, 400, 1024, 151936) == 151936 and f(BF16, 8192, 2560, 151936) == 0
+    assert f(F32, -1, 64, 10) == 0 and f(F32, 10, 64, 0) == 0 and f(F32, 10, 0, 10) == 0
 
 
 def test_linear_ce_types_and_workspace():

@@ -124,7 +124,7 @@ SIGNATURES = {
     "tt_gated_linear_bwd_workspace_size": (_I64, [_INT, _I64, _I32, _I32]),
     "tt_gated_linear_bwd": (_INT, [_INT, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _INT, _P,
                                    _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
-    "tt_linear_ce_kept_ld": (_I64, [_INT, _I64, _I64]),
+    "tt_linear_ce_kept_ld": (_I64, [_INT, _I64, _I32, _I64]),
     "tt_linear_ce_fwd_workspace_size": (_I64, [_INT, _I64, _I32, _I64, _I64]),
     "tt_linear_ce_fwd": (_INT, [_INT, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P, _F32, _P,
                                 _P, _P, _P, _I64, _P, _P]),

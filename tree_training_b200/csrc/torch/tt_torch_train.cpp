@@ -222,7 +222,7 @@ CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double sca
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
   CE r{flat ? empty({T}, x, at::kFloat) : empty({T, M}, x, at::kFloat),
        empty({T}, x, at::kFloat), Tensor()};
-  const int64_t ld = keep ? tt_linear_ce_kept_ld(dtype_code(x), T, V) : 0;
+  const int64_t ld = keep ? tt_linear_ce_kept_ld(dtype_code(x), T, (int32_t)H, V) : 0;
   if (ld) r.kept = empty({T, ld}, x, at::kFloat);
   int32_t* status = status_of(x);
   On on(x);

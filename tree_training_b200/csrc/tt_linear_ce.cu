@@ -26,9 +26,13 @@
 // about 2^14 (and divided out of the sums): softmax probabilities times weights of
 // 1 / T lie below fp16's smallest number.
 //
+// Where one piece holds all logits (a quarter of a gigabyte of fp32 at most: few rows or
+// a small vocabulary) the forward leaves them for the backward, whose fourth product
+// would cost a third more.  (16-bit: not where k is so short that forming them again
+// takes less than their 8 bytes each way.)
+//
 // fp32: the same steps with products on the CUDA cores and passes over the logits
-// of a piece.  Where one piece holds all logits (a quarter of a gigabyte at most) the
-// forward leaves them for the backward, whose fourth product would cost a third more.
+// of a piece.
 #include <cfloat>
 
 #include "tt_gemm_sm100.cuh"
@@ -85,7 +89,8 @@ __device__ __forceinline__ void take(const float (&z)[N], float& m, float& s) {
   m = top;
 }
 
-template <bool kB>
+// (kKeep: a form of its own, since the stores cost the registers that the sums need)
+template <bool kB, bool kKeep>
 struct LseEpi {
   static constexpr bool kBf16 = kB, kChunks = true;
   struct Args {
@@ -93,6 +98,8 @@ struct LseEpi {
     Labels labels;
     float* picked;                         // [T][M]
     float scale;
+    float* kept;                           // kKeep: the logits
+    int64_t kept_ld;
   };
   static __device__ __forceinline__ void finish(const Args& a, const gemm::Problem& p,
                                                 const gemm::TileAt& t, int row, int c0,
@@ -103,6 +110,21 @@ struct LseEpi {
 #pragma unroll
     for (int i = 0; i < 64; ++i) z[i] = i < cols ? z[i] * a.scale : -INFINITY;
     take<64>(z, m, s);
+    if constexpr (kKeep) {
+      float* to = a.kept + (int64_t)row * a.kept_ld + n0;
+      if (cols == 64) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 8) {
+          const float u[4] = {z[i], z[i + 1], z[i + 2], z[i + 3]};
+          const float v[4] = {z[i + 4], z[i + 5], z[i + 6], z[i + 7]};
+          gemm::store32(to + i, vec::pack<float, 4>(u), vec::pack<float, 4>(v));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i < cols) to[i] = z[i];
+      }
+    }
     a.part[(int64_t)(4 * t.n + c0 / 64) * p.M + row] = make_float2(m, s);
     const int count = a.labels.count[row];
     for (int k = 0; k < count; ++k) {
@@ -325,10 +347,61 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// The same to 16-bit dz (and what its rounding took off, or null), in packs of 8; rows
+// of z and dz begin on 32- and 16-byte boundaries and have whole packs.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    grad_16_kernel(const float* z, int64_t z_ld, T* dz, T* rest, int64_t rows, int n, int64_t ld,
+                   int segment, const Grad g) {
+  const int c0 = blockIdx.y * segment, c1 = min(n, c0 + segment);
+  const float f = g.factor ? *g.factor : 1.f;
+  for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
+    const int count = g.g_loss ? g.labels.count[t] : 0;
+    const int2* list = g.labels.list + t * g.labels.M;
+    const float w = g.weight[t] * f, lse = g.lse[t];
+    const float* from = z + t * z_ld;
+    auto put = [&](int64_t at, float v) {
+      dz[at] = from_f32<T>(v);
+      if (rest) rest[at] = from_f32<T>(v - to_f32(from_f32<T>(v)));
+    };
+    for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from + c + i);
+        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = w * exp2f((v[i] - lse) * kLog2e);
+      vec::store<T, 8>(dz + t * ld + c, v);
+      if (rest) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] -= to_f32(from_f32<T>(v[i]));
+        vec::store<T, 8>(rest + t * ld + c, v);
+      }
+    }
+    __syncthreads();
+    // a thread a label, the first of those that are equal
+    for (int k = threadIdx.x; k < count; k += blockDim.x) {
+      const int at = list[k].x;
+      if (at < c0 || at >= c1) continue;
+      float sum = 0.f;
+      bool first = true;
+      for (int j = 0; j < count; ++j)
+        if (list[j].x == at) {
+          first &= j >= k;
+          sum += g.g_loss[t * g.labels.M + list[j].y];
+        }
+      if (first) put(t * ld + at, w * exp2f((from[at] - lse) * kLog2e) - sum * g.scale * f);
+    }
+    __syncthreads();
+  }
+}
+
 // Columns of a segment: four blocks an SM where there are few rows.
 int segment_of(int64_t T, int64_t n) {
   const int64_t want = std::max<int64_t>(1, 4 * vec::kSMs / T);
-  return (int)std::max<int64_t>(512, (n + want - 1) / want);
+  return (int)std::max<int64_t>(512, (n + want - 1) / want + 7) / 8 * 8;
 }
 int64_t segments_of(int64_t T, int64_t n) {
   return (n + segment_of(T, n) - 1) / segment_of(T, n);
@@ -353,16 +426,21 @@ constexpr int64_t kPieceBytes = (int64_t)1 << 28;
 int64_t dz_size(int dtype, int64_t T) { return dtype == TT_F32 || two_terms(dtype, T) ? 4 : 2; }
 
 // Columns of a piece of the vocabulary: a quarter of a gigabyte of dz, at least 4,096.
-int64_t piece_of(int dtype, int64_t T, int64_t V) {
+int64_t most_columns(int dtype, int64_t T) {
   const int64_t wide = kPieceBytes / (dz_size(dtype, T) * std::max<int64_t>(T, 1));
-  return std::min((V + 255) / 256 * 256, std::max<int64_t>(4096, wide / 256 * 256));
+  return std::max<int64_t>(4096, wide / 256 * 256);
+}
+int64_t piece_of(int dtype, int64_t T, int64_t V) {
+  return std::min((V + 255) / 256 * 256, most_columns(dtype, T));
 }
 
 // The row stride of the logits that the forward leaves for the backward; 0: none.
-int64_t kept_ld(int dtype, int64_t T, int64_t V) {
+int64_t kept_ld(int dtype, int64_t T, int32_t H, int64_t V) {
   const int64_t ld = (V + 7) / 8 * 8;
-  return dtype == TT_F32 && T > 0 && T * ld * 4 <= kPieceBytes && piece_of(dtype, T, V) >= V ? ld
-                                                                                             : 0;
+  // (forming them again takes 2 H operations each at 1.4e15 a second, or W's 2 H bytes
+  // for T of them at 6.5e12; keeping them 8 bytes)
+  const bool worth = dtype == TT_F32 || H >= 1024 || H > 4 * T;
+  return worth && T > 0 && T * ld * 4 <= kPieceBytes && V <= most_columns(dtype, T) ? ld : 0;
 }
 
 int64_t labels_bytes(int64_t T, int64_t M) { return round256(4 * T) + round256(8 * T * M); }
@@ -402,16 +480,18 @@ struct Shape {
 
 template <bool kB>
 int forward_16(const Shape& s, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
-               const Labels& l, float scale, float2* part, float* picked, int* parts,
-               int32_t* status, cudaStream_t st) {
-  using Epi = LseEpi<kB>;
+               const Labels& l, float scale, float2* part, float* picked, float* kept,
+               int* parts, int32_t* status, cudaStream_t st) {
   const gemm::Plan plan = forward_plan(s.T, s.H, s.V);
   const gemm::Term term{{x, x_ld, false}, {w, w_ld, false}, s.H};
   gemm::Problem q;
   if (!gemm::set_up(&q, plan, kB, s.T, s.V, &term, 1, false, status)) return TT_ERR_UNSUPPORTED;
   *parts = 4 * q.tiles_n;
-  typename Epi::Args ea{part, l, picked, scale};
-  return gemm::launch<false, false, Epi>(plan, q, ea, st);
+  if (kept)
+    return gemm::launch<false, false, LseEpi<kB, true>>(
+        plan, q, {part, l, picked, scale, kept, kept_ld(s.dtype, s.T, s.H, s.V)}, st);
+  return gemm::launch<false, false, LseEpi<kB, false>>(plan, q,
+                                                       {part, l, picked, scale, nullptr, 0}, st);
 }
 
 template <bool kB>
@@ -446,8 +526,9 @@ const char* row_of(const Shape& s, const void* w, int64_t w_ld, int64_t v) {
 using namespace tt;
 using namespace tt::linear_ce;
 
-extern "C" int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int64_t V) {
-  return sizes_ok(T, 1, V, 0) ? kept_ld(dtype, T, V) : 0;
+extern "C" int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int32_t H, int64_t V) {
+  if (!sizes_ok(T, H, V, 0) || dtype < TT_F32 || dtype > TT_F16) return 0;
+  return kept_ld(dtype, T, H, V);
 }
 
 extern "C" int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V,
@@ -472,7 +553,7 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   const Shape s{dtype, T, H, V, M};
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
-  if (!lse || (M > 0 && !losses) || (kept && !kept_ld(dtype, T, V))) return TT_ERR_INVALID_ARG;
+  if (!lse || (M > 0 && !losses) || (kept && !kept_ld(dtype, T, H, V))) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_fwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -487,7 +568,7 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
     parts = 0;
     float* room = ws.take<float>(4 * T * P);
     float* z = kept ? kept : room;
-    const int64_t ld = kept ? kept_ld(dtype, T, V) : P;
+    const int64_t ld = kept ? kept_ld(dtype, T, H, V) : P;
     for (int64_t v0 = 0; v0 < V; v0 += P) {
       const int64_t n = std::min(P, V - v0);
       const gemm::Term term{{x, x_ld, false}, {row_of(s, w, w_ld, v0), w_ld, false}, H};
@@ -503,10 +584,10 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
     }
   } else {
     part = (float2*)ws.p;
-    rc = dtype == TT_BF16 ? forward_16<true>(s, x, x_ld, w, w_ld, l, scale, part, picked, &parts,
-                                             status, st)
-                          : forward_16<false>(s, x, x_ld, w, w_ld, l, scale, part, picked, &parts,
-                                              status, st);
+    rc = dtype == TT_BF16 ? forward_16<true>(s, x, x_ld, w, w_ld, l, scale, part, picked, kept,
+                                             &parts, status, st)
+                          : forward_16<false>(s, x, x_ld, w, w_ld, l, scale, part, picked, kept,
+                                              &parts, status, st);
     if (rc) return rc;
   }
   // 32 rows a block read whole lines of the parts; with few rows there are more blocks
@@ -547,7 +628,7 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   const Shape s{dtype, T, H, V, M};
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
-  if (!lse || (kept && !kept_ld(dtype, T, V))) return TT_ERR_INVALID_ARG;
+  if (!lse || (kept && !kept_ld(dtype, T, H, V))) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_bwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -596,8 +677,19 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
         return rc;
       const int segment = segment_of(T, P);
       grad_kernel<<<dim3(row_blocks(T), (unsigned)((n + segment - 1) / segment)), 256, 0, st>>>(
-          kept ? kept : (const float*)dz, kept ? kept_ld(dtype, T, V) : P, (float*)dz, T, (int)n, P,
+          kept ? kept : (const float*)dz, kept ? kept_ld(dtype, T, H, V) : P, (float*)dz, T, (int)n, P,
           segment, g);
+      tt_count_launches(1);
+    } else if (kept) {
+      const int segment = segment_of(T, P);
+      const dim3 grid(row_blocks(T), (unsigned)((n + segment - 1) / segment));
+      const int64_t z_ld = kept_ld(dtype, T, H, V);
+      if (dtype == TT_BF16)
+        grad_16_kernel<<<grid, 256, 0, st>>>(kept, z_ld, (__nv_bfloat16*)dz, (__nv_bfloat16*)rest,
+                                             T, (int)n, P, segment, g);
+      else
+        grad_16_kernel<<<grid, 256, 0, st>>>(kept, z_ld, (__half*)dz, (__half*)rest, T, (int)n, P,
+                                             segment, g);
       tt_count_launches(1);
     } else {
       rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st)
