@@ -112,18 +112,14 @@ struct LseEpi {
     take<64>(z, m, s);
     if constexpr (kKeep) {
       float* to = a.kept + (int64_t)row * a.kept_ld + n0;
-      if (cols == 64) {
+      // (tiles are multiples of 16 wide: eights that go over the end go into the row's pad)
 #pragma unroll
-        for (int i = 0; i < 64; i += 8) {
-          const float u[4] = {z[i], z[i + 1], z[i + 2], z[i + 3]};
-          const float v[4] = {z[i + 4], z[i + 5], z[i + 6], z[i + 7]};
-          gemm::store32(to + i, vec::pack<float, 4>(u), vec::pack<float, 4>(v));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < cols) to[i] = z[i];
-      }
+      for (int i = 0; i < 64; i += 8)
+        if (i < cols)
+          asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i),
+                       "f"(z[i]), "f"(z[i + 1]), "f"(z[i + 2]), "f"(z[i + 3]), "f"(z[i + 4]),
+                       "f"(z[i + 5]), "f"(z[i + 6]), "f"(z[i + 7])
+                       : "memory");
     }
     a.part[(int64_t)(4 * t.n + c0 / 64) * p.M + row] = make_float2(m, s);
     const int count = a.labels.count[row];
