@@ -23,6 +23,10 @@
 // 33 for three).
 //
 // fp32: the products on the CUDA cores (see tt_gemm_fp32.cu), h by a pass over g and u.
+//
+// Measured on a B200, bf16, 8,192 x 2,560 x 9,728, single launches: forward 537 us with g
+// and u kept (495 without), dg and du 158 (7.1 TB/s), dx 501, both weights' gradients 528;
+// a pass back to back 2,080 to 2,170 us, at the power limit.
 #include "tt_gemm_sm100.cuh"
 
 namespace tt {
