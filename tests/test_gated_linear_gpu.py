@@ -250,3 +250,22 @@ def test_modules_that_do_more_keep_their_forward():
     assert tt.fuse_gated_mlps(m) == 4
     for b, w in zip(m, want):
         assert float((b(x) - w).norm() / w.norm()) < 100 * EPS
+
+
+@pytest.mark.parametrize("dtype,largest", [(BF, 1e18), (F16, 6e4 * 6e4)])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_gradients_far_below_zero(act, dtype, largest):
+    """Where the activation is nothing its slope is, however large the product: dg and
+    du are 0 there (the cube in tanh's argument reaches 1e54, past fp32)."""
+    sizes = torch.logspace(1, torch.tensor(largest).log10().item() / 2, 24, device=DEV)
+    for r in sizes.tolist():                # feature 0: g = -r^2, u = 1
+        x = torch.zeros(1, 16, device=DEV, dtype=dtype)
+        wg, wu = (torch.zeros(8, 16, device=DEV, dtype=dtype) for _ in range(2))
+        x[0, 0], wg[0, 0] = r, -r
+        x[0, 1] = wu[:, 1] = 1
+        leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
+        h = tt.gated_linear(*leaves, activation=act)
+        dx, dwg, dwu = torch.autograd.grad(h, leaves, torch.ones_like(h))
+        for got in (h[0, 0], dx[0, 0], dwg[0], dwu[0]):
+            assert float(got.abs().max()) == 0, (r, got)
+    tt.check_device_status()

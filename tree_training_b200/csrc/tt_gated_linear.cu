@@ -85,12 +85,13 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
 template <int A>
 __device__ __forceinline__ void act_grad_16(float g, float& a, float& d) {
   if constexpr (A == kSilu || A == kGeluTanh) {
-    // s = 1 / (1 + exp(-z)), 1 - s = exp(-z) s; past -80 both are nothing beside 1
+    // s = 1 / (1 + exp(-z)), 1 - s = exp(-z) s; past -80, where exp(-z) s would leave
+    // fp32, s is 0 (not 2e-35: g and its cube may be as large)
     const float z = A == kSilu ? g : 2.f * kTanhA * (g + kTanhB * g * g * g);
-    const float e = __expf(-fmaxf(z, -80.f)), s = __fdividef(1.f, 1.f + e);
+    const float e = __expf(-fmaxf(z, -80.f)), s = z < -80.f ? 0.f : __fdividef(1.f, 1.f + e);
     const float dz = A == kSilu ? 1.f : 2.f * kTanhA * (1.f + 3.f * kTanhB * g * g);
     a = g * s;
-    d = s * (1.f + g * dz * (e * s));
+    d = s * (1.f + g * (e * s * dz));
   } else {
     act_grad<A>(g, a, d);
   }
