@@ -574,7 +574,8 @@ int tt_token_logprobs_bwd(int dtype, int64_t n_rows, int32_t vocab, const void* 
 /* ---- embedding ------------------------------------------------------------- *
  * y[t] = scale * weight[ids[t]]: y [n, H] contiguous, weight [V, H] with row
  * stride ld, ids int64 (ids64) or int32.  An id outside [0, V) gives a row of NaN
- * and writes TT_ERR_INVALID_ARG into *status.  n, V < 2^31. */
+ * and writes TT_ERR_INVALID_ARG into *status.  n, V < 2^31, H <= 2^22.  (Workspaces,
+ * here and below: on a 16-byte boundary.) */
 int tt_embedding_fwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids, int ids64,
                      const void* weight, int64_t ld, float scale, void* y, int32_t* status,
                      void* stream);
@@ -598,7 +599,7 @@ int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void*
  * boundaries (else TT_ERR_UNSUPPORTED).  g and u (fp32; null for 16-bit inputs: not
  * kept) are the two products, which the backward takes: on 16-byte boundaries, their
  * row stride keep_ld a multiple of 4 and at least round_up(F, 8).  What stands past
- * column F is not read as a value. */
+ * column F is not read as a value.  T, H < 2^31 - 256, F <= 2^30 - 256. */
 int64_t tt_gated_linear_fwd_workspace_size(int dtype, int64_t T, int32_t H, int32_t F);
 int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, const void* x, int64_t x_ld,
                         const void* wg, int64_t wg_ld, const void* wu, int64_t wu_ld, int act,
@@ -617,7 +618,8 @@ int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* 
  * lse[t] - z[t, labels[t, m]], 0 for labels (int64 [T, M]) outside [0, V).  16-bit
  * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED).  kept (null, or
  * [T][tt_linear_ce_kept_ld] fp32 where that is not 0) takes the logits for the
- * backward, which forms them again without it. */
+ * backward, which forms them again without it: on a 32-byte boundary.  T, H, V <
+ * 2^31 - 256. */
 int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int32_t H, int64_t V);
 int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
 int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,

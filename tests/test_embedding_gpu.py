@@ -147,3 +147,16 @@ def test_refusals():
     g, = torch.autograd.grad(tt.embedding(ids, w).sum(), w, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_the_widest_row_and_wider_ones():
+    H = 1 << 22
+    w = torch.randn(2, H, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    ids = torch.tensor([1, 1, 0], device="cuda")
+    y = tt.embedding(ids, w)
+    assert torch.equal(y, w[ids])
+    dw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(dw, torch.tensor([[1.], [2.]], device="cuda").bfloat16().expand(2, H))
+    tt.check_device_status()
+    with pytest.raises(ValueError):
+        tt.embedding(ids, torch.zeros(2, H + 1, device="cuda", dtype=torch.bfloat16))

@@ -269,3 +269,12 @@ def test_gradients_far_below_zero(act, dtype, largest):
         for got in (h[0, 0], dx[0, 0], dwg[0], dwu[0]):
             assert float(got.abs().max()) == 0, (r, got)
     tt.check_device_status()
+
+
+def test_widths_that_32_bits_do_not_count():
+    one = torch.ones(1, 1, device=DEV, dtype=BF)
+    with pytest.raises(ValueError):
+        tt.gated_linear(one, *[one.expand((1 << 30) - 255, 1)] * 2)
+    wide = one.expand(1, (1 << 31) - 257)
+    with pytest.raises(ValueError):
+        tt.gated_linear(wide, wide, wide)

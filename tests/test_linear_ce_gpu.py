@@ -243,3 +243,13 @@ def test_16_bit_logits_that_are_left_for_the_backward(dtype, T, H, V, M):
     compare(*make(T, H, V, M, dtype, T))
     x, w, _, gl, ge = make(T, H, V, M, dtype, T)
     compare(x, w, torch.full((T, M), V - 1, device=DEV), gl, ge)        # one label for all
+
+
+def test_widths_that_32_bits_do_not_count():
+    one = torch.ones(1, 1, device="cuda", dtype=torch.bfloat16)
+    wide = one.expand(1, (1 << 31) - 257)
+    with pytest.raises(ValueError):
+        tt.linear_cross_entropy(wide, wide, torch.zeros(1, device="cuda", dtype=torch.int64))
+    with pytest.raises(ValueError):
+        tt.linear_cross_entropy(one, one.expand((1 << 31) - 256, 1),
+                                torch.zeros(1, device="cuda", dtype=torch.int64))

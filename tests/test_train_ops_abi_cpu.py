@@ -183,3 +183,32 @@ def test_grad_norm(call):
 def test_clip_outputs():
     assert clip(outs=arrays(at=None)[2]) == INVALID
     assert clip(outs=arrays(at=P + 1)[2]) == INVALID
+
+
+@pytest.mark.parametrize("call,wide", [
+    (embed, dict(H=(1 << 22) + 1, ld=1 << 23)), (embed_bwd, dict(H=(1 << 22) + 1, ld=1 << 23)),
+    (gated, dict(F=(1 << 30) - 255)), (gated_bwd, dict(F=(1 << 30) - 255, ld=1 << 30,
+                                                      dh_ld=1 << 30)),
+    (gated, dict(H=(1 << 31) - 257, x_ld=1 << 31, wg_ld=1 << 31, wu_ld=1 << 31)),
+    (gated_bwd, dict(H=(1 << 31) - 257, x_ld=1 << 31, wg_ld=1 << 31, wu_ld=1 << 31)),
+    (ce, dict(H=(1 << 31) - 257, x_ld=1 << 31, w_ld=1 << 31)),
+    (ce_bwd, dict(H=(1 << 31) - 257, x_ld=1 << 31, w_ld=1 << 31))])
+def test_widths_that_32_bits_do_not_count(call, wide):
+    assert call(**wide) == INVALID
+
+
+def test_the_largest_widths_have_a_workspace():
+    size = lambda name, *a: status(f"tt_{name}_workspace_size", *a)
+    assert size("embedding_bwd", 1, 1, 1 << 22) > 1 << 22
+    assert size("gated_linear_bwd", BF16, 1, 1, (1 << 30) - 256) > 1 << 32
+    assert size("linear_ce_fwd", BF16, 1, (1 << 31) - 258, 1, 1) > 0
+
+
+@pytest.mark.parametrize("call", [embed_bwd, gated, gated_bwd, ce, ce_bwd, norm, clip])
+def test_a_workspace_off_its_boundary(call):
+    assert call(ws=P + 4) == INVALID
+
+
+@pytest.mark.parametrize("call", [ce, ce_bwd])
+def test_kept_logits_off_their_boundary(call):
+    assert call(dtype=F32, kept=P + 16) == INVALID

@@ -97,7 +97,7 @@ Tensor embedding(const Tensor& ids_, const Tensor& w_, double scale,
     value_error("embedding: weight must be [V, H]");
   const int64_t V = w_.size(0);
   need_size(op, "a vocabulary", V);
-  need_size(op, "a row's width", w_.size(1));
+  if (w_.size(1) > (1 << 22)) value_error("embedding: a row's width is limited to 2^22");
   need_size(op, "a number of tokens", ids_.numel());
   int64_t padding = -1;
   if (padding_) {
@@ -193,8 +193,9 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
   if (wg.dim() != 2 || wg.size(0) < 1 || wg.size(1) != H)
     value_error("gated_linear: w_gate must be [F, " + std::to_string(H) + "]");
   if (wu.sizes() != wg.sizes()) value_error("gated_linear: w_up must have w_gate's shape");
-  need_size(op, "a row's width", H);
-  need_size(op, "a number of features", wg.size(0) + 8);
+  need_size(op, "a row's width", H + 257);
+  if (wg.size(0) > (1 << 30) - 256)
+    value_error("gated_linear: the number of features is limited to 2^30 - 256");
   const int64_t T = x.numel() / H;
   need_size(op, "a number of rows", T + 256);
   no_tangent(op, {&x, &wg, &wu});
@@ -296,7 +297,7 @@ std::tuple<Tensor, Tensor> linear_cross_entropy(const Tensor& x_, const Tensor& 
     value_error("linear_cross_entropy: weight must be [V, " + std::to_string(H) + "]");
   if (labels_.dim() < 1 || labels_.dim() > 2 || labels_.size(0) != T)
     value_error("linear_cross_entropy: labels must be [rows] or [rows, M]");
-  need_size(op, "a row's width", H);
+  need_size(op, "a row's width", H + 257);
   need_size(op, "a vocabulary", w.size(0) + 256);
   need_size(op, "a number of rows", T + 256);
   if (!std::isfinite((float)scale)) value_error("linear_cross_entropy: scale must be finite");

@@ -517,7 +517,8 @@ int sort_blocks(int64_t n, int digits) {
 int64_t round16(int64_t b) { return (b + 15) / 16 * 16; }
 
 bool ok_sizes(int64_t n, int64_t V, int H) {
-  return n >= 0 && n <= 0x7fffffff && V >= 1 && V <= 0x7fffffff && H >= 1 && H <= (1 << 30);
+  // (the gradient's columns are shared out over the grid's second side, of 65,535 blocks)
+  return n >= 0 && n <= 0x7fffffff && V >= 1 && V <= 0x7fffffff && H >= 1 && H <= (1 << 22);
 }
 
 }  // namespace
@@ -638,7 +639,8 @@ extern "C" int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, cons
                                 int64_t padding_idx, void* dweight, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   if (!ok_sizes(n, V, H) || (n > 1 && dy_ld < H)) return TT_ERR_INVALID_ARG;
-  if (!dweight || (n > 0 && (!ids || !dy))) return TT_ERR_INVALID_ARG;
+  if (!dweight || (n > 0 && (!ids || !dy)) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return TT_ERR_INVALID_ARG;
   if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
   const Layout l(n, V, H);
   if (workspace_bytes < l.all || !workspace) return TT_ERR_WORKSPACE;

@@ -277,7 +277,9 @@ int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 bool sizes_ok(int64_t T, int32_t H, int32_t F) {
-  return T >= 0 && T < ((int64_t)1 << 31) - 256 && H >= 1 && F >= 1;
+  // (dg and du side by side, a pad and a tile past them are counted in 32 bits)
+  return T >= 0 && T < ((int64_t)1 << 31) - 256 && H >= 1 && H < INT32_MAX - 256 && F >= 1 &&
+         F <= (1 << 30) - 256;
 }
 
 int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
@@ -285,7 +287,7 @@ int size_of(int dtype) { return dtype == TT_F32 ? 4 : 2; }
 template <typename T, int A>
 void run_backward(const float* g, const float* u, int64_t keep_ld, const void* dh, int64_t dh_ld,
                   int64_t rows, int F, void* dg, void* du, int64_t ld, cudaStream_t st) {
-  const int packs = (F * (int)sizeof(T) + 15) / 16;
+  const int packs = (int)((F * (int64_t)sizeof(T) + 15) / 16);
   const dim3 grid((unsigned)std::min((packs + 255) / 256, 64),
                   (unsigned)std::min<int64_t>(rows, 32768));
   backward_kernel<T, A><<<grid, 256, 0, st>>>(g, u, keep_ld, (const T*)dh, dh_ld, rows, F, (T*)dg,
@@ -339,7 +341,8 @@ extern "C" int tt_gated_linear_fwd(int dtype, int64_t T, int32_t H, int32_t F, c
   if (!sizes_ok(T, H, F) || act < kSilu || act > kRelu || x_ld < H || wg_ld < H || wu_ld < H ||
       !g != !u ||
       (g && (keep_ld < round8(F) || keep_ld % 4 ||
-             ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15))))
+             ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15))) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15))
     return TT_ERR_INVALID_ARG;
   if (dtype < TT_F32 || dtype > TT_F16) return TT_ERR_UNSUPPORTED;
   if (T == 0) return TT_OK;
@@ -401,7 +404,8 @@ extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, c
   if (T == 0) return TT_OK;
   if (!x || !wg || !wu || !g || !u || !dh) return TT_ERR_INVALID_ARG;
   if (keep_ld < round8(F) || keep_ld % 4 ||
-      ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u)) & 15))
+      ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15))
     return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_gated_linear_bwd_workspace_size(dtype, T, H, F))
     return TT_ERR_WORKSPACE;

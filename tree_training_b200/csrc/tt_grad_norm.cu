@@ -293,7 +293,7 @@ int check(int32_t count, const int32_t* dtypes, const int64_t* sizes, const void
   for (int32_t i = 0; i < count; ++i) {
     if (dtypes[i] < TT_F32 || dtypes[i] > TT_F16) return TT_ERR_UNSUPPORTED;
     // (a tensor's chunks are counted in 32 bits: 2^31 of them are 64 TB)
-    if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 44) || (sizes[i] > 0 && !src[i]))
+    if (sizes[i] < 0 || sizes[i] >= ((int64_t)1 << 44) || (sizes[i] > 0 && !src[i]))
       return TT_ERR_INVALID_ARG;
     const uintptr_t b = dtypes[i] == TT_F32 ? 3 : 1;
     if (reinterpret_cast<uintptr_t>(src[i]) & b) return TT_ERR_INVALID_ARG;
@@ -342,7 +342,7 @@ extern "C" int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t*
                             const void* const* tensors, double norm_type, float* norm,
                             void* workspace, int64_t workspace_bytes, void* stream) {
   const int kind = kind_of(norm_type);
-  if (kind < 0 || !norm) return TT_ERR_INVALID_ARG;
+  if (kind < 0 || !norm || (reinterpret_cast<uintptr_t>(workspace) & 7)) return TT_ERR_INVALID_ARG;
   if (const int rc = check(count, dtypes, sizes, tensors)) return rc;
   if (!workspace || workspace_bytes < tt_grad_norm_workspace_size(count)) return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -363,7 +363,7 @@ extern "C" int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int
                                  const float* given_norm, float max_norm, float eps, float* norm,
                                  void* workspace, int64_t workspace_bytes, void* stream) {
   const int kind = kind_of(norm_type);
-  if (kind < 0 || !norm) return TT_ERR_INVALID_ARG;
+  if (kind < 0 || !norm || (reinterpret_cast<uintptr_t>(workspace) & 7)) return TT_ERR_INVALID_ARG;
   if (const int rc = check(count, dtypes, sizes, tensors)) return rc;
   if (const int rc = check(count, dtypes, sizes, outs)) return rc;
   if (!workspace || workspace_bytes < tt_grad_norm_workspace_size(count)) return TT_ERR_WORKSPACE;

@@ -413,7 +413,7 @@ int64_t segments_of(int64_t T, int64_t n) {
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 bool sizes_ok(int64_t T, int32_t H, int64_t V, int64_t M) {
-  return T >= 0 && T < ((int64_t)1 << 31) - 256 && H >= 1 && V >= 1 &&
+  return T >= 0 && T < ((int64_t)1 << 31) - 256 && H >= 1 && H < INT32_MAX - 256 && V >= 1 &&
          V < ((int64_t)1 << 31) - 256 && M >= 0 && M <= 0x7fffffff;
 }
 
@@ -516,6 +516,9 @@ int check(const Shape& s, const void* x, int64_t x_ld, const void* w, int64_t w_
   return TT_OK;
 }
 
+// Whether p is off a boundary of n bytes.
+bool off(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
 const char* row_of(const Shape& s, const void* w, int64_t w_ld, int64_t v) {
   return (const char*)w + v * w_ld * (s.dtype == TT_F32 ? 4 : 2);
 }
@@ -555,6 +558,7 @@ extern "C" int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
   if (!lse || (M > 0 && !losses) || (kept && !kept_ld(dtype, T, H, V))) return TT_ERR_INVALID_ARG;
+  if (off(kept, 32) || off(workspace, 16)) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_fwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -630,6 +634,7 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
   if (!lse || (kept && !kept_ld(dtype, T, H, V))) return TT_ERR_INVALID_ARG;
+  if (off(kept, 32) || off(workspace, 16)) return TT_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < tt_linear_ce_bwd_workspace_size(dtype, T, H, V, M))
     return TT_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;

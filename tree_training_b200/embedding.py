@@ -15,7 +15,7 @@ from . import _ops
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> torch.Tensor:
     """scale * weight[ids]: ids [...] int64/int32, weight [V, H] fp32/bf16/fp16
-    (any row stride) -> [..., H] of weight's type, rounded once.
+    (any row stride, H up to 2^22) -> [..., H] of weight's type, rounded once.
 
     Differentiable in weight: a word's gradient is scale times the sum of its
     tokens' gradients in the order of the tokens, rounded once; ``padding_idx``

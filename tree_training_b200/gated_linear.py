@@ -17,8 +17,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                  activation: str = "silu") -> torch.Tensor:
     """h = activation(x @ w_gate.T) * (x @ w_up.T)
 
-    x [..., H], w_gate and w_up [F, H] of one type (fp32/bf16/fp16) -> [..., F];
-    activation one of silu, gelu, gelu_tanh, relu.  Sums are fp32, h is rounded
+    x [..., H], w_gate and w_up [F, H] of one type (fp32/bf16/fp16), F below 2^30 - 255
+    -> [..., F]; activation one of silu, gelu, gelu_tanh, relu.  Sums are fp32, h is rounded
     once.  Any row strides; 16-bit rows that do not start on 16-byte boundaries are
     copied first.  The two weights may be halves of one tensor.
 
