@@ -643,7 +643,8 @@ int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
                  const void* const* tensors, double norm_type, float* norm, void* workspace,
                  int64_t workspace_bytes, void* stream);
 /* outs[i] = tensors[i] * min(1, max_norm / (norm + eps)); outs[i] may be tensors[i].
- * given_norm (device; null: computed here) is the norm to go by; *norm gets it. */
+ * given_norm (device, no part of outs; null: computed here) is the norm to go by;
+ * *norm gets it. */
 int tt_clip_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
                       const void* const* tensors, void* const* outs, double norm_type,
                       const float* given_norm, float max_norm, float eps, float* norm,

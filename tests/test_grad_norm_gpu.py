@@ -186,3 +186,13 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         tt.grad_norm([t[0], t[1].cpu()])
     assert float(tt.grad_norm([t[0], t[0]])) == pytest.approx(float(t[0].norm()) * 2 ** 0.5, rel=1e-6)
+
+
+def test_a_norm_among_the_written():
+    flat = torch.ones(40, device="cuda")
+    with pytest.raises(ValueError):
+        tt.clip_grad_norm([flat[:30]], 1.0, norm=flat[29:30])
+    with pytest.raises(ValueError):
+        tt.clip_grad_norm([flat[:10]], 1.0, norm=flat[20:21], out=[flat[20:30]])
+    tt.clip_grad_norm([flat[:30]], 0.5, norm=flat[30:31], eps=0.0)
+    assert torch.equal(flat, torch.tensor([0.5] * 30 + [1.0] * 10, device="cuda"))

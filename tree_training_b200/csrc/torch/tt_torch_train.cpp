@@ -419,6 +419,11 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, double 
     if (norm_->numel() != 1 || norm_->scalar_type() != at::kFloat)
       type_error("clip_grad_norm: norm must be one float32");
     given = *norm_;
+    // (every block reads it, others may have written by then)
+    const int64_t at = (int64_t)(uintptr_t)given.const_data_ptr();
+    for (size_t i = 0; i < dst.sizes.size(); ++i)
+      if (dst.sizes[i] && at + 4 > (int64_t)(uintptr_t)dst.data[i] && at < end_of(dst, i))
+        value_error("clip_grad_norm: norm is a part of a tensor that is written");
   }
   // what is written has a new version: autograd refuses what it saved of it (and
   // inference tensors are not written outside inference mode)

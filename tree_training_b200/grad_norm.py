@@ -26,7 +26,8 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float, norm_type: fl
 
     In place, or into ``out`` (one tensor for each gradient, of its shape, type and
     strides; it may be the gradient itself).  ``norm`` [1 element, fp32, on the
-    device]: go by this norm (one summed over ranks, say) instead of computing it.
+    device, no part of what is written]: go by this norm (one summed over ranks, say)
+    instead of computing it.
     Where the norm is not finite the factor is 0 or NaN, as the formula gives it.
 
     Tensors that are written must fill their memory without gaps, and none may share
