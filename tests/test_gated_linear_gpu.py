@@ -278,3 +278,54 @@ def test_widths_that_32_bits_do_not_count():
     wide = one.expand(1, (1 << 31) - 257)
     with pytest.raises(ValueError):
         tt.gated_linear(wide, wide, wide)
+
+
+def test_modules_that_are_wrapped_or_watched_keep_their_forward():
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.qwen3.modeling_qwen3 import Qwen3MLP
+    cfg = transformers.Qwen3Config(hidden_size=64, intermediate_size=96, num_hidden_layers=1)
+
+    class Dropping(Qwen3MLP):
+        def forward(self, x):
+            return torch.nn.functional.dropout(super().forward(x), 0.5, self.training)
+
+    class Normed(Qwen3MLP):
+        def __init__(self, cfg):
+            super().__init__(cfg)
+            self.norm = torch.nn.LayerNorm(64)
+    seen = []
+    wrapped, hooked, double, plain = (Qwen3MLP(cfg) for _ in range(4))
+    forward = wrapped.forward
+    wrapped.forward = lambda x: (seen.append(1), forward(x))[1]
+    hooked.up_proj.register_forward_hook(lambda *a: seen.append(2))
+    m = torch.nn.ModuleList([wrapped, hooked, double.double(), Dropping(cfg), Normed(cfg)]).to(DEV)
+    m.eval()
+    state = torch.cuda.get_rng_state(), torch.get_rng_state()
+    assert tt.fuse_gated_mlps(m) == 0
+    assert torch.equal(torch.cuda.get_rng_state(), state[0])
+    assert torch.equal(torch.get_rng_state(), state[1])
+    assert not any(b.training for b in m)
+    seen.clear()
+    x = torch.randn(3, 64, device=DEV)
+    wrapped(x), hooked(x)
+    assert seen == [1, 2]
+    plain = torch.nn.ModuleList([plain]).to(DEV)
+    assert tt.fuse_gated_mlps(plain) == 1 and tt.fuse_gated_mlps(plain) == 0
+
+
+def test_fused_and_then_checkpointed():
+    from types import SimpleNamespace
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.qwen3.modeling_qwen3 import Qwen3MLP
+    from tree_training_b200.hybrid import checkpoint_mlps
+    cfg = transformers.Qwen3Config(hidden_size=64, intermediate_size=96, num_hidden_layers=1)
+    mlp = Qwen3MLP(cfg).to(DEV)
+    x = torch.randn(5, 64, device=DEV, requires_grad=True)
+    ps = [x, *mlp.parameters()]
+    assert tt.fuse_gated_mlps(torch.nn.ModuleList([mlp])) == 1
+    want = torch.autograd.grad(mlp(x).sum(), ps)
+    layer = SimpleNamespace(mlp=mlp)
+    assert checkpoint_mlps(SimpleNamespace(model=SimpleNamespace(layers=[layer]))) == 1
+    got = torch.autograd.grad(mlp(x).sum(), ps)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))     # the same kernels, run again
+    assert tt.fuse_gated_mlps(torch.nn.ModuleList([mlp])) == 0   # (and the wrapper stays)

@@ -44,14 +44,25 @@ def _activation_of(fn):
 @torch.no_grad()
 def _is_plain(mod) -> bool:
     """Whether the module's forward is down(act(gate(x)) * up(x)) and nothing else
-    (no dropout, sparsity or clamp), by what it gives for a few rows."""
+    (no dropout, sparsity or clamp), by what it gives for a few rows in training."""
     w = mod.gate_proj.weight
     x = torch.linspace(-3, 3, 4 * w.shape[1], dtype=torch.float32).view(4, -1).sin()
     x = x.to(w.device, w.dtype)
-    y = mod.forward(x)
+    training = mod.training
+    mod.training = True
+    try:
+        with torch.random.fork_rng(devices=[w.device] if w.is_cuda else []):
+            y = mod.forward(x)
+    finally:
+        mod.training = training
     want = mod.down_proj(mod.act_fn(mod.gate_proj(x)) * mod.up_proj(x))
     return isinstance(y, torch.Tensor) and y.shape == want.shape and \
         torch.allclose(y.float(), want.float(), rtol=2e-2, atol=1e-3 * float(want.abs().max()))
+
+
+def _has_hooks(mod) -> bool:
+    return any(getattr(mod, a) for a in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks",
+                                         "_backward_pre_hooks"))
 
 
 def _gated_mlp_forward(self, x):
@@ -62,12 +73,19 @@ def _gated_mlp_forward(self, x):
 def fuse_gated_mlps(model) -> int:
     """Routes every gated feed-forward module of an HF model (``gate_proj``,
     ``up_proj`` and ``down_proj`` without biases, ``act_fn`` one of the activations)
-    through :func:`gated_linear`.  Returns how many modules were patched; modules
-    of another form (or whose forward does more than that) keep their own forward."""
+    through :func:`gated_linear`.  Returns how many modules were patched; modules of
+    another form or type keep their own forward, and so do those whose forward does
+    more than that, has been replaced (by this function or another: wrap it after
+    this call, as ``checkpoint_mlps`` does), or whose gate or up projection has hooks."""
     n = 0
     for mod in model.modules():
         parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
-        if not all(type(p) is torch.nn.Linear for p in parts) or not hasattr(mod, "act_fn"):
+        if not all(type(p) is torch.nn.Linear for p in parts) or not hasattr(mod, "act_fn") \
+                or getattr(mod.forward, "__func__", None) is not type(mod).forward \
+                or _has_hooks(parts[0]) or _has_hooks(parts[1]):
+            continue
+        if parts[0].weight.dtype not in (torch.float32, torch.bfloat16, torch.float16) or \
+                any(c not in (*parts, mod.act_fn) for c in mod.children()):
             continue
         name = _activation_of(mod.act_fn)
         if name is None or parts[0].bias is not None or parts[1].bias is not None \
