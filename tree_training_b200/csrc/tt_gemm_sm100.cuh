@@ -523,7 +523,9 @@ inline int64_t slice_clocks(int cg, int bn) {
 // over 64 tokens: 39 us by pairs, 29 by single CTAs; over 512: 52 and 48).  The gated
 // product's is longer than that wait (8,192 x 256 x 1,024: 31 us by pairs, 39).
 inline int64_t epilogue_clocks(int cg, int bn, bool dual) {
-  return (dual ? 8000 : cg == 1 ? 5000 : 8000) * bn / 256;
+  // (a warp has 32 columns of every 64: a few of 64 take as long as all)
+  const int blocks = ((dual ? bn / 2 : bn) + 63) / 64;
+  return dual ? 4000 * blocks : (cg == 1 ? 1250 : 2000) * blocks;
 }
 
 // The cheapest of the forms by the tiles' waves.  `n_step`: what widths of the
@@ -637,7 +639,7 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
 
 // A 32 x 32 block of C: each lane 32 values of a row of its own at `p` (null: none), of
 // which `left` are in C.  Where rows are on 16-byte boundaries (wide) a lane stores its
-// own; else the warp stores row after row out of shared memory, 32 elements next to
+// own, of a narrower block as many packs as are whole; else the warp stores row after row out of shared memory, 32 elements next to
 // one another (elements of 32 rows at a time cost an odd width three times the rest).
 template <typename T>
 __device__ __forceinline__ void store_block(T* p, const float (&v)[32], int left, bool wide,
@@ -658,6 +660,23 @@ __device__ __forceinline__ void store_block(T* p, const float (&v)[32], int left
       } else {
         *reinterpret_cast<uint4*>(p + i) = a;
         *reinterpret_cast<uint4*>(p + i + V) = b;
+      }
+    }
+    return;
+  }
+  if (wide) {
+    if (!p) return;
+#pragma unroll
+    for (int i = 0; i < 32; i += V) {
+      if (i + V <= left) {
+        float w[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = v[i + j];
+        vec::store<T, V>(p + i, w);
+      } else if (i < left) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (i + j < left) p[i + j] = from_f32<T>(v[i + j]);
       }
     }
     return;
