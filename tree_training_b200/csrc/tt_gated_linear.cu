@@ -19,8 +19,8 @@
 //
 // Up to kFewRows tokens (a rollout's single ones) no tensor core is needed: a warp a
 // feature reads its two rows once, 16 bytes a lane, and multiplies by fma (2,560 x
-// 9,728 bf16: 21 us a token, 25 two; the tensor cores take 29 for 3 to 128 tokens, fma
-// 33 for three).
+// 9,728 bf16: 21 us a token, 25 two; the tensor cores take 23 to 25 for 2 to 128 tokens,
+// so that two go there if the weights are large: 1,024 x 4,096 8 us and 13).
 //
 // fp32: the products on the CUDA cores (see tt_gemm_fp32.cu), h by a pass over g and u.
 //
@@ -148,6 +148,7 @@ struct GatedEpi {
 
 constexpr int kFewRows = 2;
 constexpr int kFewBytes = 40960;           // of x in shared memory
+constexpr int64_t kFewWeights = 1 << 24;   // elements of a weight, for two rows
 
 // A warp a feature, N rows of x.
 template <typename T, int A, int N>
@@ -303,7 +304,8 @@ int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void*
     const gemm::Factor all[3] = {{x, x_ld, false}, {wg, wg_ld, false}, {wu, wu_ld, false}};
     for (const gemm::Factor& f : all)
       if (!gemm::copyable(f)) return TT_ERR_UNSUPPORTED;
-    if (T <= kFewRows && T * ((H + 7) / 8) * 16 <= kFewBytes)
+    if (T <= kFewRows && T * ((H + 7) / 8) * 16 <= kFewBytes &&
+        (T == 1 || (int64_t)H * F <= kFewWeights))
       return few_rows<typename std::conditional<kB, __nv_bfloat16, __half>::type,
                       decltype(a)::value>(x, x_ld, wg, wg_ld, wu, wu_ld, (int)T, H, F, h, g, u,
                                           keep_ld, st);
