@@ -592,6 +592,10 @@ int tt_embedding_bwd(int dtype, int64_t n, int64_t V, int32_t H, const void* ids
  * next multiple of 8 are zeroed. */
 int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
                   int64_t dst_ld, void* stream);
+/* The same for up to four arrays (host arrays of `count`) in one launch. */
+int tt_align_rows_of(int32_t count, const int64_t* rows, const int64_t* cols,
+                     const void* const* src, const int64_t* ld, void* const* dst,
+                     const int64_t* dst_ld, void* stream);
 
 /* ---- the gated half of a feed-forward block --------------------------------- *
  * h = act(x wg^T) * (x wu^T): x [T, H], wg and wu [F, H], h [T, F] contiguous; act

@@ -212,3 +212,20 @@ def test_a_workspace_off_its_boundary(call):
 @pytest.mark.parametrize("call", [ce, ce_bwd])
 def test_kept_logits_off_their_boundary(call):
     assert call(dtype=F32, kept=P + 16) == INVALID
+
+
+def align_many(n=2, rows=4, cols=9, src=P, ld=9, dst=P, dst_ld=16, null=None):
+    I, V = ctypes.c_int64 * max(n, 1), ctypes.c_void_p * max(n, 1)
+    tables = [I(*[rows] * n), I(*[cols] * n), V(*[src] * n), I(*[ld] * n), V(*[dst] * n),
+              I(*[dst_ld] * n)]
+    return status("tt_align_rows_of", n, *[None if i == null else t for i, t in enumerate(tables)],
+                  None)
+
+
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=5), dict(rows=-1), dict(cols=0), dict(ld=8),
+                                 dict(dst_ld=8), dict(dst_ld=17), dict(src=None), dict(dst=None),
+                                 dict(dst=P + 8), dict(src=P + 1), *[dict(null=i) for i in range(6)]])
+def test_align_rows_of(bad):
+    assert align_many(**bad) == INVALID
+    assert align_many(n=0) == _lib.TT_OK
+    assert align_many(rows=0, src=None, dst=None) == _lib.TT_OK

@@ -118,6 +118,7 @@ SIGNATURES = {
     "tt_embedding_bwd": (_INT, [_INT, _I64, _I64, _I32, _P, _INT, _P, _I64, _F32, _I64, _P, _P,
                                 _I64, _P]),
     "tt_align_rows": (_INT, [_I64, _I64, _P, _I64, _P, _I64, _P]),
+    "tt_align_rows_of": (_INT, [_I32, _P, _P, _P, _P, _P, _P, _P]),
     "tt_gated_linear_fwd_workspace_size": (_I64, [_INT, _I64, _I32, _I32]),
     "tt_gated_linear_fwd": (_INT, [_INT, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _INT, _P,
                                    _P, _P, _I64, _P, _I64, _P, _P]),

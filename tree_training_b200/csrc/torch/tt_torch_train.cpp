@@ -16,22 +16,32 @@ Tensor bytes(int64_t n, const Tensor& like) { return empty({std::max<int64_t>(n,
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // [rows, n] with unit last stride whose rows the tensor cores' copies can read: on
-// 16-byte boundaries (else a padded copy).  fp32 rows as they are.
-Tensor rows16(const Tensor& t_) {
-  const Tensor t = rows2d(t_);
-  if (t.scalar_type() == at::kFloat) return t;
-  if (t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0) return t;
-  if (t.size(0) == 1 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 &&
-      t.size(1) % 8 == 0)
-    return t;
-  const int64_t ld = pad8(t.size(1));
-  Tensor c = empty({t.size(0), ld}, t, t.scalar_type());
-  On on(t);
-  check_status("tt_align_rows", tt_align_rows(t.size(0), t.size(1), ptr(t),
-                                              std::max(t.stride(0), t.size(1)), out(c), ld,
-                                              on.stream));
+// 16-byte boundaries (else padded copies, all by one launch).  fp32 rows as they are.
+template <size_t N>
+std::array<Tensor, N> rows16(const std::array<const Tensor*, N>& ts) {
+  std::array<Tensor, N> r, copy;
+  int64_t rows[N], cols[N], ld[N], to_ld[N];
+  const void* src[N];
+  void* dst[N];
+  int32_t n = 0;
+  for (size_t i = 0; i < N; ++i) {
+    const Tensor& t = r[i] = rows2d(*ts[i]);
+    if (t.scalar_type() == at::kFloat) continue;
+    if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 &&
+        (t.stride(0) % 8 == 0 || (t.size(0) == 1 && t.size(1) % 8 == 0)))
+      continue;
+    copy[i] = empty({t.size(0), pad8(t.size(1))}, t, t.scalar_type());
+    rows[n] = t.size(0), cols[n] = t.size(1), ld[n] = std::max(t.stride(0), t.size(1));
+    to_ld[n] = pad8(t.size(1)), src[n] = ptr(t), dst[n++] = out(copy[i]);
+  }
+  if (n == 0) return r;
+  On on(r[0]);
+  check_status("tt_align_rows_of",
+               tt_align_rows_of(n, rows, cols, src, ld, dst, to_ld, on.stream));
   at::NoGradGuard no_grad;
-  return c.narrow(1, 0, t.size(1));
+  for (size_t i = 0; i < N; ++i)
+    if (copy[i].defined()) r[i] = copy[i].narrow(1, 0, r[i].size(1));
+  return r;
 }
 
 // The stride of rows (of one row: its own width, rounded up).
@@ -141,7 +151,7 @@ Gated gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
 struct GatedFunction : Function<GatedFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
                         int64_t act) {
-    const Tensor x2 = rows16(x), g2 = rows16(wg), u2 = rows16(wu);
+    const auto [x2, g2, u2] = rows16<3>({&x, &wg, &wu});
     Gated r = gated_forward(x2, g2, u2, act, true);
     // (with odd widths the copies that were made)
     ctx->save_for_backward({x2, g2, u2, r.g, r.u});
@@ -203,8 +213,10 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
   Tensor h;
   if (wants_grad({&x, &wg, &wu}))
     h = GatedFunction::apply(x2, wg, wu, act);
-  else
-    h = gated_forward(rows16(x2), rows16(wg), rows16(wu), act, false).h;
+  else {
+    const auto [xr, gr, ur] = rows16<3>({&x2, &wg, &wu});
+    h = gated_forward(xr, gr, ur, act, false).h;
+  }
   if (x.dim() == 2) return h;
   auto sizes = x.sizes().vec();
   sizes.back() = wg.size(0);
@@ -240,7 +252,7 @@ CE ce_forward(const Tensor& x, const Tensor& w, const Tensor& labels, double sca
 struct LinearCEFunction : Function<LinearCEFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
                                const Tensor& labels, double scale, bool flat) {
-    const Tensor x2 = rows16(x), w2 = rows16(w);
+    const auto [x2, w2] = rows16<2>({&x, &w});
     CE r = ce_forward(x2, w2, labels, scale, flat, true);
     // (with odd widths the copies that were made)
     ctx->save_for_backward({x2, w2, labels, r.lse, r.kept});
@@ -310,7 +322,8 @@ std::tuple<Tensor, Tensor> linear_cross_entropy(const Tensor& x_, const Tensor& 
     variable_list v = LinearCEFunction::apply(x_, w, labels, scale, labels_.dim() == 1);
     losses = v[0], lse = v[1];
   } else {
-    CE r = ce_forward(rows16(x_), rows16(w), labels, scale, labels_.dim() == 1, false);
+    const auto [x, wr] = rows16<2>({&x_, &w});
+    CE r = ce_forward(x, wr, labels, scale, labels_.dim() == 1, false);
     losses = r.losses, lse = r.lse;
   }
   return {losses, lse};

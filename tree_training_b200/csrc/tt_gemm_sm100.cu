@@ -137,17 +137,30 @@ int product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& 
   });
 }
 
-// 16-bit rows onto 16-byte boundaries, in packs of 8; columns past the last are zero.
-__global__ void __launch_bounds__(256)
-    align_rows_kernel(const __nv_bfloat16* src, int64_t ld, int64_t rows, int64_t cols,
-                      __nv_bfloat16* dst, int64_t dst_ld) {
-  const __nv_bfloat16* hi = src + (rows - 1) * ld + cols;
-  const int64_t packs = (cols + 7) / 8;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int64_t p = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; p < packs;
-         p += (int64_t)gridDim.x * blockDim.x)
-      *reinterpret_cast<uint4*>(dst + r * dst_ld + p * 8) =
-          vec::load_any_of<__nv_bfloat16>(src + r * ld, p * 8, cols, src, hi);
+// 16-bit rows of up to kMaxAligned arrays onto 16-byte boundaries, in packs of 8; columns
+// past the last are zero.  A block a row, or 128 packs of a longer one.
+constexpr int kMaxAligned = 4, kAlignThreads = 128;
+
+struct Aligned {
+  const __nv_bfloat16* src[kMaxAligned];
+  __nv_bfloat16* dst[kMaxAligned];
+  int64_t ld[kMaxAligned], dst_ld[kMaxAligned], rows[kMaxAligned], cols[kMaxAligned];
+  int64_t pieces[kMaxAligned];             // of a row
+  int64_t first[kMaxAligned + 1];          // piece of an array
+};
+
+__global__ void __launch_bounds__(kAlignThreads) align_rows_kernel(const __grid_constant__ Aligned a) {
+  for (int64_t i = blockIdx.x; i < a.first[kMaxAligned]; i += gridDim.x) {
+    int t = 0;
+#pragma unroll
+    for (int k = 1; k < kMaxAligned; ++k) t = i >= a.first[k] ? k : t;
+    const int64_t at = i - a.first[t], n = a.pieces[t];
+    const int64_t r = n == 1 ? at : at / n, p = (at - r * n) * kAlignThreads + threadIdx.x;
+    if (p * 8 >= a.cols[t]) continue;
+    const __nv_bfloat16* src = a.src[t];
+    *reinterpret_cast<uint4*>(a.dst[t] + r * a.dst_ld[t] + p * 8) = vec::load_any_of<__nv_bfloat16>(
+        src + r * a.ld[t], p * 8, a.cols[t], src, src + (a.rows[t] - 1) * a.ld[t] + a.cols[t]);
+  }
 }
 
 }  // namespace
@@ -169,19 +182,38 @@ int tc_product(bool bf16, int64_t M, int64_t N, const Term* terms, int n_terms, 
 }  // namespace gemm
 }  // namespace tt
 
-extern "C" int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
-                             int64_t dst_ld, void* stream) {
-  if (rows < 0 || cols < 1 || (rows > 1 && ld < cols) || dst_ld < cols || dst_ld % 8 != 0)
+extern "C" int tt_align_rows_of(int32_t count, const int64_t* rows, const int64_t* cols,
+                                const void* const* src, const int64_t* ld, void* const* dst,
+                                const int64_t* dst_ld, void* stream) {
+  using namespace tt::gemm;
+  if (count < 0 || count > kMaxAligned ||
+      (count > 0 && (!rows || !cols || !src || !ld || !dst || !dst_ld)))
     return TT_ERR_INVALID_ARG;
-  if (rows == 0) return TT_OK;
-  if (!src || !dst || (reinterpret_cast<uintptr_t>(dst) & 15) ||
-      (reinterpret_cast<uintptr_t>(src) & 1))
-    return TT_ERR_INVALID_ARG;
-  const int64_t packs = (cols + 7) / 8;
-  const dim3 grid((unsigned)std::min<int64_t>((packs + 255) / 256, 64),
-                  (unsigned)std::min<int64_t>(rows, 65535));
-  tt::gemm::align_rows_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
-      (const __nv_bfloat16*)src, ld, rows, cols, (__nv_bfloat16*)dst, dst_ld);
+  Aligned a{};
+  for (int i = 0; i < kMaxAligned; ++i) {
+    a.first[i + 1] = a.first[i];
+    if (i >= count) continue;
+    if (rows[i] < 0 || cols[i] < 1 || (rows[i] > 1 && ld[i] < cols[i]) || dst_ld[i] < cols[i] ||
+        dst_ld[i] % 8 != 0)
+      return TT_ERR_INVALID_ARG;
+    if (rows[i] == 0) continue;
+    if (!src[i] || !dst[i] || (reinterpret_cast<uintptr_t>(dst[i]) & 15) ||
+        (reinterpret_cast<uintptr_t>(src[i]) & 1))
+      return TT_ERR_INVALID_ARG;
+    a.src[i] = (const __nv_bfloat16*)src[i], a.dst[i] = (__nv_bfloat16*)dst[i];
+    a.ld[i] = ld[i], a.dst_ld[i] = dst_ld[i], a.rows[i] = rows[i], a.cols[i] = cols[i];
+    a.pieces[i] = (cols[i] + 8 * kAlignThreads - 1) / (8 * kAlignThreads);
+    a.first[i + 1] += rows[i] * a.pieces[i];
+  }
+  const int64_t pieces = a.first[kMaxAligned];
+  if (pieces == 0) return TT_OK;
+  align_rows_kernel<<<(unsigned)std::min<int64_t>(pieces, 16 * tt::vec::kSMs), kAlignThreads, 0,
+                      (cudaStream_t)stream>>>(a);
   tt_count_launches(1);
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
+extern "C" int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
+                             int64_t dst_ld, void* stream) {
+  return tt_align_rows_of(1, &rows, &cols, &src, &ld, &dst, &dst_ld, stream);
 }
