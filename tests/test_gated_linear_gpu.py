@@ -329,3 +329,29 @@ def test_fused_and_then_checkpointed():
     got = torch.autograd.grad(mlp(x).sum(), ps)
     assert all(torch.equal(a, b) for a, b in zip(got, want))     # the same kernels, run again
     assert tt.fuse_gated_mlps(torch.nn.ModuleList([mlp])) == 0   # (and the wrapper stays)
+
+
+@pytest.mark.parametrize("T,H,F", [(208, 4288, 4544), (1024, 2560, 4864), (300, 8192, 4096),
+                                   (130, 1001, 2735)])
+def test_signs_of_products_near_zero(T, H, F):
+    """relu is open where the product is above 0, whatever the sums' own error: a sum in
+    64 bits of products of bf16 (exact) errs by H 2^-53 of its terms' magnitudes."""
+    x, wg, wu, _ = make(T, H, F, BF, seed=7)
+    g = torch.cat([x.double() @ w.double().t() for w in wg.split(1024)], 1)
+    size = torch.cat([x.abs().double() @ w.abs().double().t() for w in wg.split(1024)], 1)
+    h = tt.gated_linear(x, wg, wu, activation="relu")
+    tt.check_device_status()
+    u = torch.cat([x.double() @ w.double().t() for w in wu.split(1024)], 1)
+    sure = (g.abs() > H * 2.0 ** -53 * size) & (u.abs() > 1e-3) & (g.abs() > 1e-30)
+    wrong = sure & ((h != 0) != (g > 0))
+    assert int(wrong.sum()) == 0, g[wrong]
+
+
+def test_rows_of_zeros_and_of_very_different_sizes():
+    """Products of exactly 0, and rows in which nearly all are small beside one: as every
+    other activation's (no sum is formed again for them, or few are)."""
+    x, wg, wu, dh = make(300, 512, 1000, BF, seed=8)
+    wg[::3] = 0
+    wg[1::64] *= 2.0 ** 20
+    x[::7] = 0
+    compare(x, wg, wu, dh, "relu")

@@ -108,6 +108,81 @@ int dispatch_act(int act, F f) {
   }
 }
 
+// relu's slope jumps at 0: of a product that the tensor cores' cut-off sums leave within
+// their own error of 0 (208 x 4,288 x 4,544: one of 945,000, which was 1.5e-3 of a weight's
+// gradient) the sign is found again, by a sum in 64 bits.  Their error is about 2^-24 of
+// the sums on the way for every 16 of k; these are as large as the row's other products.
+// The whole warp forms such a sum; a row with more than kMostDoubts of them in 32 is
+// left as it is (columns of very different sizes: the estimate says nothing there).  It
+// costs the forward 3 to 15% (64 x 2,560 x 9,728 23.1 -> 25.5 us, 4,096 x 1,536 x 4,096 67
+// -> 78, 8,192 x 2,560 x 9,728 kept 600 -> 632), a pass with gradients a quarter of that.
+constexpr int kMostDoubts = 4;
+
+struct Doubts {
+  const void *x, *w;
+  int64_t x_ld, w_ld;
+  int H;
+  float share;                             // of the sum of 32 products' magnitudes
+};
+
+template <typename T>
+__device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live, int feature,
+                                             int left, float (&g)[32]) {
+  const int lane = threadIdx.x & 31;
+  float sum_of[2] = {0.f, 0.f}, least[2] = {INFINITY, INFINITY};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    sum_of[i & 1] += fabsf(g[i]);
+    least[i & 1] = fminf(least[i & 1], fabsf(g[i]));
+  }
+  const float doubt = (sum_of[0] + sum_of[1]) * d.share;
+  if (!__any_sync(0xffffffffu, live && fminf(least[0], least[1]) < doubt)) return;
+  uint32_t mask = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (live && i < left && g[i] != 0.f && fabsf(g[i]) < doubt) mask |= 1u << i;
+  if (__popc(mask) > kMostDoubts) mask = 0;
+  for (uint32_t who; (who = __ballot_sync(0xffffffffu, mask != 0)) != 0;) {
+    const int from = __ffs(who) - 1;
+    const int i = __shfl_sync(0xffffffffu, __ffs(mask) - 1, from);
+    const T* a = reinterpret_cast<const T*>(d.x) + (int64_t)__shfl_sync(0xffffffffu, row, from) * d.x_ld;
+    const T* b = reinterpret_cast<const T*>(d.w) + (int64_t)(feature + i) * d.w_ld;
+    constexpr int kAhead = 5;              // packs of a row that are fetched together
+    double sum = 0.0, more = 0.0;
+    for (int64_t p0 = lane * 8; p0 < d.H; p0 += 256 * kAhead) {
+      uint4 ra[kAhead], rb[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t p = p0 + 256 * k;
+        const bool whole = p + 8 <= d.H;
+        ra[k] = whole ? __ldg(reinterpret_cast<const uint4*>(a + p))
+                      : vec::load_any_of<T>(a, p, d.H, a, a);
+        rb[k] = whole ? __ldg(reinterpret_cast<const uint4*>(b + p))
+                      : vec::load_any_of<T>(b, p, d.H, b, b);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        float va[8], vb[8];
+        vec::unpack<T, 8>(ra[k], va);
+        vec::unpack<T, 8>(rb[k], vb);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          sum = fma((double)va[j], (double)vb[j], sum);
+          more = fma((double)va[j + 1], (double)vb[j + 1], more);
+        }
+      }
+    }
+    sum += more;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == from) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (i == j) g[j] = (float)sum;
+      mask &= mask - 1;
+    }
+  }
+}
+
 template <bool kB, int A>
 struct GatedEpi {
   static constexpr bool kBf16 = kB, kChunks = false;
@@ -117,6 +192,7 @@ struct GatedEpi {
     float *g, *u;                          // null: not kept
     int64_t keep_ld;
     int F, wide;
+    Doubts doubts;
   };
   static __device__ __forceinline__ void tile(const Args& a, const gemm::Problem& p,
                                               const gemm::TileAt& t, int row, uint32_t acc, int c0,
@@ -129,6 +205,7 @@ struct GatedEpi {
       __syncwarp();                          // (the loads are the whole warp's)
       sm100::tmem_ld32x2(acc + c, acc + half + c, g, u);
       const int left = cols - c;
+      if constexpr (A == kRelu) settle_signs<T>(a.doubts, row, live, n0 + c, left, g);
       if (a.g) {
         const int64_t at = (int64_t)row * a.keep_ld + n0 + c;
         gemm::store_block(live ? a.g + at : nullptr, g, left, true, block);
@@ -318,6 +395,7 @@ int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void*
     if (!gemm::set_up(&q, plan, kB, T, F, terms, 2, true, status)) return TT_ERR_UNSUPPORTED;
     typename Epi::Args ea{};
     ea.h = h, ea.h_ld = F, ea.g = g, ea.u = u, ea.keep_ld = keep_ld, ea.F = F;
+    ea.doubts = {x, wg, x_ld, wg_ld, H, (float)(H / 16 + 4) * 0x1p-29f};
     ea.wide = F % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
     return gemm::launch<false, false, Epi>(plan, q, ea, st);
   });
