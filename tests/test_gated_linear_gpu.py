@@ -355,3 +355,9 @@ def test_rows_of_zeros_and_of_very_different_sizes():
     wg[1::64] *= 2.0 ** 20
     x[::7] = 0
     compare(x, wg, wu, dh, "relu")
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 7, 8, 13, 16, 17])
+@pytest.mark.parametrize("H,F", [(1001, 735), (4096, 520), (256, 9001)])
+def test_few_rows_of_fp32(T, H, F):
+    compare(*make(T, H, F, F32, seed=T))

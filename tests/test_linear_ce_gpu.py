@@ -253,3 +253,9 @@ def test_widths_that_32_bits_do_not_count():
     with pytest.raises(ValueError):
         tt.linear_cross_entropy(one, one.expand((1 << 31) - 256, 1),
                                 torch.zeros(1, device="cuda", dtype=torch.int64))
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 7, 8, 13, 16, 17])
+@pytest.mark.parametrize("H,V", [(1001, 735), (2048, 333), (96, 20001)])
+def test_few_rows_of_fp32(T, H, V):
+    compare(*make(T, H, V, 2, torch.float32, seed=T))

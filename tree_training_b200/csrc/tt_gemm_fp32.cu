@@ -8,7 +8,7 @@
 // 64 where there are few rows or tiles, which would leave SMs idle); slices of 16 of k
 // are loaded into registers while the slice before is multiplied out of shared memory.
 // Bound by the fma rate (measured on a B200 at 4,096 a side: 51 to 58 TFLOP/s of 74; the
-// library's 57).  Where there are few tiles the sum over k is split over blocks, whose
+// library's 57).  Up to eight rows have kernels of their own.  Where there are few tiles the sum over k is split over blocks, whose
 // parts are added up in order by a second kernel.
 #include <algorithm>
 
@@ -172,6 +172,147 @@ __global__ void __launch_bounds__(kThreads, 2) product_kernel(const Args a) {
   }
 }
 
+// ---- few rows ---------------------------------------------------------------------
+//
+// Up to kFewRows rows of A: bound by B's bytes; a tile of 64 rows would spend its time on
+// rows that are not there.  Both products of 2,560 x 9,728 (200 MB): 40 us one row, 41
+// two, 55 four, 91 eight, where tiles take 214 to 220; A comes out of L1, whose loads bound
+// it from four rows on (two rows of B a warp and two steps ahead; four of either: 62 to 67
+// and 117 to 127).  For 16 it would be 180 to 400, tiles 225.
+
+constexpr int kFewRows = 8;
+
+// Four elements at p, of which `left` are there.
+__device__ __forceinline__ float4 load4(const float* p, int64_t left) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (left > 0) v.x = __ldg(p);
+  if (left > 1) v.y = __ldg(p + 1);
+  if (left > 2) v.z = __ldg(p + 2);
+  if (left > 3) v.w = __ldg(p + 3);
+  return v;
+}
+
+// Rows of B contiguous in k: a warp R rows of B, its lanes over k, R x MR sums a lane.
+template <int MR, int R>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const Args a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = blockIdx.y;
+  const int64_t n0 = ((int64_t)blockIdx.x * (kThreads / 32) + warp) * R;
+  if (n0 >= a.N) return;
+  float acc[MR][R];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[m][r] = 0.f;
+  const int last = a.batch > 1 ? which + 1 : a.terms;
+  for (int term = which; term < last; ++term) {
+    const float* rows[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      rows[r] = a.b[term] + min(n0 + r, (int64_t)a.N - 1) * a.b_ld[term];
+    const int64_t K = a.k[term];
+    auto step = [&](int64_t k, auto load) {
+      float4 b[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) b[r] = load(rows[r] + k);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const float4 x = load(a.a[term] + (int64_t)min(m, a.M - 1) * a.a_ld[term] + k);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          acc[m][r] = fmaf(x.x, b[r].x, acc[m][r]);
+          acc[m][r] = fmaf(x.y, b[r].y, acc[m][r]);
+          acc[m][r] = fmaf(x.z, b[r].z, acc[m][r]);
+          acc[m][r] = fmaf(x.w, b[r].w, acc[m][r]);
+        }
+      }
+    };
+    // (a loop without branches: its loads wait for none)
+    const int64_t whole = a.vec_a && a.vec_b ? K / 4 * 4 : 0;
+#pragma unroll 2
+    for (int64_t k = lane * 4; k < whole; k += 128)
+      step(k, [](const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); });
+    for (int64_t k = whole + lane * 4; k < K; k += 128)
+      step(k, [&](const float* p) { return load4(p, K - k); });
+  }
+  const float alpha = a.alpha * (a.alpha_dev ? *a.alpha_dev : 1.f);
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v = acc[m][r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == (m * R + r) % 32 && m < a.M && n0 + r < a.N) {
+        v *= alpha;
+        if (a.cin) v += a.cin[m * a.cin_ld + n0 + r];
+        a.c[which][m * a.c_ld + n0 + r] = v;
+      }
+    }
+}
+
+// Columns of B contiguous: a thread four columns and all rows, over a part of k, of which
+// A's elements stand in shared memory.
+constexpr int kFewThreads = 128, kFewK = 64;
+
+template <int MR>
+__global__ void __launch_bounds__(kFewThreads) few_columns_kernel(const Args a) {
+  constexpr int kAhead = 8;                // rows of B fetched together
+  __shared__ float sa[kFewK][MR];
+  const int part = blockIdx.y % a.parts, which = blockIdx.y / a.parts;
+  const int64_t col = ((int64_t)blockIdx.x * kFewThreads + threadIdx.x) * 4, left = a.N - col;
+  float4 acc[MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) acc[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+  int64_t from = part * a.k_part, to = from + a.k_part;
+  const int last = a.batch > 1 ? which + 1 : a.terms;
+  for (int term = which; term < last; ++term) {
+    const int64_t k_all = a.k[term];
+    const int64_t kb = min(max(from, (int64_t)0), k_all), ke = min(max(to, (int64_t)0), k_all);
+    from -= k_all, to -= k_all;
+    for (int64_t k0 = kb; k0 < ke; k0 += kFewK) {
+      const int n = (int)min((int64_t)kFewK, ke - k0);
+      __syncthreads();                     // (the rows before are multiplied)
+      for (int i = threadIdx.x; i < kFewK * MR; i += kFewThreads) {
+        const int m = i / kFewK, kk = i % kFewK;
+        sa[kk][m] = m < a.M && kk < n ? __ldg(a.a[term] + m * a.a_ld[term] + k0 + kk) : 0.f;
+      }
+      __syncthreads();
+      const float* b = a.b[term] + k0 * a.b_ld[term] + col;
+      for (int k = 0; k < n; k += kAhead) {
+        float4 y[kAhead];
+        if (a.vec_b && left >= 4 && k + kAhead <= n) {
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j)
+            y[j] = __ldg(reinterpret_cast<const float4*>(b + (k + j) * a.b_ld[term]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j)
+            y[j] = load4(b + (k + j) * a.b_ld[term], k + j < n ? left : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+            const float x = sa[k + j][m];
+            acc[m].x = fmaf(x, y[j].x, acc[m].x), acc[m].y = fmaf(x, y[j].y, acc[m].y);
+            acc[m].z = fmaf(x, y[j].z, acc[m].z), acc[m].w = fmaf(x, y[j].w, acc[m].w);
+          }
+      }
+    }
+  }
+  const float alpha = a.alpha * (a.alpha_dev ? *a.alpha_dev : 1.f);
+  float* c = a.c[which] + part * a.c_part;
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+    if (m >= a.M) continue;
+    const float v[4] = {acc[m].x, acc[m].y, acc[m].z, acc[m].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left)
+        c[m * a.c_ld + col + j] = v[j] * alpha + (a.cin ? a.cin[m * a.cin_ld + col + j] : 0.f);
+  }
+}
+
 // C = the parts, added up in order, + cin; blockIdx.y: of a batch.  A block 32 elements
 // at a time, each warp a run of the parts.
 __global__ void __launch_bounds__(256)
@@ -228,6 +369,39 @@ Form form_of(int64_t M, int64_t N, int64_t k, int batch, bool split) {
   return best;
 }
 
+// Parts of a sum whose B has contiguous columns, for few rows: eight blocks an SM, parts
+// of 32 of k at least, and no more bytes of parts, there and back, than half of B's.
+int64_t few_parts(int64_t M, int64_t N, int64_t k, int batch) {
+  const int64_t blocks = (N + 4 * kFewThreads - 1) / (4 * kFewThreads) * batch;
+  return std::max<int64_t>(1, std::min({8 * vec::kSMs / blocks, k / 32, k / (4 * M)}));
+}
+
+template <int MR>
+void launch_few(const Args& a, bool bmn, cudaStream_t st) {
+  if (bmn) {
+    const dim3 grid((unsigned)((a.N + 4ll * kFewThreads - 1) / (4 * kFewThreads)),
+                    (unsigned)(a.parts * a.batch));
+    few_columns_kernel<MR><<<grid, kFewThreads, 0, st>>>(a);
+    return;
+  }
+  // (two rows of B share the loads of A, where that leaves eight warps an SM)
+  constexpr int R = 2, W = kThreads / 32;
+  if ((int64_t)a.N * a.batch >= (int64_t)R * W * vec::kSMs)
+    few_rows_kernel<MR, R><<<dim3((unsigned)((a.N + R * W - 1) / (R * W)), a.batch), kThreads, 0,
+                             st>>>(a);
+  else
+    few_rows_kernel<MR, 1><<<dim3((unsigned)((a.N + W - 1) / W), a.batch), kThreads, 0, st>>>(a);
+}
+
+int launch_few(const Args& a, bool bmn, cudaStream_t st) {
+  if (a.M == 1) launch_few<1>(a, bmn, st);
+  else if (a.M == 2) launch_few<2>(a, bmn, st);
+  else if (a.M <= 4) launch_few<4>(a, bmn, st);
+  else launch_few<8>(a, bmn, st);
+  tt_count_launches(1);
+  return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
+}
+
 template <int SM, int SN>
 int launch_product(const Args& a, const dim3& grid, bool amn, bool bmn, cudaStream_t st) {
   if (amn && bmn) product_kernel<SM, SN, true, true><<<grid, kThreads, 0, st>>>(a);
@@ -257,8 +431,11 @@ int run(int64_t M, int64_t N, const Term* terms, int n_terms, const Result* r, i
       return TT_ERR_INVALID_ARG;
     k = batch > 1 ? terms[i].k : k + terms[i].k;
   }
-  Form f = form_of(M, N, k, batch, true);
-  if (f.parts > 1 && (!work || f.parts * batch * M * N * 4 > work_bytes))
+  const bool amn = terms[0].a.mn, bmn = terms[0].b.mn, few = M <= kFewRows && !amn;
+  Form f = few ? Form{kFewRows, 4, bmn ? few_parts(M, N, k, batch) : 1}
+               : form_of(M, N, k, batch, true);
+  if (few && f.parts * batch * M * N * 4 > (work ? work_bytes : 0)) f.parts = 1;
+  if (!few && f.parts > 1 && (!work || f.parts * batch * M * N * 4 > work_bytes))
     f = form_of(M, N, k, batch, false);
   // (whole slices a part: 16-byte loads stay on their boundaries)
   a.k_part = f.parts > 1 ? ((k + f.parts - 1) / f.parts + kK - 1) / kK * kK
@@ -275,8 +452,8 @@ int run(int64_t M, int64_t N, const Term* terms, int n_terms, const Result* r, i
   if (rows * cols > 0x7fffffff) return TT_ERR_UNSUPPORTED;
   a.tiles_n = (uint32_t)cols;
   const dim3 grid((unsigned)(rows * cols), (unsigned)(a.parts * batch));
-  const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
-  const int rc = f.rows == 128   ? launch_product<128, 128>(a, grid, amn, bmn, st)
+  const int rc = few             ? launch_few(a, bmn, st)
+                 : f.rows == 128 ? launch_product<128, 128>(a, grid, amn, bmn, st)
                  : f.cols == 128 ? launch_product<64, 128>(a, grid, amn, bmn, st)
                                  : launch_product<64, 64>(a, grid, amn, bmn, st);
   if (rc != TT_OK || a.parts == 1) return rc;
@@ -292,8 +469,9 @@ int run(int64_t M, int64_t N, const Term* terms, int n_terms, const Result* r, i
 
 int64_t fp32_work(int64_t M, int64_t N, int64_t k, int batch) {
   if (M <= 0 || N <= 0) return 0;
-  const Form f = form_of(M, N, k, batch, true);
-  return f.parts > 1 ? f.parts * batch * M * N * 4 : 0;
+  const int64_t parts = std::max(form_of(M, N, k, batch, true).parts,
+                                 M <= kFewRows ? few_parts(M, N, k, batch) : 1);
+  return parts > 1 ? parts * batch * M * N * 4 : 0;
 }
 
 int fp32_product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& r, void* work,
