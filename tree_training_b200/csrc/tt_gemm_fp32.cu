@@ -350,7 +350,9 @@ struct Form {
 // The cheapest form: tiles of 128 x 128 take 2,048 clocks of fma a slice and SM, 64 x
 // 128 half of that and some, 64 x 64 a quarter and some (their operands are read from
 // shared memory more often); parts have at least 64 of k, and cost a launch and their
-// way through L2.
+// way through L2.  From five blocks an SM on the rate counts more than how the last of
+// them come out, and the smaller tiles' clocks are a quarter more (2,000 x 1,500 x 2,500
+// 2,355 us by 64 x 128, 2,106 by 128 x 128; 700 x 512 x 3,000, of 3.6 an SM, 369 and 395).
 Form form_of(int64_t M, int64_t N, int64_t k, int batch, bool split) {
   constexpr int kForms[3][3] = {{128, 128, 2048}, {64, 128, 1100}, {64, 64, 650}};
   Form best{128, 128, 1};
@@ -361,7 +363,9 @@ Form form_of(int64_t M, int64_t N, int64_t k, int batch, bool split) {
         split ? std::max<int64_t>(1, std::min<int64_t>(k / 64, 4 * vec::kSMs / tiles)) : 1;
     for (int64_t parts = 1; parts <= most; parts = next_parts(parts, most)) {
       const double slices = (double)((k + parts - 1) / parts + kK - 1) / kK;
-      double t = (double)((tiles * parts + vec::kSMs - 1) / vec::kSMs) * slices * f[2] + 1500;
+      const bool full = f[0] * f[1] < 128 * 128 && tiles * parts >= 5 * vec::kSMs;
+      double t = (double)((tiles * parts + vec::kSMs - 1) / vec::kSMs) * slices * f[2] *
+                     (full ? 1.25 : 1.0) + 1500;
       if (parts > 1) t += 5000 + (double)(parts + 1) * batch * M * N * 4 / 1500;
       if (t < least * 0.99) least = t, best = Form{f[0], f[1], parts};
     }
