@@ -7,6 +7,7 @@ from __future__ import annotations
 import types
 
 import torch
+from torch.overrides import TorchFunctionMode
 
 from . import _ops
 
@@ -33,31 +34,102 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     return _ops.ext().gated_linear(x, w_gate, w_up, ACTIVATIONS[activation])
 
 
+# Modules that are these activations and nothing else, by where they are defined: another
+# class of the same name, or one derived from them, may do more.
+_KNOWN = {
+    "torch.nn.modules.activation": {"SiLU": "silu", "ReLU": "relu", "GELU": "gelu"},
+    "transformers.activations": {"SiLUActivation": "silu", "GELUActivation": "gelu",
+                                 "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"},
+}
+_MULTIPLY = (torch.mul, torch.multiply, torch.Tensor.mul, torch.Tensor.multiply,
+             torch.Tensor.__mul__, torch.Tensor.__rmul__)
+
+
 def _activation_of(fn):
     """The name of a module's activation, None where it is not one of these."""
-    if isinstance(fn, torch.nn.GELU):
-        return "gelu_tanh" if fn.approximate == "tanh" else "gelu"
-    return {"SiLU": "silu", "SiLUActivation": "silu", "ReLU": "relu", "GELUActivation": "gelu",
-            "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"}.get(type(fn).__name__)
+    cls = type(fn)
+    name = _KNOWN.get(cls.__module__, {}).get(cls.__name__)
+    if name is None or "forward" in fn.__dict__ or _has_hooks(fn):
+        return None
+    return "gelu_tanh" if cls is torch.nn.GELU and fn.approximate == "tanh" else name
 
 
-@torch.no_grad()
+class _Calls(TorchFunctionMode):
+    """Every call that is made on tensors, but those inside the activation's module,
+    which counts as one."""
+
+    def __init__(self, act):
+        super().__init__()
+        self.calls, self.act, self.inside = [], act, False
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if not self.inside:
+            self.note(func, args, kwargs, out)
+        return out
+
+    def note(self, func, args, kwargs, out):
+        self.calls.append((func, args, kwargs, out, torch.is_grad_enabled(),
+                           torch.is_autocast_enabled()))
+
+    def enter(self, mod, args):
+        self.inside = True
+
+    def leave(self, mod, args, out):
+        self.inside = False
+        self.note(self.act, args, None, out)
+
+
 def _is_plain(mod) -> bool:
-    """Whether the module's forward is down(act(gate(x)) * up(x)) and nothing else
-    (no dropout, sparsity or clamp), by what it gives for a few rows in training."""
-    w = mod.gate_proj.weight
-    x = torch.linspace(-3, 3, 4 * w.shape[1], dtype=torch.float32).view(4, -1).sin()
-    x = x.to(w.device, w.dtype)
+    """Whether the module's forward is down(act(gate(x)) * up(x)) and nothing else, by
+    the calls that it makes (a bound, dropout or a shape that is asked for is one more).
+    Values show too little of it: a bound that they do not reach, zeros."""
+    gate, up, down, act = mod.gate_proj, mod.up_proj, mod.down_proj, mod.act_fn
+    x = torch.ones(2, gate.in_features, dtype=gate.weight.dtype, device=gate.weight.device)
+
+    def plain(training) -> bool:
+        mode = _Calls(act)
+        hooks = [act.register_forward_pre_hook(mode.enter), act.register_forward_hook(mode.leave)]
+        context = [training, torch.is_autocast_enabled()]
+        mod.training = training
+        try:
+            with torch.set_grad_enabled(training), mode:
+                result = mod.forward(x)
+        except Exception:                     # (other arguments, say)
+            return False
+        finally:
+            for hook in hooks:
+                hook.remove()
+        made = {}
+        for func, args, kwargs, out, *within in mode.calls:
+            if kwargs or within != context:
+                return False
+            if func is torch.nn.functional.linear and len(args) == 3:
+                part = [p for p in (gate, up, down) if args[1] is p.weight and args[2] is p.bias]
+            elif func is act and len(args) == 1:
+                part = [act]
+            elif func in _MULTIPLY and len(args) == 2:
+                part = ["product"]
+            else:
+                return False
+            if len(part) != 1 or part[0] in made:
+                return False
+            made[part[0]] = (args, out)
+        if set(made) != {gate, up, down, act, "product"}:
+            return False
+        a, b = made["product"][0]
+        if made[act][1] is not a:
+            a, b = b, a
+        return made[gate][0][0] is x and made[up][0][0] is x and made[act][0][0] is made[gate][1] \
+            and a is made[act][1] and b is made[up][1] and made[down][0][0] is made["product"][1] \
+            and result is made[down][1]
     training = mod.training
-    mod.training = True
+    devices = [x.device] if x.is_cuda else []
     try:
-        with torch.random.fork_rng(devices=[w.device] if w.is_cuda else []):
-            y = mod.forward(x)
+        with torch.random.fork_rng(devices=devices):
+            return plain(True) and plain(False)
     finally:
         mod.training = training
-    want = mod.down_proj(mod.act_fn(mod.gate_proj(x)) * mod.up_proj(x))
-    return isinstance(y, torch.Tensor) and y.shape == want.shape and \
-        torch.allclose(y.float(), want.float(), rtol=2e-2, atol=1e-3 * float(want.abs().max()))
 
 
 def _has_hooks(mod) -> bool:
@@ -74,18 +146,23 @@ def fuse_gated_mlps(model) -> int:
     """Routes every gated feed-forward module of an HF model (``gate_proj``,
     ``up_proj`` and ``down_proj`` without biases, ``act_fn`` one of the activations)
     through :func:`gated_linear`.  Returns how many modules were patched; modules of
-    another form or type keep their own forward, and so do those whose forward does
-    more than that, has been replaced (by this function or another: wrap it after
-    this call, as ``checkpoint_mlps`` does), or whose gate or up projection has hooks."""
+    another form or type keep their own forward, and so do those whose forward makes any
+    other call on tensors (a bound, dropout, a branch on a shape; it is run twice to see
+    them), has been replaced (by this function or another: wrap it after this call, as
+    ``checkpoint_mlps`` does), or whose gate or up projection or activation has hooks."""
     n = 0
     for mod in model.modules():
         parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
-        if not all(type(p) is torch.nn.Linear for p in parts) or not hasattr(mod, "act_fn") \
+        if not all(type(p) is torch.nn.Linear and "forward" not in p.__dict__ for p in parts) \
+                or not isinstance(getattr(mod, "act_fn", None), torch.nn.Module) \
                 or getattr(mod.forward, "__func__", None) is not type(mod).forward \
                 or _has_hooks(parts[0]) or _has_hooks(parts[1]):
             continue
-        if parts[0].weight.dtype not in (torch.float32, torch.bfloat16, torch.float16) or \
-                any(c not in (*parts, mod.act_fn) for c in mod.children()):
+        weights = [p.weight for p in parts[:2]]
+        if weights[0].dtype not in (torch.float32, torch.bfloat16, torch.float16) \
+                or weights[1].dtype != weights[0].dtype or weights[1].shape != weights[0].shape \
+                or any(type(w) not in (torch.nn.Parameter, torch.Tensor) for w in weights) \
+                or any(c not in (*parts, mod.act_fn) for c in mod.children()):
             continue
         name = _activation_of(mod.act_fn)
         if name is None or parts[0].bias is not None or parts[1].bias is not None \
