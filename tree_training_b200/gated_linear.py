@@ -5,8 +5,10 @@ activation and their product in one kernel, with gradients.  (The way back,
 from __future__ import annotations
 
 import types
+import weakref
 
 import torch
+from torch.nn.modules.module import _has_any_global_hook as has_any_global_hook
 from torch.overrides import TorchFunctionMode
 
 from . import _ops
@@ -133,13 +135,39 @@ def _is_plain(mod) -> bool:
 
 
 def _has_hooks(mod) -> bool:
-    return any(getattr(mod, a) for a in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks",
-                                         "_backward_pre_hooks"))
+    return bool(mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks
+                or mod._backward_pre_hooks)
 
 
-def _gated_mlp_forward(self, x):
-    return self.down_proj(gated_linear(x, self.gate_proj.weight, self.up_proj.weight,
-                                       self._tt_activation))
+def _activation_of_parts(mod):
+    """The activation's name where gate, up and activation are what the kernel computes
+    (plain projections without bias, nothing attached to them), else None."""
+    weights = []
+    for part in (getattr(mod, "gate_proj", None), getattr(mod, "up_proj", None)):
+        if type(part) is not torch.nn.Linear or part.bias is not None \
+                or "forward" in part.__dict__ or _has_hooks(part) \
+                or type(part.weight) not in (torch.nn.Parameter, torch.Tensor):
+            return None
+        weights.append(part.weight)
+    act = getattr(mod, "act_fn", None)
+    if weights[0].dtype != weights[1].dtype or weights[0].shape != weights[1].shape \
+            or not isinstance(act, torch.nn.Module):
+        return None
+    return _activation_of(act)
+
+
+# The forward of each class of which modules were taken.
+_taken = weakref.WeakKeyDictionary()
+
+
+def _gated_mlp_forward(self, *args, **kwargs):
+    cls = type(self)
+    name = _activation_of_parts(self)
+    # what has changed since the module was taken goes by its own forward
+    if name is None or kwargs or len(args) != 1 or _taken.get(cls, cls.forward) is not cls.forward \
+            or has_any_global_hook():
+        return cls.forward(self, *args, **kwargs)
+    return self.down_proj(gated_linear(args[0], self.gate_proj.weight, self.up_proj.weight, name))
 
 
 def fuse_gated_mlps(model) -> int:
@@ -149,26 +177,22 @@ def fuse_gated_mlps(model) -> int:
     another form or type keep their own forward, and so do those whose forward makes any
     other call on tensors (a bound, dropout, a branch on a shape; it is run twice to see
     them), has been replaced (by this function or another: wrap it after this call, as
-    ``checkpoint_mlps`` does), or whose gate or up projection or activation has hooks."""
+    ``checkpoint_mlps`` does), or whose gate or up projection or activation has hooks.
+
+    A patched module looks at its parts in every call: with an adapter in place of a
+    projection, a hook on one or on the activation, or an activation that the kernel does
+    not have, it goes by its class's forward for as long as that is so."""
     n = 0
     for mod in model.modules():
-        parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
-        if not all(type(p) is torch.nn.Linear and "forward" not in p.__dict__ for p in parts) \
-                or not isinstance(getattr(mod, "act_fn", None), torch.nn.Module) \
+        name, down = _activation_of_parts(mod), getattr(mod, "down_proj", None)
+        if name is None or type(down) is not torch.nn.Linear or "forward" in down.__dict__ \
                 or getattr(mod.forward, "__func__", None) is not type(mod).forward \
-                or _has_hooks(parts[0]) or _has_hooks(parts[1]):
-            continue
-        weights = [p.weight for p in parts[:2]]
-        if weights[0].dtype not in (torch.float32, torch.bfloat16, torch.float16) \
-                or weights[1].dtype != weights[0].dtype or weights[1].shape != weights[0].shape \
-                or any(type(w) not in (torch.nn.Parameter, torch.Tensor) for w in weights) \
-                or any(c not in (*parts, mod.act_fn) for c in mod.children()):
-            continue
-        name = _activation_of(mod.act_fn)
-        if name is None or parts[0].bias is not None or parts[1].bias is not None \
+                or mod.gate_proj.weight.dtype not in (torch.float32, torch.bfloat16, torch.float16) \
+                or any(c not in (mod.gate_proj, mod.up_proj, down, mod.act_fn)
+                       for c in mod.children()) \
                 or not _is_plain(mod):
             continue
-        mod._tt_activation = name
+        _taken[type(mod)] = type(mod).forward
         mod.forward = types.MethodType(_gated_mlp_forward, mod)
         n += 1
     return n
