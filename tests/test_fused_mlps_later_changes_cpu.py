@@ -176,3 +176,24 @@ def test_copies_are_of_their_own_parts(kernel):
         other.gate_proj.weight.zero_()
     x = torch.randn(5, 32)
     assert not other(x).any() and mod(x).any() and len(kernel) == 2
+
+
+@pytest.mark.parametrize("given", [torch.float32, torch.bfloat16])
+def test_under_autocast(kernel, given):
+    """In autocast's type, as the projections of the module's own forward."""
+    mod, own = fused()
+    x = torch.randn(5, 32)
+    grads = []
+    for m in (mod, own):
+        leaf = x.to(given).requires_grad_(True)
+        with torch.autocast("cpu", torch.bfloat16):
+            y = m(leaf)
+        assert y.dtype == torch.bfloat16
+        grads.append([y, *torch.autograd.grad(y.float().square().sum(), [leaf, *m.parameters()])])
+    assert kernel == [(torch.bfloat16, torch.bfloat16, "silu")]
+    for a, b in zip(*grads):
+        assert a.dtype == b.dtype
+        assert float((a - b).norm()) <= 2.0 ** -6 * float(b.norm())      # a few roundings to bf16
+    with torch.autocast("cpu", torch.bfloat16, enabled=False):
+        mod(x)
+    assert kernel[1:] == [(torch.float32, torch.float32, "silu")]

@@ -361,3 +361,28 @@ def test_rows_of_zeros_and_of_very_different_sizes():
 @pytest.mark.parametrize("H,F", [(1001, 735), (4096, 520), (256, 9001)])
 def test_few_rows_of_fp32(T, H, F):
     compare(*make(T, H, F, F32, seed=T))
+
+
+@pytest.mark.parametrize("autocast", [BF, F16])
+@pytest.mark.parametrize("given", [F32, BF])
+def test_hf_modules_under_autocast(given, autocast):
+    """Patched modules run in autocast's type: h and its gradients within a few of its
+    roundings (five on the way: both factors, the activation, the product, the result)."""
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.qwen3.modeling_qwen3 import Qwen3MLP
+    cfg = transformers.Qwen3Config(hidden_size=128, intermediate_size=264, num_hidden_layers=1)
+    torch.manual_seed(0)
+    mlp = torch.nn.ModuleList([Qwen3MLP(cfg)]).to(DEV)
+    x = torch.randn(2, 37, 128, device=DEV).to(given)
+    dy = torch.randn(2, 37, 128, device=DEV).to(autocast)
+    got = []
+    for fuse in (0, 1):
+        assert tt.fuse_gated_mlps(mlp) == 1 if fuse else True
+        leaf = x.clone().requires_grad_(True)
+        with torch.autocast("cuda", autocast):
+            y = mlp[0](leaf)
+        assert y.dtype == autocast
+        got.append([y, *torch.autograd.grad(y, [leaf, *mlp.parameters()], dy)])
+    for a, b in zip(*got):
+        assert a.dtype == b.dtype
+        assert float((a - b).norm() / b.norm()) < 5 * max(UNIT[autocast], UNIT[b.dtype])

@@ -28,7 +28,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     Differentiable in all three.  For the backward the two products are kept in
     fp32 (8 bytes an element of h); their gradients are rounded to x's type once,
     for the products that give dx and the weights' gradients: in fp16 a gradient
-    of h under 1e-7 or so is lost there, as it is in fp16 itself.
+    of h under 1e-7 or so is lost there, as it is in fp16 itself.  Autocast does not
+    change the types.
 
     CUDA tensors only (no CPU path)."""
     if activation not in ACTIVATIONS:
@@ -167,7 +168,11 @@ def _gated_mlp_forward(self, *args, **kwargs):
     if name is None or kwargs or len(args) != 1 or _taken.get(cls, cls.forward) is not cls.forward \
             or has_any_global_hook():
         return cls.forward(self, *args, **kwargs)
-    return self.down_proj(gated_linear(args[0], self.gate_proj.weight, self.up_proj.weight, name))
+    factors = [args[0], self.gate_proj.weight, self.up_proj.weight]
+    kind = factors[0].device.type
+    if torch.is_autocast_enabled(kind):       # (as the projections' own products)
+        factors = [t.to(torch.get_autocast_dtype(kind)) for t in factors]
+    return self.down_proj(gated_linear(*factors, name))
 
 
 def fuse_gated_mlps(model) -> int:
@@ -181,7 +186,8 @@ def fuse_gated_mlps(model) -> int:
 
     A patched module looks at its parts in every call: with an adapter in place of a
     projection, a hook on one or on the activation, or an activation that the kernel does
-    not have, it goes by its class's forward for as long as that is so."""
+    not have, it goes by its class's forward for as long as that is so.  Under autocast it
+    computes in autocast's type, as the projections would."""
     n = 0
     for mod in model.modules():
         name, down = _activation_of_parts(mod), getattr(mod, "down_proj", None)
