@@ -125,6 +125,26 @@ struct Doubts {
   float share;                             // of the sum of 32 products' magnitudes
 };
 
+// Eight elements of a row of d.H from the p-th on.
+template <typename T>
+__device__ __forceinline__ uint4 pack_at(const Doubts& d, const T* row, int64_t p) {
+  return p + 8 <= d.H ? __ldg(reinterpret_cast<const uint4*>(row + p))
+                      : vec::load_any_of<T>(row, p, d.H, row, row);
+}
+
+// Whether a feature has a weight other than 0.
+template <typename T>
+__device__ __forceinline__ bool any_weight(const Doubts& d, int feature) {
+  const T* w = reinterpret_cast<const T*>(d.w) + (int64_t)feature * d.w_ld;
+  uint32_t bits = 0;
+#pragma unroll 4
+  for (int64_t p = (threadIdx.x & 31) * 8; p < d.H; p += 256) {
+    const uint4 v = pack_at(d, w, p);
+    bits |= v.x | v.y | v.z | v.w;
+  }
+  return __any_sync(0xffffffffu, (bits & 0x7fff7fffu) != 0);
+}
+
 template <typename T>
 __device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live, int feature,
                                              int left, float (&g)[32]) {
@@ -137,10 +157,20 @@ __device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live
   }
   const float doubt = (sum_of[0] + sum_of[1]) * d.share;
   if (!__any_sync(0xffffffffu, live && fminf(least[0], least[1]) < doubt)) return;
-  uint32_t mask = 0;
+  uint32_t mask = 0, zero = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (live && i < left && g[i] != 0.f && fabsf(g[i]) < doubt) mask |= 1u << i;
+  for (int i = 0; i < 32; ++i) {
+    if (live && i < left && fabsf(g[i]) < doubt) mask |= 1u << i;
+    if (g[i] == 0.f) zero |= 1u << i;
+  }
+  // exactly 0: cut off altogether, or a feature without weights
+  const uint32_t features = __reduce_or_sync(0xffffffffu, zero & mask);
+  if (__popc(features) > kMostDoubts) mask &= ~zero;
+  else
+    for (uint32_t f = features; f; f &= f - 1) {
+      const int i = __ffs(f) - 1;
+      if (!any_weight<T>(d, feature + i)) mask &= ~(1u << i);
+    }
   if (__popc(mask) > kMostDoubts) mask = 0;
   for (uint32_t who; (who = __ballot_sync(0xffffffffu, mask != 0)) != 0;) {
     const int from = __ffs(who) - 1;
@@ -154,11 +184,8 @@ __device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int64_t p = p0 + 256 * k;
-        const bool whole = p + 8 <= d.H;
-        ra[k] = whole ? __ldg(reinterpret_cast<const uint4*>(a + p))
-                      : vec::load_any_of<T>(a, p, d.H, a, a);
-        rb[k] = whole ? __ldg(reinterpret_cast<const uint4*>(b + p))
-                      : vec::load_any_of<T>(b, p, d.H, b, b);
+        ra[k] = pack_at(d, a, p);
+        rb[k] = pack_at(d, b, p);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
