@@ -61,9 +61,26 @@ def check(x, wg, wu, features, up, pairs=False):
     assert (off <= (2.0 ** -8 + 2.0 ** -9) * want.abs()[seen[:, features]]).all()
 
 
+@pytest.mark.parametrize("up", [2.0 ** -10, 1.0, 2.0 ** 16])
+@pytest.mark.parametrize("T,H,F", [(64, 4096, 1024), (100, 1024, 688), (600, 4096, 3840),
+                                   (1024, 2560, 4864)])
+def test_whatever_the_other_factors_size(T, H, F, up):
+    features = list(range(5, F, 16))
+    check(*planted(T, H, F, features, up), features, up)
+
+
+@pytest.mark.parametrize("T,H,F,features", [
+    (64, 4096, 1025, [1024]), (600, 4096, 3841, [3840]), (2048, 2560, 2561, [2560]),
+    (2048, 2560, 2564, [2561, 2563]), (2048, 2560, 2567, [2560, 2566]), (16, 4096, 1, [0]),
+    (40, 4096, 3, [1]), (40, 4096, 5, [0, 4]), (300, 4096, 9, [8]), (1000, 2560, 2049, [2048])])
+def test_the_last_few_features(T, H, F, features):
+    check(*planted(T, H, F, features), features, 1.0)
+
+
 @pytest.mark.parametrize("T,H,F,features", [
     (600, 4096, 3840, range(5, 3840, 32)), (1024, 2560, 4864, range(0, 4864, 31)),
-    (2048, 1024, 2048, range(7, 2048, 64))])
+    (2048, 1024, 2048, range(7, 2048, 64)), (64, 4096, 1024, range(3, 1024, 16)),
+    (64, 4096, 1025, [1024]), (16, 1024, 3, [0, 2])])
 def test_terms_that_are_cut_off_altogether(T, H, F, features):
     features = list(features)
     check(*planted(T, H, F, features, pairs=True), features, 1.0, pairs=True)

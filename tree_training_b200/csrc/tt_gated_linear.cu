@@ -111,18 +111,22 @@ int dispatch_act(int act, F f) {
 // relu's slope jumps at 0: of a product that the tensor cores' cut-off sums leave within
 // their own error of 0 (208 x 4,288 x 4,544: one of 945,000, which was 1.5e-3 of a weight's
 // gradient) the sign is found again, by a sum in 64 bits.  Their error is about 2^-24 of
-// the sums on the way for every 16 of k; these are as large as the row's other products.
-// The whole warp forms such a sum; a row with more than kMostDoubts of them in 32 is
-// left as it is (columns of very different sizes: the estimate says nothing there).  It
-// costs the forward 3 to 15% (64 x 2,560 x 9,728 23.1 -> 25.5 us, 4,096 x 1,536 x 4,096 67
-// -> 78, 8,192 x 2,560 x 9,728 kept 600 -> 632), a pass with gradients a quarter of that.
+// the sums on the way for every 16 of k; these are as large as the row's other products
+// of the block (fewer than kFewest say too little: their factors' sizes then).  The whole
+// warp forms such a sum; a row with more than kMostDoubts of them in 32 is left as it is
+// (columns of very different sizes: the estimate says nothing there).  It costs the
+// forward 3 to 15% (64 x 2,560 x 9,728 23.1 -> 25.5 us, 4,096 x 1,536 x 4,096 67 -> 78, 8,192 x
+// 2,560 x 9,728 kept 600 -> 632), a pass with gradients a quarter of that; a last tile of
+// few features up to 6 us (2,048 x 2,560 x 2,567 55 -> 61, 8,192 x 2,560 x 9,729 537 -> 541),
+// features without weights up to a fifth (8,192 x 2,560 x 9,728, four in 32: 514 -> 617).
 constexpr int kMostDoubts = 4;
+constexpr int kFewest = 8;
 
 struct Doubts {
   const void *x, *w;
   int64_t x_ld, w_ld;
   int H;
-  float share;                             // of the sum of 32 products' magnitudes
+  float share;                             // of a product's usual magnitude
 };
 
 // Eight elements of a row of d.H from the p-th on.
@@ -130,6 +134,50 @@ template <typename T>
 __device__ __forceinline__ uint4 pack_at(const Doubts& d, const T* row, int64_t p) {
   return p + 8 <= d.H ? __ldg(reinterpret_cast<const uint4*>(row + p))
                       : vec::load_any_of<T>(row, p, d.H, row, row);
+}
+
+// The mean square of a row's elements, by kSampled packs of it (a lane on its own).
+template <typename T>
+__device__ __forceinline__ float mean_square(const Doubts& d, const T* row) {
+  constexpr int kSampled = 32, kAhead = 16;
+  const int whole = d.H / 8;
+  float sum = 0.f;
+  if (whole == 0) {
+    for (int k = 0; k < d.H; ++k) sum = fmaf(to_f32(row[k]), to_f32(row[k]), sum);
+    return sum / (float)d.H;
+  }
+  for (int k0 = 0; k0 < kSampled; k0 += kAhead) {
+    uint4 raw[kAhead];                     // (loads without branches: none waits for another)
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      raw[k] = __ldg(reinterpret_cast<const uint4*>(row) + (int64_t)(k0 + k) * whole / kSampled);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float v[8];
+      vec::unpack<T, 8>(raw[k], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+    }
+  }
+  return sum / (8.f * kSampled);
+}
+
+// The usual magnitude of a row's products with `left` (under kFewest) features, from
+// their factors: |x| |w| / sqrt(H), and kWider times that, since a part of the elements
+// shows their size only so far (a few may be much larger) and sums are soon formed again.
+template <typename T>
+__device__ __noinline__ float usual_of_few(const Doubts& d, int row, bool live, int feature,
+                                           int left) {
+  constexpr float kWider = 256.f;
+  const int lane = threadIdx.x & 31;
+  float xx = 0.f, ww = 0.f;
+  if (live) xx = mean_square(d, reinterpret_cast<const T*>(d.x) + (int64_t)row * d.x_ld);
+  if (lane < left)
+    ww = mean_square(d, reinterpret_cast<const T*>(d.w) + (int64_t)(feature + lane) * d.w_ld);
+  __syncwarp();
+  for (int o = 4; o; o >>= 1) ww += __shfl_xor_sync(0xffffffffu, ww, o);
+  ww = __shfl_sync(0xffffffffu, ww, 0) / (float)left;
+  return kWider * sqrtf(xx) * sqrtf(ww) * sqrtf((float)d.H);
 }
 
 // Whether a feature has a weight other than 0.
@@ -145,17 +193,30 @@ __device__ __forceinline__ bool any_weight(const Doubts& d, int feature) {
   return __any_sync(0xffffffffu, (bits & 0x7fff7fffu) != 0);
 }
 
+// g: of `left` features (those behind them are not this block's)
 template <typename T>
 __device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live, int feature,
                                              int left, float (&g)[32]) {
   const int lane = threadIdx.x & 31;
-  float sum_of[2] = {0.f, 0.f}, least[2] = {INFINITY, INFINITY};
+  float sum_of[2] = {0.f, 0.f}, least[2] = {INFINITY, INFINITY}, usual;
+  if (left >= 32) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    sum_of[i & 1] += fabsf(g[i]);
-    least[i & 1] = fminf(least[i & 1], fabsf(g[i]));
+    for (int i = 0; i < 32; ++i) {
+      sum_of[i & 1] += fabsf(g[i]);
+      least[i & 1] = fminf(least[i & 1], fabsf(g[i]));
+    }
+    usual = (sum_of[0] + sum_of[1]) / 32.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < left) {
+        sum_of[0] += fabsf(g[i]);
+        least[0] = fminf(least[0], fabsf(g[i]));
+      }
+    usual = left >= kFewest ? sum_of[0] / (float)left
+                            : usual_of_few<T>(d, row, live, feature, left);
   }
-  const float doubt = (sum_of[0] + sum_of[1]) * d.share;
+  const float doubt = usual * d.share;
   if (!__any_sync(0xffffffffu, live && fminf(least[0], least[1]) < doubt)) return;
   uint32_t mask = 0, zero = 0;
 #pragma unroll
@@ -422,7 +483,7 @@ int forward_16(int64_t T, int H, int F, const void* x, int64_t x_ld, const void*
     if (!gemm::set_up(&q, plan, kB, T, F, terms, 2, true, status)) return TT_ERR_UNSUPPORTED;
     typename Epi::Args ea{};
     ea.h = h, ea.h_ld = F, ea.g = g, ea.u = u, ea.keep_ld = keep_ld, ea.F = F;
-    ea.doubts = {x, wg, x_ld, wg_ld, H, (float)(H / 16 + 4) * 0x1p-29f};
+    ea.doubts = {x, wg, x_ld, wg_ld, H, (float)(H / 16 + 4) * 0x1p-24f};
     ea.wide = F % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
     return gemm::launch<false, false, Epi>(plan, q, ea, st);
   });
