@@ -58,6 +58,12 @@ __device__ __forceinline__ float act_16(float g) {
   return act<A>(g);
 }
 
+// Of gelu with tanh past +-20: the slope is 1 or 0 there, and the cube's derivative would
+// leave fp32 from 1e19 on (0 times infinity).  NaN stays.
+__device__ __forceinline__ float near_zero(float g) {
+  return g > 20.f ? 20.f : (g < -20.f ? -20.f : g);
+}
+
 // act(g) and its derivative.
 template <int A>
 __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
@@ -71,9 +77,9 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
     a = g * c;
     d = c + g * expf(-0.5f * g * g) * 0.3989422804014327f;
   } else if constexpr (A == kGeluTanh) {
-    const float t = tanhf(kTanhA * (g + kTanhB * g * g * g));
+    const float c = near_zero(g), t = tanhf(kTanhA * (c + kTanhB * c * c * c));
     a = 0.5f * g * (1.f + t);
-    d = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * kTanhA * (1.f + 3.f * kTanhB * g * g);
+    d = 0.5f * (1.f + t) + 0.5f * c * (1.f - t * t) * kTanhA * (1.f + 3.f * kTanhB * c * c);
   } else {
     a = act<kRelu>(g);
     d = g > 0.f ? 1.f : (g != g ? g : 0.f);
@@ -86,12 +92,13 @@ template <int A>
 __device__ __forceinline__ void act_grad_16(float g, float& a, float& d) {
   if constexpr (A == kSilu || A == kGeluTanh) {
     // s = 1 / (1 + exp(-z)), 1 - s = exp(-z) s; past -80, where exp(-z) s would leave
-    // fp32, s is 0 (not 2e-35: g and its cube may be as large)
-    const float z = A == kSilu ? g : 2.f * kTanhA * (g + kTanhB * g * g * g);
+    // fp32, s is 0 (not 2e-35: g may be as large)
+    const float c = A == kSilu ? g : near_zero(g);
+    const float z = A == kSilu ? g : 2.f * kTanhA * (c + kTanhB * c * c * c);
     const float e = __expf(-fmaxf(z, -80.f)), s = z < -80.f ? 0.f : __fdividef(1.f, 1.f + e);
-    const float dz = A == kSilu ? 1.f : 2.f * kTanhA * (1.f + 3.f * kTanhB * g * g);
+    const float dz = A == kSilu ? 1.f : 2.f * kTanhA * (1.f + 3.f * kTanhB * c * c);
     a = g * s;
-    d = s * (1.f + g * (e * s * dz));
+    d = s * (1.f + c * (e * s * dz));
   } else {
     act_grad<A>(g, a, d);
   }
