@@ -1,8 +1,15 @@
-"""The activations far from 0, of single products: what is large has slope 1 there."""
+"""The activations far from 0, of single products: what is small there is kept as far as
+the type holds it, and what is large has slope 1.
+
+Bounds.  The exponential of an argument z errs by (2 + 1.2 |z|) units of fp32, the
+argument itself (tanh's) by a few of its own: 2^-23 (8 + 8 |z|) of the value altogether,
+beside one rounding of each gradient of a product and one of the result.
+"""
 import pytest
 import torch
 
 import tree_training_b200 as tt
+from tests.op_bounds import TINY, UNIT
 from tests.test_gated_linear_gpu import act64
 
 pytestmark = pytest.mark.gpu
@@ -30,6 +37,21 @@ def run(g, T, dtype, act):
     d, = torch.autograd.grad(a.sum(), g)
     n = min(T, len(g))
     return g.detach(), a.detach(), d, h.detach(), dwg[:n, 0], dwu[:n, 1]
+
+
+@pytest.mark.parametrize("T", [1, 200])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_far_below_zero(dtype, T):
+    g = torch.arange(-103.5, -60, 0.25, device=DEV)
+    g, a, d, h, dwg, dwu = run(g, T, dtype, "silu")
+    rel = UNIT[dtype] + 2.0 ** -23 * (8 + 8 * g.abs())
+    # (fp32's own subnormals on the way: exp(-103) is one unit of them, and g times it)
+    tiny = TINY[dtype] + 2.0 ** -149 * (2 + g.abs())
+    n = len(dwg)
+    assert ((h.double() - a).abs() <= rel * a.abs() + tiny).all()
+    assert ((dwu.double() - a[:n]).abs() <= 2 * (rel * a.abs() + tiny)[:n]).all()
+    assert ((dwg.double() - d[:n]).abs() <= 2 * (rel * (1 + g.abs()) * g.exp() + tiny)[:n]).all()
+    assert (h[:, g > -87] != 0).all() and (dwu[g[:n] > -87] != 0).all()
 
 
 @pytest.mark.parametrize("T", [1, 200])

@@ -38,23 +38,32 @@ enum Act { kSilu = 0, kGelu = 1, kGeluTanh = 2, kRelu = 3 };
 constexpr float kTanhA = 0.7978845608028654f;      // sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
 
+// 1 / (1 + exp(-g)) down to where fp32 ends, which exp(-g) leaves at -88 already.
+__device__ __forceinline__ float sigmoid(float g) {
+  return g < -80.f ? expf(g) : 1.f / (1.f + expf(-g));
+}
+
 template <int A>
 __device__ __forceinline__ float act(float g) {
-  if constexpr (A == kSilu) return g / (1.f + expf(-g));
+  if constexpr (A == kSilu) return g < -80.f ? g * expf(g) : g / (1.f + expf(-g));
   if constexpr (A == kGelu) return g * normcdff(g);
   if constexpr (A == kGeluTanh)
     return 0.5f * g * (1.f + tanhf(kTanhA * (g + kTanhB * g * g * g)));
   return g > 0.f ? g : (g != g ? g : 0.f);
 }
 
-// The same for results of 16 bits, where 2^-20 of a value does not show: the epilogue
-// of the products has no time for the exact quotient.
+// The same for results of 16 bits: the epilogue of the products has no time for the exact
+// exponential and quotient.  The quick ones err by 2^-22 (3 + 0.6 |z|) of the value: 2^-16 of
+// silu(-80), 2^-20 of what is above -4, beside 2^-12 or 2^-9 of the rounding that follows.
+// 1 / (1 + exp(-z)) = exp(z) / (1 + exp(z)): by the exponential that is at most 1, so that
+// neither leaves fp32.  ((1 + tanh y) / 2 = 1 / (1 + exp(-2 y)).)
 template <int A>
 __device__ __forceinline__ float act_16(float g) {
-  if constexpr (A == kSilu) return __fdividef(g, 1.f + __expf(-g));
-  // (1 + tanh y) / 2 = 1 / (1 + exp(-2 y))
-  if constexpr (A == kGeluTanh)
-    return __fdividef(g, 1.f + __expf(-2.f * kTanhA * (g + kTanhB * g * g * g)));
+  if constexpr (A == kSilu || A == kGeluTanh) {
+    const float z = A == kSilu ? g : 2.f * kTanhA * (g + kTanhB * g * g * g);
+    const float e = __expf(-fabsf(z));
+    return __fdividef(z < 0.f ? g * e : g, 1.f + e);
+  }
   return act<A>(g);
 }
 
@@ -68,10 +77,10 @@ __device__ __forceinline__ float near_zero(float g) {
 template <int A>
 __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
   if constexpr (A == kSilu) {
-    const float q = 1.f / (1.f + expf(-g));
+    const float q = sigmoid(g);
     a = g * q;
     // (1 - q loses what little there is of it for large g: q(-g) instead)
-    d = q * (1.f + g * (1.f / (1.f + expf(g))));
+    d = q * (1.f + g * sigmoid(-g));
   } else if constexpr (A == kGelu) {
     const float c = normcdff(g);
     a = g * c;
@@ -91,14 +100,14 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
 template <int A>
 __device__ __forceinline__ void act_grad_16(float g, float& a, float& d) {
   if constexpr (A == kSilu || A == kGeluTanh) {
-    // s = 1 / (1 + exp(-z)), 1 - s = exp(-z) s; past -80, where exp(-z) s would leave
-    // fp32, s is 0 (not 2e-35: g may be as large)
+    // s = 1 / (1 + exp(-z)) and r = 1 - s, the smaller of them as exp(-|z|) times the other
     const float c = A == kSilu ? g : near_zero(g);
     const float z = A == kSilu ? g : 2.f * kTanhA * (c + kTanhB * c * c * c);
-    const float e = __expf(-fmaxf(z, -80.f)), s = z < -80.f ? 0.f : __fdividef(1.f, 1.f + e);
+    const float e = __expf(-fabsf(z)), large = __fdividef(1.f, 1.f + e), small = e * large;
+    const float s = z < 0.f ? small : large, r = z < 0.f ? large : small;
     const float dz = A == kSilu ? 1.f : 2.f * kTanhA * (1.f + 3.f * kTanhB * c * c);
     a = g * s;
-    d = s * (1.f + c * (e * s * dz));
+    d = s * (1.f + c * (r * dz));
   } else {
     act_grad<A>(g, a, d);
   }
