@@ -640,7 +640,7 @@ int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, cons
                      int32_t* status, void* stream);
 
 /* ---- the norm of many tensors ---------------------------------------------------- *
- * dtypes, sizes (elements) and tensors are host arrays of `count`.  norm_type 1, 2
+ * dtypes, sizes (elements, at most 2^43) and tensors are host arrays of `count`.  norm_type 1, 2
  * or infinity; *norm (device, fp32) is the norm of all elements together. */
 int64_t tt_grad_norm_workspace_size(int32_t count);
 int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,

@@ -292,8 +292,8 @@ int check(int32_t count, const int32_t* dtypes, const int64_t* sizes, const void
   if (count < 0 || (count > 0 && (!dtypes || !sizes || !src))) return TT_ERR_INVALID_ARG;
   for (int32_t i = 0; i < count; ++i) {
     if (dtypes[i] < TT_F32 || dtypes[i] > TT_F16) return TT_ERR_UNSUPPORTED;
-    // (a tensor's chunks are counted in 32 bits: 2^31 of them are 64 TB)
-    if (sizes[i] < 0 || sizes[i] >= ((int64_t)1 << 44) || (sizes[i] > 0 && !src[i]))
+    // (a tensor's chunks, and a launch's past its last, are counted in 32 bits)
+    if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 43) || (sizes[i] > 0 && !src[i]))
       return TT_ERR_INVALID_ARG;
     const uintptr_t b = dtypes[i] == TT_F32 ? 3 : 1;
     if (reinterpret_cast<uintptr_t>(src[i]) & b) return TT_ERR_INVALID_ARG;
