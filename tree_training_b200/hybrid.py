@@ -262,6 +262,23 @@ def _base_model(model):
     return base
 
 
+def _check_lm_head(model) -> None:
+    """The fused losses read ``lm_head.weight`` alone: whatever else stands between the
+    final hidden states and the logits would be left out without a word."""
+    _base_model(model)
+    head, config = model.lm_head, getattr(model, "config", None)
+    plain = type(head) is torch.nn.Linear and head.bias is None \
+        and "forward" not in head.__dict__ \
+        and not (head._forward_hooks or head._forward_pre_hooks or head._backward_hooks
+                 or head._backward_pre_hooks)
+    if not plain:
+        raise ValueError("fused_ce needs an LM head that is a plain Linear (no bias, adapter or "
+                         "hooks)")
+    for name in ("final_logit_softcapping", "logit_scale", "logits_scaling"):
+        if getattr(config, name, None) not in (None, 1, 1.0):
+            raise ValueError(f"fused_ce does not know the model's {name}")
+
+
 def _fused_leaf_loss(model, hidden, info, leaves, loss: TreeLeafLoss, fused_ce) -> torch.Tensor:
     """sum over the partition's loss leaves of CE(leaf logits) / n_leaves from
     the final hidden states [N, H], without materialising the logits (by chunks
@@ -415,7 +432,8 @@ def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
     with ``fused_ce`` (a ``make_tree_loss_fn`` loss, ``backward="fused"``) the
     leaf losses come from the final hidden states through the chunked LM-head
     cross-entropy of ``ce`` and no logits are formed (``fused_ce="pieces"``:
-    through ``linear_cross_entropy``, by pieces of the vocabulary);
+    through ``linear_cross_entropy``, by pieces of the vocabulary), of an LM head that
+    is a plain product;
     ``"per_leaf"`` calls backward once per leaf loss and once per gateway with
     retain_graph, as the reference does (tree_grad_hybrid.py:521-539).  Both
     accumulate the same sum of gradients; every per-leaf call traverses the
@@ -448,6 +466,8 @@ def tree_grad_hybrid(model, roots, leaf_loss_fn: Callable, max_tokens: int,
         raise ValueError("fused_ce must be False, True or 'pieces'")
     if fused_ce and (backward != "fused" or not isinstance(leaf_loss_fn, TreeLeafLoss)):
         raise ValueError("fused_ce needs backward='fused' and a make_tree_loss_fn loss")
+    if fused_ce:
+        _check_lm_head(model)
     _ensure_tree_attention(model)
     dev = next(model.parameters()).device
     parts = partition_tree(roots, max_tokens)
