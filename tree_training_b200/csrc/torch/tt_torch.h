@@ -86,8 +86,10 @@ inline bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
-// [rows, D] with unit last stride and rows that do not overlap (else a copy).
+// [rows, D] with unit last stride and rows that do not overlap (else a copy, as of
+// tensors whose sign is kept beside their memory).
 inline Tensor rows2d(const Tensor& t) {
+  if (t.is_neg()) return t.resolve_neg().contiguous();
   if (t.stride(1) == 1 && (t.stride(0) >= t.size(1) || t.size(0) <= 1)) return t;
   return t.contiguous();
 }

@@ -268,7 +268,7 @@ struct LinearCEFunction : Function<LinearCEFunction> {
     const Tensor &x = s[0], &w = s[1], &labels = s[2], &lse = s[3], &kept = s[4];
     const int64_t T = x.size(0), H = x.size(1), V = w.size(0), M = labels.size(1);
     for (int i = 0; i < 2; ++i)
-      if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();
+      if (g[i].defined()) g[i] = g[i].resolve_neg().to(at::kFloat).contiguous();
     auto like = [&](int64_t n) {
       Tensor t = empty({n, H}, x, x.scalar_type());
       return T ? t : t.zero_();
@@ -343,12 +343,15 @@ struct List {
       if (dtype_code(t) < 0)
         type_error(std::string(op) + ": " + name + " must be float32/bfloat16/float16");
       if (t.is_sparse()) type_error(std::string(op) + ": " + name + " must be dense tensors");
+      if (written && t.is_neg())
+        value_error(std::string(op) + ": " + name + " keeps its sign beside its memory "
+                                                    "(resolve_neg)");
       no_tangent(op, {&t});
       const bool dense = t.is_non_overlapping_and_dense();
       if (written && !dense)
         value_error(std::string(op) + ": a tensor that is written must fill its memory without "
                                       "gaps or overlaps");
-      hold.push_back(dense ? t : t.contiguous());
+      hold.push_back(dense ? t : t.contiguous());  // (a norm does not ask for signs)
       dtypes.push_back(dtype_code(t));
       sizes.push_back(t.numel());
       data.push_back(const_cast<void*>(hold.back().const_data_ptr()));
