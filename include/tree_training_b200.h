@@ -623,7 +623,8 @@ int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, const void* 
  * factors need rows on 16-byte boundaries (else TT_ERR_UNSUPPORTED).  kept (null, or
  * [T][tt_linear_ce_kept_ld] fp32 where that is not 0) takes the logits for the
  * backward, which forms them again without it: on a 32-byte boundary.  T, H, V <
- * 2^31 - 256. */
+ * 2^31 - 256.  The workspaces grow with T: forward about T V / 8 bytes, backward 256 MB
+ * or 8,192 T, and 4 T H. */
 int64_t tt_linear_ce_kept_ld(int dtype, int64_t T, int32_t H, int64_t V);
 int64_t tt_linear_ce_fwd_workspace_size(int dtype, int64_t T, int32_t H, int64_t V, int64_t M);
 int tt_linear_ce_fwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, const void* x,
@@ -640,8 +641,8 @@ int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M, cons
                      int32_t* status, void* stream);
 
 /* ---- the norm of many tensors ---------------------------------------------------- *
- * dtypes, sizes (elements, at most 2^43) and tensors are host arrays of `count`.  norm_type 1, 2
- * or infinity; *norm (device, fp32) is the norm of all elements together. */
+ * dtypes, sizes (elements, at most 2^43) and tensors are host arrays of `count`.
+ * norm_type 1, 2 or infinity; *norm (device, fp32) is the norm of all elements together. */
 int64_t tt_grad_norm_workspace_size(int32_t count);
 int tt_grad_norm(int32_t count, const int32_t* dtypes, const int64_t* sizes,
                  const void* const* tensors, double norm_type, float* norm, void* workspace,

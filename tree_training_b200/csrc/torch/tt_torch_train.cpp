@@ -11,7 +11,9 @@ namespace {
 
 using namespace tt_torch;
 
-Tensor bytes(int64_t n, const Tensor& like) { return empty({std::max<int64_t>(n, 16)}, like, at::kByte); }
+Tensor bytes(int64_t n, const Tensor& like) {
+  return empty({std::max<int64_t>(n, 16)}, like, at::kByte);
+}
 
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
@@ -112,7 +114,8 @@ Tensor embedding(const Tensor& ids_, const Tensor& w_, double scale,
   int64_t padding = -1;
   if (padding_) {
     padding = *padding_ < 0 ? *padding_ + V : *padding_;
-    if (padding < 0 || padding >= V) value_error("embedding: padding_idx is outside the vocabulary");
+    if (padding < 0 || padding >= V)
+      value_error("embedding: padding_idx is outside the vocabulary");
   }
   if (!std::isfinite((float)scale)) value_error("embedding: scale must be finite");
   no_tangent(op, {&w_});
@@ -286,8 +289,8 @@ struct LinearCEFunction : Function<LinearCEFunction> {
                                     ld_of(w), (const int64_t*)ptr(labels),
                                     (float)ctx->saved_data["scale"].toDouble(),
                                     (const float*)ptr(lse), (const float*)ptr(kept),
-                                    (const float*)ptr(g[0]), (const float*)ptr(g[1]), out(dx), out(dw), out(ws), size,
-                                    status, on.stream));
+                                    (const float*)ptr(g[0]), (const float*)ptr(g[1]), out(dx),
+                                    out(dw), out(ws), size, status, on.stream));
     }
     return once("linear_cross_entropy", {dx, dw, Tensor(), Tensor(), Tensor()});
   }
@@ -303,7 +306,8 @@ std::tuple<Tensor, Tensor> linear_cross_entropy(const Tensor& x_, const Tensor& 
     type_error("linear_cross_entropy: hidden and weight must share one of "
                "float32/bfloat16/float16");
   need_int(op, "labels", labels_);
-  if (x_.dim() != 2 || x_.size(1) < 1) value_error("linear_cross_entropy: hidden must be [rows, H]");
+  if (x_.dim() != 2 || x_.size(1) < 1)
+    value_error("linear_cross_entropy: hidden must be [rows, H]");
   const int64_t T = x_.size(0), H = x_.size(1);
   if (w.dim() != 2 || w.size(0) < 1 || w.size(1) != H)
     value_error("linear_cross_entropy: weight must be [V, " + std::to_string(H) + "]");
@@ -370,7 +374,8 @@ void no_overlap(const char* op, const List& src, const List& dst) {
   for (size_t i = 0; i < dst.sizes.size(); ++i)
     if (dst.sizes[i]) order.push_back(i);
   auto at = [](const List& l, size_t i) { return (int64_t)(uintptr_t)l.data[i]; };
-  std::sort(order.begin(), order.end(), [&](size_t a, size_t b) { return at(dst, a) < at(dst, b); });
+  std::sort(order.begin(), order.end(),
+            [&](size_t a, size_t b) { return at(dst, a) < at(dst, b); });
   for (size_t k = 1; k < order.size(); ++k)
     if (end_of(dst, order[k - 1]) > at(dst, order[k]))
       value_error(std::string(op) + ": two tensors that are written share memory");

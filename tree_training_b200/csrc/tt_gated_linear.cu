@@ -26,7 +26,7 @@
 //
 // Measured on a B200, bf16, 8,192 x 2,560 x 9,728, single launches: forward 537 us with g
 // and u kept (495 without), dg and du 158 (7.1 TB/s), dx 501, both weights' gradients 528;
-// a pass back to back 2,080 to 2,170 us, at the power limit.
+// a pass back to back 2,080 to 2,240 us, at the power limit.
 #include "tt_gemm_sm100.cuh"
 
 namespace tt {
@@ -252,7 +252,8 @@ __device__ __forceinline__ void settle_signs(const Doubts& d, int row, bool live
   for (uint32_t who; (who = __ballot_sync(0xffffffffu, mask != 0)) != 0;) {
     const int from = __ffs(who) - 1;
     const int i = __shfl_sync(0xffffffffu, __ffs(mask) - 1, from);
-    const T* a = reinterpret_cast<const T*>(d.x) + (int64_t)__shfl_sync(0xffffffffu, row, from) * d.x_ld;
+    const int64_t of_x = __shfl_sync(0xffffffffu, row, from);
+    const T* a = reinterpret_cast<const T*>(d.x) + of_x * d.x_ld;
     const T* b = reinterpret_cast<const T*>(d.w) + (int64_t)(feature + i) * d.w_ld;
     constexpr int kAhead = 5;              // packs of a row that are fetched together
     double sum = 0.0, more = 0.0;
@@ -327,17 +328,24 @@ struct GatedEpi {
   }
 };
 
+// Two rows go here up to kFewWeights elements of a weight (H x F; us here and by the
+// tensor cores: 1,024 x 4,096 9.4 and 14.4, 2,048 x 8,192 19.5 and 25.0, 2,560 x 9,728 25.1 and
+// 24.3, 4,096 x 12,288 45.7 and 39.6; 2,560 x 8,192, past the limit, 23.0 and 33.3: tiles of
+// a wave and a bit).
 constexpr int kFewRows = 2;
 constexpr int kFewBytes = 40960;           // of x in shared memory
-constexpr int64_t kFewWeights = 1 << 24;   // elements of a weight, for two rows
+constexpr int64_t kFewWeights = 1 << 24;
 
-// A warp a feature, N rows of x.
+// A warp a feature, N rows of x.  Of a feature's two rows five packs each are fetched
+// together: 10 loads a lane (us of one row with four, five and eight: 2,560 x 9,728 22.3, 21.0
+// and 26.9, whose 320 packs are two rounds of five; 4,096 x 12,288 39.6, 41.6 and 41.6; 3,584 x
+// 18,944 48.5, 47.7 and 51.9; 2,048 x 8,192 16.8, 17.7 and 18.2).
 template <typename T, int A, int N>
 __global__ void __launch_bounds__(256)
     few_rows_kernel(const T* x, int64_t x_ld, const T* wg, int64_t wg_ld, const T* wu,
                     int64_t wu_ld, int rows, int H, int F, T* h, float* g_out, float* u_out,
                     int64_t keep_ld) {
-  constexpr int kAhead = 5;                // packs of a row that are fetched together
+  constexpr int kAhead = 5;
   extern __shared__ uint4 xs[];            // [N][packs]
   const int packs = (H + 7) / 8, lane = threadIdx.x & 31;
   const int f = blockIdx.x * 8 + threadIdx.x / 32;
@@ -380,7 +388,10 @@ __global__ void __launch_bounds__(256)
         float vx[8];
         vec::unpack<T, 8>(xs[t * packs + p], vx);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[t] = fmaf(vg[i], vx[i], g[t]), u[t] = fmaf(vu[i], vx[i], u[t]);
+        for (int i = 0; i < 8; ++i) {
+          g[t] = fmaf(vg[i], vx[i], g[t]);
+          u[t] = fmaf(vu[i], vx[i], u[t]);
+        }
       }
     }
   }
@@ -610,7 +621,8 @@ extern "C" int tt_gated_linear_bwd(int dtype, int64_t T, int32_t H, int32_t F, c
     const gemm::Result r{dtype, c, N, nullptr, 0, 1.f, nullptr};
     return dtype == TT_F32
                ? gemm::fp32_product(M, N, terms, n, r, work, work_bytes, st)
-               : gemm::tc_product(dtype == TT_BF16, M, N, terms, n, r, work, work_bytes, status, st);
+               : gemm::tc_product(dtype == TT_BF16, M, N, terms, n, r, work, work_bytes, status,
+                                  st);
   };
   if (dx) {
     const gemm::Term terms[2] = {{{dg, ld, false}, {wg, wg_ld, true}, F},

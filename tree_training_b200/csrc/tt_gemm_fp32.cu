@@ -8,8 +8,8 @@
 // 64 where there are few rows or tiles, which would leave SMs idle); slices of 16 of k
 // are loaded into registers while the slice before is multiplied out of shared memory.
 // Bound by the fma rate (measured on a B200 at 4,096 a side: 51 to 58 TFLOP/s of 74; the
-// library's 57).  Up to eight rows have kernels of their own.  Where there are few tiles the sum over k is split over blocks, whose
-// parts are added up in order by a second kernel.
+// library's 57).  Up to eight rows have kernels of their own.  Where there are few tiles the
+// sum over k is split over blocks, whose parts are added up in order by a second kernel.
 #include <algorithm>
 
 #include "tt_gemm.cuh"

@@ -74,7 +74,8 @@ struct StoreEpi {
 template <typename T>
 __global__ void __launch_bounds__(256)
     join_tiles_kernel(const __grid_constant__ Problem p, const float* parts, T* c, T* c2,
-                      int gap, int second, int64_t ld, const float* cin, int64_t cin_ld, float alpha, const float* alpha_dev) {
+                      int gap, int second, int64_t ld, const float* cin, int64_t cin_ld,
+                      float alpha, const float* alpha_dev) {
   const TileAt t = tile_at(p, p.whole + blockIdx.x * p.parts);
   const int64_t size = (int64_t)p.tile_rows * p.bn;
   const float* q = parts + (int64_t)t.unit * size;
@@ -112,14 +113,16 @@ int product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& 
   for (int i = 0; i < n_terms; ++i) steps += (terms[i].k + kBK - 1) / kBK;
   const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
   Plan plan = plan_product(M, N, steps, bmn ? 64 : 16, false, true);
-  if (plan.work > work_bytes || !work) plan = plan_product(M, N, steps, bmn ? 64 : 16, false, false);
+  if (plan.work > work_bytes || !work)
+    plan = plan_product(M, N, steps, bmn ? 64 : 16, false, false);
   Problem q;
   if (!set_up(&q, plan, kB, M, N, terms, n_terms, false, status)) return TT_ERR_UNSUPPORTED;
   typename Epi::Args a{};
   a.alpha = r.alpha, a.alpha_dev = r.alpha_dev, a.parts = (float*)work;
   a.c = r.p, a.c2 = r.p2, a.gap = (int)r.gap, a.second = (int)r.second, a.ld = r.ld;
   a.cin = r.cin, a.cin_ld = r.cin_ld, a.f32 = r.dtype == TT_F32;
-  a.wide = ((reinterpret_cast<uintptr_t>(a.c) | reinterpret_cast<uintptr_t>(a.c2)) & 15) == 0 && a.ld * (a.f32 ? 4 : 2) % 16 == 0;
+  a.wide = ((reinterpret_cast<uintptr_t>(a.c) | reinterpret_cast<uintptr_t>(a.c2)) & 15) == 0 &&
+           a.ld * (a.f32 ? 4 : 2) % 16 == 0;
   a.cin_wide = (reinterpret_cast<uintptr_t>(a.cin) & 15) == 0 && a.cin_ld % 4 == 0;
   int rc;
   if (amn && bmn) rc = launch<true, true, Epi>(plan, q, a, st);
@@ -129,7 +132,8 @@ int product(int64_t M, int64_t N, const Term* terms, int n_terms, const Result& 
   if (rc != TT_OK || split == 0) return rc;
   return vec::dispatch_float(r.dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const dim3 grid((unsigned)split, (unsigned)std::min<int64_t>(64, std::max<int64_t>(1, 8 * vec::kSMs / split)));
+    const int64_t rows = std::min<int64_t>(64, std::max<int64_t>(1, 8 * vec::kSMs / split));
+    const dim3 grid((unsigned)split, (unsigned)rows);
     join_tiles_kernel<T><<<grid, 256, 0, st>>>(q, a.parts, (T*)r.p, (T*)r.p2, a.gap, a.second, r.ld,
                                                r.cin, r.cin_ld, r.alpha, r.alpha_dev);
     tt_count_launches(1);
@@ -149,7 +153,8 @@ struct Aligned {
   int64_t first[kMaxAligned + 1];          // piece of an array
 };
 
-__global__ void __launch_bounds__(kAlignThreads) align_rows_kernel(const __grid_constant__ Aligned a) {
+__global__ void __launch_bounds__(kAlignThreads)
+    align_rows_kernel(const __grid_constant__ Aligned a) {
   for (int64_t i = blockIdx.x; i < a.first[kMaxAligned]; i += gridDim.x) {
     int t = 0;
 #pragma unroll
@@ -213,6 +218,7 @@ extern "C" int tt_align_rows_of(int32_t count, const int64_t* rows, const int64_
   return cudaGetLastError() == cudaSuccess ? TT_OK : TT_ERR_CUDA;
 }
 
+// (for callers of the C ABI with one array: the bindings copy all of a call at once)
 extern "C" int tt_align_rows(int64_t rows, int64_t cols, const void* src, int64_t ld, void* dst,
                              int64_t dst_ld, void* stream) {
   return tt_align_rows_of(1, &rows, &cols, &src, &ld, &dst, &dst_ld, stream);

@@ -235,7 +235,10 @@ __global__ void __launch_bounds__(threads_of<Epi>(), 1)
   const volatile int32_t* abort_flag = &sh->abort;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], warps_of<Epi>() * CG);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->acc_full[b], 1);
+      mbar_init(&sh->acc_empty[b], warps_of<Epi>() * CG);
+    }
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -542,10 +545,13 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int n_step, bool d
     for (int bn = 256; bn >= step; bn -= step) {
       const int64_t cols = dual ? bn / 2 : bn;
       const int64_t tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + cols - 1) / cols);
-      const int64_t rest = tiles % slots, most = rest && split ? std::min(slots / rest, steps / 8) : 1;
-      const double clocks = (double)slice_clocks(cg, bn), end = (double)epilogue_clocks(cg, bn, dual);
+      const int64_t rest = tiles % slots;
+      const int64_t most = rest && split ? std::min(slots / rest, steps / 8) : 1;
+      const double clocks = (double)slice_clocks(cg, bn);
+      const double end = (double)epilogue_clocks(cg, bn, dual);
       auto tile = [&](int64_t n) { return std::max((double)n * clocks, end) + 600; };
-      for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); parts = next_parts(parts, most)) {
+      for (int64_t parts = 1; parts <= std::max<int64_t>(1, most);
+           parts = next_parts(parts, most)) {
         // (a tile's start and end, which nothing hides: 600 clocks; the parts' way
         // through L2 and the launch that adds them up)
         const int64_t whole = parts > 1 ? tiles - rest : tiles;
@@ -575,7 +581,8 @@ inline bool set_up(Problem* q, const Plan& plan, bool bf16, int64_t M, int64_t N
   const bool amn = terms[0].a.mn, bmn = terms[0].b.mn;
   bool k64 = true;                          // whole blocks of 64 k
   for (int i = 0; i < n_terms; ++i) k64 &= terms[i].k % 64 == 0;
-  q->a_blocks = amn ? M % 64 == 0 : k64 && cg == 2, q->b_blocks = bmn ? N % 64 == 0 : k64 && cg == 2;
+  q->a_blocks = amn ? M % 64 == 0 : k64 && cg == 2;
+  q->b_blocks = bmn ? N % 64 == 0 : k64 && cg == 2;
   const int kb = blocks_of_k(cg);
   for (int i = 0; i < 2; ++i) {
     const Term& t = terms[i < n_terms ? i : 0];
@@ -639,8 +646,9 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
 
 // A 32 x 32 block of C: each lane 32 values of a row of its own at `p` (null: none), of
 // which `left` are in C.  Where rows are on 16-byte boundaries (wide) a lane stores its
-// own, of a narrower block as many packs as are whole; else the warp stores row after row out of shared memory, 32 elements next to
-// one another (elements of 32 rows at a time cost an odd width three times the rest).
+// own, of a narrower block as many packs as are whole; else the warp stores row after row
+// out of shared memory, 32 elements next to one another (elements of 32 rows at a time
+// cost an odd width three times the rest).
 template <typename T>
 __device__ __forceinline__ void store_block(T* p, const float (&v)[32], int left, bool wide,
                                             float* block) {

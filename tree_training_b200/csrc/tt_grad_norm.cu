@@ -27,7 +27,7 @@ namespace tt {
 namespace gradnorm {
 namespace {
 
-constexpr int kMaxTensors = 512;       // of a launch: a table of 20 KB
+constexpr int kMaxTensors = 512;       // of a launch: a table of 14.9 KB
 constexpr int kThreads = 512;
 constexpr int64_t kChunkBytes = 32768, kLargeChunkBytes = 131072;
 constexpr int kBlocks = 2 * vec::kSMs; // at most, of a launch: all that are resident
@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       case TT_BF16: {
         const int64_t e = t.chunk_bytes / 2, n = min(e, t.n[i] - at * e);
-        sum = join(sum, chunk_sum<kind>(reinterpret_cast<const __nv_bfloat16*>(t.src[i]) + at * e, n),
-                   kind);
+        sum = join(
+            sum, chunk_sum<kind>(reinterpret_cast<const __nv_bfloat16*>(t.src[i]) + at * e, n), kind);
         break;
       }
       default: {

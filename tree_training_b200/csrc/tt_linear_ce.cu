@@ -16,7 +16,10 @@
 // the vocabulary, each formed again, turned into 16-bit dz by the epilogue, and
 // multiplied twice: dW's rows of the piece are complete, dx is summed up in fp32.
 // The pieces are as wide as a quarter of a gigabyte of dz allows, and at least
-// 4,096: every piece reads and writes dx's fp32 sum once.
+// 4,096: every piece reads and writes dx's fp32 sum once.  Both workspaces grow with the
+// rows: the forward's 8 bytes for 64 logits are T V / 8 (155 MB for 8,192 rows of 151,936
+// words, 2.5 GB for 131,072; more where tiles are narrower), the backward's dz 8,192 T
+// past 32,768 rows.
 //
 // dz is rounded to 16 bits once, as the tensor cores' operands need.  A row's label
 // dominates its dz, so that over few rows that one rounding (2^-9 in bf16) would show
@@ -35,7 +38,7 @@
 // of a piece.
 //
 // Measured on a B200, bf16, W of 151,936 x 2,560: 8,192 rows forward and backward 19.2 to
-// 20.5 ms (1,240 to 1,330 TFLOP/s with the logits formed again, at the power limit); 2,047
+// 20.8 ms (1,230 to 1,330 TFLOP/s with the logits formed again, at the power limit); 2,047
 // rows forward 1.25 ms (1,280 TFLOP/s), 47 rows 140 us forward (5.6 TB/s) and 543 with the
 // backward.
 #include <cfloat>
@@ -627,9 +630,9 @@ extern "C" int64_t tt_linear_ce_bwd_workspace_size(int dtype, int64_t T, int32_t
 extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int64_t M,
                                 const void* x, int64_t x_ld, const void* w, int64_t w_ld,
                                 const int64_t* labels, float scale, const float* lse,
-                                const float* kept, const float* g_loss, const float* g_lse, void* dx, void* dw,
-                                void* workspace, int64_t workspace_bytes, int32_t* status,
-                                void* stream) {
+                                const float* kept, const float* g_loss, const float* g_lse,
+                                void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                                int32_t* status, void* stream) {
   const Shape s{dtype, T, H, V, M};
   if (const int rc = check(s, x, x_ld, w, w_ld, labels)) return rc;
   if (T == 0) return TT_OK;
@@ -683,8 +686,8 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
         return rc;
       const int segment = segment_of(T, P);
       grad_kernel<<<dim3(row_blocks(T), (unsigned)((n + segment - 1) / segment)), 256, 0, st>>>(
-          kept ? kept : (const float*)dz, kept ? kept_ld(dtype, T, H, V) : P, (float*)dz, T, (int)n, P,
-          segment, g);
+          kept ? kept : (const float*)dz, kept ? kept_ld(dtype, T, H, V) : P, (float*)dz, T,
+          (int)n, P, segment, g);
       tt_count_launches(1);
     } else if (kept) {
       const int segment = segment_of(T, P);
@@ -698,8 +701,8 @@ extern "C" int tt_linear_ce_bwd(int dtype, int64_t T, int32_t H, int64_t V, int6
                                              segment, g);
       tt_count_launches(1);
     } else {
-      rc = dtype == TT_BF16 ? gradient_16<true>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st)
-                            : gradient_16<false>(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st);
+      auto* form = dtype == TT_BF16 ? gradient_16<true> : gradient_16<false>;
+      rc = form(s, x, x_ld, wp, w_ld, n, g, dz, rest, P, status, st);
       if (rc) return rc;
     }
     if (dx) {

@@ -193,7 +193,8 @@ def fuse_gated_mlps(model) -> int:
         name, down = _activation_of_parts(mod), getattr(mod, "down_proj", None)
         if name is None or type(down) is not torch.nn.Linear or "forward" in down.__dict__ \
                 or getattr(mod.forward, "__func__", None) is not type(mod).forward \
-                or mod.gate_proj.weight.dtype not in (torch.float32, torch.bfloat16, torch.float16) \
+                or mod.gate_proj.weight.dtype not in (torch.float32, torch.bfloat16,
+                                                      torch.float16) \
                 or any(c not in (mod.gate_proj, mod.up_proj, down, mod.act_fn)
                        for c in mod.children()) \
                 or not _is_plain(mod):
