@@ -182,3 +182,22 @@ def test_state_is_left_as_it_was():
     assert not any(b._forward_hooks or b._forward_pre_hooks for b in m.modules())
     assert all(p.grad is None for p in m.parameters())
     assert tt.fuse_gated_mlps(m) == 0
+
+
+@pytest.mark.parametrize("enabled", [False, True])
+@pytest.mark.filterwarnings("ignore:.*CUDA is not available")
+def test_forwards_that_set_autocast_themselves(enabled):
+    class Setting(Mlp):
+        def forward(self, x):
+            with torch.autocast("cuda", torch.bfloat16, enabled=enabled):
+                return super().forward(x)
+
+    class Frozen(Mlp):
+        def forward(self, x):
+            with torch.no_grad():
+                g = self.gate_proj(x)
+            return self.down_proj(self.act_fn(g) * self.up_proj(x))
+    before = torch.is_autocast_enabled("cuda")
+    assert taken(Setting()) == 0
+    assert taken(Frozen()) == 0
+    assert torch.is_autocast_enabled("cuda") == before

@@ -73,7 +73,7 @@ class _Calls(TorchFunctionMode):
 
     def note(self, func, args, kwargs, out):
         self.calls.append((func, args, kwargs, out, torch.is_grad_enabled(),
-                           torch.is_autocast_enabled()))
+                           torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")))
 
     def enter(self, mod, args):
         self.inside = True
@@ -90,17 +90,22 @@ def _is_plain(mod) -> bool:
     gate, up, down, act = mod.gate_proj, mod.up_proj, mod.down_proj, mod.act_fn
     x = torch.ones(2, gate.in_features, dtype=gate.weight.dtype, device=gate.weight.device)
 
-    def plain(training) -> bool:
+    def plain(training, autocast) -> bool:
         mode = _Calls(act)
         hooks = [act.register_forward_pre_hook(mode.enter), act.register_forward_hook(mode.leave)]
-        context = [training, torch.is_autocast_enabled()]
+        before = torch.is_autocast_enabled("cuda")
+        context = [training, autocast, torch.get_autocast_dtype("cuda")]
         mod.training = training
+        torch.set_autocast_enabled("cuda", autocast)
         try:
             with torch.set_grad_enabled(training), mode:
                 result = mod.forward(x)
         except Exception:                     # (other arguments, say)
             return False
         finally:
+            torch.set_autocast_enabled("cuda", before)
+            if not before:
+                torch.clear_autocast_cache()
             for hook in hooks:
                 hook.remove()
         made = {}
@@ -130,7 +135,8 @@ def _is_plain(mod) -> bool:
     devices = [x.device] if x.is_cuda else []
     try:
         with torch.random.fork_rng(devices=devices):
-            return plain(True) and plain(False)
+            # (one that sets autocast itself shows only where it changes it)
+            return plain(True, False) and plain(False, False) and plain(True, True)
     finally:
         mod.training = training
 
@@ -180,9 +186,10 @@ def fuse_gated_mlps(model) -> int:
     ``up_proj`` and ``down_proj`` without biases, ``act_fn`` one of the activations)
     through :func:`gated_linear`.  Returns how many modules were patched; modules of
     another form or type keep their own forward, and so do those whose forward makes any
-    other call on tensors (a bound, dropout, a branch on a shape; it is run twice to see
-    them), has been replaced (by this function or another: wrap it after this call, as
-    ``checkpoint_mlps`` does), or whose gate or up projection or activation has hooks.
+    other call on tensors (a bound, dropout, a branch on a shape; it is run to see them),
+    sets autocast itself, has been replaced (by this function or another: wrap it after
+    this call, as ``checkpoint_mlps`` does), or whose gate or up projection or activation
+    has hooks.
 
     A patched module looks at its parts in every call: with an adapter in place of a
     projection, a hook on one or on the activation, or an activation that the kernel does
